@@ -277,6 +277,69 @@ int fdwt_specsoftmax_backward(int dtype, int64_t rows, int64_t n, const void* x,
                               void* gh, void* gv, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Layer norm over the last axis (no counterpart in the reference): rows of `dim` values,
+ *   y = (x - mean x) / sqrt(mean (x - mean x)^2 + eps) * weight + bias.
+ * weight and bias may be NULL (1 and 0); their type is param_dtype, the rows' type or FDWT_F32
+ * (fp64 rows: FDWT_F64).  stats, (rows, 2) fp32 (fp64 for fp64 rows), receives the mean and
+ * 1 / sqrt(...) of each row that the backward pass takes; NULL skips it.
+ * ---------------------------------------------------------------------------------------- */
+int fdwt_layer_norm_forward(int dtype, int param_dtype, int64_t rows, int64_t dim, const void* x,
+                            const void* weight, const void* bias, double eps, void* y,
+                            void* stats, void* stream);
+/* dL/dx (rows, dim), dL/dweight and dL/dbias (dim, param_dtype) from dL/dy; each may be NULL.
+ * The sums over rows are added in a fixed order (the same bits every run). */
+size_t fdwt_layer_norm_backward_workspace(int dtype, int64_t rows, int64_t dim, int need_params);
+int fdwt_layer_norm_backward(int dtype, int param_dtype, int64_t rows, int64_t dim,
+                             const void* dy, const void* x, const void* weight,
+                             const void* stats, void* dx, void* dweight, void* dbias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no counterpart in the reference).  Head h has a
+ * state S (dk, dv) and a log decay a = log_decay[h]; over the tokens t of a sequence
+ *   S <- e^a S + k_t v_t^T,   o_t = scale * q_t^T S.
+ * Query head h reads key and value head h / (heads / kv_heads).  q, k, v and out are addressed
+ * by (batch, token, head) strides in elements, their last axis contiguous.  log_decay (heads)
+ * and the states (batch, heads, dk, dv; contiguous) are fp32, fp64 when dtype is FDWT_F64.
+ * lengths (batch, int32, may be NULL: every sequence is full) gives the tokens that count,
+ * clamped to [0, length]: outputs and gradients after them are zero and the state stops there.
+ * Head sizes up to 256.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct {
+  int32_t dtype;
+  int32_t heads, kv_heads;
+  int32_t dk, dv;
+  int64_t batch, length;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* batch, token, head */
+  double scale;
+} fdwt_linattn_desc;
+
+/* out and the states after the sequences (final_state; may be NULL) from initial_state (NULL:
+ * zeros). */
+size_t fdwt_linattn_forward_workspace(const fdwt_linattn_desc* desc);
+int fdwt_linattn_forward(const fdwt_linattn_desc* desc, const void* q, const void* k,
+                         const void* v, const void* log_decay, const void* initial_state,
+                         const int32_t* lengths, void* out, void* final_state, void* workspace,
+                         size_t workspace_bytes, void* stream);
+/* dL/dq (batch, length, heads, dk), dL/dk, dL/dv (batch, length, kv_heads, ...), contiguous, and
+ * dL/dinitial_state (may be NULL) from dL/dout (strides o_stride) and dL/dfinal_state (NULL:
+ * zeros). */
+size_t fdwt_linattn_backward_workspace(const fdwt_linattn_desc* desc);
+int fdwt_linattn_backward(const fdwt_linattn_desc* desc, const void* q, const void* k,
+                          const void* v, const void* log_decay, const void* initial_state,
+                          const int32_t* lengths, const void* d_out, const void* d_final_state,
+                          void* dq, void* dk, void* dv, void* d_initial_state, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* One token for each of desc->batch sequences (desc->length is 1; the token strides are not
+ * used): the states in `state` (state_slots, heads, dk, dv) are updated in place.  slots (batch,
+ * int32; NULL: sequence b has state b) names each sequence's state; a slot outside
+ * [0, state_slots) leaves every state as it is and gives a zero output row.  No two sequences
+ * may name the same slot. */
+int fdwt_linattn_step(const fdwt_linattn_desc* desc, const void* q, const void* k, const void* v,
+                      const void* log_decay, void* state, int64_t state_slots,
+                      const int32_t* slots, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ or the tensors are not on a CUDA device, the call raises.  Status codes other th
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -21,6 +22,7 @@ c_dblp = ctypes.POINTER(ctypes.c_double)
 c_voidpp = ctypes.POINTER(ctypes.c_void_p)
 
 DTYPES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
+DTYPE_OF = {code: dtype for dtype, code in DTYPES.items()}
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -94,6 +96,24 @@ SIGNATURES = {
     "fdwt_dwt_synthesis_workspace": (ctypes.c_size_t, [
         ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, c_i64p, c_i64p, ctypes.c_int,
         ctypes.c_int, ctypes.c_int]),
+    "fdwt_layer_norm_forward": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p]),
+    "fdwt_layer_norm_backward_workspace": (ctypes.c_size_t, [
+        ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "fdwt_layer_norm_backward": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_linattn_forward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_linattn_forward": (ctypes.c_int, [ctypes.c_void_p] * 10 + [
+        ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_linattn_backward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_linattn_backward": (ctypes.c_int, [ctypes.c_void_p] * 14 + [
+        ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_linattn_step": (ctypes.c_int, [ctypes.c_void_p] * 6 + [
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -152,6 +172,16 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing to enter where it is current already."""
+    if torch.cuda.current_device() == device.index:
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 def i64_array(values):

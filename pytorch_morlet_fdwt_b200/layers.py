@@ -11,6 +11,8 @@ reference's parameters).  The forward passes run on this package's fused kernels
 - :class:`MorletAttention` and :class:`MorletChannelMixAttention`, ``(B, H, C, T, D)`` -> the
   same shape: each channel's T*D samples as one signal; per position, a softmax over the CWT
   frequencies weights learned per-channel values (or the channel-mixed input).
+- :class:`DecayTokenMixer`, ``(B, L, D) -> (B, L, D)`` (no counterpart in the reference): a causal
+  mixer with a state, for training, prompts and single tokens.
 """
 
 from __future__ import annotations
@@ -23,9 +25,12 @@ from torch import nn
 
 from .cwt import CWT1D, morlet_mix_tokens, spectral_softmax
 from .dwt import wavedec, waverec
+from .linear_attention import linear_attention, linear_attention_step
+from .norm import LayerNorm
 from .wavelets import WaveletLike
 
-__all__ = ["MorletTokenMixer", "WaveletTokenMixer", "MorletAttention", "MorletChannelMixAttention"]
+__all__ = ["MorletTokenMixer", "WaveletTokenMixer", "MorletAttention", "MorletChannelMixAttention",
+           "DecayTokenMixer"]
 
 
 def _randn_over(rows: int, cols: int, fan: int) -> torch.Tensor:
@@ -233,3 +238,88 @@ class MorletChannelMixAttention(_MorletPatchAttention):
         values = x.reshape(B, H, C, T * D).to(_compute_dtype(x))
         U = torch.matmul(self.freq_to_channel.to(values.dtype), values)  # (B, H, f, T*D)
         return self._spectral_softmax(x, U.reshape(B * H, self.num_freqs, T * D))
+
+
+class DecayTokenMixer(nn.Module):
+    """Causal token mixing by linear attention with a decay for each head, with the norm before
+    it and the residual around it::
+
+        y = x + out_proj(attention(qkv_proj(norm(x))))
+
+    Unlike the wavelet mixers it never looks ahead, so it also answers token by token: a prompt's
+    :meth:`forward` returns the state that :meth:`step` carries on.  Head h forgets
+    ``2 ** -(5 + 7 h / (num_heads - 1))`` of its state a token (memories of about 32 to 4096
+    tokens), a fixed schedule.
+
+    Args: ``dim`` (D), ``num_heads``, ``num_kv_heads`` (heads of the keys and values, shared by
+    groups of query heads; ``num_heads`` by default), ``head_dim`` and ``value_dim`` (sizes of a
+    query/key and of a value head, ``dim // num_heads`` by default), ``eps`` (of the norm).
+    """
+
+    def __init__(self, dim: int, num_heads: int = 4, num_kv_heads: Optional[int] = None,
+                 head_dim: Optional[int] = None, value_dim: Optional[int] = None,
+                 eps: float = 1e-5):
+        super().__init__()
+        kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        if num_heads < 1 or kv_heads < 1 or num_heads % kv_heads:
+            raise ValueError(f"num_heads must be a multiple of num_kv_heads, got {num_heads} and "
+                             f"{kv_heads}")
+        if head_dim is None or value_dim is None:
+            if dim % num_heads:
+                raise ValueError(f"dim {dim} is not a multiple of num_heads {num_heads}: give "
+                                 "head_dim and value_dim")
+        self.num_heads, self.num_kv_heads = num_heads, kv_heads
+        self.head_dim = dim // num_heads if head_dim is None else head_dim
+        self.value_dim = dim // num_heads if value_dim is None else value_dim
+        self.norm = LayerNorm(dim, eps)
+        self._sizes = (num_heads * self.head_dim, kv_heads * self.head_dim,
+                       kv_heads * self.value_dim)
+        self.qkv_proj = nn.Linear(dim, sum(self._sizes))
+        self.out_proj = nn.Linear(num_heads * self.value_dim, dim)
+        self._log_decay = [math.log1p(-2.0 ** -(5 + 7 * h / max(1, num_heads - 1)))
+                           for h in range(num_heads)]
+        self._on_device = {}
+
+    def log_decay(self, device) -> torch.Tensor:
+        """The schedule on ``device`` in fp64's nearest fp32 (kept out of the buffers: a module
+        cast to 16 bits must not round it)."""
+        device = torch.device(device)
+        if device not in self._on_device:
+            self._on_device[device] = torch.tensor(self._log_decay, dtype=torch.float32,
+                                                   device=device)
+        return self._on_device[device]
+
+    def init_state(self, batch: int, device, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Zero states for ``batch`` sequences (or slots of a pool)."""
+        return torch.zeros(batch, self.num_heads, self.head_dim, self.value_dim, device=device,
+                           dtype=dtype)
+
+    def _qkv(self, x: torch.Tensor):
+        q, k, v = self.qkv_proj(self.norm(x)).split(self._sizes, dim=-1)
+        return (q.unflatten(-1, (self.num_heads, self.head_dim)),
+                k.unflatten(-1, (self.num_kv_heads, self.head_dim)),
+                v.unflatten(-1, (self.num_kv_heads, self.value_dim)))
+
+    def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None,
+                lengths: Optional[torch.Tensor] = None, return_state: bool = False):
+        """``x (B, L, D)`` -> ``y (B, L, D)``, or ``(y, state)`` with ``return_state``; ``state``
+        and ``lengths`` as ``initial_state`` and ``lengths`` of
+        :func:`~pytorch_morlet_fdwt_b200.linear_attention`."""
+        if x.dim() != 3:
+            raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
+        q, k, v = self._qkv(x)
+        mixed, state = linear_attention(q, k, v, self.log_decay(x.device), initial_state=state,
+                                        lengths=lengths)
+        y = x + self.out_proj(mixed.flatten(-2))
+        return (y, state) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: torch.Tensor,
+             slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token for each sequence: ``x (B, D)`` -> ``y (B, D)``; ``state`` (of a prompt, or
+        a pool indexed by ``slots``) is updated in place."""
+        if x.dim() != 2:
+            raise ValueError(f"expected (B, D) input, got shape {tuple(x.shape)}")
+        q, k, v = self._qkv(x)
+        mixed = linear_attention_step(q, k, v, self.log_decay(x.device), state, slots=slots)
+        return x + self.out_proj(mixed.flatten(-2))
