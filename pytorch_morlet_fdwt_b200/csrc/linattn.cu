@@ -104,7 +104,9 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
   const T* q = static_cast<const T*>(job.q) + b * job.qs[0] + (h / job.q_group) * job.qs[2];
   const T* k = static_cast<const T*>(job.k) + b * job.ks[0] + (h / job.k_group) * job.ks[2];
   const T* v = static_cast<const T*>(job.v) + b * job.vs[0] + (h / job.v_group) * job.vs[2] + v0;
-  T* o = static_cast<T*>(job.o) + b * job.os[0] + h * job.os[2] + v0;
+  const int64_t o_head = b * job.os[0] + h * job.os[2] + v0;
+  T* o = static_cast<T*>(job.o) + o_head;
+  float* wide = static_cast<float*>(job.o) + o_head;
   A* segs = static_cast<A*>(job.seg) + bh * (call.nseg - 1) * job.dk * job.dv;
   const int64_t state_size = int64_t(job.dk) * job.dv;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -221,8 +223,13 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
       for (int i = 0; i < TM; ++i) {
         const int t = ty + 16 * i;
         if (t < m) {
-          T* row = o + token_of(l0 + t, n, job.reverse) * job.os[1];
-          if (job.o_vec && TN * sizeof(T) % 8 == 0 && tx * TN + TN <= vcols) {
+          const int64_t at = token_of(l0 + t, n, job.reverse) * job.os[1];
+          T* row = o + at;
+          if (job.o_wide) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              if (tx * TN + j < vcols) wide[at + tx * TN + j] = static_cast<float>(out[i][j]);
+          } else if (job.o_vec && TN * sizeof(T) % 8 == 0 && tx * TN + TN <= vcols) {
             Pack<T, TN> w;
 #pragma unroll
             for (int j = 0; j < TN; ++j) w.v[j] = from_acc<T>(out[i][j]);
@@ -264,7 +271,10 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
   }
   if (!STATES) {  // rows after the sequence's end
     for (int64_t l = imax(begin, n) + ty; l < row_end; l += 16)
-      for (int c = tx; c < vcols; c += 16) o[l * job.os[1] + c] = from_acc<T>(A(0));
+      for (int c = tx; c < vcols; c += 16) {
+        if (job.o_wide) wide[l * job.os[1] + c] = 0.0f;
+        else o[l * job.os[1] + c] = from_acc<T>(A(0));
+      }
   }
   A* dst = STATES ? segs + seg * state_size
                   : (seg == last && job.fin != nullptr ? static_cast<A*>(job.fin) + bh * state_size
@@ -306,18 +316,18 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant
 }
 
 // Gradients of shared key or value heads: the sum over the heads that read them, in the order of
-// the heads.
+// the heads; the heads' own gradients are 32 bits (64 for fp64), rounded once here.
 template <typename T>
 __global__ void __launch_bounds__(256)
-linattn_group_sum_kernel(const T* __restrict__ in, T* __restrict__ out, int64_t count, int group,
-                         int dim) {
+linattn_group_sum_kernel(const typename AccOf<T>::type* __restrict__ in, T* __restrict__ out,
+                         int64_t count, int group, int dim) {
   using A = typename AccOf<T>::type;
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= count) return;
   const int64_t head = i / dim;
-  const T* p = in + head * group * dim + i % dim;
+  const A* p = in + head * group * dim + i % dim;
   A sum = A(0);
-  for (int g = 0; g < group; ++g) sum += A(to_acc(p[int64_t(g) * dim]));
+  for (int g = 0; g < group; ++g) sum += p[int64_t(g) * dim];
   out[i] = from_acc<T>(sum);
 }
 
@@ -480,7 +490,7 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
     job.q_vec = vector_ok(job.q, job.qs, job.dk, size);
     job.k_vec = vector_ok(job.k, job.ks, job.dk, size);
     job.v_vec = vector_ok(job.v, job.vs, job.dv, size);
-    job.o_vec = vector_ok(job.o, job.os, job.dv, size);
+    job.o_vec = vector_ok(job.o, job.os, job.dv, job.o_wide ? 4 : size);
   }
   const Plan p = make_plan(dtype, call, tc_supports(dtype, call));
   call.nseg = p.nseg;
@@ -654,15 +664,20 @@ extern "C" int fdwt_linattn_forward(const fdwt_linattn_desc* desc, const void* q
   return run(desc->dtype, call, workspace, s);
 }
 
+// A gradient of every query head in 32 bits (64 for fp64).
+static size_t per_head_bytes(const fdwt_linattn_desc* desc, int dim) {
+  return size_t(desc->batch) * desc->length * desc->heads * dim *
+         (desc->dtype == FDWT_F64 ? 8 : 4);
+}
+
 extern "C" size_t fdwt_linattn_backward_workspace(const fdwt_linattn_desc* desc) {
   if (!desc_ok(desc) || !desc_supported(desc) || desc->batch == 0 || desc->length == 0) return 0;
   Call call{};
   shape_jobs(desc, true, &call);
   size_t bytes = call_workspace(desc->dtype, call);
   if (desc->heads != desc->kv_heads)
-    bytes = round256(bytes) + round256(size_t(desc->batch) * desc->length * desc->heads * desc->dk *
-                                       dtype_size(desc->dtype)) +
-            size_t(desc->batch) * desc->length * desc->heads * desc->dv * dtype_size(desc->dtype);
+    bytes = round256(bytes) + round256(per_head_bytes(desc, desc->dk)) +
+            per_head_bytes(desc, desc->dv);
   return bytes;
 }
 
@@ -698,8 +713,8 @@ extern "C" int fdwt_linattn_backward(const fdwt_linattn_desc* desc, const void* 
   if (shared) {  // per query head first
     char* p = ws + round256(call_workspace(desc->dtype, call));
     dk_all = p;
-    dv_all = p + round256(size_t(desc->batch) * desc->length * desc->heads * desc->dk *
-                          dtype_size(desc->dtype));
+    dv_all = p + round256(per_head_bytes(desc, desc->dk));
+    call.job[1].o_wide = call.job[2].o_wide = dtype_size(desc->dtype) == 2;
   }
   auto set = [&](Job& j, const void* jq, const void* jk, const void* jv, void* jo,
                  const void* init, void* fin) {
@@ -725,7 +740,7 @@ extern "C" int fdwt_linattn_backward(const fdwt_linattn_desc* desc, const void* 
       const int e = pre_launch(s);
       if (e != FDWT_OK) return e;
       linattn_group_sum_kernel<T><<<static_cast<unsigned>(cdiv(count, 256)), 256, 0, s>>>(
-          static_cast<const T*>(which == 0 ? dk_all : dv_all),
+          static_cast<const typename AccOf<T>::type*>(which == 0 ? dk_all : dv_all),
           static_cast<T*>(which == 0 ? dk : dv), count, group, dim);
       const int l = launch_status();
       if (l != FDWT_OK) return l;

@@ -41,6 +41,7 @@ struct Job {
   int dk, dv, tiles;                   // tiles: column tiles of the value axis
   int reverse, off;
   int q_vec, k_vec, v_vec, o_vec;      // 16-byte accesses are aligned
+  int o_wide;                          // o is fp32 though the operands are 16 bits
   double inter, intra, write;
 };
 

@@ -23,7 +23,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, config
 
 __all__ = ["linear_attention", "linear_attention_step"]
 
@@ -128,6 +128,8 @@ def _forward(q, k, v, log_decay, initial, lengths, scale, sizes):
             None if lengths is None else lengths.data_ptr(), out.data_ptr(), final.data_ptr(),
             None if ws is None else ws.data_ptr(), nws, _lib.stream_of(dev))
     _lib.check(st, "fdwt_linattn_forward")
+    if config.check_device_errors:
+        _lib.check_device_error("fdwt_linattn_forward")
     return out, final
 
 
@@ -171,6 +173,8 @@ class _LinearAttentionFunction(torch.autograd.Function):
                 dvv.data_ptr(), None if d_initial is None else d_initial.data_ptr(),
                 None if ws is None else ws.data_ptr(), nws, _lib.stream_of(dev))
         _lib.check(st, "fdwt_linattn_backward")
+        if config.check_device_errors:
+            _lib.check_device_error("fdwt_linattn_backward")
         return dq, dkk, dvv, None, d_initial, None, None, None
 
 
