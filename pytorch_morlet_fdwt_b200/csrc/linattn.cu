@@ -426,10 +426,11 @@ int simt_launch(const Call& call, int dk, bool states, int64_t grid, cudaStream_
   return simt_launch_as<T, 256, 32, 32>(call, states, grid, stream);
 }
 
-// Accesses of 16 bytes along the last axis are aligned (and the axis ends on one).
-inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t size) {
-  const int64_t v = 16 / static_cast<int64_t>(size);
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && dim % v == 0 && strides[0] % v == 0 &&
+// Accesses of `bytes` along the last axis are aligned (and the axis ends on one).
+inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t size,
+                      size_t bytes = 16) {
+  const int64_t v = static_cast<int64_t>(bytes / size);
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && dim % v == 0 && strides[0] % v == 0 &&
          strides[1] % v == 0 && strides[2] % v == 0;
 }
 
@@ -487,10 +488,22 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
   const size_t size = dtype_size(dtype);
   for (int j = 0; j < call.jobs; ++j) {
     Job& job = call.job[j];
+    // the stride of an axis of one element is whatever the caller had there
+    auto normal = [&](int64_t* s, int group) {
+      if (call.batch == 1) s[0] = 0;
+      if (call.length == 1) s[1] = 0;
+      if (call.heads / group == 1) s[2] = 0;
+    };
+    normal(job.qs, job.q_group);
+    normal(job.ks, job.k_group);
+    normal(job.vs, job.v_group);
+    normal(job.os, 1);
     job.q_vec = vector_ok(job.q, job.qs, job.dk, size);
     job.k_vec = vector_ok(job.k, job.ks, job.dk, size);
     job.v_vec = vector_ok(job.v, job.vs, job.dv, size);
-    job.o_vec = vector_ok(job.o, job.os, job.dv, job.o_wide ? 4 : size);
+    const size_t o_size = job.o_wide ? 4 : size;
+    job.o_vec = vector_ok(job.o, job.os, job.dv, o_size, 16) +
+                vector_ok(job.o, job.os, job.dv, o_size, 32);
   }
   const Plan p = make_plan(dtype, call, tc_supports(dtype, call));
   call.nseg = p.nseg;

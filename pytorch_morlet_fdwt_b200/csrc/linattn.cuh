@@ -40,7 +40,7 @@ struct Job {
   int q_group, k_group, v_group;       // operand head = h / group
   int dk, dv, tiles;                   // tiles: column tiles of the value axis
   int reverse, off;
-  int q_vec, k_vec, v_vec, o_vec;      // 16-byte accesses are aligned
+  int q_vec, k_vec, v_vec, o_vec;      // 16-byte accesses are aligned (o_vec 2: 32-byte too)
   int o_wide;                          // o is fp32 though the operands are 16 bits
   double inter, intra, write;
 };

@@ -4,14 +4,15 @@
 // One block per SM runs one head's segment, 64 value columns of it, in chunks of 128 tokens:
 //
 //   Sc = Q K^T            (128 x 128)    shared x shared   -> TMEM, two buffers
-//   P  = Sc * M           rounded to 16 bits, TMEM -> registers -> TMEM
+//   P  = Sc * M           rounded to 16 bits, over Sc's columns in TMEM
 //   Oi = P V              (128 x 64)     TMEM x shared     -> TMEM
 //   Oe = Q S              (128 x 64)     shared x shared   -> TMEM, S the 16-bit copy of the state
-//   U  = K^T (V' + V'')   (DK x 64)      shared x shared   -> TMEM
+//   U  = K^T V'           (DK x 64)      shared x shared   -> TMEM, two buffers
 //   o  = diag(d^{l+off}) inter Oe + Oi,  S <- d^m S + write U   in registers, 32 bits
 //
-// V' + V'' is diag(d^{m-off-l}) V in two 16-bit parts: one part would leave the state 2^-9
-// (bf16) off per token, two leave 2^-17.  The scores and the copy of S that multiplies Q are
+// V' is diag(d^{m-off-l}) V in two 16-bit parts (fp16) or three (bf16): one part would leave the
+// state a 2^-9 (bf16) of each token off, two 2^-17, more than the 32-bit state's own rounding.
+// The scores and the copy of S that multiplies Q are
 // rounded once to the operands' type, as the products need it; their errors are of the size of
 // the result's own rounding.  fp16 would overflow or lose small values there: each row of P and
 // each copy of S is scaled by a power of two first, undone in the sum for o.
@@ -19,8 +20,10 @@
 // Bound: 2 (2 Dk + 2 Dv) bytes of HBM a token and head against about 4 (Dk Dv + 128 (Dk + Dv))
 // operations, 96 a byte at 128 x 128, under half of the tensor rate at the HBM rate.  What costs
 // is the chain of dependent steps in a chunk, so every step has its own warps and the chunks
-// overlap: four warps load (cp.async) and form V' + V'', one issues all products, four form P,
+// overlap: one warp issues the loads (TMA), four form V', one issues all products, four form P,
 // four keep the state, four finish o.  Every wait on a barrier has a time limit.
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "linattn.cuh"
@@ -55,6 +58,18 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
+// The same without waiting for the phase.
+__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 constexpr long long kWaitCycles = 4000000000LL;  // about two seconds
 // False: the wait ran out here or elsewhere in the block; the block then ends early.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
@@ -83,30 +98,45 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                    smem_addr(bar))
                : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+// Shared-memory operands are given by the low word of their descriptor (operand() below); the
+// high word is the same for all: 128-byte swizzle, 8-row groups 1024 bytes apart.
+constexpr uint32_t kOperandHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+// D = A B (+ D), A in shared memory or (mma_ts) in TMEM
+template <bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, %5, 0;\n"
+      " mov.b64 x, {%1, %4};\n mov.b64 y, {%2, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(kOperandHigh), "n"(ADD ? 1 : 0)
       : "memory");
 }
 // D = A B + 2^-11 D
-__device__ __forceinline__ void mma_ss_shift11(uint32_t d, uint64_t a, uint64_t b,
+__device__ __forceinline__ void mma_ss_shift11(uint32_t d, uint32_t a, uint32_t b,
                                                uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, 1, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc)
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, 1, 0;\n"
+      " mov.b64 x, {%1, %4};\n mov.b64 y, {%2, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p, 11;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(kOperandHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+template <bool ADD>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.u32 p, %5, 0;\n"
+      " mov.b64 y, {%2, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(kOperandHigh), "n"(ADD ? 1 : 0)
       : "memory");
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(is));
+  return is != 0;
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&r)[32]) {
   uint32_t u[32];
@@ -154,21 +184,32 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(in ? 16 : 0)
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)),
+               "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int token,
+                                         int head, int batch, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(token), "r"(head), "r"(batch), "r"(smem_addr(bar))
+      : "memory");
+}
+// (a, b) * (c, d)
+__device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
+      " mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
 }
 
-// Shared-memory operand descriptor: 128-byte swizzle, 8-row groups 1024 bytes apart, panels of
-// 64 elements `lead` bytes apart (used where the operand's rows run along the contraction).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
-  return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(lead >> 4) << 16) |
-         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// Low word of an operand's descriptor: its address, and `lead`, the distance of its panels of 64
+// elements (used where the operand's rows run along the contraction).  An offset of n bytes adds
+// n / 16 (addresses stay below 2^18).
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
+  return (addr >> 4) | ((lead >> 4) << 16);
 }
 // Instruction descriptor: fp32 result, 16-bit operands; a_mn / b_mn: the operand's contiguous
 // axis is M / N instead of the contraction.
@@ -219,7 +260,7 @@ __device__ __forceinline__ float scale_of(float most, float* inverse) {
 struct Where {
   const Job* job;
   int64_t bh, n, begin, end, row_end;  // valid tokens [begin, end) and rows [begin, row_end)
-  int h, b, seg, last, v0, vcols, chunks;
+  int h, b, seg, last, v0, vcols, chunks, ji;
   float a;
 };
 
@@ -233,6 +274,7 @@ __device__ __forceinline__ Where locate(const Call& call) {
   int ji = 0;
   while (tile >= call.job[ji].tiles) tile -= call.job[ji++].tiles;
   w.job = &call.job[ji];
+  w.ji = ji;
   w.b = static_cast<int>(w.bh / call.heads);
   w.h = static_cast<int>(w.bh % call.heads);
   w.v0 = tile * NV;
@@ -252,105 +294,100 @@ __device__ __forceinline__ Where locate(const Call& call) {
   return w;
 }
 
-// A loader thread's share of 128 rows x 64 PANELS columns: 16-byte column group `tid % 8` of the
-// rows tid / 8 + 16 j of each panel, zeros past the valid rows and columns.
-template <typename T, int PANELS> struct Loader {
-  const T* base;     // row 0 of the head, this thread's first column
-  int64_t stride;    // elements between tokens
-  uint32_t in_mask;  // panels whose columns exist
-  __device__ __forceinline__ void init(const void* p, const int64_t* s, int64_t b, int head,
-                                       int first, int cols, int tid) {
-    const int c = tid % 8 * 8;
-    base = static_cast<const T*>(p) + b * s[0] + head * s[2] + first;
-    stride = s[1];
-    in_mask = 0;
+// The operands of the jobs as 4-d tensors (column, token, head, batch), boxes of 64 columns x 64
+// tokens, 128-byte swizzle; what lies outside reads as zeros.
+constexpr int kBoxRows = 64, kBox = kBoxRows * 128;
+struct Maps {
+  CUtensorMap map[kMaxJobs][3];  // q, k, v
+};
+struct Source {
+  const CUtensorMap* map;
+  int head, batch;
+  __device__ __forceinline__ Source(const CUtensorMap* m, const int64_t* stride, int h, int b)
+      : map(m), head(stride[2] == 0 ? 0 : h), batch(stride[0] == 0 ? 0 : b) {}
+  // ROWS tokens from `token` on, `columns` panels of 64 columns from x on, to dst
+  template <int ROWS> __device__ __forceinline__ void load(uint32_t dst, int x, int panels,
+                                                           int64_t token, uint64_t* bar) const {
+    for (int i = 0; i < panels; ++i)
 #pragma unroll
-    for (int i = 0; i < PANELS; ++i)
-      if (c + 64 * i < cols) in_mask |= 1u << i;
-    if (in_mask) base += c;
-  }
-  // rows l0 .. l0 + 127 of the job's order, `valid` of them
-  __device__ __forceinline__ void load(uint32_t dst, int64_t l0, int64_t n, int reverse, int valid,
-                                       int tid) const {
-    const int r0 = tid / 8;
-    const uint32_t cell = dst + r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
-    const int64_t step = reverse ? -stride : stride;
-    const T* row = base + (reverse ? n - 1 - l0 : l0) * stride;
-#pragma unroll
-    for (int j = 0; j < C / 16; ++j) {
-      const bool in = r0 + 16 * j < valid;
-      const T* src = in ? row + (r0 + 16 * j) * step : base;
-#pragma unroll
-      for (int i = 0; i < PANELS; ++i) {
-        const bool ok = in && (in_mask >> i & 1);
-        cp_async16(cell + i * kPanel + j * 16 * 128, ok ? src + 64 * i : base, ok);
-      }
-    }
+      for (int r = 0; r < ROWS / kBoxRows; ++r)
+        tma_load(dst + (i * (ROWS / kBoxRows) + r) * kBox, map, x + 64 * i,
+                 static_cast<int>(token) + r * kBoxRows, head, batch, bar);
   }
 };
 
-// The second part of a weighted value is held times 2^11 in fp16: where the first part is
+// Parts of a weighted value.  The second part is held times 2^11 in fp16: where the first part is
 // subnormal (a small value, far behind), an unscaled second part would have no bits left.
-template <typename T> constexpr float kLowScale = std::is_same<T, __half>::value ? 2048.0f : 1.0f;
+template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
+template <typename T> constexpr int kParts = kIsHalf<T> ? 2 : 3;
+constexpr float kLowScale = 2048.0f;
 
-// diag(weight) V in two 16-bit parts.  A loader thread reads back the groups it copied itself.
-template <typename T>
-__device__ __forceinline__ void split_values(const unsigned char* v, unsigned char* high,
-                                             unsigned char* low, const float (&weight)[C / 16],
-                                             int tid) {
+// V' = diag(weight) V in parts, `lead` bytes apart; thread tid takes the 16-byte column group
+// tid % 8 of the rows tid / 8 + 16 j.
+template <typename T, int ROWS>
+__device__ __forceinline__ void split_values(const unsigned char* v, unsigned char* parts, int lead,
+                                             const float (&weight)[ROWS / 16], int tid) {
   const int r0 = tid / 8;
   const int cell = r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
-#pragma unroll
-  for (int j = 0; j < C / 16; ++j) {
+#pragma unroll 2
+  for (int j = 0; j < ROWS / 16; ++j) {
     const int at = cell + j * 16 * 128;
     const uint4 x = *reinterpret_cast<const uint4*>(v + at);
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-    uint32_t hi[4], lo[4];
+    uint32_t out[kParts<T>][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 f = unpack<T>(in[i]);
       f.x *= weight[j];
       f.y *= weight[j];
-      hi[i] = pack<T>(f.x, f.y);
-      const float2 g = unpack<T>(hi[i]);
-      lo[i] = pack<T>((f.x - g.x) * kLowScale<T>, (f.y - g.y) * kLowScale<T>);
-    }
-    *reinterpret_cast<uint4*>(high + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(low + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-  }
-}
-
-// D (+)= K^T B over a chunk: M runs along the heads' size, the contraction over the tokens.
-// shift: D counts 2^-11 in the sum.
-template <typename T, int DK, bool SHIFT>
-__device__ __forceinline__ void issue_update(uint32_t d, uint32_t k, uint32_t b, bool add) {
-  constexpr uint32_t id = instr<T>(DK, NV, true, true);
 #pragma unroll
-  for (int i = 0; i < C / 16; ++i) {
-    const uint64_t x = operand(k + i * 2048, kPanel), y = operand(b + i * 2048, kPanel);
-    if (SHIFT && i == 0) mma_ss_shift11(d, x, y, id);
-    else mma_ss(d, x, y, id, add || i > 0);
+      for (int p = 0; p < kParts<T>; ++p) {
+        out[p][i] = pack<T>(f.x, f.y);
+        const float2 g = unpack<T>(out[p][i]);
+        f.x -= g.x;
+        f.y -= g.y;
+        if (kIsHalf<T>) {
+          f.x *= kLowScale;
+          f.y *= kLowScale;
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kParts<T>; ++p)
+      *reinterpret_cast<uint4*>(parts + p * lead + at) =
+          make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
   }
 }
 
-constexpr int kThreads = 544;  // 4 warps each: P, o, state, loads; one issues the products
-constexpr uint32_t kColumns = 512;
-// TMEM columns
-constexpr uint32_t kSc = 0, kP = 256, kOe = 320, kOi = 384, kU = 448;
+// D (+)= K^T B over ROWS tokens (FIRST: the first product does not add; SHIFT: D counts 2^-11 in
+// it): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
+template <typename T, int DK, int ROWS, bool FIRST, bool SHIFT>
+__device__ __forceinline__ void issue_update(uint32_t d, uint32_t k, uint32_t b) {
+  constexpr uint32_t id = instr<T>(DK, NV, true, true);
+  if (SHIFT) mma_ss_shift11(d, k, b, id);
+  else mma_ss<!FIRST>(d, k, b, id);
+#pragma unroll
+  for (int i = 1; i < ROWS / 16; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
+}
 
-template <int DK> struct Smem {
+constexpr int kThreads = 576;  // 4 warps each: P, o, state, V'; one for the products, one loads
+constexpr uint32_t kColumns = 512;
+// TMEM columns; P lies over its Sc
+constexpr uint32_t kSc = 0, kOe = 256, kOi = 320, kU = 384;
+// The state launch takes 64 tokens at a time: more stages, two buffers of V'.
+constexpr int kStateRows = 64, kStatePanel = kStateRows * 128;
+
+template <typename T, int DK> struct Smem {
   static constexpr int panels = DK / 64;
   static constexpr int stages = DK == 64 ? 3 : 2;
   static constexpr int q = 0, k = panels * kPanel, v = 2 * panels * kPanel;
   static constexpr int stage = (2 * panels + 1) * kPanel;
-  static constexpr int high = stages * stage, low = high + kPanel, s = low + kPanel;
-  static constexpr int out = s + DK * 128;
-  static constexpr int bytes = out + kPanel + 1024;  // 1024: room to align the base
-  // the state launch: K, V, and two buffers of V' + V''
-  static constexpr int st_stage = (panels + 1) * kPanel;
-  static constexpr int st_stages = 3;
-  static constexpr int st_high = st_stages * st_stage;
-  static constexpr int st_bytes = st_high + 4 * kPanel + 1024;
+  static constexpr int parts = stages * stage, s = parts + kParts<T> * kPanel;
+  static constexpr int bytes = s + DK * 128 + 1024;  // 1024: room to align the base
+  static constexpr int st_stages = 4;
+  static constexpr int st_stage = (panels + 1) * kStatePanel;
+  static constexpr int st_parts = st_stages * st_stage;
+  static constexpr int st_bytes = st_parts + 2 * kParts<T> * kStatePanel + 1024;
 };
 
 __device__ __forceinline__ unsigned char* align_smem(unsigned char* p) {
@@ -369,43 +406,78 @@ __device__ __forceinline__ void tmem_free(uint32_t base) {
                : "memory");
 }
 
+// 16 columns of a row (`cols` of them exist), in whole 32-byte sectors where these are aligned
+// (vec 2), else in 16 bytes (vec 1) or single elements.
+__device__ __forceinline__ void store8(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d,
+                                       uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b),
+               "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, const float (&x)[16], int cols, int vec) {
+  uint32_t u[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) u[c] = pack<T>(x[2 * c], x[2 * c + 1]);
+  if (vec == 2) {
+    if (cols > 0) store8(dst, u[0], u[1], u[2], u[3], u[4], u[5], u[6], u[7]);
+  } else if (vec == 1) {
+    if (cols > 0) *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+    if (cols > 8) *reinterpret_cast<uint4*>(dst + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c < cols) dst[c] = from_acc<T>(x[c]);
+  }
+}
+// The 32-bit form (results that are added over heads later): contiguous, columns in eights.
+__device__ __forceinline__ void store_wide(float* dst, const float (&x)[16], int cols) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if (g * 8 < cols)
+      store8(dst + g * 8, __float_as_uint(x[g * 8]), __float_as_uint(x[g * 8 + 1]),
+             __float_as_uint(x[g * 8 + 2]), __float_as_uint(x[g * 8 + 3]),
+             __float_as_uint(x[g * 8 + 4]), __float_as_uint(x[g * 8 + 5]),
+             __float_as_uint(x[g * 8 + 6]), __float_as_uint(x[g * 8 + 7]));
+}
+
 // ------------------------------------------------------------------------------ main launch
 template <typename T, int DK>
 __global__ void __launch_bounds__(kThreads, 1)
-linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
-  using Z = Smem<DK>;
-  constexpr bool kHalf = std::is_same<T, __half>::value;
+linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Maps maps,
+                  int* error) {
+  using Z = Smem<T, DK>;
+  constexpr bool kHalf = kIsHalf<T>;
   constexpr int S = Z::stages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = align_smem(raw);
-  __shared__ uint64_t full[S], empty[S], sc_full[2], sc_empty[2], p_full, o_full, o_empty, s_full,
-      u_full, u_empty, vp_full, most_full, drain;
+  __shared__ uint64_t full[S], empty[S], sc_full[2], p_full, o_full, o_empty, s_full, u_full[2],
+      u_empty[2], v_full, most_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
-  __shared__ float power[64];          // power[31 + n] = intra d^n, n = 0 .. 31
+  __shared__ float power[64];          // at 31 + t - s: intra d^|t-s|, 0 for a masked pair
   __shared__ float p_inv[2][C];        // fp16: inverse scales of P's rows
   __shared__ float s_inv[2];           // fp16: inverse scale of the state's copy
   __shared__ volatile float s_most[4];  // fp16: largest magnitude of each warp's rows
 
   const Where w = locate(call);
   const Job& job = *w.job;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      bar_init(&full[i], 128);
+      bar_init(&full[i], 1);
       bar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sc_full[i], 1);
-      bar_init(&sc_empty[i], 128);
+      bar_init(&u_full[i], 1);
+      bar_init(&u_empty[i], 128);
     }
     bar_init(&p_full, 128);
     bar_init(&o_full, 1);
     bar_init(&o_empty, 128);
     bar_init(&s_full, 128);
-    bar_init(&u_full, 1);
-    bar_init(&u_empty, 128);
-    bar_init(&vp_full, 128);
+    bar_init(&v_full, 128);
     bar_init(&most_full, 4);
     bar_init(&drain, 1);
     failed = 0;
@@ -413,7 +485,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
   }
   if (threadIdx.x >= 64 && threadIdx.x < 128) {
     const int i = threadIdx.x - 64;
-    power[i] = i < 31 ? 0.0f : float(job.intra) * decay_pow(w.a, float(i - 31));
+    const int n = job.reverse ? 31 - i : i - 31;
+    power[i] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
   }
   if (warp == 16) tmem_alloc(&tmem_slot);
   tc_before();
@@ -425,151 +498,117 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
   const int chunks = w.chunks;
 
   if (warp < 4) {
-    // ---- P = Sc * M.  Row t = 32 warp + lane; 32 columns at a time, those above the diagonal
-    // are zero once and for all.  Off the diagonal block d^{t-s} = (intra d^{32(w-j-1)+lane+1})
-    // d^{31-c}: both powers are at least 0, nothing overflows.
-    float tab[32];
+    // ---- P = Sc * M.  Row t = 32 warp + lane, 32 columns at a time from the left: the 16-bit
+    // scores of a block go over columns whose scores have been read.  Off the diagonal block
+    // (forward; the mirror image back in time) d^{t-s} = d^{32(w-j-1)+lane+1} d^{31-c}: both
+    // powers are at least 0, nothing overflows.
+    const bool rev = job.reverse != 0;
+    float tab[32], lead[4];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) tab[c] = decay_pow(w.a, float(31 - c));
-    float lead = float(job.intra) * decay_pow(w.a, float(lane + 1));
-    const float block = decay_pow(w.a, 32.0f);
-    {
-      uint32_t zero[16];
+    for (int c = 0; c < 32; ++c) tab[c] = decay_pow(w.a, float(rev ? c + 1 : 31 - c));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) zero[i] = 0;
-      for (int j = warp + 1; j < 4; ++j) tmem_st16(tmem + lanes + kP + j * 16, zero);
-      tmem_st_wait();
+    for (int j = 0; j < 4; ++j) {
+      const int n = rev ? 32 * (j - warp - 1) + 31 - lane : 32 * (warp - j - 1) + lane + 1;
+      lead[j] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
     }
+    const float* diagonal = power + 31 + lane;
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
-      ok = bar_wait(&sc_full[i & 1], (i >> 1) & 1, &failed);
-      if (ok && i > 0) ok = bar_wait(&o_full, (i - 1) & 1, &failed);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, bar_wait(&sc_full[i & 1], (i >> 1) & 1, &failed));
       if (!ok) break;
       tc_after();
       const uint32_t sc = tmem + lanes + kSc + (i & 1) * 128;
       float scale = 1.0f;
       if (kHalf) {
-        float most = 0.0f, f = lead;
-        for (int j = warp; j >= 0; --j) {
-          float x[32];
+        float most = 0.0f;
+#pragma unroll 1
+        for (int j = rev ? warp : 0; j <= (rev ? 3 : warp); ++j) {
+          const float f = j == 0 ? lead[0] : (j == 1 ? lead[1] : (j == 2 ? lead[2] : lead[3]));
+          float x[32], block = 0.0f;
           tmem_ld32(sc + j * 32, x);
           tmem_ld_wait(x);
           if (j == warp) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c <= lane) most = fmaxf(most, fabsf(x[c] * power[31 + lane - c]));
+            for (int c = 0; c < 32; ++c) {
+              const float p = diagonal[-c];
+              if (p != 0.0f) most = fmaxf(most, fabsf(x[c] * p));
+            }
           } else {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) most = fmaxf(most, fabsf(x[c] * (f * tab[c])));
-            f *= block;
+            for (int c = 0; c < 32; ++c) block = fmaxf(block, fabsf(x[c] * tab[c]));
+            most = fmaxf(most, block * fabsf(f));
           }
         }
         float inv;
         scale = scale_of(most, &inv);
         p_inv[i & 1][warp * 32 + lane] = inv;
       }
-      float f = lead * scale;
-      for (int j = warp; j >= 0; --j) {
-        float x[32];
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
         uint32_t u[16];
-        tmem_ld32(sc + j * 32, x);
-        tmem_ld_wait(x);
-        if (j == warp) {
+        if (rev ? j < warp : j > warp) {  // all masked
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float p = x[c] * power[31 + lane - c];
-            x[c] = c <= lane ? (kHalf ? p * scale : p) : 0.0f;
-          }
+          for (int c = 0; c < 16; ++c) u[c] = 0;
         } else {
+          float x[32];
+          tmem_ld32(sc + j * 32, x);
+          tmem_ld_wait(x);
+          if (j == warp) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] *= f * tab[c];
-          f *= block;
+            for (int c = 0; c < 32; ++c) {
+              const float p = diagonal[-c];
+              x[c] = p != 0.0f ? (kHalf ? x[c] * p * scale : x[c] * p) : 0.0f;
+            }
+          } else {
+            const float f =
+                (j == 0 ? lead[0] : (j == 1 ? lead[1] : (j == 2 ? lead[2] : lead[3]))) * scale;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              mul2(x[c], x[c + 1], tab[c], tab[c + 1]);
+              mul2(x[c], x[c + 1], f, f);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) u[c] = pack<T>(x[2 * c], x[2 * c + 1]);
         }
-#pragma unroll
-        for (int c = 0; c < 16; ++c) u[c] = pack<T>(x[2 * c], x[2 * c + 1]);
-        tmem_st16(tmem + lanes + kP + j * 16, u);
+        tmem_st16(sc + j * 16, u);
       }
       tmem_st_wait();
       tc_before();
-      bar_arrive(&sc_empty[i & 1]);
       bar_arrive(&p_full);
     }
   } else if (warp < 8) {
-    // ---- o = inter d^{t+off} Oe + Oi, through shared memory into whole 128-byte rows
-    const int t = (warp - 4) * 32 + lane;
-    const float read = float(job.inter) * decay_pow(w.a, float(t + job.off));
-    unsigned char* stage = sm + Z::out + (warp - 4) * 4096;
-    const size_t head = size_t(int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0);
+    // ---- o = inter d^{l+off} Oe + Oi, a row of 64 columns a thread, 16 at a time
+    const int t = (warp - 4) * 32 + lane, l = job.reverse ? C - 1 - t : t;
+    const float read = float(job.inter) * decay_pow(w.a, float(l + job.off));
+    const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
       ok = __all_sync(0xffffffffu, bar_wait(&o_full, i & 1, &failed));
       if (!ok) break;
       tc_after();
       const int64_t l0 = w.begin + int64_t(i) * C;
-      const int m = static_cast<int>(imin(C, w.end - l0));
+      const bool in = l0 + l < w.end;
+      const int64_t token = (job.reverse ? w.n - C - l0 : l0) + t;
+      const int64_t at = head + token * job.os[1];
       const float fe = kHalf ? read * s_inv[i & 1] : read;
       const float fi = kHalf ? p_inv[i & 1][t] : 1.0f;
-      const int64_t first = job.reverse ? w.n - 1 - l0 : l0;  // token of row 0
-      const int64_t step = job.reverse ? -job.os[1] : job.os[1];
-      const int row0 = (warp - 4) * 32, rows = m - row0;  // rows of this warp
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float e[32], x[32];
-        tmem_ld32(tmem + lanes + kOe + half * 32, e);
-        tmem_ld32(tmem + lanes + kOi + half * 32, x);
+#pragma unroll 2
+      for (int c0 = 0; c0 < NV; c0 += 16) {
+        float e[16], x[16];
+        tmem_ld16(tmem + lanes + kOe + c0, e);
+        tmem_ld16(tmem + lanes + kOi + c0, x);
         tmem_ld_wait(e);
         tmem_ld_wait(x);
-        if (half == 1) {
-          tc_before();
-          bar_arrive(&o_empty);
-        }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = kHalf ? fe * e[c] + fi * x[c] : fe * e[c] + x[c];
-        if (!job.o_wide) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float* y = x + g * 8;
-            *reinterpret_cast<uint4*>(stage + lane * 128 + (((half * 4 + g) ^ (lane & 7)) << 4)) =
-                make_uint4(pack<T>(y[0], y[1]), pack<T>(y[2], y[3]), pack<T>(y[4], y[5]),
-                           pack<T>(y[6], y[7]));
-          }
-        } else {  // 32-bit results (added over heads later), 32 columns at a time
-          float* o = static_cast<float*>(job.o) + head + first * job.os[1];
-#pragma unroll
-          for (int g = 0; g < 8; ++g)
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((g ^ (lane & 7)) << 4)) =
-                make_float4(x[g * 4], x[g * 4 + 1], x[g * 4 + 2], x[g * 4 + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = j * 4 + lane / 8, g = lane % 8, c = half * 32 + g * 4;
-            if (r < rows && c < w.vcols)
-              *reinterpret_cast<float4*>(o + (row0 + r) * step + c) =
-                  *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-          }
-          __syncwarp();
+        for (int c = 0; c < 16; ++c) x[c] = kHalf ? fe * e[c] + fi * x[c] : fe * e[c] + x[c];
+        if (in) {
+          if (job.o_wide) store_wide(static_cast<float*>(job.o) + at + c0, x, w.vcols - c0);
+          else store_row(static_cast<T*>(job.o) + at + c0, x, w.vcols - c0, job.o_vec);
         }
       }
-      if (!job.o_wide) {
-        __syncwarp();
-        T* o = static_cast<T*>(job.o) + head + first * job.os[1];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = j * 4 + lane / 8, g = lane % 8;
-          if (r < rows && g * 8 < w.vcols) {
-            const uint4 u = *reinterpret_cast<const uint4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-            T* dst = o + (row0 + r) * step + g * 8;
-            if (job.o_vec) {
-              *reinterpret_cast<uint4*>(dst) = u;
-            } else {
-              const T* e = reinterpret_cast<const T*>(&u);
-              for (int c = 0; c < 8 && g * 8 + c < w.vcols; ++c) dst[c] = e[c];
-            }
-          }
-        }
-        __syncwarp();
-      }
+      tc_before();
+      bar_arrive(&o_empty);
     }
   } else if (warp < 12) {
     // ---- the state, a row of 64 columns a thread (DK = 64: 16 rows a warp, the lanes that a
@@ -599,7 +638,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
     bool ok = true;
     for (int i = 0; i <= chunks && ok; ++i) {
       if (i > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(&u_full, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&u_full[(i - 1) & 1], ((i - 1) >> 1) & 1, &failed));
         if (!ok) break;
         tc_after();
         const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i - 1) * C)));
@@ -607,7 +646,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
           float x[16];
-          tmem_ld16(tmem + lanes + kU + part * 16, x);
+          tmem_ld16(tmem + lanes + kU + ((i - 1) & 1) * 64 + part * 16, x);
           tmem_ld_wait(x);
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
@@ -616,7 +655,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
           }
         }
         tc_before();
-        bar_arrive(&u_empty);
+        bar_arrive(&u_empty[(i - 1) & 1]);
         if (i == chunks) break;
         ok = __all_sync(0xffffffffu, bar_wait(&o_full, (i - 1) & 1, &failed));
         if (!ok) break;
@@ -667,107 +706,134 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
         if (c < w.vcols) dst[c] = s[c / 32][c % 32];
     }
   } else if (warp < 16) {
-    // ---- loads, and V' + V''
+    // ---- V'
     const int tid = threadIdx.x - 384;
-    Loader<T, Z::panels> lq, lk;
-    Loader<T, 1> lv;
-    lq.init(job.q, job.qs, w.b, w.h / job.q_group, 0, job.dk, tid);
-    lk.init(job.k, job.ks, w.b, w.h / job.k_group, 0, job.dk, tid);
-    lv.init(job.v, job.vs, w.b, w.h / job.v_group, w.v0, w.vcols, tid);
-    auto load = [&](int i) {
-      const int64_t l0 = w.begin + int64_t(i) * C;
-      const int m = static_cast<int>(imin(C, w.end - l0));
-      const uint32_t at = base + (i % S) * Z::stage;
-      lq.load(at + Z::q, l0, w.n, job.reverse, m, tid);
-      lk.load(at + Z::k, l0, w.n, job.reverse, m, tid);
-      lv.load(at + Z::v, l0, w.n, job.reverse, m, tid);
-    };
     float weight[C / 16];
     int weight_m = 0;
-    for (int i = 0; i < S - 1; ++i) {
-      if (i < chunks) load(i);
-      cp_commit();
-    }
     for (int i = 0; i < chunks; ++i) {
-      cp_wait<S - 2>();
-      fence_async();
-      bar_arrive(&full[i % S]);
       const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
       if (m != weight_m) {
         weight_m = m;
 #pragma unroll
         for (int j = 0; j < C / 16; ++j) {
-          const int age = m - job.off - (tid / 8 + 16 * j);
+          const int r = tid / 8 + 16 * j;
+          const int age = m - job.off - (job.reverse ? C - 1 - r : r);
           weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
         }
       }
-      if (i > 0 && !bar_wait(&u_full, (i - 1) & 1, &failed)) break;
-      split_values<T>(sm + (i % S) * Z::stage + Z::v, sm + Z::high, sm + Z::low, weight, tid);
-      fence_async();
-      bar_arrive(&vp_full);
-      const int next = i + S - 1;
-      if (next < chunks) {
-        if (i > 0 && !bar_wait(&empty[next % S], (next / S - 1) & 1, &failed)) break;
-        load(next);
+      if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
+      unsigned char* stage = sm + (i % S) * Z::stage;
+      if (m < C && !job.reverse && w.n < call.length) {
+        // padding after the sequence's end: the products take zeros for its keys and values
+        // (scores with them are masked, whichever of the two they read).  A thread clears the
+        // values that it reads below.
+        for (int r = tid / 8; r < C; r += 16) {
+          if (r < m) continue;
+          const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
+#pragma unroll
+          for (int p = 0; p < Z::panels; ++p)
+            *reinterpret_cast<uint4*>(stage + Z::k + p * kPanel + at) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(stage + Z::v + at) = make_uint4(0, 0, 0, 0);
+        }
       }
-      cp_commit();
+      if (i > 0 && !bar_wait(&u_full[(i - 1) & 1], ((i - 1) >> 1) & 1, &failed)) break;
+      split_values<T, C>(stage + Z::v, sm + Z::parts, kPanel, weight, tid);
+      fence_async();
+      bar_arrive(&v_full);
     }
-    cp_wait<0>();
+  } else if (warp == 17) {
+    // ---- loads
+    const CUtensorMap* map = maps.map[w.ji];
+    const Source q(map, job.qs, w.h / job.q_group, w.b), k(map + 1, job.ks, w.h / job.k_group, w.b),
+        v(map + 2, job.vs, w.h / job.v_group, w.b);
+    const bool one = elect_one();
+    int issued = 0;
+    bool ok = true;
+    for (; issued < chunks && ok; ++issued) {
+      const int i = issued, st = i % S;
+      ok = __all_sync(0xffffffffu, i < S || bar_wait(&empty[st], (i / S - 1) & 1, &failed));
+      if (!ok) break;
+      if (one) {
+        const int64_t l0 = w.begin + int64_t(i) * C;
+        const int64_t token = job.reverse ? w.n - C - l0 : l0;
+        const uint32_t at = base + st * Z::stage;
+        bar_expect(&full[st], Z::stage);
+        k.template load<C>(at + Z::k, 0, Z::panels, token, &full[st]);
+        q.template load<C>(at + Z::q, 0, Z::panels, token, &full[st]);
+        v.template load<C>(at + Z::v, w.v0, 1, token, &full[st]);
+      }
+      __syncwarp();
+    }
+    if (!ok) {  // copies in flight land before the block ends
+      const long long start = clock64();
+      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
+        while (!bar_try(&full[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
+        }
+    }
   } else {
     // ---- all products, issued by one lane
     constexpr uint32_t id_sc = instr<T>(C, C, false, false);
     constexpr uint32_t id_o = instr<T>(C, NV, false, true);
+    // operands of stage 0, and of what has one buffer
+    const uint32_t oq = operand(base + Z::q, kPanel);
+    const uint32_t os = operand(base + Z::s, kPanel), op = operand(base + Z::parts, kPanel);
+    const bool one = elect_one();
     auto scores = [&](int i) {
-      if (lane == 0) {
+      const uint32_t q = oq + (i % S) * (Z::stage / 16), k = q + (Z::k - Z::q) / 16;
+      const uint32_t d = tmem + kSc + (i & 1) * 128;
+      if (one) {
         tc_after();
-        const uint32_t at = base + (i % S) * Z::stage;
+        mma_ss<false>(d, q, k, id_sc);
 #pragma unroll
-        for (int j = 0; j < DK / 16; ++j) {
-          const uint32_t off = j / 4 * kPanel + j % 4 * 32;
-          mma_ss(tmem + kSc + (i & 1) * 128, operand(at + Z::q + off, kPanel),
-                 operand(at + Z::k + off, kPanel), id_sc, j > 0);
-        }
+        for (int j = 1; j < DK / 16; ++j)
+          mma_ss<true>(d, q + j / 4 * (kPanel / 16) + j % 4 * 2, k + j / 4 * (kPanel / 16) + j % 4 * 2,
+                       id_sc);
         tc_commit(&sc_full[i & 1]);
       }
       __syncwarp();
     };
-    // true: chunk i's operands are there and its score buffer is free
-    auto ready = [&](int i) {
-      return bar_wait(&full[i % S], (i / S) & 1, &failed) &&
-             (i < 2 || bar_wait(&sc_empty[i & 1], ((i >> 1) - 1) & 1, &failed));
-    };
+    // the score buffer of chunk i is free once P V of chunk i - 2 has been issued before
+    auto ready = [&](int i) { return bar_wait(&full[i % S], (i / S) & 1, &failed); };
     bool ok = true;
     if (chunks > 0) {
       ok = __all_sync(0xffffffffu, ready(0));
       if (ok) scores(0);
     }
     for (int i = 0; i < chunks && ok; ++i) {
-      const uint32_t at = base + (i % S) * Z::stage;
-      ok = bar_wait(&vp_full, i & 1, &failed) &&
-           (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
+      const uint32_t q = oq + (i % S) * (Z::stage / 16);
+      const uint32_t k = q + (Z::k - Z::q) / 16, v = q + (Z::v - Z::q) / 16;
+      ok = bar_wait(&v_full, i & 1, &failed) &&
+           (i < 2 || bar_wait(&u_empty[i & 1], ((i >> 1) - 1) & 1, &failed));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (lane == 0) {
+      if (one) {
         tc_after();
-        issue_update<T, DK, false>(tmem + kU, at + Z::k, base + Z::low, false);
-        issue_update<T, DK, kHalf>(tmem + kU, at + Z::k, base + Z::high, true);
-        tc_commit(&u_full);
+        const uint32_t d = tmem + kU + (i & 1) * 64;
+        if (kHalf) {
+          issue_update<T, DK, C, true, false>(d, k, op + kPanel / 16);
+          issue_update<T, DK, C, false, true>(d, k, op);
+        } else {  // small parts first
+          issue_update<T, DK, C, true, false>(d, k, op + 2 * (kPanel / 16));
+          issue_update<T, DK, C, false, false>(d, k, op + kPanel / 16);
+          issue_update<T, DK, C, false, false>(d, k, op);
+        }
+        tc_commit(&u_full[i & 1]);
       }
       __syncwarp();
       ok = bar_wait(&s_full, i & 1, &failed) &&
            (i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (lane == 0) {
+      if (one) {
         tc_after();
+        mma_ss<false>(tmem + kOe, q, os, id_o);
 #pragma unroll
-        for (int j = 0; j < DK / 16; ++j)
-          mma_ss(tmem + kOe, operand(at + Z::q + j / 4 * kPanel + j % 4 * 32, kPanel),
-                 operand(base + Z::s + j * 2048, kPanel), id_o, j > 0);
+        for (int j = 1; j < DK / 16; ++j)
+          mma_ss<true>(tmem + kOe, q + j / 4 * (kPanel / 16) + j % 4 * 2, os + j * 128, id_o);
       }
       __syncwarp();
       // the next chunk's scores go before this one's P V where their operands are there already
-      bool ahead = i + 1 < chunks && bar_try(&full[(i + 1) % S], ((i + 1) / S) & 1);
+      bool ahead = i + 1 < chunks && bar_test(&full[(i + 1) % S], ((i + 1) / S) & 1);
       ahead = __all_sync(0xffffffffu, ahead);
       if (ahead) {
         ok = __all_sync(0xffffffffu, ready(i + 1));
@@ -776,11 +842,12 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
       }
       ok = __all_sync(0xffffffffu, bar_wait(&p_full, i & 1, &failed));
       if (!ok) break;
-      if (lane == 0) {
+      if (one) {
         tc_after();
+        const uint32_t p = tmem + kSc + (i & 1) * 128;
+        mma_ts<false>(tmem + kOi, p, v, id_o);
 #pragma unroll
-        for (int j = 0; j < C / 16; ++j)
-          mma_ts(tmem + kOi, tmem + kP + j * 8, operand(at + Z::v + j * 2048, kPanel), id_o, j > 0);
+        for (int j = 1; j < C / 16; ++j) mma_ts<true>(tmem + kOi, p + j * 8, v + j * 128, id_o);
         tc_commit(&o_full);
         tc_commit(&empty[i % S]);
       }
@@ -791,7 +858,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
       }
     }
     if (!ok) {  // let the products in flight end before TMEM goes
-      if (lane == 0) tc_commit(&drain);
+      if (one) tc_commit(&drain);
       __syncwarp();
       const long long start = clock64();
       while (!bar_try(&drain, 0) && clock64() - start < kWaitCycles) {
@@ -819,27 +886,33 @@ linattn_tc_kernel(const __grid_constant__ Call call, int* error) {
 }
 
 // ------------------------------------------------------------------------------ state launch
-// A segment's own end state: U += K^T (V' + V''), V' + V'' = diag(d^{end-off-l}) V weighted
-// towards the segment's end, so that the sum stays in TMEM over all chunks.
-constexpr int kStateThreads = 288;  // loads, result, products: 4 + 4 + 1 warps
+// A segment's own end state: U += K^T V' with V' = diag(d^{end-off-l}) V weighted towards the
+// segment's end, so that the sums stay in TMEM over all tokens (the second part's apart in fp16).
+constexpr int kStateThreads = 320;  // V', result, products, loads: 4 + 4 + 1 + 1 warps
 
 template <typename T, int DK>
 __global__ void __launch_bounds__(kStateThreads, 1)
-linattn_tc_state_kernel(const __grid_constant__ Call call, int* error) {
-  using Z = Smem<DK>;
+linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant__ Maps maps,
+                        int* error) {
+  using Z = Smem<T, DK>;
+  constexpr bool kHalf = kIsHalf<T>;
+  constexpr int R = kStateRows;
   constexpr int S = Z::st_stages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = align_smem(raw);
-  __shared__ uint64_t vp_full[2], used[S], done;
+  __shared__ uint64_t full[S], v_full[2], used[S], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   const Where w = locate(call);
   const Job& job = *w.job;
   if (w.seg >= w.last) return;  // the whole block
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) bar_init(&vp_full[i], 128);
-    for (int i = 0; i < S; ++i) bar_init(&used[i], 1);
+    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 128);
+    for (int i = 0; i < S; ++i) {
+      bar_init(&full[i], 1);
+      bar_init(&used[i], 1);
+    }
     bar_init(&done, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -850,48 +923,28 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, int* error) {
   tc_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t base = smem_addr(sm);
-  const int chunks = w.chunks;  // whole ones: every segment before the last is full
+  const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
 
   if (warp < 4) {
     const int tid = threadIdx.x;
-    Loader<T, Z::panels> lk;
-    Loader<T, 1> lv;
-    lk.init(job.k, job.ks, w.b, w.h / job.k_group, 0, job.dk, tid);
-    lv.init(job.v, job.vs, w.b, w.h / job.v_group, w.v0, w.vcols, tid);
-    auto load = [&](int i) {
-      const int64_t l0 = w.begin + int64_t(i) * C;
-      const uint32_t at = base + (i % S) * Z::st_stage;
-      lk.load(at, l0, w.n, job.reverse, C, tid);
-      lv.load(at + Z::panels * kPanel, l0, w.n, job.reverse, C, tid);
-    };
-    for (int i = 0; i < S - 1; ++i) {
-      if (i < chunks) load(i);
-      cp_commit();
-    }
     for (int i = 0; i < chunks; ++i) {
-      cp_wait<S - 2>();
-      float weight[C / 16];
-      const int64_t ages = w.end - job.off - (w.begin + int64_t(i) * C + tid / 8);
+      float weight[R / 16];
 #pragma unroll
-      for (int j = 0; j < C / 16; ++j) {
-        const int64_t age = ages - 16 * j;
+      for (int j = 0; j < R / 16; ++j) {
+        const int r = tid / 8 + 16 * j;
+        const int64_t age =
+            w.end - job.off - (w.begin + int64_t(i) * R + (job.reverse ? R - 1 - r : r));
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
       }
-      // buffer i % 2 of V' + V'' is free when the products of chunk i - 2 have ended
+      if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
+      // buffer i % 2 of V' is free when the products of chunk i - 2 have ended
       if (i >= 2 && !bar_wait(&used[(i - 2) % S], ((i - 2) / S) & 1, &failed)) break;
-      unsigned char* high = sm + Z::st_high + (i & 1) * 2 * kPanel;
-      split_values<T>(sm + (i % S) * Z::st_stage + Z::panels * kPanel, high, high + kPanel, weight,
-                      tid);
+      split_values<T, R>(sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
+                         sm + Z::st_parts + (i & 1) * kParts<T> * kStatePanel, kStatePanel, weight,
+                         tid);
       fence_async();
-      bar_arrive(&vp_full[i & 1]);
-      const int next = i + S - 1;
-      if (next < chunks) {
-        if (i > 0 && !bar_wait(&used[(i - 1) % S], ((i - 1) / S) & 1, &failed)) break;
-        load(next);
-      }
-      cp_commit();
+      bar_arrive(&v_full[i & 1]);
     }
-    cp_wait<0>();
   } else if (warp < 8) {
     const bool ok = __all_sync(0xffffffffu, bar_wait(&done, 0, &failed));
     if (ok) {
@@ -904,36 +957,78 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, int* error) {
       const float write = float(job.write);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float x[32], y[32];
+        float x[32];
         const uint32_t at = tmem + (uint32_t(warp % 4 * 32) << 16) + half * 32;
         tmem_ld32(at, x);
-        tmem_ld32(at + NV, y);
         tmem_ld_wait(x);
-        tmem_ld_wait(y);
+        if (kIsHalf<T>) {
+          float y[32];
+          tmem_ld32(at + NV, y);
+          tmem_ld_wait(y);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] += y[c] * (1.0f / kLowScale);
+        }
         if (mine) {
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (half * 32 + c < w.vcols) dst[half * 32 + c] = write * (x[c] + y[c] / kLowScale<T>);
+            if (half * 32 + c < w.vcols) dst[half * 32 + c] = write * x[c];
         }
       }
     }
+  } else if (warp == 9) {
+    const CUtensorMap* map = maps.map[w.ji];
+    const Source k(map + 1, job.ks, w.h / job.k_group, w.b),
+        v(map + 2, job.vs, w.h / job.v_group, w.b);
+    const bool one = elect_one();
+    int issued = 0;
+    bool ok = true;
+    for (; issued < chunks && ok; ++issued) {
+      const int i = issued, st = i % S;
+      ok = __all_sync(0xffffffffu, i < S || bar_wait(&used[st], (i / S - 1) & 1, &failed));
+      if (!ok) break;
+      if (one) {
+        const int64_t l0 = w.begin + int64_t(i) * R;
+        const int64_t token = job.reverse ? w.n - R - l0 : l0;
+        const uint32_t at = base + st * Z::st_stage;
+        bar_expect(&full[st], Z::st_stage);
+        k.template load<R>(at, 0, Z::panels, token, &full[st]);
+        v.template load<R>(at + Z::panels * kStatePanel, w.v0, 1, token, &full[st]);
+      }
+      __syncwarp();
+    }
+    if (!ok) {  // copies in flight land before the block ends
+      const long long start = clock64();
+      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
+        while (!bar_try(&full[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
+        }
+    }
   } else {
+    const uint32_t ok0 = operand(base, kStatePanel), op0 = operand(base + Z::st_parts, kStatePanel);
+    const bool one = elect_one();
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
-      ok = __all_sync(0xffffffffu, bar_wait(&vp_full[i & 1], (i >> 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&v_full[i & 1], (i >> 1) & 1, &failed));
       if (!ok) break;
-      if (lane == 0) {
+      const uint32_t k = ok0 + (i % S) * (Z::st_stage / 16);
+      const uint32_t parts = op0 + (i & 1) * (kParts<T> * kStatePanel / 16);
+      if (one) {
         tc_after();
-        const uint32_t high = base + Z::st_high + (i & 1) * 2 * kPanel;
-        const uint32_t k = base + (i % S) * Z::st_stage;
-        issue_update<T, DK, false>(tmem, k, high, i > 0);
-        issue_update<T, DK, false>(tmem + NV, k, high + kPanel, i > 0);
+        if (i == 0) issue_update<T, DK, R, true, false>(tmem, k, parts);
+        else issue_update<T, DK, R, false, false>(tmem, k, parts);
+        if (kHalf) {
+          if (i == 0) issue_update<T, DK, R, true, false>(tmem + NV, k, parts + kStatePanel / 16);
+          else issue_update<T, DK, R, false, false>(tmem + NV, k, parts + kStatePanel / 16);
+        } else {
+#pragma unroll
+          for (int p = 1; p < kParts<T>; ++p)
+            issue_update<T, DK, R, false, false>(tmem, k, parts + p * (kStatePanel / 16));
+        }
         tc_commit(&used[i % S]);
       }
       __syncwarp();
     }
     // also after a failed wait: the products in flight end before TMEM goes
-    if (lane == 0) tc_commit(&done);
+    if (one) tc_commit(&done);
     __syncwarp();
     const long long start = clock64();
     while (!bar_try(&done, 0) && clock64() - start < kWaitCycles) {
@@ -948,8 +1043,50 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, int* error) {
   }
 }
 
+// ------------------------------------------------------------------------------ launches
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                            CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                            CUtensorMapFloatOOBfill);
+Encode encoder() {
+  static const Encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return fn;
+}
+
+int encode(Encode fn, int dtype, CUtensorMap* map, const void* p, const int64_t* stride, int dim,
+           int64_t length, int64_t heads, int64_t batch) {
+  // an axis of one element, or broadcast with stride 0, is one coordinate
+  const int64_t some = (dim + 7) / 8 * 16;
+  const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(stride[1] == 0 ? 1 : length),
+                              cuuint64_t(stride[2] == 0 ? 1 : heads),
+                              cuuint64_t(stride[0] == 0 ? 1 : batch)};
+  const cuuint64_t strides[3] = {cuuint64_t(stride[1] == 0 ? some : stride[1] * 2),
+                                 cuuint64_t(stride[2] == 0 ? some : stride[2] * 2),
+                                 cuuint64_t(stride[0] == 0 ? some : stride[0] * 2)};
+  const cuuint32_t box[4] = {64, kBoxRows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type =
+      dtype == FDWT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int tries = 0; tries < 2; ++tries) {
+    if (fn(map, type, 4, const_cast<void*>(p), dims, strides, box, one,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+      return FDWT_OK;
+    // a thread's first CUDA call (autograd's) finds no current context: bind the device's
+    if (tries == 0) FDWT_CUDA(cudaFree(nullptr));
+  }
+  return FDWT_ERR_UNSUPPORTED;
+}
+
 template <typename T, int DK>
-int launch_as(const Call& call, bool states, cudaStream_t stream) {
+int launch_as(const Call& call, const Maps& maps, bool states, cudaStream_t stream) {
   auto kernel = states ? linattn_tc_state_kernel<T, DK> : linattn_tc_kernel<T, DK>;
   const int64_t heads = call.batch * call.heads;
   const int64_t grid = heads * call.tiles * (states ? call.nseg - 1 : call.nseg);
@@ -959,7 +1096,7 @@ int launch_as(const Call& call, bool states, cudaStream_t stream) {
   if (st == FDWT_OK) st = pre_launch(stream);
   if (st != FDWT_OK) return st;
   kernel<<<static_cast<unsigned>(grid), states ? kStateThreads : kThreads,
-           states ? Smem<DK>::st_bytes : Smem<DK>::bytes, stream>>>(call, error);
+           states ? Smem<T, DK>::st_bytes : Smem<T, DK>::bytes, stream>>>(call, maps, error);
   return launch_status();
 }
 
@@ -967,21 +1104,41 @@ int launch_as(const Call& call, bool states, cudaStream_t stream) {
 
 bool tc_supports(int dtype, const Call& call) {
   if (dtype != FDWT_F16 && dtype != FDWT_BF16) return false;
+  if (call.length > INT32_MAX - 2 * C || call.batch > INT32_MAX || encoder() == nullptr) return false;
   for (int j = 0; j < call.jobs; ++j) {
     const Job& job = call.job[j];
     if (job.dk > 128 || !job.q_vec || !job.k_vec || !job.v_vec) return false;
+    // tensor maps: no broadcast tokens, no negative strides, strides below 2^40 bytes
+    for (const int64_t* s : {job.qs, job.ks, job.vs}) {
+      if (call.length > 1 && s[1] == 0) return false;
+      for (int i = 0; i < 3; ++i)
+        if (s[i] < 0 || s[i] >= int64_t(1) << 39) return false;
+    }
   }
   return true;
 }
 
 int tc_launch(int dtype, const Call& call, bool states, cudaStream_t stream) {
+  const Encode fn = encoder();
+  Maps maps;
   int dk = 0;
-  for (int j = 0; j < call.jobs; ++j) dk = call.job[j].dk > dk ? call.job[j].dk : dk;
+  for (int j = 0; j < call.jobs; ++j) {
+    const Job& job = call.job[j];
+    dk = job.dk > dk ? job.dk : dk;
+    const void* p[3] = {job.q, job.k, job.v};
+    const int64_t* stride[3] = {job.qs, job.ks, job.vs};
+    const int group[3] = {job.q_group, job.k_group, job.v_group};
+    for (int i = states ? 1 : 0; i < 3; ++i) {
+      const int st = encode(fn, dtype, &maps.map[j][i], p[i], stride[i], i == 2 ? job.dv : job.dk,
+                            call.length, call.heads / group[i], call.batch);
+      if (st != FDWT_OK) return st;
+    }
+  }
   if (dtype == FDWT_F16)
-    return dk <= 64 ? launch_as<__half, 64>(call, states, stream)
-                    : launch_as<__half, 128>(call, states, stream);
-  return dk <= 64 ? launch_as<__nv_bfloat16, 64>(call, states, stream)
-                  : launch_as<__nv_bfloat16, 128>(call, states, stream);
+    return dk <= 64 ? launch_as<__half, 64>(call, maps, states, stream)
+                    : launch_as<__half, 128>(call, maps, states, stream);
+  return dk <= 64 ? launch_as<__nv_bfloat16, 64>(call, maps, states, stream)
+                  : launch_as<__nv_bfloat16, 128>(call, maps, states, stream);
 }
 
 }  // namespace linattn
