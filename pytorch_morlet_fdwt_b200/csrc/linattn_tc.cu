@@ -4,10 +4,10 @@
 // One block per SM runs one head's segment, 64 value columns of it, in chunks of 128 tokens:
 //
 //   Sc = Q K^T            (128 x 128)    shared x shared   -> TMEM, two buffers
-//   P  = Sc * M           rounded to 16 bits, over Sc's columns in TMEM
-//   Oi = P V              (128 x 64)     TMEM x shared     -> TMEM
+//   P  = Sc * M           rounded to 16 bits, over the first half of Sc's columns
+//   Oi = P V              (128 x 64)     TMEM x shared     -> TMEM, the second half of them
 //   Oe = Q S              (128 x 64)     shared x shared   -> TMEM, S the 16-bit copy of the state
-//   U  = K^T V'           (DK x 64)      shared x shared   -> TMEM, two buffers
+//   U  = K^T V'           (DK x 64 each part)  shared x shared -> TMEM
 //   o  = diag(d^{l+off}) inter Oe + Oi,  S <- d^m S + write U   in registers, 32 bits
 //
 // V' is diag(d^{m-off-l}) V in two 16-bit parts (fp16) or three (bf16): one part would leave the
@@ -20,8 +20,9 @@
 // Bound: 2 (2 Dk + 2 Dv) bytes of HBM a token and head against about 4 (Dk Dv + 128 (Dk + Dv))
 // operations, 96 a byte at 128 x 128, under half of the tensor rate at the HBM rate.  What costs
 // is the chain of dependent steps in a chunk, so every step has its own warps and the chunks
-// overlap: one warp issues the loads (TMA), four form V', one issues all products, four form P,
-// four keep the state, four finish o.  Every wait on a barrier has a time limit.
+// overlap: one warp issues the loads (TMA), one all products, four form P, eight form V' and
+// finish o, four keep the state.  All parts of V' are one product (N = 64 parts), so that K is read
+// once: the shared-memory rate binds the products more than the tensor rate.  Every wait on a barrier has a time limit.
 #include <cuda.h>
 
 #include <type_traits>
@@ -111,16 +112,6 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint3
       "r"(a), "r"(b), "r"(idesc), "n"(kOperandHigh), "n"(ADD ? 1 : 0)
       : "memory");
 }
-// D = A B + 2^-11 D
-__device__ __forceinline__ void mma_ss_shift11(uint32_t d, uint32_t a, uint32_t b,
-                                               uint32_t idesc) {
-  asm volatile(
-      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, 1, 0;\n"
-      " mov.b64 x, {%1, %4};\n mov.b64 y, {%2, %4};\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p, 11;\n}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "n"(kOperandHigh)
-      : "memory");
-}
 template <bool ADD>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
@@ -173,6 +164,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&r)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float (&r)[8]) {
+  uint32_t u[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
+                 "=r"(u[6]), "=r"(u[7])
+               : "r"(addr)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = __uint_as_float(u[i]);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -196,6 +197,25 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(map), "r"(x), "r"(token), "r"(head), "r"(batch), "r"(smem_addr(bar))
       : "memory");
+}
+// (a, b) -= (c, d);  (a, b) += (c, d);  (a, b) = (a, b) * f + (c, d)
+__device__ __forceinline__ void sub2(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
+      " sub.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void fma2(float& a, float& b, float f, float c, float d) {
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
+      " mov.b64 z, {%4, %4};\n fma.rn.f32x2 x, x, z, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d), "f"(f));
 }
 // (a, b) * (c, d)
 __device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {
@@ -322,34 +342,30 @@ template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
 template <typename T> constexpr int kParts = kIsHalf<T> ? 2 : 3;
 constexpr float kLowScale = 2048.0f;
 
-// V' = diag(weight) V in parts, `lead` bytes apart; thread tid takes the 16-byte column group
-// tid % 8 of the rows tid / 8 + 16 j.
+// V' = diag(weight) V in parts, `lead` bytes apart; thread tid of 256 takes the 16-byte column
+// group tid % 8 of the rows tid / 8 + 32 j.
 template <typename T, int ROWS>
 __device__ __forceinline__ void split_values(const unsigned char* v, unsigned char* parts, int lead,
-                                             const float (&weight)[ROWS / 16], int tid) {
+                                             const float (&weight)[ROWS / 32], int tid) {
   const int r0 = tid / 8;
   const int cell = r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
-#pragma unroll 2
-  for (int j = 0; j < ROWS / 16; ++j) {
-    const int at = cell + j * 16 * 128;
+#pragma unroll
+  for (int j = 0; j < ROWS / 32; ++j) {
+    const int at = cell + j * 32 * 128;
     const uint4 x = *reinterpret_cast<const uint4*>(v + at);
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
     uint32_t out[kParts<T>][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 f = unpack<T>(in[i]);
-      f.x *= weight[j];
-      f.y *= weight[j];
+      mul2(f.x, f.y, weight[j], weight[j]);
 #pragma unroll
       for (int p = 0; p < kParts<T>; ++p) {
         out[p][i] = pack<T>(f.x, f.y);
+        if (p + 1 == kParts<T>) break;
         const float2 g = unpack<T>(out[p][i]);
-        f.x -= g.x;
-        f.y -= g.y;
-        if (kIsHalf<T>) {
-          f.x *= kLowScale;
-          f.y *= kLowScale;
-        }
+        sub2(f.x, f.y, g.x, g.y);
+        if (kIsHalf<T>) mul2(f.x, f.y, kLowScale, kLowScale);
       }
     }
 #pragma unroll
@@ -359,21 +375,39 @@ __device__ __forceinline__ void split_values(const unsigned char* v, unsigned ch
   }
 }
 
-// D (+)= K^T B over ROWS tokens (FIRST: the first product does not add; SHIFT: D counts 2^-11 in
-// it): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
-template <typename T, int DK, int ROWS, bool FIRST, bool SHIFT>
+// D (+)= K^T V' over ROWS tokens, all parts at once, 64 columns each (FIRST: the first product
+// does not add): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
+template <typename T, int DK, int ROWS, bool FIRST>
 __device__ __forceinline__ void issue_update(uint32_t d, uint32_t k, uint32_t b) {
-  constexpr uint32_t id = instr<T>(DK, NV, true, true);
-  if (SHIFT) mma_ss_shift11(d, k, b, id);
-  else mma_ss<!FIRST>(d, k, b, id);
+  constexpr uint32_t id = instr<T>(DK, NV * kParts<T>, true, true);
+  mma_ss<!FIRST>(d, k, b, id);
 #pragma unroll
   for (int i = 1; i < ROWS / 16; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
 }
+// 8 columns of U from the parts' sums.
+template <typename T> __device__ __forceinline__ void load_update(uint32_t addr, float (&x)[8]) {
+  float y[8], z[8];
+  tmem_ld8(addr, x);
+  tmem_ld8(addr + NV, y);
+  if (!kIsHalf<T>) tmem_ld8(addr + 2 * NV, z);
+  tmem_ld_wait(x);
+  tmem_ld_wait(y);
+#pragma unroll
+  for (int c = 0; c < 8; c += 2) {
+    if (kIsHalf<T>) {
+      mul2(y[c], y[c + 1], 1.0f / kLowScale, 1.0f / kLowScale);
+    } else {
+      if (c == 0) tmem_ld_wait(z);
+      add2(y[c], y[c + 1], z[c], z[c + 1]);
+    }
+    add2(x[c], x[c + 1], y[c], y[c + 1]);
+  }
+}
 
-constexpr int kThreads = 576;  // 4 warps each: P, o, state, V'; one for the products, one loads
+constexpr int kThreads = 576;  // P: 4 warps, V' and o: 8, state: 4, products: 1, loads: 1
 constexpr uint32_t kColumns = 512;
-// TMEM columns; P lies over its Sc
-constexpr uint32_t kSc = 0, kOe = 256, kOi = 320, kU = 384;
+// TMEM columns: two buffers of Sc (P over its first 64 columns, Oi over the others), Oe, U
+constexpr uint32_t kSc = 0, kOi = 64, kOe = 256, kU = 320;
 // The state launch takes 64 tokens at a time: more stages, two buffers of V'.
 constexpr int kStateRows = 64, kStatePanel = kStateRows * 128;
 
@@ -451,8 +485,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   constexpr int S = Z::stages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = align_smem(raw);
-  __shared__ uint64_t full[S], empty[S], sc_full[2], p_full, o_full, o_empty, s_full, u_full[2],
-      u_empty[2], v_full, most_full, drain;
+  __shared__ uint64_t full[S], empty[S], sc_full[2], p_full, o_full, o_empty, s_full, u_full,
+      u_empty, v_full, most_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float power[64];          // at 31 + t - s: intra d^|t-s|, 0 for a masked pair
@@ -470,14 +504,14 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sc_full[i], 1);
-      bar_init(&u_full[i], 1);
-      bar_init(&u_empty[i], 128);
     }
     bar_init(&p_full, 128);
     bar_init(&o_full, 1);
-    bar_init(&o_empty, 128);
+    bar_init(&o_empty, 256);
     bar_init(&s_full, 128);
-    bar_init(&v_full, 128);
+    bar_init(&u_full, 1);
+    bar_init(&u_empty, 128);
+    bar_init(&v_full, 256);
     bar_init(&most_full, 4);
     bar_init(&drain, 1);
     failed = 0;
@@ -577,43 +611,85 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       tc_before();
       bar_arrive(&p_full);
     }
-  } else if (warp < 8) {
-    // ---- o = inter d^{l+off} Oe + Oi, a row of 64 columns a thread, 16 at a time
-    const int t = (warp - 4) * 32 + lane, l = job.reverse ? C - 1 - t : t;
+  } else if (warp < 12) {
+    // ---- V' of a chunk, then o = inter d^{l+off} Oe + Oi of the chunk before: half a row of 64
+    // columns a thread
+    const int tid = threadIdx.x - 128;
+    const int t = warp % 4 * 32 + lane, l = job.reverse ? C - 1 - t : t;
+    const int c_half = (warp - 4) / 4 * 32;
     const float read = float(job.inter) * decay_pow(w.a, float(l + job.off));
     const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
-    bool ok = true;
-    for (int i = 0; i < chunks && ok; ++i) {
-      ok = __all_sync(0xffffffffu, bar_wait(&o_full, i & 1, &failed));
-      if (!ok) break;
+    float weight[C / 32];
+    int weight_m = 0;
+    for (int i = 0; i <= chunks; ++i) {
+      if (i < chunks) {
+        const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
+        if (m != weight_m) {
+          weight_m = m;
+#pragma unroll
+          for (int j = 0; j < C / 32; ++j) {
+            const int r = tid / 8 + 32 * j;
+            const int age = m - job.off - (job.reverse ? C - 1 - r : r);
+            weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
+          }
+        }
+        bool ok = bar_wait(&full[i % S], (i / S) & 1, &failed);
+        unsigned char* stage = sm + (i % S) * Z::stage;
+        if (ok && m < C && !job.reverse && w.n < call.length) {
+          // padding after the sequence's end: the products take zeros for its keys and values
+          // (scores with them are masked, whichever of the two they read).  A thread clears the
+          // values that it reads below.
+          for (int r = tid / 8; r < C; r += 32) {
+            if (r < m) continue;
+            const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
+#pragma unroll
+            for (int p = 0; p < Z::panels; ++p)
+              *reinterpret_cast<uint4*>(stage + Z::k + p * kPanel + at) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(stage + Z::v + at) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        ok = ok && (i == 0 || bar_wait(&u_full, (i - 1) & 1, &failed));
+        if (!__all_sync(0xffffffffu, ok)) break;
+        split_values<T, C>(stage + Z::v, sm + Z::parts, kPanel, weight, tid);
+        fence_async();
+        bar_arrive(&v_full);
+      }
+      if (i == 0) continue;
+      const int e = i - 1;  // the chunk whose o is finished
+      if (!__all_sync(0xffffffffu, bar_wait(&o_full, e & 1, &failed))) break;
       tc_after();
-      const int64_t l0 = w.begin + int64_t(i) * C;
+      const int64_t l0 = w.begin + int64_t(e) * C;
       const bool in = l0 + l < w.end;
       const int64_t token = (job.reverse ? w.n - C - l0 : l0) + t;
       const int64_t at = head + token * job.os[1];
-      const float fe = kHalf ? read * s_inv[i & 1] : read;
-      const float fi = kHalf ? p_inv[i & 1][t] : 1.0f;
-#pragma unroll 2
-      for (int c0 = 0; c0 < NV; c0 += 16) {
-        float e[16], x[16];
-        tmem_ld16(tmem + lanes + kOe + c0, e);
-        tmem_ld16(tmem + lanes + kOi + c0, x);
-        tmem_ld_wait(e);
-        tmem_ld_wait(x);
+      const float fe = kHalf ? read * s_inv[e & 1] : read;
+      const float fi = kHalf ? p_inv[e & 1][t] : 1.0f;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) x[c] = kHalf ? fe * e[c] + fi * x[c] : fe * e[c] + x[c];
+      for (int c0 = c_half; c0 < c_half + 32; c0 += 16) {
+        float y[16], x[16];
+        tmem_ld16(tmem + lanes + kOe + c0, y);
+        tmem_ld16(tmem + lanes + kSc + (e & 1) * 128 + kOi + c0, x);
+        tmem_ld_wait(y);
+        tmem_ld_wait(x);
+        if (c0 > c_half) {
+          tc_before();
+          bar_arrive(&o_empty);
+        }
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          if (kHalf) mul2(x[c], x[c + 1], fi, fi);
+          fma2(y[c], y[c + 1], fe, x[c], x[c + 1]);
+        }
         if (in) {
-          if (job.o_wide) store_wide(static_cast<float*>(job.o) + at + c0, x, w.vcols - c0);
-          else store_row(static_cast<T*>(job.o) + at + c0, x, w.vcols - c0, job.o_vec);
+          if (job.o_wide) store_wide(static_cast<float*>(job.o) + at + c0, y, w.vcols - c0);
+          else store_row(static_cast<T*>(job.o) + at + c0, y, w.vcols - c0, job.o_vec);
         }
       }
-      tc_before();
-      bar_arrive(&o_empty);
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ---- the state, a row of 64 columns a thread (DK = 64: 16 rows a warp, the lanes that a
     // product with M = 64 fills)
-    const int r = DK == 128 ? (warp - 8) * 32 + lane : (warp - 8) * 16 + (lane & 15);
+    const int r = DK == 128 ? (warp - 12) * 32 + lane : (warp - 12) * 16 + (lane & 15);
     const bool mine = DK == 128 || lane < 16;
     const int64_t size = int64_t(job.dk) * job.dv;
     const float write = float(job.write);
@@ -638,24 +714,24 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     bool ok = true;
     for (int i = 0; i <= chunks && ok; ++i) {
       if (i > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(&u_full[(i - 1) & 1], ((i - 1) >> 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&u_full, (i - 1) & 1, &failed));
         if (!ok) break;
         tc_after();
         const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i - 1) * C)));
         const float keep = decay_pow(w.a, float(m));
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          float x[16];
-          tmem_ld16(tmem + lanes + kU + ((i - 1) & 1) * 64 + part * 16, x);
-          tmem_ld_wait(x);
+        for (int g = 0; g < 8; ++g) {
+          float x[8];
+          load_update<T>(tmem + lanes + kU + g * 8, x);
+          float* y = &s[g / 4][g % 4 * 8];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            float& y = s[part / 2][part % 2 * 16 + c];
-            y = keep * y + write * x[c];
+          for (int c = 0; c < 8; c += 2) {
+            mul2(x[c], x[c + 1], write, write);
+            fma2(y[c], y[c + 1], keep, x[c], x[c + 1]);
           }
         }
         tc_before();
-        bar_arrive(&u_empty[(i - 1) & 1]);
+        bar_arrive(&u_empty);
         if (i == chunks) break;
         ok = __all_sync(0xffffffffu, bar_wait(&o_full, (i - 1) & 1, &failed));
         if (!ok) break;
@@ -673,7 +749,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         // (rewritten only after o_full of this chunk, which follows every warp's s_full)
         if (lane == 0) {
-          s_most[warp - 8] = most;
+          s_most[warp - 12] = most;
           bar_arrive(&most_full);
         }
         ok = __all_sync(0xffffffffu, bar_wait(&most_full, i & 1, &failed));
@@ -681,7 +757,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
         float inv;
         scale = scale_of(most, &inv);
-        if (warp == 8 && lane == 0) s_inv[i & 1] = inv;
+        if (warp == 12 && lane == 0) s_inv[i & 1] = inv;
       }
       if (mine) {
         unsigned char* row = sm + Z::s + r * 128;
@@ -704,42 +780,6 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
       for (int c = 0; c < NV; ++c)
         if (c < w.vcols) dst[c] = s[c / 32][c % 32];
-    }
-  } else if (warp < 16) {
-    // ---- V'
-    const int tid = threadIdx.x - 384;
-    float weight[C / 16];
-    int weight_m = 0;
-    for (int i = 0; i < chunks; ++i) {
-      const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
-      if (m != weight_m) {
-        weight_m = m;
-#pragma unroll
-        for (int j = 0; j < C / 16; ++j) {
-          const int r = tid / 8 + 16 * j;
-          const int age = m - job.off - (job.reverse ? C - 1 - r : r);
-          weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
-        }
-      }
-      if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
-      unsigned char* stage = sm + (i % S) * Z::stage;
-      if (m < C && !job.reverse && w.n < call.length) {
-        // padding after the sequence's end: the products take zeros for its keys and values
-        // (scores with them are masked, whichever of the two they read).  A thread clears the
-        // values that it reads below.
-        for (int r = tid / 8; r < C; r += 16) {
-          if (r < m) continue;
-          const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
-#pragma unroll
-          for (int p = 0; p < Z::panels; ++p)
-            *reinterpret_cast<uint4*>(stage + Z::k + p * kPanel + at) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(stage + Z::v + at) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (i > 0 && !bar_wait(&u_full[(i - 1) & 1], ((i - 1) >> 1) & 1, &failed)) break;
-      split_values<T, C>(stage + Z::v, sm + Z::parts, kPanel, weight, tid);
-      fence_async();
-      bar_arrive(&v_full);
     }
   } else if (warp == 17) {
     // ---- loads
@@ -792,7 +832,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       }
       __syncwarp();
     };
-    // the score buffer of chunk i is free once P V of chunk i - 2 has been issued before
+    // (the score buffer is free: o of chunk i - 2, which ends in it, was waited for before)
     auto ready = [&](int i) { return bar_wait(&full[i % S], (i / S) & 1, &failed); };
     bool ok = true;
     if (chunks > 0) {
@@ -803,21 +843,13 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       const uint32_t q = oq + (i % S) * (Z::stage / 16);
       const uint32_t k = q + (Z::k - Z::q) / 16, v = q + (Z::v - Z::q) / 16;
       ok = bar_wait(&v_full, i & 1, &failed) &&
-           (i < 2 || bar_wait(&u_empty[i & 1], ((i >> 1) - 1) & 1, &failed));
+           (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (one) {
         tc_after();
-        const uint32_t d = tmem + kU + (i & 1) * 64;
-        if (kHalf) {
-          issue_update<T, DK, C, true, false>(d, k, op + kPanel / 16);
-          issue_update<T, DK, C, false, true>(d, k, op);
-        } else {  // small parts first
-          issue_update<T, DK, C, true, false>(d, k, op + 2 * (kPanel / 16));
-          issue_update<T, DK, C, false, false>(d, k, op + kPanel / 16);
-          issue_update<T, DK, C, false, false>(d, k, op);
-        }
-        tc_commit(&u_full[i & 1]);
+        issue_update<T, DK, C, true>(tmem + kU, k, op);
+        tc_commit(&u_full);
       }
       __syncwarp();
       ok = bar_wait(&s_full, i & 1, &failed) &&
@@ -845,9 +877,9 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       if (one) {
         tc_after();
         const uint32_t p = tmem + kSc + (i & 1) * 128;
-        mma_ts<false>(tmem + kOi, p, v, id_o);
+        mma_ts<false>(p + kOi, p, v, id_o);
 #pragma unroll
-        for (int j = 1; j < C / 16; ++j) mma_ts<true>(tmem + kOi, p + j * 8, v + j * 128, id_o);
+        for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
         tc_commit(&o_full);
         tc_commit(&empty[i % S]);
       }
@@ -887,15 +919,14 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 
 // ------------------------------------------------------------------------------ state launch
 // A segment's own end state: U += K^T V' with V' = diag(d^{end-off-l}) V weighted towards the
-// segment's end, so that the sums stay in TMEM over all tokens (the second part's apart in fp16).
-constexpr int kStateThreads = 320;  // V', result, products, loads: 4 + 4 + 1 + 1 warps
+// segment's end, so that the sums stay in TMEM over all tokens.
+constexpr int kStateThreads = 320;  // V' (and the result): 8 warps, products: 1, loads: 1
 
 template <typename T, int DK>
 __global__ void __launch_bounds__(kStateThreads, 1)
 linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant__ Maps maps,
                         int* error) {
   using Z = Smem<T, DK>;
-  constexpr bool kHalf = kIsHalf<T>;
   constexpr int R = kStateRows;
   constexpr int S = Z::st_stages;
   extern __shared__ unsigned char raw[];
@@ -908,7 +939,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   if (w.seg >= w.last) return;  // the whole block
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 128);
+    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 256);
     for (int i = 0; i < S; ++i) {
       bar_init(&full[i], 1);
       bar_init(&used[i], 1);
@@ -925,13 +956,13 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   const uint32_t base = smem_addr(sm);
   const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
 
-  if (warp < 4) {
+  if (warp < 8) {
     const int tid = threadIdx.x;
     for (int i = 0; i < chunks; ++i) {
-      float weight[R / 16];
+      float weight[R / 32];
 #pragma unroll
-      for (int j = 0; j < R / 16; ++j) {
-        const int r = tid / 8 + 16 * j;
+      for (int j = 0; j < R / 32; ++j) {
+        const int r = tid / 8 + 32 * j;
         const int64_t age =
             w.end - job.off - (w.begin + int64_t(i) * R + (job.reverse ? R - 1 - r : r));
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
@@ -945,33 +976,21 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       fence_async();
       bar_arrive(&v_full[i & 1]);
     }
-  } else if (warp < 8) {
-    const bool ok = __all_sync(0xffffffffu, bar_wait(&done, 0, &failed));
-    if (ok) {
+    if (warp < 4 && __all_sync(0xffffffffu, bar_wait(&done, 0, &failed)) && !failed) {
       tc_after();
-      const int r = DK == 128 ? (warp - 4) * 32 + lane : (warp - 4) * 16 + (lane & 15);
+      const int r = DK == 128 ? warp * 32 + lane : warp * 16 + (lane & 15);
       const bool mine = (DK == 128 || lane < 16) && r < job.dk;
       float* dst = static_cast<float*>(job.seg) +
                    (w.bh * (call.nseg - 1) + w.seg) * (int64_t(job.dk) * job.dv) +
                    int64_t(r) * job.dv + w.v0;
       const float write = float(job.write);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float x[32];
-        const uint32_t at = tmem + (uint32_t(warp % 4 * 32) << 16) + half * 32;
-        tmem_ld32(at, x);
-        tmem_ld_wait(x);
-        if (kIsHalf<T>) {
-          float y[32];
-          tmem_ld32(at + NV, y);
-          tmem_ld_wait(y);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] += y[c] * (1.0f / kLowScale);
-        }
+      for (int g = 0; g < NV; g += 8) {
+        float x[8];
+        load_update<T>(tmem + (uint32_t(warp * 32) << 16) + g, x);
         if (mine) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (half * 32 + c < w.vcols) dst[half * 32 + c] = write * x[c];
+          for (int c = 0; c < 8; ++c)
+            if (g + c < w.vcols) dst[g + c] = write * x[c];
         }
       }
     }
@@ -1013,16 +1032,8 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       const uint32_t parts = op0 + (i & 1) * (kParts<T> * kStatePanel / 16);
       if (one) {
         tc_after();
-        if (i == 0) issue_update<T, DK, R, true, false>(tmem, k, parts);
-        else issue_update<T, DK, R, false, false>(tmem, k, parts);
-        if (kHalf) {
-          if (i == 0) issue_update<T, DK, R, true, false>(tmem + NV, k, parts + kStatePanel / 16);
-          else issue_update<T, DK, R, false, false>(tmem + NV, k, parts + kStatePanel / 16);
-        } else {
-#pragma unroll
-          for (int p = 1; p < kParts<T>; ++p)
-            issue_update<T, DK, R, false, false>(tmem, k, parts + p * (kStatePanel / 16));
-        }
+        if (i == 0) issue_update<T, DK, R, true>(tmem, k, parts);
+        else issue_update<T, DK, R, false>(tmem, k, parts);
         tc_commit(&used[i % S]);
       }
       __syncwarp();
