@@ -404,7 +404,16 @@ template <typename T> __device__ __forceinline__ void load_update(uint32_t addr,
   }
 }
 
-constexpr int kThreads = 576;  // P: 4 warps, V' and o: 8, state: 4, products: 1, loads: 1
+// P: 4 warps, V' and o: 8, state: 4, products: 1, loads: 1 (and 2 that only give their registers)
+constexpr int kThreads = 640;
+// Registers a thread: 640 threads leave 96 each; the five groups of four warps share the 480 as
+// 112 (P), 2 x 96 (V' and o), 136 (state, 64 of it its rows) and 40.
+template <int N> __device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 constexpr uint32_t kColumns = 512;
 // TMEM columns: two buffers of Sc (P over its first 64 columns, Oi over the others), Oe, U
 constexpr uint32_t kSc = 0, kOi = 64, kOe = 256, kU = 320;
@@ -532,6 +541,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   const int chunks = w.chunks;
 
   if (warp < 4) {
+    take_registers<112>();
     // ---- P = Sc * M.  Row t = 32 warp + lane, 32 columns at a time from the left: the 16-bit
     // scores of a block go over columns whose scores have been read.  Off the diagonal block
     // (forward; the mirror image back in time) d^{t-s} = d^{32(w-j-1)+lane+1} d^{31-c}: both
@@ -687,6 +697,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       }
     }
   } else if (warp < 16) {
+    take_registers<136>();
     // ---- the state, a row of 64 columns a thread (DK = 64: 16 rows a warp, the lanes that a
     // product with M = 64 fills)
     const int r = DK == 128 ? (warp - 12) * 32 + lane : (warp - 12) * 16 + (lane & 15);
@@ -782,6 +793,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         if (c < w.vcols) dst[c] = s[c / 32][c % 32];
     }
   } else if (warp == 17) {
+    give_registers<40>();
     // ---- loads
     const CUtensorMap* map = maps.map[w.ji];
     const Source q(map, job.qs, w.h / job.q_group, w.b), k(map + 1, job.ks, w.h / job.k_group, w.b),
@@ -810,7 +822,10 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         while (!bar_try(&full[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
         }
     }
+  } else if (warp > 17) {
+    give_registers<40>();
   } else {
+    give_registers<40>();
     // ---- all products, issued by one lane
     constexpr uint32_t id_sc = instr<T>(C, C, false, false);
     constexpr uint32_t id_o = instr<T>(C, NV, false, true);
