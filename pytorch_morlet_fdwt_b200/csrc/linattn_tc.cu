@@ -20,8 +20,8 @@
 // Bound: 2 (2 Dk + 2 Dv) bytes of HBM a token and head against about 4 (Dk Dv + 128 (Dk + Dv))
 // operations, 96 a byte at 128 x 128, under half of the tensor rate at the HBM rate.  What costs
 // is the chain of dependent steps in a chunk, so every step has its own warps and the chunks
-// overlap: one warp issues the loads (TMA), one all products, four form P, eight form V' and
-// finish o, four keep the state.  All parts of V' are one product (N = 64 parts), so that K is read
+// overlap: one warp issues the loads (TMA), one all products, four form P, eight V', four finish
+// o, four keep the state.  All parts of V' are one product (N = 64 parts), so that K is read
 // once: the shared-memory rate binds the products more than the tensor rate.  Every wait on a barrier has a time limit.
 #include <cuda.h>
 
@@ -342,47 +342,58 @@ template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
 template <typename T> constexpr int kParts = kIsHalf<T> ? 2 : 3;
 constexpr float kLowScale = 2048.0f;
 
-// V' = diag(weight) V in parts, `lead` bytes apart; thread tid of 256 takes the 16-byte column
-// group tid % 8 of the rows tid / 8 + 32 j.
-template <typename T, int ROWS>
-__device__ __forceinline__ void split_values(const unsigned char* v, unsigned char* parts, int lead,
-                                             const float (&weight)[ROWS / 32], int tid) {
+// V' = diag(weight) V in parts: one 16-byte group.
+template <typename T>
+__device__ __forceinline__ void split_group(const unsigned char* v, float weight,
+                                            uint4 (&out)[kParts<T>]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(v);
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t u[kParts<T>][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f = unpack<T>(in[i]);
+    mul2(f.x, f.y, weight, weight);
+#pragma unroll
+    for (int p = 0; p < kParts<T>; ++p) {
+      u[p][i] = pack<T>(f.x, f.y);
+      if (p + 1 == kParts<T>) break;
+      const float2 g = unpack<T>(u[p][i]);
+      sub2(f.x, f.y, g.x, g.y);
+      if (kIsHalf<T>) mul2(f.x, f.y, kLowScale, kLowScale);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kParts<T>; ++p) out[p] = make_uint4(u[p][0], u[p][1], u[p][2], u[p][3]);
+}
+// 64 rows of it by 128 threads: thread tid takes the column group tid % 8 of the rows tid / 8 + 16 j.
+// `ready()` (false: give up) is asked for between forming the first two groups and storing them.
+template <typename T, typename F>
+__device__ __forceinline__ bool split_values(const unsigned char* v, unsigned char* parts, int lead,
+                                             const float (&weight)[4], int tid, F ready) {
   const int r0 = tid / 8;
   const int cell = r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
+  uint4 a[2][kParts<T>];
 #pragma unroll
-  for (int j = 0; j < ROWS / 32; ++j) {
-    const int at = cell + j * 32 * 128;
-    const uint4 x = *reinterpret_cast<const uint4*>(v + at);
-    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-    uint32_t out[kParts<T>][4];
+  for (int j = 0; j < 2; ++j) split_group<T>(v + cell + j * 2048, weight[j], a[j]);
+  if (!ready()) return false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 f = unpack<T>(in[i]);
-      mul2(f.x, f.y, weight[j], weight[j]);
-#pragma unroll
-      for (int p = 0; p < kParts<T>; ++p) {
-        out[p][i] = pack<T>(f.x, f.y);
-        if (p + 1 == kParts<T>) break;
-        const float2 g = unpack<T>(out[p][i]);
-        sub2(f.x, f.y, g.x, g.y);
-        if (kIsHalf<T>) mul2(f.x, f.y, kLowScale, kLowScale);
-      }
-    }
+  for (int j = 0; j < 4; ++j) {
+    if (j >= 2) split_group<T>(v + cell + j * 2048, weight[j], a[j - 2]);
 #pragma unroll
     for (int p = 0; p < kParts<T>; ++p)
-      *reinterpret_cast<uint4*>(parts + p * lead + at) =
-          make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
+      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048) = a[j & 1][p];
   }
+  return true;
 }
 
-// D (+)= K^T V' over ROWS tokens, all parts at once, 64 columns each (FIRST: the first product
-// does not add): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
-template <typename T, int DK, int ROWS, bool FIRST>
+// D (+)= K^T V' over 64 tokens, all parts at once, 64 columns each (FIRST: the first product does
+// not add): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
+template <typename T, int DK, bool FIRST>
 __device__ __forceinline__ void issue_update(uint32_t d, uint32_t k, uint32_t b) {
   constexpr uint32_t id = instr<T>(DK, NV * kParts<T>, true, true);
   mma_ss<!FIRST>(d, k, b, id);
 #pragma unroll
-  for (int i = 1; i < ROWS / 16; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
+  for (int i = 1; i < 4; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
 }
 // 8 columns of U from the parts' sums.
 template <typename T> __device__ __forceinline__ void load_update(uint32_t addr, float (&x)[8]) {
@@ -404,10 +415,11 @@ template <typename T> __device__ __forceinline__ void load_update(uint32_t addr,
   }
 }
 
-// P: 4 warps, V' and o: 8, state: 4, products: 1, loads: 1 (and 2 that only give their registers)
-constexpr int kThreads = 640;
-// Registers a thread: 640 threads leave 96 each; the five groups of four warps share the 480 as
-// 112 (P), 2 x 96 (V' and o), 136 (state, 64 of it its rows) and 40.
+// Products: warp 0, loads: 1 (2 and 3 only give registers; the first warps go first where several
+// could), P: 4 warps, V': 8, o: 4, state: 4.
+constexpr int kThreads = 768;
+// Registers a thread: 768 threads leave 80 each; the six groups of four warps share the 480 as
+// 96 (P), 2 x 56 (V'), 96 (o), 136 (state, 64 of it its rows) and 40.
 template <int N> __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
@@ -423,9 +435,8 @@ constexpr int kStateRows = 64, kStatePanel = kStateRows * 128;
 template <typename T, int DK> struct Smem {
   static constexpr int panels = DK / 64;
   static constexpr int stages = DK == 64 ? 3 : 2;
-  static constexpr int q = 0, k = panels * kPanel, v = 2 * panels * kPanel;
-  static constexpr int stage = (2 * panels + 1) * kPanel;
-  static constexpr int parts = stages * stage, s = parts + kParts<T> * kPanel;
+  static constexpr int q = 0, k = stages * panels * kPanel, v = 2 * k;  // rings of stages
+  static constexpr int parts = v + stages * kPanel, s = parts + kParts<T> * kPanel;
   static constexpr int bytes = s + DK * 128 + 1024;  // 1024: room to align the base
   static constexpr int st_stages = 4;
   static constexpr int st_stage = (panels + 1) * kStatePanel;
@@ -494,8 +505,9 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   constexpr int S = Z::stages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = align_smem(raw);
-  __shared__ uint64_t full[S], empty[S], sc_full[2], p_full, o_full, o_empty, s_full, u_full,
-      u_empty, v_full, most_full, drain;
+  __shared__ uint64_t k_full[S], q_full[S], v_in[S], k_empty[S], q_empty[S], v_empty[S];
+  __shared__ uint64_t sc_full[2], p_full[2], oe_full, oe_empty, o_full, o_empty, s_full, u_full,
+      u_empty, v_full[2], v_free[2], most_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float power[64];          // at 31 + t - s: intra d^|t-s|, 0 for a masked pair
@@ -508,19 +520,26 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      bar_init(&full[i], 1);
-      bar_init(&empty[i], 1);
+      bar_init(&k_full[i], 1);
+      bar_init(&q_full[i], 1);
+      bar_init(&v_in[i], 1);
+      bar_init(&k_empty[i], 1);
+      bar_init(&q_empty[i], 1);
+      bar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sc_full[i], 1);
+      bar_init(&p_full[i], 128);
+      bar_init(&v_full[i], 128);
+      bar_init(&v_free[i], 1);
     }
-    bar_init(&p_full, 128);
+    bar_init(&oe_full, 1);
+    bar_init(&oe_empty, 128);
     bar_init(&o_full, 1);
-    bar_init(&o_empty, 256);
+    bar_init(&o_empty, 128);
     bar_init(&s_full, 128);
     bar_init(&u_full, 1);
     bar_init(&u_empty, 128);
-    bar_init(&v_full, 256);
     bar_init(&most_full, 4);
     bar_init(&drain, 1);
     failed = 0;
@@ -531,7 +550,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const int n = job.reverse ? 31 - i : i - 31;
     power[i] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
   }
-  if (warp == 16) tmem_alloc(&tmem_slot);
+  if (warp == 0) tmem_alloc(&tmem_slot);
   tc_before();
   __syncthreads();
   tc_after();
@@ -540,9 +559,10 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   const uint32_t base = smem_addr(sm);
   const int chunks = w.chunks;
 
-  if (warp < 4) {
-    take_registers<112>();
-    // ---- P = Sc * M.  Row t = 32 warp + lane, 32 columns at a time from the left: the 16-bit
+  if (warp >= 4 && warp < 8) {
+    take_registers<96>();
+    const int row_warp = warp - 4;
+    // ---- P = Sc * M.  Row t = 32 row_warp + lane, 32 columns at a time from the left: the 16-bit
     // scores of a block go over columns whose scores have been read.  Off the diagonal block
     // (forward; the mirror image back in time) d^{t-s} = d^{32(w-j-1)+lane+1} d^{31-c}: both
     // powers are at least 0, nothing overflows.
@@ -552,7 +572,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     for (int c = 0; c < 32; ++c) tab[c] = decay_pow(w.a, float(rev ? c + 1 : 31 - c));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int n = rev ? 32 * (j - warp - 1) + 31 - lane : 32 * (warp - j - 1) + lane + 1;
+      const int n = rev ? 32 * (j - row_warp - 1) + 31 - lane : 32 * (row_warp - j - 1) + lane + 1;
       lead[j] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
     }
     const float* diagonal = power + 31 + lane;
@@ -566,12 +586,12 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       if (kHalf) {
         float most = 0.0f;
 #pragma unroll 1
-        for (int j = rev ? warp : 0; j <= (rev ? 3 : warp); ++j) {
+        for (int j = rev ? row_warp : 0; j <= (rev ? 3 : row_warp); ++j) {
           const float f = j == 0 ? lead[0] : (j == 1 ? lead[1] : (j == 2 ? lead[2] : lead[3]));
           float x[32], block = 0.0f;
           tmem_ld32(sc + j * 32, x);
           tmem_ld_wait(x);
-          if (j == warp) {
+          if (j == row_warp) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
               const float p = diagonal[-c];
@@ -585,19 +605,19 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         }
         float inv;
         scale = scale_of(most, &inv);
-        p_inv[i & 1][warp * 32 + lane] = inv;
+        p_inv[i & 1][row_warp * 32 + lane] = inv;
       }
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
         uint32_t u[16];
-        if (rev ? j < warp : j > warp) {  // all masked
+        if (rev ? j < row_warp : j > row_warp) {  // all masked
 #pragma unroll
           for (int c = 0; c < 16; ++c) u[c] = 0;
         } else {
           float x[32];
           tmem_ld32(sc + j * 32, x);
           tmem_ld_wait(x);
-          if (j == warp) {
+          if (j == row_warp) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
               const float p = diagonal[-c];
@@ -619,88 +639,103 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       }
       tmem_st_wait();
       tc_before();
-      bar_arrive(&p_full);
+      bar_arrive(&p_full[i & 1]);
     }
-  } else if (warp < 12) {
-    // ---- V' of a chunk, then o = inter d^{l+off} Oe + Oi of the chunk before: half a row of 64
-    // columns a thread
-    const int tid = threadIdx.x - 128;
+  } else if (warp >= 8 && warp < 16) {
+    give_registers<56>();
+    // ---- V', four warps each for the first and the last 64 tokens, which are multiplied one
+    // after the other: a half is formed anew while the other one is still in use
+    const int tid = threadIdx.x % 128, half = (warp - 8) / 4;
+    const int cell0 = half * 64 * 128;
+    float weight[4];
+    int weight_m = 0;
+    for (int i = 0; i < chunks; ++i) {
+      const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
+      if (m != weight_m) {
+        weight_m = m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = half * 64 + tid / 8 + 16 * j;
+          const int age = m - job.off - (job.reverse ? C - 1 - r : r);
+          weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
+        }
+      }
+      if (!bar_wait(&v_in[i % S], (i / S) & 1, &failed)) break;
+      unsigned char* v = sm + Z::v + (i % S) * kPanel;
+      if (m < C && !job.reverse && w.n < call.length) {
+        // padding after the sequence's end: the products take zeros for its keys and values
+        // (scores with them are masked, whichever of the two they read).  A thread clears the
+        // values that it reads below.
+        if (!bar_wait(&k_full[i % S], (i / S) & 1, &failed)) break;
+        unsigned char* k = sm + Z::k + (i % S) * Z::panels * kPanel;
+        for (int r = half * 64 + tid / 8; r < half * 64 + 64; r += 16) {
+          if (r < m) continue;
+          const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
+#pragma unroll
+          for (int p = 0; p < Z::panels; ++p)
+            *reinterpret_cast<uint4*>(k + p * kPanel + at) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + at) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      const bool ok = split_values<T>(v + cell0, sm + Z::parts + cell0, kPanel, weight, tid, [&] {
+        return i == 0 || bar_wait(&v_free[half], (i - 1) & 1, &failed);
+      });
+      if (!ok) break;
+      fence_async();
+      bar_arrive(&v_full[half]);
+    }
+  } else if (warp >= 16 && warp < 20) {
+    take_registers<96>();
+    // ---- o = inter d^{l+off} Oe + Oi, a row of 64 columns a thread; Oe is taken as soon as it is
+    // there, so that the next chunk's can follow
     const int t = warp % 4 * 32 + lane, l = job.reverse ? C - 1 - t : t;
-    const int c_half = (warp - 4) / 4 * 32;
     const float read = float(job.inter) * decay_pow(w.a, float(l + job.off));
     const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
-    float weight[C / 32];
-    int weight_m = 0;
-    for (int i = 0; i <= chunks; ++i) {
-      if (i < chunks) {
-        const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
-        if (m != weight_m) {
-          weight_m = m;
-#pragma unroll
-          for (int j = 0; j < C / 32; ++j) {
-            const int r = tid / 8 + 32 * j;
-            const int age = m - job.off - (job.reverse ? C - 1 - r : r);
-            weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
-          }
-        }
-        bool ok = bar_wait(&full[i % S], (i / S) & 1, &failed);
-        unsigned char* stage = sm + (i % S) * Z::stage;
-        if (ok && m < C && !job.reverse && w.n < call.length) {
-          // padding after the sequence's end: the products take zeros for its keys and values
-          // (scores with them are masked, whichever of the two they read).  A thread clears the
-          // values that it reads below.
-          for (int r = tid / 8; r < C; r += 32) {
-            if (r < m) continue;
-            const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
-#pragma unroll
-            for (int p = 0; p < Z::panels; ++p)
-              *reinterpret_cast<uint4*>(stage + Z::k + p * kPanel + at) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(stage + Z::v + at) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        ok = ok && (i == 0 || bar_wait(&u_full, (i - 1) & 1, &failed));
-        if (!__all_sync(0xffffffffu, ok)) break;
-        split_values<T, C>(stage + Z::v, sm + Z::parts, kPanel, weight, tid);
-        fence_async();
-        bar_arrive(&v_full);
-      }
-      if (i == 0) continue;
-      const int e = i - 1;  // the chunk whose o is finished
-      if (!__all_sync(0xffffffffu, bar_wait(&o_full, e & 1, &failed))) break;
+    for (int i = 0; i < chunks; ++i) {
+      if (!__all_sync(0xffffffffu, bar_wait(&oe_full, i & 1, &failed))) break;
       tc_after();
-      const int64_t l0 = w.begin + int64_t(e) * C;
+      const int64_t l0 = w.begin + int64_t(i) * C;
       const bool in = l0 + l < w.end;
       const int64_t token = (job.reverse ? w.n - C - l0 : l0) + t;
       const int64_t at = head + token * job.os[1];
-      const float fe = kHalf ? read * s_inv[e & 1] : read;
-      const float fi = kHalf ? p_inv[e & 1][t] : 1.0f;
+      const float fe = kHalf ? read * s_inv[i & 1] : read;
+      float y[NV / 16][16];
 #pragma unroll
-      for (int c0 = c_half; c0 < c_half + 32; c0 += 16) {
-        float y[16], x[16];
-        tmem_ld16(tmem + lanes + kOe + c0, y);
-        tmem_ld16(tmem + lanes + kSc + (e & 1) * 128 + kOi + c0, x);
-        tmem_ld_wait(y);
+      for (int g = 0; g < NV / 16; ++g) tmem_ld16(tmem + lanes + kOe + g * 16, y[g]);
+#pragma unroll
+      for (int g = 0; g < NV / 16; ++g) tmem_ld_wait(y[g]);
+      tc_before();
+      bar_arrive(&oe_empty);
+      if (!__all_sync(0xffffffffu, bar_wait(&o_full, i & 1, &failed))) break;
+      tc_after();
+      const float fi = kHalf ? p_inv[i & 1][t] : 1.0f;
+#pragma unroll
+      for (int g = 0; g < NV / 16; ++g) {
+        float x[16];
+        tmem_ld16(tmem + lanes + kSc + (i & 1) * 128 + kOi + g * 16, x);
         tmem_ld_wait(x);
-        if (c0 > c_half) {
+        if (g == NV / 16 - 1) {
           tc_before();
           bar_arrive(&o_empty);
         }
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
           if (kHalf) mul2(x[c], x[c + 1], fi, fi);
-          fma2(y[c], y[c + 1], fe, x[c], x[c + 1]);
+          fma2(y[g][c], y[g][c + 1], fe, x[c], x[c + 1]);
         }
         if (in) {
-          if (job.o_wide) store_wide(static_cast<float*>(job.o) + at + c0, y, w.vcols - c0);
-          else store_row(static_cast<T*>(job.o) + at + c0, y, w.vcols - c0, job.o_vec);
+          if (job.o_wide)
+            store_wide(static_cast<float*>(job.o) + at + g * 16, y[g], w.vcols - g * 16);
+          else
+            store_row(static_cast<T*>(job.o) + at + g * 16, y[g], w.vcols - g * 16, job.o_vec);
         }
       }
     }
-  } else if (warp < 16) {
+  } else if (warp >= 20) {
     take_registers<136>();
     // ---- the state, a row of 64 columns a thread (DK = 64: 16 rows a warp, the lanes that a
     // product with M = 64 fills)
-    const int r = DK == 128 ? (warp - 12) * 32 + lane : (warp - 12) * 16 + (lane & 15);
+    const int r = DK == 128 ? (warp - 20) * 32 + lane : (warp - 20) * 16 + (lane & 15);
     const bool mine = DK == 128 || lane < 16;
     const int64_t size = int64_t(job.dk) * job.dv;
     const float write = float(job.write);
@@ -744,7 +779,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         tc_before();
         bar_arrive(&u_empty);
         if (i == chunks) break;
-        ok = __all_sync(0xffffffffu, bar_wait(&o_full, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&oe_full, (i - 1) & 1, &failed));
         if (!ok) break;
       }
       if (chunks == 0) break;
@@ -758,9 +793,9 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // (rewritten only after o_full of this chunk, which follows every warp's s_full)
+        // (rewritten only after oe_full of this chunk, which follows every warp's s_full)
         if (lane == 0) {
-          s_most[warp - 12] = most;
+          s_most[warp - 20] = most;
           bar_arrive(&most_full);
         }
         ok = __all_sync(0xffffffffu, bar_wait(&most_full, i & 1, &failed));
@@ -768,7 +803,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
         float inv;
         scale = scale_of(most, &inv);
-        if (warp == 12 && lane == 0) s_inv[i & 1] = inv;
+        if (warp == 20 && lane == 0) s_inv[i & 1] = inv;
       }
       if (mine) {
         unsigned char* row = sm + Z::s + r * 128;
@@ -792,37 +827,46 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       for (int c = 0; c < NV; ++c)
         if (c < w.vcols) dst[c] = s[c / 32][c % 32];
     }
-  } else if (warp == 17) {
+  } else if (warp == 1) {
     give_registers<40>();
     // ---- loads
     const CUtensorMap* map = maps.map[w.ji];
     const Source q(map, job.qs, w.h / job.q_group, w.b), k(map + 1, job.ks, w.h / job.k_group, w.b),
         v(map + 2, job.vs, w.h / job.v_group, w.b);
     const bool one = elect_one();
-    int issued = 0;
+    // an operand's buffer is loaded again as soon as its own last product has ended
+    int issued = 0;  // loads begun, three a chunk: K, Q, V
     bool ok = true;
-    for (; issued < chunks && ok; ++issued) {
-      const int i = issued, st = i % S;
+    for (; issued < 3 * chunks; ++issued) {
+      const int i = issued / 3, which = issued % 3, st = i % S;
+      uint64_t* empty = which == 0 ? k_empty : (which == 1 ? q_empty : v_empty);
       ok = __all_sync(0xffffffffu, i < S || bar_wait(&empty[st], (i / S - 1) & 1, &failed));
       if (!ok) break;
       if (one) {
         const int64_t l0 = w.begin + int64_t(i) * C;
         const int64_t token = job.reverse ? w.n - C - l0 : l0;
-        const uint32_t at = base + st * Z::stage;
-        bar_expect(&full[st], Z::stage);
-        k.template load<C>(at + Z::k, 0, Z::panels, token, &full[st]);
-        q.template load<C>(at + Z::q, 0, Z::panels, token, &full[st]);
-        v.template load<C>(at + Z::v, w.v0, 1, token, &full[st]);
+        if (which == 2) {
+          bar_expect(&v_in[st], kPanel);
+          v.template load<C>(base + Z::v + st * kPanel, w.v0, 1, token, &v_in[st]);
+        } else {
+          uint64_t* bar = which == 0 ? &k_full[st] : &q_full[st];
+          bar_expect(bar, Z::panels * kPanel);
+          (which == 0 ? k : q).template load<C>(
+              base + (which == 0 ? Z::k : Z::q) + st * Z::panels * kPanel, 0, Z::panels, token, bar);
+        }
       }
       __syncwarp();
     }
     if (!ok) {  // copies in flight land before the block ends
       const long long start = clock64();
-      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
-        while (!bar_try(&full[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
+      for (int j = issued > 3 * S ? issued - 3 * S : 0; j < issued; ++j) {
+        const int i = j / 3, which = j % 3;
+        uint64_t* bar = which == 0 ? k_full : (which == 1 ? q_full : v_in);
+        while (!bar_try(&bar[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
         }
+      }
     }
-  } else if (warp > 17) {
+  } else if (warp > 1) {
     give_registers<40>();
   } else {
     give_registers<40>();
@@ -830,11 +874,13 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     constexpr uint32_t id_sc = instr<T>(C, C, false, false);
     constexpr uint32_t id_o = instr<T>(C, NV, false, true);
     // operands of stage 0, and of what has one buffer
-    const uint32_t oq = operand(base + Z::q, kPanel);
+    const uint32_t oq = operand(base + Z::q, kPanel), ok0 = operand(base + Z::k, kPanel);
+    const uint32_t ov = operand(base + Z::v, kPanel);
     const uint32_t os = operand(base + Z::s, kPanel), op = operand(base + Z::parts, kPanel);
     const bool one = elect_one();
     auto scores = [&](int i) {
-      const uint32_t q = oq + (i % S) * (Z::stage / 16), k = q + (Z::k - Z::q) / 16;
+      const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
+      const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
       const uint32_t d = tmem + kSc + (i & 1) * 128;
       if (one) {
         tc_after();
@@ -847,28 +893,41 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       }
       __syncwarp();
     };
-    // (the score buffer is free: o of chunk i - 2, which ends in it, was waited for before)
-    auto ready = [&](int i) { return bar_wait(&full[i % S], (i / S) & 1, &failed); };
+    auto ready = [&](int i) {
+      return bar_wait(&k_full[i % S], (i / S) & 1, &failed) &&
+             bar_wait(&q_full[i % S], (i / S) & 1, &failed);
+    };
     bool ok = true;
     if (chunks > 0) {
       ok = __all_sync(0xffffffffu, ready(0));
       if (ok) scores(0);
     }
     for (int i = 0; i < chunks && ok; ++i) {
-      const uint32_t q = oq + (i % S) * (Z::stage / 16);
-      const uint32_t k = q + (Z::k - Z::q) / 16, v = q + (Z::v - Z::q) / 16;
-      ok = bar_wait(&v_full, i & 1, &failed) &&
+      const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
+      const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
+      const uint32_t v = ov + (i % S) * (kPanel / 16);
+      ok = bar_wait(&v_full[0], i & 1, &failed) &&
            (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (one) {
         tc_after();
-        issue_update<T, DK, C, true>(tmem + kU, k, op);
+        issue_update<T, DK, true>(tmem + kU, k, op);
+        tc_commit(&v_free[0]);
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, &failed));
+      if (!ok) break;
+      if (one) {
+        tc_after();
+        issue_update<T, DK, false>(tmem + kU, k + 512, op + 512);
+        tc_commit(&v_free[1]);
         tc_commit(&u_full);
+        tc_commit(&k_empty[i % S]);
       }
       __syncwarp();
       ok = bar_wait(&s_full, i & 1, &failed) &&
-           (i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+           (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, &failed));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (one) {
@@ -877,17 +936,20 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
         for (int j = 1; j < DK / 16; ++j)
           mma_ss<true>(tmem + kOe, q + j / 4 * (kPanel / 16) + j % 4 * 2, os + j * 128, id_o);
+        tc_commit(&oe_full);
+        tc_commit(&q_empty[i % S]);
       }
       __syncwarp();
-      // the next chunk's scores go before this one's P V where their operands are there already
-      bool ahead = i + 1 < chunks && bar_test(&full[(i + 1) % S], ((i + 1) / S) & 1);
+      // the next chunk's scores go before this one's P V where its operands are there already.
+      // Their buffer held Oi of the chunk before.  (This wait comes before P V, whose o frees the
+      // other buffer: a barrier must not be two phases ahead of who waits for it.)
+      ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+      if (!ok) break;
+      bool ahead = i + 1 < chunks && bar_test(&k_full[(i + 1) % S], ((i + 1) / S) & 1) &&
+                   bar_test(&q_full[(i + 1) % S], ((i + 1) / S) & 1);
       ahead = __all_sync(0xffffffffu, ahead);
-      if (ahead) {
-        ok = __all_sync(0xffffffffu, ready(i + 1));
-        if (!ok) break;
-        scores(i + 1);
-      }
-      ok = __all_sync(0xffffffffu, bar_wait(&p_full, i & 1, &failed));
+      if (ahead) scores(i + 1);
+      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed));
       if (!ok) break;
       if (one) {
         tc_after();
@@ -896,7 +958,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
         for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
         tc_commit(&o_full);
-        tc_commit(&empty[i % S]);
+        tc_commit(&v_empty[i % S]);
       }
       __syncwarp();
       if (!ahead && i + 1 < chunks) {
@@ -925,7 +987,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   }
   tc_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 0) {
     tc_after();
     tmem_free(tmem);
     if (lane == 0 && failed) *error = kErrCopyTimeout;
@@ -954,7 +1016,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   if (w.seg >= w.last) return;  // the whole block
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 256);
+    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 128);
     for (int i = 0; i < S; ++i) {
       bar_init(&full[i], 1);
       bar_init(&used[i], 1);
@@ -972,29 +1034,31 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
 
   if (warp < 8) {
-    const int tid = threadIdx.x;
-    for (int i = 0; i < chunks; ++i) {
-      float weight[R / 32];
+    // four warps take the even blocks of 64 tokens, four the odd ones, each their buffer of V'
+    const int tid = threadIdx.x % 128, mine = warp / 4;
+    for (int i = mine; i < chunks; i += 2) {
+      float weight[4];
 #pragma unroll
-      for (int j = 0; j < R / 32; ++j) {
-        const int r = tid / 8 + 32 * j;
+      for (int j = 0; j < 4; ++j) {
+        const int r = tid / 8 + 16 * j;
         const int64_t age =
             w.end - job.off - (w.begin + int64_t(i) * R + (job.reverse ? R - 1 - r : r));
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
       }
       if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
-      // buffer i % 2 of V' is free when the products of chunk i - 2 have ended
-      if (i >= 2 && !bar_wait(&used[(i - 2) % S], ((i - 2) / S) & 1, &failed)) break;
-      split_values<T, R>(sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
-                         sm + Z::st_parts + (i & 1) * kParts<T> * kStatePanel, kStatePanel, weight,
-                         tid);
+      const bool ok = split_values<T>(
+          sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
+          sm + Z::st_parts + mine * kParts<T> * kStatePanel, kStatePanel, weight, tid,
+          // the products of block i - 2 have ended
+          [&] { return i < 2 || bar_wait(&used[(i - 2) % S], ((i - 2) / S) & 1, &failed); });
+      if (!ok) break;
       fence_async();
-      bar_arrive(&v_full[i & 1]);
+      bar_arrive(&v_full[mine]);
     }
     if (warp < 4 && __all_sync(0xffffffffu, bar_wait(&done, 0, &failed)) && !failed) {
       tc_after();
       const int r = DK == 128 ? warp * 32 + lane : warp * 16 + (lane & 15);
-      const bool mine = (DK == 128 || lane < 16) && r < job.dk;
+      const bool in = (DK == 128 || lane < 16) && r < job.dk;
       float* dst = static_cast<float*>(job.seg) +
                    (w.bh * (call.nseg - 1) + w.seg) * (int64_t(job.dk) * job.dv) +
                    int64_t(r) * job.dv + w.v0;
@@ -1002,7 +1066,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       for (int g = 0; g < NV; g += 8) {
         float x[8];
         load_update<T>(tmem + (uint32_t(warp * 32) << 16) + g, x);
-        if (mine) {
+        if (in) {
 #pragma unroll
           for (int c = 0; c < 8; ++c)
             if (g + c < w.vcols) dst[g + c] = write * x[c];
@@ -1047,8 +1111,8 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       const uint32_t parts = op0 + (i & 1) * (kParts<T> * kStatePanel / 16);
       if (one) {
         tc_after();
-        if (i == 0) issue_update<T, DK, R, true>(tmem, k, parts);
-        else issue_update<T, DK, R, false>(tmem, k, parts);
+        if (i == 0) issue_update<T, DK, true>(tmem, k, parts);
+        else issue_update<T, DK, false>(tmem, k, parts);
         tc_commit(&used[i % S]);
       }
       __syncwarp();
