@@ -59,31 +59,23 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// The same without waiting for the phase.
-__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n"
-      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-constexpr long long kWaitCycles = 4000000000LL;  // about two seconds
+// Polls of a wait (each may sleep for a while in hardware): well under a second in all.
+constexpr int kWaitTries = 1 << 22;
 // False: the wait ran out here or elsewhere in the block; the block then ends early.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (bar_try(bar, parity)) return true;
-  const long long start = clock64();
-  while (!bar_try(bar, parity)) {
+#pragma unroll 1
+  for (int i = 0; i < kWaitTries; ++i) {
+    if (bar_try(bar, parity)) return true;
     if (*failed) return false;
-    if (clock64() - start > kWaitCycles) {
-      *failed = 1;
-      return false;
-    }
   }
-  return true;
+  *failed = 1;
+  return false;
+}
+// For what is in flight after a failure: no regard to `failed`.
+__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < kWaitTries && !bar_try(bar, parity); ++i) {
+  }
 }
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -279,38 +271,38 @@ __device__ __forceinline__ float scale_of(float most, float* inverse) {
 // ------------------------------------------------------------------------------ a block's work
 struct Where {
   const Job* job;
-  int64_t bh, n, begin, end, row_end;  // valid tokens [begin, end) and rows [begin, row_end)
+  int bh, n, begin, end, row_end;  // valid tokens [begin, end) and rows [begin, row_end)
   int h, b, seg, last, v0, vcols, chunks, ji;
   float a;
 };
 
+// Block (value tile of the jobs, sequence and head, segment).
 __device__ __forceinline__ Where locate(const Call& call) {
   Where w;
-  int tile = blockIdx.x % call.tiles;
-  const int64_t rest = blockIdx.x / call.tiles;
-  const int64_t heads = call.batch * call.heads;
-  w.bh = rest % heads;
-  w.seg = static_cast<int>(rest / heads);
+  int tile = blockIdx.x;
+  w.bh = blockIdx.y;
+  w.seg = blockIdx.z;
   int ji = 0;
   while (tile >= call.job[ji].tiles) tile -= call.job[ji++].tiles;
   w.job = &call.job[ji];
   w.ji = ji;
-  w.b = static_cast<int>(w.bh / call.heads);
-  w.h = static_cast<int>(w.bh % call.heads);
+  w.b = static_cast<int>(blockIdx.y / static_cast<unsigned>(call.heads));
+  w.h = w.bh - w.b * call.heads;
   w.v0 = tile * NV;
   w.vcols = w.job->dv - w.v0 < NV ? w.job->dv - w.v0 : NV;
-  int64_t n = call.length;
+  const int length = static_cast<int>(call.length), seg_len = static_cast<int>(call.seg_len);
+  int n = length;
   if (call.lengths != nullptr) {
     n = call.lengths[w.b];
-    n = n < 0 ? 0 : (n > call.length ? call.length : n);
+    n = n < 0 ? 0 : (n > length ? length : n);
   }
   w.n = n;
-  w.last = n == 0 ? 0 : static_cast<int>((n - 1) / call.seg_len);
+  w.last = n == 0 ? 0 : static_cast<int>(unsigned(n - 1) / unsigned(seg_len));
   w.a = static_cast<const float*>(call.log_decay)[w.h];
-  w.begin = int64_t(w.seg) * call.seg_len;
-  w.row_end = imin(w.begin + call.seg_len, call.length);
-  w.end = imin(w.row_end, n);
-  w.chunks = w.end > w.begin ? static_cast<int>(cdiv(w.end - w.begin, C)) : 0;
+  w.begin = w.seg * seg_len;
+  w.row_end = length - w.begin < seg_len ? length : w.begin + seg_len;
+  w.end = w.row_end < n ? w.row_end : n;
+  w.chunks = w.end > w.begin ? (w.end - w.begin + C - 1) / C : 0;
   return w;
 }
 
@@ -327,12 +319,13 @@ struct Source {
       : map(m), head(stride[2] == 0 ? 0 : h), batch(stride[0] == 0 ? 0 : b) {}
   // ROWS tokens from `token` on, `columns` panels of 64 columns from x on, to dst
   template <int ROWS> __device__ __forceinline__ void load(uint32_t dst, int x, int panels,
-                                                           int64_t token, uint64_t* bar) const {
+                                                           int token, uint64_t* bar) const {
+#pragma unroll 1
     for (int i = 0; i < panels; ++i)
 #pragma unroll
       for (int r = 0; r < ROWS / kBoxRows; ++r)
         tma_load(dst + (i * (ROWS / kBoxRows) + r) * kBox, map, x + 64 * i,
-                 static_cast<int>(token) + r * kBoxRows, head, batch, bar);
+                 token + r * kBoxRows, head, batch, bar);
   }
 };
 
@@ -372,16 +365,17 @@ __device__ __forceinline__ bool split_values(const unsigned char* v, unsigned ch
                                              const float (&weight)[4], int tid, F ready) {
   const int r0 = tid / 8;
   const int cell = r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
-  uint4 a[2][kParts<T>];
+#pragma unroll 1
+  for (int j = 0; j < 4; j += 2) {
+    uint4 a[2][kParts<T>];
+    split_group<T>(v + cell + j * 2048, j == 0 ? weight[0] : weight[2], a[0]);
+    split_group<T>(v + cell + j * 2048 + 2048, j == 0 ? weight[1] : weight[3], a[1]);
+    if (j == 0 && !ready()) return false;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) split_group<T>(v + cell + j * 2048, weight[j], a[j]);
-  if (!ready()) return false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= 2) split_group<T>(v + cell + j * 2048, weight[j], a[j - 2]);
-#pragma unroll
-    for (int p = 0; p < kParts<T>; ++p)
-      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048) = a[j & 1][p];
+    for (int p = 0; p < kParts<T>; ++p) {
+      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048) = a[0][p];
+      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048 + 2048) = a[1][p];
+    }
   }
   return true;
 }
@@ -460,8 +454,8 @@ __device__ __forceinline__ void tmem_free(uint32_t base) {
                : "memory");
 }
 
-// 16 columns of a row (`cols` of them exist), in whole 32-byte sectors where these are aligned
-// (vec 2), else in 16 bytes (vec 1) or single elements.
+// 16 columns of a row (`cols` of them exist, a multiple of 8), in whole 32-byte sectors where
+// these are aligned (vec 2), else in 16 bytes.
 __device__ __forceinline__ void store8(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d,
                                        uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b),
@@ -475,13 +469,9 @@ __device__ __forceinline__ void store_row(T* dst, const float (&x)[16], int cols
   for (int c = 0; c < 8; ++c) u[c] = pack<T>(x[2 * c], x[2 * c + 1]);
   if (vec == 2) {
     if (cols > 0) store8(dst, u[0], u[1], u[2], u[3], u[4], u[5], u[6], u[7]);
-  } else if (vec == 1) {
+  } else {
     if (cols > 0) *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
     if (cols > 8) *reinterpret_cast<uint4*>(dst + 8) = make_uint4(u[4], u[5], u[6], u[7]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < 16; ++c)
-      if (c < cols) dst[c] = from_acc<T>(x[c]);
   }
 }
 // The 32-bit form (results that are added over heads later): contiguous, columns in eights.
@@ -515,10 +505,34 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   __shared__ float s_inv[2];           // fp16: inverse scale of the state's copy
   __shared__ volatile float s_most[4];  // fp16: largest magnitude of each warp's rows
 
+  __shared__ float dpow[C + 1];  // d^n
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  if (warp == 0) tmem_alloc(&tmem_slot);
   const Where w = locate(call);
   const Job& job = *w.job;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) {
+  const uint32_t base = smem_addr(sm);
+  const int chunks = w.chunks;
+  // loads: j = 3 i + (0: K, 1: Q, 2: V) of chunk i
+  auto load = [&](int j) {
+    const int i = j / 3, which = j % 3, st = i % S;
+    const CUtensorMap* map = maps.map[w.ji];
+    const int l0 = w.begin + i * C, token = job.reverse ? w.n - C - l0 : l0;
+    if (which == 2) {
+      bar_expect(&v_in[st], kPanel);
+      Source(map + 2, job.vs, w.h / job.v_group, w.b)
+          .template load<C>(base + Z::v + st * kPanel, w.v0, 1, token, &v_in[st]);
+    } else {
+      const bool k = which == 0;
+      uint64_t* bar = k ? &k_full[st] : &q_full[st];
+      bar_expect(bar, Z::panels * kPanel);
+      Source(k ? map + 1 : map, k ? job.ks : job.qs, w.h / (k ? job.k_group : job.q_group), w.b)
+          .template load<C>(base + (k ? Z::k : Z::q) + st * Z::panels * kPanel, 0, Z::panels, token,
+                            bar);
+    }
+  };
+  const int first_loads = 3 * (chunks < S ? chunks : S);
+  if (threadIdx.x == 32) {
     for (int i = 0; i < S; ++i) {
       bar_init(&k_full[i], 1);
       bar_init(&q_full[i], 1);
@@ -544,20 +558,23 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     bar_init(&drain, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+#pragma unroll 1
+    for (int j = 0; j < first_loads; ++j) load(j);
   }
   if (threadIdx.x >= 64 && threadIdx.x < 128) {
     const int i = threadIdx.x - 64;
     const int n = job.reverse ? 31 - i : i - 31;
     power[i] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
   }
-  if (warp == 0) tmem_alloc(&tmem_slot);
+  if (threadIdx.x >= 128 && threadIdx.x <= 128 + C)
+    dpow[threadIdx.x - 128] = decay_pow(w.a, float(threadIdx.x - 128));
+  __syncwarp();
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
-  const uint32_t base = smem_addr(sm);
-  const int chunks = w.chunks;
 
   if (warp >= 4 && warp < 8) {
     take_registers<96>();
@@ -569,11 +586,11 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const bool rev = job.reverse != 0;
     float tab[32], lead[4];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) tab[c] = decay_pow(w.a, float(rev ? c + 1 : 31 - c));
+    for (int c = 0; c < 32; ++c) tab[c] = dpow[rev ? c + 1 : 31 - c];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = rev ? 32 * (j - row_warp - 1) + 31 - lane : 32 * (row_warp - j - 1) + lane + 1;
-      lead[j] = n < 0 ? 0.0f : float(job.intra) * decay_pow(w.a, float(n));
+      lead[j] = n < 0 || n > C ? 0.0f : float(job.intra) * dpow[n];
     }
     const float* diagonal = power + 31 + lane;
     bool ok = true;
@@ -650,14 +667,14 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     float weight[4];
     int weight_m = 0;
     for (int i = 0; i < chunks; ++i) {
-      const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i) * C)));
+      const int left = w.end - (w.begin + i * C), m = left < C ? left : C;
       if (m != weight_m) {
         weight_m = m;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = half * 64 + tid / 8 + 16 * j;
           const int age = m - job.off - (job.reverse ? C - 1 - r : r);
-          weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
+          weight[j] = age < 0 ? 0.0f : dpow[age];
         }
       }
       if (!bar_wait(&v_in[i % S], (i / S) & 1, &failed)) break;
@@ -689,15 +706,15 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     // ---- o = inter d^{l+off} Oe + Oi, a row of 64 columns a thread; Oe is taken as soon as it is
     // there, so that the next chunk's can follow
     const int t = warp % 4 * 32 + lane, l = job.reverse ? C - 1 - t : t;
-    const float read = float(job.inter) * decay_pow(w.a, float(l + job.off));
+    const float read = float(job.inter) * dpow[l + job.off];
     const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
     for (int i = 0; i < chunks; ++i) {
       if (!__all_sync(0xffffffffu, bar_wait(&oe_full, i & 1, &failed))) break;
       tc_after();
-      const int64_t l0 = w.begin + int64_t(i) * C;
+      const int l0 = w.begin + i * C;
       const bool in = l0 + l < w.end;
-      const int64_t token = (job.reverse ? w.n - C - l0 : l0) + t;
-      const int64_t at = head + token * job.os[1];
+      const int token = (job.reverse ? w.n - C - l0 : l0) + t;
+      const int64_t at = head + int64_t(token) * job.os[1];
       const float fe = kHalf ? read * s_inv[i & 1] : read;
       float y[NV / 16][16];
 #pragma unroll
@@ -750,12 +767,16 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           col = job.init_col;
         }
       } else if (w.seg <= w.last) {
-        src = static_cast<const float*>(job.seg) + (w.bh * (call.nseg - 1) + w.seg - 1) * size;
+        src = static_cast<const float*>(job.seg) +
+              (int64_t(w.bh) * (call.nseg - 1) + w.seg - 1) * size;
       }
-      const bool in = src != nullptr && mine && r < job.dk;
+      const int cols = src != nullptr && mine && r < job.dk ? w.vcols : 0;
+      src += r * row + w.v0 * col;
 #pragma unroll
-      for (int c = 0; c < NV; ++c)
-        s[c / 32][c % 32] = in && c < w.vcols ? src[r * row + (w.v0 + c) * col] : 0.0f;
+      for (int c = 0; c < NV; ++c) {
+        s[c / 32][c % 32] = c < cols ? *src : 0.0f;
+        src += col;
+      }
     }
     bool ok = true;
     for (int i = 0; i <= chunks && ok; ++i) {
@@ -763,8 +784,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         ok = __all_sync(0xffffffffu, bar_wait(&u_full, (i - 1) & 1, &failed));
         if (!ok) break;
         tc_after();
-        const int m = static_cast<int>(imin(C, w.end - (w.begin + int64_t(i - 1) * C)));
-        const float keep = decay_pow(w.a, float(m));
+        const int left = w.end - (w.begin + (i - 1) * C);
+        const float keep = dpow[left < C ? left : C];
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
           float x[8];
@@ -829,41 +850,23 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     }
   } else if (warp == 1) {
     give_registers<40>();
-    // ---- loads
-    const CUtensorMap* map = maps.map[w.ji];
-    const Source q(map, job.qs, w.h / job.q_group, w.b), k(map + 1, job.ks, w.h / job.k_group, w.b),
-        v(map + 2, job.vs, w.h / job.v_group, w.b);
+    // ---- loads: an operand's buffer is loaded again as soon as its own last product has ended
     const bool one = elect_one();
-    // an operand's buffer is loaded again as soon as its own last product has ended
-    int issued = 0;  // loads begun, three a chunk: K, Q, V
+    int issued = first_loads;
     bool ok = true;
     for (; issued < 3 * chunks; ++issued) {
       const int i = issued / 3, which = issued % 3, st = i % S;
       uint64_t* empty = which == 0 ? k_empty : (which == 1 ? q_empty : v_empty);
-      ok = __all_sync(0xffffffffu, i < S || bar_wait(&empty[st], (i / S - 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&empty[st], (i / S - 1) & 1, &failed));
       if (!ok) break;
-      if (one) {
-        const int64_t l0 = w.begin + int64_t(i) * C;
-        const int64_t token = job.reverse ? w.n - C - l0 : l0;
-        if (which == 2) {
-          bar_expect(&v_in[st], kPanel);
-          v.template load<C>(base + Z::v + st * kPanel, w.v0, 1, token, &v_in[st]);
-        } else {
-          uint64_t* bar = which == 0 ? &k_full[st] : &q_full[st];
-          bar_expect(bar, Z::panels * kPanel);
-          (which == 0 ? k : q).template load<C>(
-              base + (which == 0 ? Z::k : Z::q) + st * Z::panels * kPanel, 0, Z::panels, token, bar);
-        }
-      }
+      if (one) load(issued);
       __syncwarp();
     }
-    if (!ok) {  // copies in flight land before the block ends
-      const long long start = clock64();
+    if (!ok || failed) {  // copies in flight land before the block ends
       for (int j = issued > 3 * S ? issued - 3 * S : 0; j < issued; ++j) {
         const int i = j / 3, which = j % 3;
         uint64_t* bar = which == 0 ? k_full : (which == 1 ? q_full : v_in);
-        while (!bar_try(&bar[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
-        }
+        bar_drain(&bar[i % S], (i / S) & 1);
       }
     }
   } else if (warp > 1) {
@@ -878,109 +881,98 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const uint32_t ov = operand(base + Z::v, kPanel);
     const uint32_t os = operand(base + Z::s, kPanel), op = operand(base + Z::parts, kPanel);
     const bool one = elect_one();
-    auto scores = [&](int i) {
-      const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
-      const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
-      const uint32_t d = tmem + kSc + (i & 1) * 128;
+    bool ok = true;
+    for (int i = -1; i < chunks; ++i) {
+      if (i >= 0) {
+        const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
+        const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
+        const uint32_t v = ov + (i % S) * (kPanel / 16);
+        ok = bar_wait(&v_full[0], i & 1, &failed) &&
+             (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (one) {
+          tc_after();
+          issue_update<T, DK, true>(tmem + kU, k, op);
+          tc_commit(&v_free[0]);
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, &failed));
+        if (!ok) break;
+        if (one) {
+          tc_after();
+          issue_update<T, DK, false>(tmem + kU, k + 512, op + 512);
+          tc_commit(&v_free[1]);
+          tc_commit(&u_full);
+          tc_commit(&k_empty[i % S]);
+        }
+        __syncwarp();
+        ok = bar_wait(&s_full, i & 1, &failed) &&
+             (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (one) {
+          tc_after();
+          mma_ss<false>(tmem + kOe, q, os, id_o);
+#pragma unroll
+          for (int j = 1; j < DK / 16; ++j)
+            mma_ss<true>(tmem + kOe, q + j / 4 * (kPanel / 16) + j % 4 * 2, os + j * 128, id_o);
+          tc_commit(&oe_full);
+          tc_commit(&q_empty[i % S]);
+        }
+        __syncwarp();
+        // (o of the chunk before is out: its buffer takes the next scores.  The wait comes before
+        // P V, whose o frees the other buffer: a barrier must not be two phases ahead of who waits
+        // for it.)
+        ok = bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed) &&
+             (i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (one) {
+          tc_after();
+          const uint32_t p = tmem + kSc + (i & 1) * 128;
+          mma_ts<false>(p + kOi, p, v, id_o);
+#pragma unroll
+          for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
+          tc_commit(&o_full);
+          tc_commit(&v_empty[i % S]);
+        }
+        __syncwarp();
+      }
+      const int n = i + 1;
+      if (n == chunks) break;
+      ok = bar_wait(&k_full[n % S], (n / S) & 1, &failed) &&
+           bar_wait(&q_full[n % S], (n / S) & 1, &failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       if (one) {
         tc_after();
+        const uint32_t q = oq + (n % S) * (Z::panels * kPanel / 16);
+        const uint32_t k = ok0 + (n % S) * (Z::panels * kPanel / 16);
+        const uint32_t d = tmem + kSc + (n & 1) * 128;
         mma_ss<false>(d, q, k, id_sc);
 #pragma unroll
         for (int j = 1; j < DK / 16; ++j)
           mma_ss<true>(d, q + j / 4 * (kPanel / 16) + j % 4 * 2, k + j / 4 * (kPanel / 16) + j % 4 * 2,
                        id_sc);
-        tc_commit(&sc_full[i & 1]);
+        tc_commit(&sc_full[n & 1]);
       }
       __syncwarp();
-    };
-    auto ready = [&](int i) {
-      return bar_wait(&k_full[i % S], (i / S) & 1, &failed) &&
-             bar_wait(&q_full[i % S], (i / S) & 1, &failed);
-    };
-    bool ok = true;
-    if (chunks > 0) {
-      ok = __all_sync(0xffffffffu, ready(0));
-      if (ok) scores(0);
-    }
-    for (int i = 0; i < chunks && ok; ++i) {
-      const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
-      const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
-      const uint32_t v = ov + (i % S) * (kPanel / 16);
-      ok = bar_wait(&v_full[0], i & 1, &failed) &&
-           (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (one) {
-        tc_after();
-        issue_update<T, DK, true>(tmem + kU, k, op);
-        tc_commit(&v_free[0]);
-      }
-      __syncwarp();
-      ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, &failed));
-      if (!ok) break;
-      if (one) {
-        tc_after();
-        issue_update<T, DK, false>(tmem + kU, k + 512, op + 512);
-        tc_commit(&v_free[1]);
-        tc_commit(&u_full);
-        tc_commit(&k_empty[i % S]);
-      }
-      __syncwarp();
-      ok = bar_wait(&s_full, i & 1, &failed) &&
-           (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, &failed));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (one) {
-        tc_after();
-        mma_ss<false>(tmem + kOe, q, os, id_o);
-#pragma unroll
-        for (int j = 1; j < DK / 16; ++j)
-          mma_ss<true>(tmem + kOe, q + j / 4 * (kPanel / 16) + j % 4 * 2, os + j * 128, id_o);
-        tc_commit(&oe_full);
-        tc_commit(&q_empty[i % S]);
-      }
-      __syncwarp();
-      // the next chunk's scores go before this one's P V where its operands are there already.
-      // Their buffer held Oi of the chunk before.  (This wait comes before P V, whose o frees the
-      // other buffer: a barrier must not be two phases ahead of who waits for it.)
-      ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
-      if (!ok) break;
-      bool ahead = i + 1 < chunks && bar_test(&k_full[(i + 1) % S], ((i + 1) / S) & 1) &&
-                   bar_test(&q_full[(i + 1) % S], ((i + 1) / S) & 1);
-      ahead = __all_sync(0xffffffffu, ahead);
-      if (ahead) scores(i + 1);
-      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed));
-      if (!ok) break;
-      if (one) {
-        tc_after();
-        const uint32_t p = tmem + kSc + (i & 1) * 128;
-        mma_ts<false>(p + kOi, p, v, id_o);
-#pragma unroll
-        for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
-        tc_commit(&o_full);
-        tc_commit(&v_empty[i % S]);
-      }
-      __syncwarp();
-      if (!ahead && i + 1 < chunks) {
-        ok = __all_sync(0xffffffffu, ready(i + 1));
-        if (ok) scores(i + 1);
-      }
     }
     if (!ok) {  // let the products in flight end before TMEM goes
       if (one) tc_commit(&drain);
       __syncwarp();
-      const long long start = clock64();
-      while (!bar_try(&drain, 0) && clock64() - start < kWaitCycles) {
-      }
+      bar_drain(&drain, 0);
     }
   }
   // rows after the sequence's end
   {
-    const int64_t from = imax(w.begin, w.n);
-    const int64_t cells = (w.row_end - from) * w.vcols;
+    const int from = w.begin > w.n ? w.begin : w.n;
+    const int64_t cells = int64_t(w.row_end - from) * w.vcols;
     for (int64_t i = threadIdx.x; i < cells; i += kThreads) {
+      const unsigned row = unsigned(i) / unsigned(w.vcols), c = unsigned(i) - row * w.vcols;
       const int64_t at = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0 +
-                         (from + i / w.vcols) * job.os[1] + i % w.vcols;
+                         (from + int64_t(row)) * job.os[1] + c;
       if (job.o_wide) static_cast<float*>(job.o)[at] = 0.0f;
       else static_cast<T*>(job.o)[at] = from_acc<T>(0.0f);
     }
@@ -1041,8 +1033,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = tid / 8 + 16 * j;
-        const int64_t age =
-            w.end - job.off - (w.begin + int64_t(i) * R + (job.reverse ? R - 1 - r : r));
+        const int age = w.end - job.off - (w.begin + i * R + (job.reverse ? R - 1 - r : r));
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
       }
       if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
@@ -1060,7 +1051,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       const int r = DK == 128 ? warp * 32 + lane : warp * 16 + (lane & 15);
       const bool in = (DK == 128 || lane < 16) && r < job.dk;
       float* dst = static_cast<float*>(job.seg) +
-                   (w.bh * (call.nseg - 1) + w.seg) * (int64_t(job.dk) * job.dv) +
+                   (int64_t(w.bh) * (call.nseg - 1) + w.seg) * (int64_t(job.dk) * job.dv) +
                    int64_t(r) * job.dv + w.v0;
       const float write = float(job.write);
       for (int g = 0; g < NV; g += 8) {
@@ -1085,8 +1076,8 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       ok = __all_sync(0xffffffffu, i < S || bar_wait(&used[st], (i / S - 1) & 1, &failed));
       if (!ok) break;
       if (one) {
-        const int64_t l0 = w.begin + int64_t(i) * R;
-        const int64_t token = job.reverse ? w.n - R - l0 : l0;
+        const int l0 = w.begin + i * R;
+        const int token = job.reverse ? w.n - R - l0 : l0;
         const uint32_t at = base + st * Z::st_stage;
         bar_expect(&full[st], Z::st_stage);
         k.template load<R>(at, 0, Z::panels, token, &full[st]);
@@ -1095,10 +1086,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       __syncwarp();
     }
     if (!ok) {  // copies in flight land before the block ends
-      const long long start = clock64();
-      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
-        while (!bar_try(&full[i % S], (i / S) & 1) && clock64() - start < kWaitCycles) {
-        }
+      for (int i = issued > S ? issued - S : 0; i < issued; ++i) bar_drain(&full[i % S], (i / S) & 1);
     }
   } else {
     const uint32_t ok0 = operand(base, kStatePanel), op0 = operand(base + Z::st_parts, kStatePanel);
@@ -1120,9 +1108,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     // also after a failed wait: the products in flight end before TMEM goes
     if (one) tc_commit(&done);
     __syncwarp();
-    const long long start = clock64();
-    while (!bar_try(&done, 0) && clock64() - start < kWaitCycles) {
-    }
+    bar_drain(&done, 0);
   }
   tc_before();
   __syncthreads();
@@ -1179,13 +1165,14 @@ template <typename T, int DK>
 int launch_as(const Call& call, const Maps& maps, bool states, cudaStream_t stream) {
   auto kernel = states ? linattn_tc_state_kernel<T, DK> : linattn_tc_kernel<T, DK>;
   const int64_t heads = call.batch * call.heads;
-  const int64_t grid = heads * call.tiles * (states ? call.nseg - 1 : call.nseg);
+  const dim3 grid(static_cast<unsigned>(call.tiles), static_cast<unsigned>(heads),
+                  static_cast<unsigned>(states ? call.nseg - 1 : call.nseg));
   int* error = device_error_flag();
   if (error == nullptr) return FDWT_ERR_CUDA;
   int st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
   if (st == FDWT_OK) st = pre_launch(stream);
   if (st != FDWT_OK) return st;
-  kernel<<<static_cast<unsigned>(grid), states ? kStateThreads : kThreads,
+  kernel<<<grid, states ? kStateThreads : kThreads,
            states ? Smem<T, DK>::st_bytes : Smem<T, DK>::bytes, stream>>>(call, maps, error);
   return launch_status();
 }
@@ -1197,7 +1184,7 @@ bool tc_supports(int dtype, const Call& call) {
   if (call.length > INT32_MAX - 2 * C || call.batch > INT32_MAX || encoder() == nullptr) return false;
   for (int j = 0; j < call.jobs; ++j) {
     const Job& job = call.job[j];
-    if (job.dk > 128 || !job.q_vec || !job.k_vec || !job.v_vec) return false;
+    if (job.dk > 128 || !job.q_vec || !job.k_vec || !job.v_vec || !job.o_vec) return false;
     // tensor maps: no broadcast tokens, no negative strides, strides below 2^40 bytes
     for (const int64_t* s : {job.qs, job.ks, job.vs}) {
       if (call.length > 1 && s[1] == 0) return false;
