@@ -882,11 +882,12 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const uint32_t os = operand(base + Z::s, kPanel), op = operand(base + Z::parts, kPanel);
     const bool one = elect_one();
     bool ok = true;
+    // each turn: U, Oe of chunk i, the scores of chunk i + 1, Oi of chunk i (turn -1: the scores
+    // alone), so that P of the next chunk is formed beside the rest
     for (int i = -1; i < chunks; ++i) {
       if (i >= 0) {
         const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
         const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
-        const uint32_t v = ov + (i % S) * (kPanel / 16);
         ok = bar_wait(&v_full[0], i & 1, &failed) &&
              (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
         ok = __all_sync(0xffffffffu, ok);
@@ -921,41 +922,44 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           tc_commit(&q_empty[i % S]);
         }
         __syncwarp();
-        // (o of the chunk before is out: its buffer takes the next scores.  The wait comes before
-        // P V, whose o frees the other buffer: a barrier must not be two phases ahead of who waits
-        // for it.)
-        ok = bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed) &&
-             (i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+        // Oi of the chunk before is out: its buffer takes the next scores.  (The wait is also due
+        // before P V, whose o frees the other buffer: no barrier may be two phases ahead of who
+        // waits for it.)
+        ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+        if (!ok) break;
+      }
+      const int n = i + 1;
+      if (n < chunks) {
+        ok = bar_wait(&k_full[n % S], (n / S) & 1, &failed) &&
+             bar_wait(&q_full[n % S], (n / S) & 1, &failed);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (one) {
           tc_after();
-          const uint32_t p = tmem + kSc + (i & 1) * 128;
-          mma_ts<false>(p + kOi, p, v, id_o);
+          const uint32_t q = oq + (n % S) * (Z::panels * kPanel / 16);
+          const uint32_t k = ok0 + (n % S) * (Z::panels * kPanel / 16);
+          const uint32_t d = tmem + kSc + (n & 1) * 128;
+          mma_ss<false>(d, q, k, id_sc);
 #pragma unroll
-          for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
-          tc_commit(&o_full);
-          tc_commit(&v_empty[i % S]);
+          for (int j = 1; j < DK / 16; ++j)
+            mma_ss<true>(d, q + j / 4 * (kPanel / 16) + j % 4 * 2,
+                         k + j / 4 * (kPanel / 16) + j % 4 * 2, id_sc);
+          tc_commit(&sc_full[n & 1]);
         }
         __syncwarp();
       }
-      const int n = i + 1;
-      if (n == chunks) break;
-      ok = bar_wait(&k_full[n % S], (n / S) & 1, &failed) &&
-           bar_wait(&q_full[n % S], (n / S) & 1, &failed);
-      ok = __all_sync(0xffffffffu, ok);
+      if (i < 0) continue;
+      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed));
       if (!ok) break;
       if (one) {
         tc_after();
-        const uint32_t q = oq + (n % S) * (Z::panels * kPanel / 16);
-        const uint32_t k = ok0 + (n % S) * (Z::panels * kPanel / 16);
-        const uint32_t d = tmem + kSc + (n & 1) * 128;
-        mma_ss<false>(d, q, k, id_sc);
+        const uint32_t v = ov + (i % S) * (kPanel / 16);
+        const uint32_t p = tmem + kSc + (i & 1) * 128;
+        mma_ts<false>(p + kOi, p, v, id_o);
 #pragma unroll
-        for (int j = 1; j < DK / 16; ++j)
-          mma_ss<true>(d, q + j / 4 * (kPanel / 16) + j % 4 * 2, k + j / 4 * (kPanel / 16) + j % 4 * 2,
-                       id_sc);
-        tc_commit(&sc_full[n & 1]);
+        for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
+        tc_commit(&o_full);
+        tc_commit(&v_empty[i % S]);
       }
       __syncwarp();
     }
