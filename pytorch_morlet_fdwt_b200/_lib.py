@@ -174,6 +174,12 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current stream's handle by device index, without the Stream object around it (2 us a call);
+# through the object where this torch does not offer it.
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 _NO_GUARD = contextlib.nullcontext()
 
 

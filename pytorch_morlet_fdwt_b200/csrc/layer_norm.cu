@@ -14,33 +14,121 @@
 namespace fdwt {
 namespace {
 
-// One aligned group of V elements of type T, loaded and stored as a whole.
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
-  T v[V];
-};
-
-template <typename A> __device__ __forceinline__ A warp_sum(A v) {
+// A group of V neighbouring elements, loaded and stored as a whole (16 bytes, two elements, or one),
+// and its values in the type of the sums.
+template <typename T, int V> struct Group {
+  struct alignas(sizeof(T) * V) Raw {
+    T v[V];
+  };
+  using A = typename AccOf<T>::type;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const Raw*>(p);
+  }
+  static __device__ __forceinline__ void values(const Raw& r, A* x) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+    for (int j = 0; j < V; ++j) x[j] = to_acc(r.v[j]);
+  }
+  static __device__ __forceinline__ void store(T* p, const A* x) {
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = from_acc<T>(x[j]);
+    *reinterpret_cast<Raw*>(p) = r;
+  }
+};
+// 16-bit types in pairs: one conversion instruction a pair.
+template <typename T> struct Half2;
+template <> struct Half2<__nv_bfloat16> {
+  static __device__ __forceinline__ void split(uint32_t u, float* x) {
+    x[0] = __uint_as_float(u << 16);
+    x[1] = __uint_as_float(u & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t join(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+};
+template <> struct Half2<__half> {
+  static __device__ __forceinline__ void split(uint32_t u, float* x) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    x[0] = f.x;
+    x[1] = f.y;
+  }
+  static __device__ __forceinline__ uint32_t join(float a, float b) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+};
+template <typename T> struct Group16 {
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const uint4*>(p);
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float* x) {
+    Half2<T>::split(r.x, x);
+    Half2<T>::split(r.y, x + 2);
+    Half2<T>::split(r.z, x + 4);
+    Half2<T>::split(r.w, x + 6);
+  }
+  static __device__ __forceinline__ void store(T* p, const float* x) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(Half2<T>::join(x[0], x[1]), Half2<T>::join(x[2], x[3]),
+                   Half2<T>::join(x[4], x[5]), Half2<T>::join(x[6], x[7]));
+  }
+};
+template <typename T> struct Group4 {
+  using Raw = uint32_t;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const uint32_t*>(p);
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float* x) { Half2<T>::split(r, x); }
+  static __device__ __forceinline__ void store(T* p, const float* x) {
+    *reinterpret_cast<uint32_t*>(p) = Half2<T>::join(x[0], x[1]);
+  }
+};
+template <> struct Group<__half, 2> : Group4<__half> {};
+template <> struct Group<__nv_bfloat16, 2> : Group4<__nv_bfloat16> {};
+template <> struct Group<__half, 8> : Group16<__half> {};
+template <> struct Group<__nv_bfloat16, 8> : Group16<__nv_bfloat16> {};
+
+// V parameters (weight or bias) as values; their group is 16 or 32 bytes.
+template <typename P, int V, typename A>
+__device__ __forceinline__ void load_params(const P* p, A* x) {
+  if constexpr (sizeof(P) * V == 32) {
+    float y[4];
+    Group<float, 4>::values(Group<float, 4>::load(p), y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = y[j];
+    Group<float, 4>::values(Group<float, 4>::load(p + 4), y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 + j] = y[j];
+  } else {
+    Group<P, V>::values(Group<P, V>::load(p), x);
+  }
 }
 
-// Sum of N values over the threads of a row (blockDim.x of them; a multiple of 32).  `slot`
-// points at 32 * N cells of shared memory; consecutive calls take different slots, so that one
-// barrier a call is enough.
+// Sums of N values over the threads of a row: blockDim.x of them, either a power of two up to 32
+// (lanes of one warp) or whole warps.  `slot` points at 32 N cells of shared memory; consecutive
+// calls take different slots, so that one barrier a call is enough.
 template <typename A, int N>
 __device__ __forceinline__ void row_sum(A (&v)[N], A* slot) {
+  const int lanes = blockDim.x < 32 ? blockDim.x : 32;
+  for (int o = lanes / 2; o > 0; o >>= 1) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if (blockDim.x == 32) return;
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  if (blockDim.x <= 32) return;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) slot[i * 32 + warp] = v[i];
+    for (int i = 0; i < N; ++i) slot[warp * N + i] = v[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? slot[i * 32 + lane] : A(0));
+  for (int i = 0; i < N; ++i) v[i] = A(0);
+  for (int k = 0; k < warps; ++k) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += slot[k * N + i];
+  }
 }
 
 template <typename A> __device__ __forceinline__ A inv_sqrt(A v);
@@ -48,68 +136,83 @@ template <> __device__ __forceinline__ float inv_sqrt(float v) { return 1.0f / s
 template <> __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
 
 // ------------------------------------------------------------------------------ forward
+// Threads a block may have when each keeps e elements.
+constexpr int fwd_max_threads(int e) { return e <= 16 ? 1024 : (e <= 32 ? 512 : 256); }
+
 // A row is held by blockDim.x threads, IT groups of V elements each (group i of thread t starts
-// at (i * blockDim.x + t) * V: neighbouring lanes read neighbouring groups).  blockDim.y rows a
-// block: more than one only where a single warp holds a row.
+// at (i * blockDim.x + t) * V: neighbouring lanes read neighbouring groups), blockDim.y rows a
+// block (more than one only where a row has at most a warp).
 template <typename T, typename P, int V, int IT>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(fwd_max_threads(V * IT))
 layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
                       const P* __restrict__ bias, T* __restrict__ y,
                       typename AccOf<T>::type* __restrict__ stats, int64_t rows, int dim,
                       typename AccOf<T>::type eps) {
   using A = typename AccOf<T>::type;
+  using G = Group<T, V>;
   __shared__ A slots[2][32];
-  const int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (row >= rows) return;  // whole warps: blockDim.y > 1 only with one warp a row
-  const T* xr = x + row * dim;
-  Pack<T, V> in[IT];
-  A sum[1] = {A(0)};
+  int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  const bool in = row < rows;
+  if (!in) row = rows - 1;  // the lanes of a warp stay together
+  const T* xr = x + row * dim + threadIdx.x * V;
+  const int step = blockDim.x * V, left = dim - threadIdx.x * V;
+  typename G::Raw raw[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+    if (i * step < left) raw[i] = G::load(xr + i * step);
+  A v[IT * V];
+  A sum[1] = {A(0)}, part[4] = {A(0), A(0), A(0), A(0)};
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * V;
-    if (c < dim) {
-      in[i] = *reinterpret_cast<const Pack<T, V>*>(xr + c);
+    if (i * step < left) {
+      G::values(raw[i], v + i * V);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[0] += to_acc(in[i].v[j]);
+      for (int j = 0; j < V; ++j) part[(i * V + j) % 4] += v[i * V + j];
     }
   }
+  sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
   row_sum(sum, slots[0]);
   const A mean = sum[0] / A(dim);
-  A sq[1] = {A(0)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) part[k] = A(0);
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * V;
-    if (c < dim) {
+    if (i * step < left) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const A d = to_acc(in[i].v[j]) - mean;
-        sq[0] += d * d;
+        A& d = v[i * V + j];
+        d -= mean;
+        part[(i * V + j) % 4] += d * d;
       }
     }
   }
-  row_sum(sq, slots[1]);
-  const A rstd = inv_sqrt(sq[0] / A(dim) + eps);
+  sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
+  row_sum(sum, slots[1]);
+  const A rstd = inv_sqrt(sum[0] / A(dim) + eps);
+  if (!in) return;
   if (stats != nullptr && threadIdx.x == 0) {
     stats[2 * row] = mean;
     stats[2 * row + 1] = rstd;
   }
-  T* yr = y + row * dim;
+  T* yr = y + row * dim + threadIdx.x * V;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * V;
-    if (c < dim) {
-      Pack<P, V> w, b;
-      if (weight != nullptr) w = *reinterpret_cast<const Pack<P, V>*>(weight + c);
-      if (bias != nullptr) b = *reinterpret_cast<const Pack<P, V>*>(bias + c);
-      Pack<T, V> out;
+    if (i * step < left) {
+      A p[V];
+      A* d = v + i * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        A h = (to_acc(in[i].v[j]) - mean) * rstd;
-        if (weight != nullptr) h *= A(to_acc(w.v[j]));
-        if (bias != nullptr) h += A(to_acc(b.v[j]));
-        out.v[j] = from_acc<T>(h);
+      for (int j = 0; j < V; ++j) d[j] *= rstd;
+      if (weight != nullptr) {
+        load_params<P, V>(weight + threadIdx.x * V + i * step, p);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] *= p[j];
       }
-      *reinterpret_cast<Pack<T, V>*>(yr + c) = out;
+      if (bias != nullptr) {
+        load_params<P, V>(bias + threadIdx.x * V + i * step, p);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] += p[j];
+      }
+      G::store(yr + i * step, d);
     }
   }
 }
@@ -155,8 +258,7 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, const P* __restrict__ weight
 // sums in shared memory (blockDim.y > 1) and writing one (dw, db) partial row.  The partial rows
 // are added in a fixed order by layer_norm_params_kernel: no atomics, the same bits every run.
 // The next row's x and dy are loaded before the current row's sums are joined.
-// Registers: 2 E sums, E weights and the current and next rows' groups (E / 2 each at 16 bits),
-// E = V IT elements a thread; h and g are formed twice rather than kept.
+// Registers, E = V IT elements a thread: 2 E sums, E weights, 2 E values, and the next row's groups.
 template <typename A> constexpr int bwd_max_threads(int e) {
   const int words = e * int(sizeof(A) / 4);
   return words <= 4 ? 1024 : (words <= 16 ? 512 : 256);
@@ -169,123 +271,117 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                       const typename AccOf<T>::type* __restrict__ stats, T* __restrict__ dx,
                       typename AccOf<T>::type* __restrict__ partial, int64_t rows, int dim) {
   using A = typename AccOf<T>::type;
+  using G = Group<T, V>;
   __shared__ A slots[2][64];
-  extern __shared__ unsigned char smem_raw[];
-  A* joined = reinterpret_cast<A*>(smem_raw);  // [blockDim.y - 1][2][dim], only blockDim.y > 1
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  A* joined = reinterpret_cast<A*>(smem_raw);  // [blockDim.y][2][dim], only blockDim.y > 1
 
+  const int col = threadIdx.x * V, step = blockDim.x * V, left = dim - col;
   A dw[IT * V], db[IT * V], w[IT * V];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * V;
-    Pack<P, V> pw;
-    if (weight != nullptr && c < dim) pw = *reinterpret_cast<const Pack<P, V>*>(weight + c);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      dw[i * V + j] = db[i * V + j] = A(0);
-      w[i * V + j] = (weight != nullptr && c < dim) ? A(to_acc(pw.v[j])) : A(1);
-    }
+  for (int e = 0; e < IT * V; ++e) {
+    dw[e] = db[e] = A(0);
+    w[e] = A(1);
   }
-  const int64_t step = int64_t(gridDim.x) * blockDim.y;
+  if (weight != nullptr) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      if (i * step < left) load_params<P, V>(weight + col + i * step, w + i * V);
+  }
+  const int64_t rows_step = int64_t(gridDim.x) * blockDim.y;
+  // rows of the block's last round past the end are read as the last row and left out of the sums
   int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  Pack<T, V> nx[IT], ny[IT];
+  const int64_t rounds = (rows - int64_t(blockIdx.x) * blockDim.y + rows_step - 1) / rows_step;
+  typename G::Raw nx[IT], ny[IT];
+  A mean, rstd;
   auto fetch = [&](int64_t r) {
+    if (r >= rows) r = rows - 1;
+    const T* px = x + r * dim + col;
+    const T* py = dy + r * dim + col;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * V;
-      if (c < dim) {
-        nx[i] = *reinterpret_cast<const Pack<T, V>*>(x + r * dim + c);
-        ny[i] = *reinterpret_cast<const Pack<T, V>*>(dy + r * dim + c);
+      if (i * step < left) {
+        nx[i] = G::load(px + i * step);
+        ny[i] = G::load(py + i * step);
       }
     }
+    mean = stats[2 * r];
+    rstd = stats[2 * r + 1];
   };
-  A mean = A(0), rstd = A(0);
-  if (row < rows) {
-    fetch(row);
-    mean = stats[2 * row];
-    rstd = stats[2 * row + 1];
-  }
-  int parity = 0;
-  for (; row < rows; row += step, parity ^= 1) {
-    Pack<T, V> cx[IT], cy[IT];
+  fetch(row);
+  const A inv = A(1) / A(dim);
+  for (int64_t k = 0; k < rounds; ++k, row += rows_step) {
+    const bool in = row < rows;
     const A m = mean, r = rstd;
-    A s[2] = {A(0), A(0)};
+    A h[IT * V], g[IT * V];
+    A s[2] = {A(0), A(0)}, s1[2] = {A(0), A(0)};
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * V;
-      if (c < dim) {
+      if (i * step < left) {
+        A d[V];
+        G::values(nx[i], h + i * V);
+        G::values(ny[i], d);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int e = i * V + j;
-          const A d = to_acc(ny[i].v[j]);
-          const A h = (to_acc(nx[i].v[j]) - m) * r;
-          const A g = d * w[e];
-          dw[e] += d * h;
-          db[e] += d;
-          s[0] += g;
-          s[1] += g * h;
+          h[e] = (h[e] - m) * r;
+          if (!in) d[j] = A(0);
+          g[e] = d[j] * w[e];
+          dw[e] += d[j] * h[e];
+          db[e] += d[j];
+          s[e % 2] += g[e];
+          s1[e % 2] += g[e] * h[e];
         }
-        cx[i] = nx[i];
-        cy[i] = ny[i];
       }
     }
-    const int64_t next = row + step;
-    if (next < rows) {
-      fetch(next);
-      mean = stats[2 * next];
-      rstd = stats[2 * next + 1];
-    }
-    row_sum(s, slots[parity]);
-    const A mg = s[0] / A(dim), mgh = s[1] / A(dim);
-    if (dx != nullptr) {
+    if (k + 1 < rounds) fetch(row + rows_step);
+    s[0] += s[1];
+    s[1] = s1[0] + s1[1];
+    row_sum(s, slots[k & 1]);
+    const A mg = s[0] * inv, mgh = s[1] * inv;
+    if (dx != nullptr && in) {
+      T* out = dx + row * dim + col;
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const int c = (i * blockDim.x + threadIdx.x) * V;
-        if (c < dim) {
-          Pack<T, V> out;
+        if (i * step < left) {
+          A d[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const A h = (to_acc(cx[i].v[j]) - m) * r;
-            const A g = to_acc(cy[i].v[j]) * w[i * V + j];
-            out.v[j] = from_acc<T>(r * (g - mg - h * mgh));
-          }
-          *reinterpret_cast<Pack<T, V>*>(dx + row * dim + c) = out;
+          for (int j = 0; j < V; ++j) d[j] = r * (g[i * V + j] - mg - h[i * V + j] * mgh);
+          G::store(out + i * step, d);
         }
       }
     }
   }
   if (partial == nullptr) return;
-  if (blockDim.y > 1) {
-    if (threadIdx.y > 0) {
-      A* mine = joined + int64_t(threadIdx.y - 1) * 2 * dim;
+  if (blockDim.y > 1) {  // join the block's rows in shared memory, a fixed order
+    A* mine = joined + int64_t(threadIdx.y) * 2 * dim;
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int c = (i * blockDim.x + threadIdx.x) * V;
-        if (c < dim) {
+    for (int i = 0; i < IT; ++i) {
+      if (i * step < left) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            mine[c + j] = dw[i * V + j];
-            mine[dim + c + j] = db[i * V + j];
-          }
+        for (int j = 0; j < V; ++j) {
+          mine[col + i * step + j] = dw[i * V + j];
+          mine[dim + col + i * step + j] = db[i * V + j];
         }
       }
     }
     __syncthreads();
-    if (threadIdx.y > 0) return;
+    const int threads = blockDim.x * blockDim.y;
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * dim; c += threads) {
+      A a = joined[c];
+      for (int y = 1; y < blockDim.y; ++y) a += joined[int64_t(y) * 2 * dim + c];
+      partial[int64_t(blockIdx.x) * 2 * dim + c] = a;
+    }
+    return;
   }
-  A* out = partial + int64_t(blockIdx.x) * 2 * dim;
+  A* out = partial + int64_t(blockIdx.x) * 2 * dim + col;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * V;
-    if (c < dim) {
+    if (i * step < left) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        A a = dw[i * V + j], b = db[i * V + j];
-        for (int k = 1; k < blockDim.y; ++k) {
-          a += joined[int64_t(k - 1) * 2 * dim + c + j];
-          b += joined[int64_t(k - 1) * 2 * dim + dim + c + j];
-        }
-        out[c + j] = a;
-        out[dim + c + j] = b;
+        out[i * step + j] = dw[i * V + j];
+        out[dim + i * step + j] = db[i * V + j];
       }
     }
   }
@@ -369,67 +465,79 @@ struct Shape {
   int threads, items, rows;
 };
 
-// A thread takes about 8 elements where that fits (enough loads in flight, few threads to join);
-// a warp holds a row of up to `warp_elems` elements a lane without any barrier; more items only
-// where the row needs them.  False: the row does not fit (the long forms take it).
-inline bool row_shape(int64_t groups, int v, int warp_elems, int (*limit)(int), Shape* s) {
-  const int most = v > 1 ? 4 : 16;
-  if (groups * v <= 32 * warp_elems) {
-    int items = 1;
-    while (32 * items < groups) items *= 2;
-    if (items <= most) {
-      *s = {32, items, 8};
-      return true;
-    }
+// Lanes and groups of a row that one warp holds: with few elements a row several rows share a warp
+// (no lanes idle), with many a lane takes more (no barrier, more loads in flight).
+inline bool warp_shape(int64_t groups, int v, int most_items, Shape* s, int block) {
+  int threads = 1, items = 1;
+  while (threads * items < groups) {
+    // 32 bytes a row and load keep the sectors whole; then items up to about 8 elements a lane,
+    // then lanes, then items again
+    if (threads < 4 || (threads < 32 && items * v >= 8)) threads *= 2;
+    else if (items * v < 8) items *= 2;
+    else items *= 2;
+    if (items > most_items) return false;
   }
-  for (int items = v >= 8 ? 1 : 8 / v > most ? most : 8 / v; items <= most; items *= 2) {
+  *s = {threads, items, block / threads};
+  return true;
+}
+inline bool forward_shape(int64_t groups, int v, int acc_size, Shape* s) {
+  if (warp_shape(groups, v, v <= 2 ? 8 : (acc_size == 8 ? 32 : 64) / v, s, 128)) return true;
+  for (int items = v >= 8 ? 2 : (v <= 2 ? 8 : 16 / v); items * v <= 32; items *= 2) {
     const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
-    if (threads <= limit(v * items)) {
+    if (threads <= fwd_max_threads(items * v)) {
       *s = {static_cast<int>(threads), items, 1};
       return true;
     }
   }
   return false;
 }
-inline int forward_limit(int) { return 1024; }
-template <typename A> int backward_limit(int e) { return bwd_max_threads<A>(e); }
-inline bool forward_shape(int64_t groups, int v, Shape* s) {
-  return row_shape(groups, v, v > 1 ? 32 : 16, forward_limit, s);
-}
 template <typename A> bool backward_shape(int64_t groups, int v, Shape* s) {
-  return row_shape(groups, v, 64 / int(sizeof(A)), backward_limit<A>, s);
+  if (warp_shape(groups, v, (sizeof(A) == 8 ? 8 : 16) / v, s, 256)) return true;
+  for (int items = v >= 8 ? 1 : 8 / v; items * v <= 32; items *= 2) {
+    const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
+    if (threads <= bwd_max_threads<A>(v * items)) {
+      *s = {static_cast<int>(threads), items, 1};
+      return true;
+    }
+  }
+  return false;
 }
 
-// fn(std::integral_constant<int, items>) for the items that row_shape returns.
-template <int V, typename F> int with_items(int items, F fn) {
+// fn(std::integral_constant<int, items>); items V at most `MOST` elements.
+template <int V, int MOST, typename F> int with_items(int items, F fn) {
   switch (items) {
     case 1: return fn(std::integral_constant<int, 1>{});
     case 2: return fn(std::integral_constant<int, 2>{});
-    case 4: return fn(std::integral_constant<int, 4>{});
+    case 4:
+      if constexpr (4 * V <= MOST) return fn(std::integral_constant<int, 4>{});
+      break;
+    case 8:
+      if constexpr (8 * V <= MOST) return fn(std::integral_constant<int, 8>{});
+      break;
+    case 16:
+      if constexpr (16 * V <= MOST) return fn(std::integral_constant<int, 16>{});
+      break;
+    case 32:
+      if constexpr (32 * V <= MOST) return fn(std::integral_constant<int, 32>{});
+      break;
     default: break;
-  }
-  if constexpr (V == 1) {
-    if (items == 8) return fn(std::integral_constant<int, 8>{});
-    return fn(std::integral_constant<int, 16>{});
   }
   return FDWT_ERR_INVALID;
 }
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T, typename P, int V>
 int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const void* b, double eps,
               void* y, void* stats, bool* done, cudaStream_t stream) {
   using A = typename AccOf<T>::type;
   Shape s;
-  if (!forward_shape(dim / V, V, &s)) return FDWT_OK;
+  if (!forward_shape(dim / V, V, sizeof(A), &s)) return FDWT_OK;
   *done = true;
   const dim3 block(s.threads, s.rows);
   const int64_t grid = cdiv(rows, s.rows);
   if (grid > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   const int st = pre_launch(stream);
   if (st != FDWT_OK) return st;
-  return with_items<V>(s.items, [&](auto items) {
+  return with_items<V, (sizeof(A) == 8 ? 32 : 64)>(s.items, [&](auto items) {
     constexpr int IT = decltype(items)::value;
     layer_norm_fwd_kernel<T, P, V, IT><<<static_cast<unsigned>(grid), block, 0, stream>>>(
         static_cast<const T*>(x), static_cast<const P*>(w), static_cast<const P*>(b),
@@ -439,6 +547,16 @@ int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const voi
   });
 }
 
+// Elements of a group: 16 bytes, two elements or one, whatever rows and pointers are aligned to.
+template <typename T, typename... Ptr> int group_of(int64_t dim, Ptr... p) {
+  uintptr_t all = 0;
+  for (const void* q : {static_cast<const void*>(p)...}) all |= reinterpret_cast<uintptr_t>(q);
+  constexpr int V = 16 / sizeof(T);
+  if (dim % V == 0 && all % 16 == 0) return V;
+  if (V > 2 && dim % 2 == 0 && all % (2 * sizeof(T)) == 0) return 2;
+  return 1;
+}
+
 template <typename T, typename P>
 int forward(int64_t rows, int64_t dim, const void* x, const void* w, const void* b, double eps,
             void* y, void* stats, cudaStream_t stream) {
@@ -446,13 +564,11 @@ int forward(int64_t rows, int64_t dim, const void* x, const void* w, const void*
   constexpr int V = 16 / sizeof(T);
   bool done = false;
   int st;
-  if (dim % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b)) {
-    st = forward_v<T, P, V>(rows, dim, x, w, b, eps, y, stats, &done, stream);
-    if (done) return st;
-  } else {
-    st = forward_v<T, P, 1>(rows, dim, x, w, b, eps, y, stats, &done, stream);
-    if (done) return st;
-  }
+  const int v = group_of<T>(dim, x, y, w, b);
+  if (v == V) st = forward_v<T, P, V>(rows, dim, x, w, b, eps, y, stats, &done, stream);
+  else if (v == 2) st = forward_v<T, P, 2>(rows, dim, x, w, b, eps, y, stats, &done, stream);
+  else st = forward_v<T, P, 1>(rows, dim, x, w, b, eps, y, stats, &done, stream);
+  if (done) return st;
   if (rows > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   st = pre_launch(stream);
   if (st != FDWT_OK) return st;
@@ -462,25 +578,23 @@ int forward(int64_t rows, int64_t dim, const void* x, const void* w, const void*
   return launch_status();
 }
 
-// Blocks of the backward pass: what is resident at once, at most one a row group.  The number
-// of partial rows, so also a part of the workspace's size.
-inline int64_t backward_blocks(int64_t rows, const Shape& s) {
-  const int resident = s.rows > 1 ? 4 : (s.threads <= 256 ? 4 : (s.threads <= 512 ? 2 : 1));
+// Blocks of the backward pass: `resident` a multiprocessor, at most one a row group.  Their number
+// is that of the partial rows, so the workspace takes the most that can be resident.
+inline int64_t backward_blocks(int64_t rows, const Shape& s, int resident) {
   return imin(cdiv(rows, s.rows), int64_t(sm_count()) * resident);
 }
-constexpr int kLongParts = 64;
+constexpr int kLongParts = 64, kMostResident = 8;
 
-// The largest of the counts that the aligned and the unaligned form use, so that the query needs
-// no pointers.
+// The largest of the counts that the forms for every alignment use: the query has no pointers.
 inline int64_t backward_parts(int dtype, int64_t rows, int64_t dim) {
   const int v = static_cast<int>(16 / dtype_size(dtype));
   int64_t parts = 0;
-  for (int per : {v, 1}) {
+  for (int per : {v, 2, 1}) {
     if (per > 1 && dim % per != 0) continue;
     Shape s;
     const bool fits = dtype == FDWT_F64 ? backward_shape<double>(dim / per, per, &s)
                                         : backward_shape<float>(dim / per, per, &s);
-    parts = imax(parts, fits ? backward_blocks(rows, s) : imin(rows, kLongParts));
+    parts = imax(parts, fits ? backward_blocks(rows, s, kMostResident) : imin(rows, kLongParts));
   }
   return parts;
 }
@@ -504,16 +618,21 @@ int backward_v(int64_t rows, int64_t dim, const void* dy, const void* x, const v
   using A = typename AccOf<T>::type;
   Shape s;
   if (!backward_shape<A>(dim / V, V, &s)) return FDWT_OK;
-  const int64_t grid = backward_blocks(rows, s);
-  *parts = grid;
   const dim3 block(s.threads, s.rows);
-  const size_t smem = partial == nullptr ? 0 : size_t(s.rows - 1) * 2 * dim * sizeof(A);
-  return with_items<V>(s.items, [&](auto items) -> int {
+  const size_t smem =
+      partial == nullptr || s.rows == 1 ? 0 : size_t(s.rows) * 2 * dim * sizeof(A);
+  return with_items<V, 32>(s.items, [&](auto items) -> int {
     constexpr int IT = decltype(items)::value;
     auto kernel = layer_norm_bwd_kernel<T, P, V, IT>;
+    int resident = 1;
     int st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
+    if (st == FDWT_OK)
+      st = occupancy(reinterpret_cast<const void*>(kernel), s.threads * s.rows, smem, &resident);
     if (st == FDWT_OK) st = pre_launch(stream);
     if (st != FDWT_OK) return st;
+    const int64_t grid =
+        backward_blocks(rows, s, resident < kMostResident ? (resident < 1 ? 1 : resident) : kMostResident);
+    *parts = grid;
     kernel<<<static_cast<unsigned>(grid), block, smem, stream>>>(
         static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const P*>(w),
         static_cast<const A*>(stats), static_cast<T*>(dx), static_cast<A*>(partial), rows,
@@ -530,10 +649,10 @@ int backward(int64_t rows, int64_t dim, const void* dy, const void* x, const voi
   void* partial = (dw != nullptr || db != nullptr) ? ws : nullptr;
   int64_t parts = 0;
   int st;
-  if (dim % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(w))
-    st = backward_v<T, P, V>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
-  else
-    st = backward_v<T, P, 1>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
+  const int v = group_of<T>(dim, x, dy, dx, w);
+  if (v == V) st = backward_v<T, P, V>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
+  else if (v == 2) st = backward_v<T, P, 2>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
+  else st = backward_v<T, P, 1>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
   if (st != FDWT_OK) return st;
   if (parts == 0) {  // long rows
     if (rows > INT32_MAX) return FDWT_ERR_UNSUPPORTED;

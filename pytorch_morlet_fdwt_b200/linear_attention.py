@@ -73,16 +73,17 @@ def _check_heads(q, k, v, log_decay, names):
     code = _lib.dtype_code(q.dtype)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.dim() != len(names) or k.dim() != q.dim() or v.dim() != q.dim():
-        raise ValueError(f"expected q, k, v of shape ({', '.join(names)}), got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape[:-2] != q.shape[:-2] or v.shape[:-1] != k.shape[:-1]:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != len(names) or len(ks) != len(qs) or len(vs) != len(qs):
+        raise ValueError(f"expected q, k, v of shape ({', '.join(names)}), got {tuple(qs)}, "
+                         f"{tuple(ks)}, {tuple(vs)}")
+    if ks[:-2] != qs[:-2] or vs[:-1] != ks[:-1]:
         raise ValueError(f"q, k and v must agree in {', '.join(names[:-2])} and k and v in their "
-                         f"heads, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    heads, dk = q.shape[-2:]
-    kv_heads, dv = v.shape[-2:]
-    if k.shape[-1] != dk:
-        raise ValueError(f"q and k must have one head size, got {dk} and {k.shape[-1]}")
+                         f"heads, got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    heads, dk = qs[-2:]
+    kv_heads, dv = vs[-2:]
+    if ks[-1] != dk:
+        raise ValueError(f"q and k must have one head size, got {dk} and {ks[-1]}")
     if not (1 <= dk <= _MAX_HEAD and 1 <= dv <= _MAX_HEAD):
         raise ValueError(f"head sizes must be 1 to {_MAX_HEAD}, got {dk} and {dv}")
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
@@ -126,8 +127,9 @@ def _forward(q, k, v, log_decay, initial, lengths, scale, sizes):
             desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
             None if initial is None else initial.data_ptr(),
             None if lengths is None else lengths.data_ptr(), out.data_ptr(), final.data_ptr(),
-            None if ws is None else ws.data_ptr(), nws, _lib.stream_of(dev))
-    _lib.check(st, "fdwt_linattn_forward")
+            None if ws is None else ws.data_ptr(), nws, _lib.raw_stream(dev.index))
+    if st:
+        _lib.check(st, "fdwt_linattn_forward")
     if config.check_device_errors:
         _lib.check_device_error("fdwt_linattn_forward")
     return out, final
@@ -171,8 +173,9 @@ class _LinearAttentionFunction(torch.autograd.Function):
                 None if lengths is None else lengths.data_ptr(), d_out.data_ptr(),
                 None if d_final is None else d_final.data_ptr(), dq.data_ptr(), dkk.data_ptr(),
                 dvv.data_ptr(), None if d_initial is None else d_initial.data_ptr(),
-                None if ws is None else ws.data_ptr(), nws, _lib.stream_of(dev))
-        _lib.check(st, "fdwt_linattn_backward")
+                None if ws is None else ws.data_ptr(), nws, _lib.raw_stream(dev.index))
+        if st:
+            _lib.check(st, "fdwt_linattn_backward")
         if config.check_device_errors:
             _lib.check_device_error("fdwt_linattn_backward")
         return dq, dkk, dvv, None, d_initial, None, None, None
@@ -205,7 +208,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     code, heads, kv_heads, dk, dv = sizes
     batch, length = q.shape[:2]
     acc = _acc(q.dtype)
-    log_decay = log_decay.to(acc).contiguous()
+    if log_decay.dtype != acc or not log_decay.is_contiguous():
+        log_decay = log_decay.to(acc).contiguous()
     if initial_state is not None:
         _lib.require_cuda(q, initial_state)
         _check_state(initial_state, (batch, heads, dk, dv), acc)
@@ -250,19 +254,22 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                            "torch.no_grad()")
     if slots is not None:
         slots = _indexes(slots, batch, -1, pool, "slots")
-    log_decay = log_decay.to(acc).contiguous()
+    if log_decay.dtype != acc or not log_decay.is_contiguous():
+        log_decay = log_decay.to(acc).contiguous()
     scale = float(dk) ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
     dev = q.device
     out = torch.empty((batch, heads, dv), device=dev, dtype=q.dtype)
     # (batch, head) strides with an unused token stride between them
-    qs, ks, vs, os = ((t.stride(0), 0, t.stride(1)) for t in (q, k, v, out))
     with _lib.device_guard(dev):
-        _, desc, _, _ = _describe(code, batch, 1, heads, kv_heads, dk, dv, qs, ks, vs, os, scale,
+        _, desc, _, _ = _describe(code, batch, 1, heads, kv_heads, dk, dv,
+                                  (q.stride(0), 0, q.stride(1)), (k.stride(0), 0, k.stride(1)),
+                                  (v.stride(0), 0, v.stride(1)), (heads * dv, 0, dv), scale,
                                   dev.index)
         st = _lib.load().fdwt_linattn_step(
             desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
             state.data_ptr(), pool, None if slots is None else slots.data_ptr(), out.data_ptr(),
-            _lib.stream_of(dev))
-    _lib.check(st, "fdwt_linattn_step")
+            _lib.raw_stream(dev.index))
+    if st:
+        _lib.check(st, "fdwt_linattn_step")
     return out

@@ -10,6 +10,7 @@ for fp64 inputs).
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -26,20 +27,28 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _forward(x, weight, bias, eps: float, codes, want_stats: bool):
-    dim = x.shape[-1]
+    shape = x.shape
+    dim = shape[-1]
     rows = x.numel() // dim
     dev = x.device
     y = torch.empty_like(x)
     stats = None
     if want_stats:
-        acc = torch.float64 if x.dtype == torch.float64 else torch.float32
-        stats = torch.empty((rows, 2), device=dev, dtype=acc)
+        stats = torch.empty((rows, 2), device=dev,
+                            dtype=torch.float64 if codes[0] == 1 else torch.float32)
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_layer_norm_forward(
             codes[0], codes[1], rows, dim, x.data_ptr(), _ptr(weight), _ptr(bias), eps,
-            y.data_ptr(), _ptr(stats), _lib.stream_of(dev))
-    _lib.check(st, "fdwt_layer_norm_forward")
+            y.data_ptr(), _ptr(stats), _lib.raw_stream(dev.index))
+    if st:
+        _lib.check(st, "fdwt_layer_norm_forward")
     return y, stats
+
+
+@lru_cache(maxsize=1024)
+def _backward_ws(code: int, rows: int, dim: int, need_params: int, device_index: int) -> int:
+    """Workspace bytes of a backward call (a pure function of its sizes on one device)."""
+    return int(_lib.load().fdwt_layer_norm_backward_workspace(code, rows, dim, need_params))
 
 
 class _LayerNormFunction(torch.autograd.Function):
@@ -54,26 +63,34 @@ class _LayerNormFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+        code, param = ctx.codes
         dy = dy.contiguous()
         dim = x.shape[-1]
         rows = x.numel() // dim
         dev = x.device
-        param = _lib.DTYPE_OF[ctx.codes[1]]
         dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(dim, device=dev, dtype=param) if need_w else None
-        db = torch.empty(dim, device=dev, dtype=param) if need_b else None
-        lib = _lib.load()
+        dw = torch.empty(dim, device=dev, dtype=_lib.DTYPE_OF[param]) if need_w else None
+        db = torch.empty(dim, device=dev, dtype=_lib.DTYPE_OF[param]) if need_b else None
         with _lib.device_guard(dev):
-            nws = lib.fdwt_layer_norm_backward_workspace(ctx.codes[0], rows, dim,
-                                                         int(need_w or need_b))
+            nws = _backward_ws(code, rows, dim, int(need_w or need_b), dev.index)
             ws = _lib.workspace(nws, dev)
-            st = lib.fdwt_layer_norm_backward(
-                ctx.codes[0], ctx.codes[1], rows, dim, dy.data_ptr(), x.data_ptr(), _ptr(weight),
+            st = _lib.load().fdwt_layer_norm_backward(
+                code, param, rows, dim, dy.data_ptr(), x.data_ptr(), _ptr(weight),
                 stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nws,
-                _lib.stream_of(dev))
-        _lib.check(st, "fdwt_layer_norm_backward")
+                _lib.raw_stream(dev.index))
+        if st:
+            _lib.check(st, "fdwt_layer_norm_backward")
         return dx, dw, db, None, None
+
+
+def _parameter(name: str, p: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    if p.shape != x.shape[-1:]:
+        raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(p.shape)}")
+    if p.dtype != x.dtype and (p.dtype != torch.float32 or x.dtype == torch.float64):
+        raise TypeError(f"{name} must be {x.dtype} or torch.float32 "
+                        f"(torch.float64 for float64 inputs), got {p.dtype}")
+    return p.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -87,27 +104,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
         raise ValueError(f"expected (..., D) with D >= 1, got shape {tuple(x.shape)}")
     if not 0 <= eps < float("inf"):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    param = code
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.shape != x.shape[-1:]:
-            raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(p.shape)}")
-        if p.dtype != x.dtype and (p.dtype != torch.float32 or x.dtype == torch.float64):
-            raise TypeError(f"{name} must be {x.dtype} or torch.float32 "
-                            f"(torch.float64 for float64 inputs), got {p.dtype}")
-        param = _lib.dtype_code(p.dtype)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     x = x.contiguous()
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    codes = (code, param)
-    if torch.is_grad_enabled() and (
-            x.requires_grad or (weight is not None and weight.requires_grad)
-            or (bias is not None and bias.requires_grad)):
-        return _LayerNormFunction.apply(x, weight, bias, float(eps), codes)
-    return _forward(x, weight, bias, float(eps), codes, False)[0]
+    param, needs = code, x.requires_grad
+    if weight is not None:
+        weight = _parameter("weight", weight, x)
+        param, needs = _lib.DTYPES[weight.dtype], needs or weight.requires_grad
+    if bias is not None:
+        bias = _parameter("bias", bias, x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError(f"weight and bias must have one type, got {weight.dtype} and "
+                            f"{bias.dtype}")
+        param, needs = _lib.DTYPES[bias.dtype], needs or bias.requires_grad
+    if needs and torch.is_grad_enabled():
+        return _LayerNormFunction.apply(x, weight, bias, float(eps), (code, param))
+    return _forward(x, weight, bias, float(eps), (code, param), False)[0]
 
 
 class LayerNorm(nn.Module):
