@@ -106,29 +106,35 @@ __device__ __forceinline__ void load_params(const P* p, A* x) {
   }
 }
 
+template <typename A> __device__ __forceinline__ A warp_sum(A v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Sums of N values over the threads of a row: blockDim.x of them, either a power of two up to 32
 // (lanes of one warp) or whole warps.  `slot` points at 32 N cells of shared memory; consecutive
 // calls take different slots, so that one barrier a call is enough.
 template <typename A, int N>
 __device__ __forceinline__ void row_sum(A (&v)[N], A* slot) {
-  const int lanes = blockDim.x < 32 ? blockDim.x : 32;
-  for (int o = lanes / 2; o > 0; o >>= 1) {
+  if (blockDim.x < 32) {
+    for (int o = blockDim.x / 2; o > 0; o >>= 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+    return;
   }
-  if (blockDim.x <= 32) return;
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) slot[warp * N + i] = v[i];
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if (blockDim.x == 32) return;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) slot[i * 32 + warp] = v[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = A(0);
-  for (int k = 0; k < warps; ++k) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += slot[k * N + i];
-  }
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? slot[i * 32 + lane] : A(0));
 }
 
 template <typename A> __device__ __forceinline__ A inv_sqrt(A v);
@@ -138,12 +144,15 @@ template <> __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / 
 // ------------------------------------------------------------------------------ forward
 // Threads a block may have when each keeps e elements.
 constexpr int fwd_max_threads(int e) { return e <= 16 ? 1024 : (e <= 32 ? 512 : 256); }
+// Blocks of that size a multiprocessor must hold: loads in flight count for more than registers
+// (65536 x 2048 bf16: 106 us without, 96 us with).
+constexpr int fwd_min_blocks(int e) { return e <= 8 ? 2 : (e <= 16 ? 1 : (e <= 32 ? 2 : 3)); }
 
 // A row is held by blockDim.x threads, IT groups of V elements each (group i of thread t starts
 // at (i * blockDim.x + t) * V: neighbouring lanes read neighbouring groups), blockDim.y rows a
 // block (more than one only where a row has at most a warp).
 template <typename T, typename P, int V, int IT>
-__global__ void __launch_bounds__(fwd_max_threads(V * IT))
+__global__ void __launch_bounds__(fwd_max_threads(V * IT), fwd_min_blocks(V * IT))
 layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
                       const P* __restrict__ bias, T* __restrict__ y,
                       typename AccOf<T>::type* __restrict__ stats, int64_t rows, int dim,
@@ -482,7 +491,7 @@ inline bool warp_shape(int64_t groups, int v, int most_items, Shape* s, int bloc
 }
 inline bool forward_shape(int64_t groups, int v, int acc_size, Shape* s) {
   if (warp_shape(groups, v, v <= 2 ? 8 : (acc_size == 8 ? 32 : 64) / v, s, 128)) return true;
-  for (int items = v >= 8 ? 2 : (v <= 2 ? 8 : 16 / v); items * v <= 32; items *= 2) {
+  for (int items = v >= 8 ? 4 : (v <= 2 ? 8 : 32 / v); items * v <= 32; items *= 2) {
     const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
     if (threads <= fwd_max_threads(items * v)) {
       *s = {static_cast<int>(threads), items, 1};
@@ -492,8 +501,8 @@ inline bool forward_shape(int64_t groups, int v, int acc_size, Shape* s) {
   return false;
 }
 template <typename A> bool backward_shape(int64_t groups, int v, Shape* s) {
-  if (warp_shape(groups, v, (sizeof(A) == 8 ? 8 : 16) / v, s, 256)) return true;
-  for (int items = v >= 8 ? 1 : 8 / v; items * v <= 32; items *= 2) {
+  if (warp_shape(groups, v, (sizeof(A) == 8 ? 8 : (v > 2 ? 32 : 16)) / v, s, 256)) return true;
+  for (int items = v >= 8 ? 2 : (v <= 2 ? 8 : 16) / v; items * v <= 32; items *= 2) {
     const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
     if (threads <= bwd_max_threads<A>(v * items)) {
       *s = {static_cast<int>(threads), items, 1};
