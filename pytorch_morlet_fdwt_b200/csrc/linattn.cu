@@ -317,18 +317,30 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant
 
 // Gradients of shared key or value heads: the sum over the heads that read them, in the order of
 // the heads; the heads' own gradients are 32 bits (64 for fp64), rounded once here.
-template <typename T>
+// A thread takes W neighbouring columns.
+template <typename T, int W>
 __global__ void __launch_bounds__(256)
 linattn_group_sum_kernel(const typename AccOf<T>::type* __restrict__ in, T* __restrict__ out,
-                         int64_t count, int group, int dim) {
+                         int64_t rows, int group, int dim) {
   using A = typename AccOf<T>::type;
-  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= count) return;
-  const int64_t head = i / dim;
-  const A* p = in + head * group * dim + i % dim;
-  A sum = A(0);
-  for (int g = 0; g < group; ++g) sum += p[int64_t(g) * dim];
-  out[i] = from_acc<T>(sum);
+  const int per = dim / W, here = blockDim.x / per;  // whole rows a block
+  const int64_t row = int64_t(blockIdx.x) * here + threadIdx.x / per;
+  if (int(threadIdx.x) >= here * per || row >= rows) return;
+  const int c = threadIdx.x % per * W;
+  const A* p = in + row * group * dim + c;
+  Pack<A, W> sum;
+#pragma unroll
+  for (int j = 0; j < W; ++j) sum.v[j] = A(0);
+#pragma unroll 4
+  for (int g = 0; g < group; ++g) {
+    const Pack<A, W> x = *reinterpret_cast<const Pack<A, W>*>(p + int64_t(g) * dim);
+#pragma unroll
+    for (int j = 0; j < W; ++j) sum.v[j] += x.v[j];
+  }
+  Pack<T, W> y;
+#pragma unroll
+  for (int j = 0; j < W; ++j) y.v[j] = from_acc<T>(sum.v[j]);
+  *reinterpret_cast<Pack<T, W>*>(out + row * dim + c) = y;
 }
 
 // ------------------------------------------------------------------------------ one token
@@ -460,7 +472,10 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   // the general kernel: blocks an SM holds by its shared memory
   const int64_t slots = int64_t(sm_count()) * (tc || dtype == FDWT_F64 || dk > 64 ? 1 : 2);
   const int64_t units = tiles * call.batch * call.heads;
-  const int64_t c = cdiv(chunks, plan_segments(units, chunks, slots, 0.5));
+  // microseconds for the tensor cores (measured; 128 tokens), chunks of 64 or 32 tokens for the
+  // general kernel
+  const Cost cost = tc ? Cost{dk <= 64 ? 1.9 : 2.3, 0.75, 6.0, 4.0} : Cost{1.0, 0.4, 1.5, 2.0};
+  const int64_t c = cdiv(chunks, plan_segments(units, chunks, slots, cost));
   p.nseg = static_cast<int>(cdiv(chunks, c));
   p.seg_len = c * p.chunk;
   return p;
@@ -533,10 +548,13 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
       default: return simt_launch<__nv_bfloat16>(call, dk, states, blocks, stream);
     }
   };
+  call.scan_inside = p.tc && p.nseg <= kScanInside;
   if (p.nseg > 1) {
     int st = launch(true);
     if (st != FDWT_OK) return st;
-    st = pre_launch(stream);
+  }
+  if (p.nseg > 1 && !call.scan_inside) {
+    int st = pre_launch(stream);
     if (st != FDWT_OK) return st;
     const dim3 blocks(static_cast<unsigned>(cdiv(elems, 256)), static_cast<unsigned>(heads),
                       static_cast<unsigned>(call.jobs));
@@ -748,13 +766,21 @@ extern "C" int fdwt_linattn_backward(const fdwt_linattn_desc* desc, const void* 
     using T = decltype(tag);
     for (int which = 0; which < 2; ++which) {
       const int dim = which == 0 ? desc->dk : desc->dv;
-      const int64_t count = desc->batch * desc->length * desc->kv_heads * dim;
-      if (cdiv(count, 256) > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+      const int64_t rows = desc->batch * desc->length * desc->kv_heads;
+      void* to = which == 0 ? dk : dv;
+      const bool wide = dim % 4 == 0 && reinterpret_cast<uintptr_t>(to) % (4 * sizeof(T)) == 0;
+      const int64_t blocks = cdiv(rows, 256 / (wide ? dim / 4 : dim));
+      if (blocks > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
       const int e = pre_launch(s);
       if (e != FDWT_OK) return e;
-      linattn_group_sum_kernel<T><<<static_cast<unsigned>(cdiv(count, 256)), 256, 0, s>>>(
-          static_cast<const typename AccOf<T>::type*>(which == 0 ? dk_all : dv_all),
-          static_cast<T*>(which == 0 ? dk : dv), count, group, dim);
+      auto go = [&](auto width) {
+        linattn_group_sum_kernel<T, decltype(width)::value>
+            <<<static_cast<unsigned>(blocks), 256, 0, s>>>(
+                static_cast<const typename AccOf<T>::type*>(which == 0 ? dk_all : dv_all),
+                static_cast<T*>(to), rows, group, dim);
+      };
+      if (wide) go(std::integral_constant<int, 4>{});
+      else go(std::integral_constant<int, 1>{});
       const int l = launch_status();
       if (l != FDWT_OK) return l;
     }

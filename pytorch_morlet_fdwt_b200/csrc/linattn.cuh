@@ -54,22 +54,30 @@ struct Call {
   const int32_t* lengths;
   int64_t batch, length, seg_len;
   int heads, nseg;
+  int scan_inside;  // the main launch adds up the segments' end states itself
 };
 
-// Segments for `units` independent blocks of `chunks` chunks on `slots` resident blocks, by the
-// modelled time in chunks: a segment of c chunks costs c + 2 in the main launch, `state_cost` c
-// + 2 in the state launch, and the two extra launches 4.
-inline int plan_segments(int64_t units, int64_t chunks, int64_t slots, double state_cost) {
+// Times of the launches, in any unit: a block of c chunks takes `fixed + c chunk` in the main launch
+// and `fixed + c state` in the state launch, each launch `launch` once.
+struct Cost {
+  double chunk, state, fixed, launch;
+};
+// Up to this many segments the main launch adds up their end states, beyond it a launch of its own.
+constexpr int kScanInside = 8;
+
+// Segments for `units` independent blocks of `chunks` chunks, `slots` of them resident.
+inline int plan_segments(int64_t units, int64_t chunks, int64_t slots, const Cost& k) {
   int best = 1;
-  double best_cost = double(cdiv(units, slots)) * double(chunks + 2);
+  double best_time = double(cdiv(units, slots)) * (k.fixed + double(chunks) * k.chunk);
   const int64_t most = imin(chunks, 64);
   for (int64_t s = 2; s <= most; ++s) {
     const int64_t c = cdiv(chunks, s);
     const int64_t real = cdiv(chunks, c);
-    const double cost = double(cdiv(units * real, slots)) * double(c + 2) +
-                        double(cdiv(units * (real - 1), slots)) * (state_cost * double(c) + 2) + 4;
-    if (cost < best_cost) {
-      best_cost = cost;
+    const double time = double(cdiv(units * real, slots)) * (k.fixed + double(c) * k.chunk) +
+                        double(cdiv(units * (real - 1), slots)) * (k.fixed + double(c) * k.state) +
+                        k.launch * (real > kScanInside ? 2 : 1);
+    if (time < best_time) {
+      best_time = time;
       best = static_cast<int>(real);
     }
   }

@@ -423,8 +423,9 @@ template <int N> __device__ __forceinline__ void give_registers() {
 constexpr uint32_t kColumns = 512;
 // TMEM columns: two buffers of Sc (P over its first 64 columns, Oi over the others), Oe, U
 constexpr uint32_t kSc = 0, kOi = 64, kOe = 256, kU = 320;
-// The state launch takes 64 tokens at a time: more stages, two buffers of V'.
-constexpr int kStateRows = 64, kStatePanel = kStateRows * 128;
+// The state launch takes 64 tokens at a time.  A stage is held from its load to the end of its
+// product, some 2.5 us, so what counts is their number (4: 140 us for 1 x 65536 x 16 x 128).
+constexpr int kStateRows = 64, kStatePanel = kStateRows * 128, kStateGroups = 4, kStateParts = 2;
 
 template <typename T, int DK> struct Smem {
   static constexpr int panels = DK / 64;
@@ -432,10 +433,10 @@ template <typename T, int DK> struct Smem {
   static constexpr int q = 0, k = stages * panels * kPanel, v = 2 * k;  // rings of stages
   static constexpr int parts = v + stages * kPanel, s = parts + kParts<T> * kPanel;
   static constexpr int bytes = s + DK * 128 + 1024;  // 1024: room to align the base
-  static constexpr int st_stages = 4;
+  static constexpr int st_stages = DK == 64 ? 8 : 6;
   static constexpr int st_stage = (panels + 1) * kStatePanel;
   static constexpr int st_parts = st_stages * st_stage;
-  static constexpr int st_bytes = st_parts + 2 * kParts<T> * kStatePanel + 1024;
+  static constexpr int st_bytes = st_parts + kStateParts * kParts<T> * kStatePanel + 1024;
 };
 
 __device__ __forceinline__ unsigned char* align_smem(unsigned char* p) {
@@ -758,24 +759,40 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const float write = float(job.write);
     float s[2][32];
     {
-      const float* src = nullptr;
-      int64_t row = job.dv, col = 1;
-      if (w.seg == 0) {
-        if (job.init != nullptr) {
-          src = static_cast<const float*>(job.init) + w.bh * size;
-          row = job.init_row;
-          col = job.init_col;
-        }
-      } else if (w.seg <= w.last) {
-        src = static_cast<const float*>(job.seg) +
-              (int64_t(w.bh) * (call.nseg - 1) + w.seg - 1) * size;
-      }
-      const int cols = src != nullptr && mine && r < job.dk ? w.vcols : 0;
-      src += r * row + w.v0 * col;
+      // the first state, or what the segments before leave: their own end states are added up
+      // here where there are few, by a launch before this one where there are many
+      const bool inside = call.scan_inside != 0;
+      const int cols = mine && r < job.dk && w.seg <= w.last ? w.vcols : 0;
+      const int64_t first = int64_t(w.bh) * size;
+      if (job.init != nullptr && (w.seg == 0 || inside)) {
+        const float* src = static_cast<const float*>(job.init) + first + r * job.init_row +
+                           w.v0 * job.init_col;
 #pragma unroll
-      for (int c = 0; c < NV; ++c) {
-        s[c / 32][c % 32] = c < cols ? *src : 0.0f;
-        src += col;
+        for (int c = 0; c < NV; ++c) {
+          s[c / 32][c % 32] = c < cols ? *src : 0.0f;
+          src += job.init_col;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) s[c / 32][c % 32] = 0.0f;
+      }
+      const float* src = static_cast<const float*>(job.seg) + first * (call.nseg - 1) +
+                         int64_t(r) * job.dv + w.v0;
+      const float keep = inside ? decay_pow(w.a, float(call.seg_len)) : 0.0f;
+#pragma unroll 1
+      for (int j = inside ? 0 : w.seg - 1; j < w.seg; ++j) {
+        if (j < 0) continue;
+#pragma unroll
+        for (int c = 0; c < NV; c += 4) {
+          if (c < cols) {
+            const float4 u = *reinterpret_cast<const float4*>(src + j * size + c);
+            float* y = &s[c / 32][c % 32];
+            y[0] = keep * y[0] + u.x;
+            y[1] = keep * y[1] + u.y;
+            y[2] = keep * y[2] + u.z;
+            y[3] = keep * y[3] + u.w;
+          }
+        }
       }
     }
     bool ok = true;
@@ -993,7 +1010,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 // ------------------------------------------------------------------------------ state launch
 // A segment's own end state: U += K^T V' with V' = diag(d^{end-off-l}) V weighted towards the
 // segment's end, so that the sums stay in TMEM over all tokens.
-constexpr int kStateThreads = 320;  // V' (and the result): 8 warps, products: 1, loads: 1
+constexpr int kStateThreads = 576;  // V' (and the result): 16 warps, products: 1, loads: 1
 
 template <typename T, int DK>
 __global__ void __launch_bounds__(kStateThreads, 1)
@@ -1004,7 +1021,8 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   constexpr int S = Z::st_stages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = align_smem(raw);
-  __shared__ uint64_t full[S], v_full[2], used[S], done;
+  constexpr int NB = kStateParts, kGroups = kStateGroups;
+  __shared__ uint64_t full[S], v_full[NB], used[S], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   const Where w = locate(call);
@@ -1012,7 +1030,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   if (w.seg >= w.last) return;  // the whole block
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) bar_init(&v_full[i], 128);
+    for (int i = 0; i < NB; ++i) bar_init(&v_full[i], 128);
     for (int i = 0; i < S; ++i) {
       bar_init(&full[i], 1);
       bar_init(&used[i], 1);
@@ -1021,7 +1039,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tmem_alloc(&tmem_slot);
+  if (warp == 16) tmem_alloc(&tmem_slot);
   tc_before();
   __syncthreads();
   tc_after();
@@ -1029,10 +1047,10 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   const uint32_t base = smem_addr(sm);
   const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
 
-  if (warp < 8) {
-    // four warps take the even blocks of 64 tokens, four the odd ones, each their buffer of V'
+  if (warp < 4 * kGroups) {
+    // groups of four warps take the blocks of 64 tokens by turns
     const int tid = threadIdx.x % 128, mine = warp / 4;
-    for (int i = mine; i < chunks; i += 2) {
+    for (int i = mine; i < chunks; i += kGroups) {
       float weight[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1043,12 +1061,12 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
       const bool ok = split_values<T>(
           sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
-          sm + Z::st_parts + mine * kParts<T> * kStatePanel, kStatePanel, weight, tid,
-          // the products of block i - 2 have ended
-          [&] { return i < 2 || bar_wait(&used[(i - 2) % S], ((i - 2) / S) & 1, &failed); });
+          sm + Z::st_parts + i % NB * kParts<T> * kStatePanel, kStatePanel, weight, tid,
+          // the products of block i - NB have ended
+          [&] { return i < NB || bar_wait(&used[(i - NB) % S], ((i - NB) / S) & 1, &failed); });
       if (!ok) break;
       fence_async();
-      bar_arrive(&v_full[mine]);
+      bar_arrive(&v_full[i % NB]);
     }
     if (warp < 4 && __all_sync(0xffffffffu, bar_wait(&done, 0, &failed)) && !failed) {
       tc_after();
@@ -1068,7 +1086,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
         }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     const CUtensorMap* map = maps.map[w.ji];
     const Source k(map + 1, job.ks, w.h / job.k_group, w.b),
         v(map + 2, job.vs, w.h / job.v_group, w.b);
@@ -1097,10 +1115,10 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     const bool one = elect_one();
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
-      ok = __all_sync(0xffffffffu, bar_wait(&v_full[i & 1], (i >> 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&v_full[i % NB], (i / NB) & 1, &failed));
       if (!ok) break;
       const uint32_t k = ok0 + (i % S) * (Z::st_stage / 16);
-      const uint32_t parts = op0 + (i & 1) * (kParts<T> * kStatePanel / 16);
+      const uint32_t parts = op0 + (i % NB) * (kParts<T> * kStatePanel / 16);
       if (one) {
         tc_after();
         if (i == 0) issue_update<T, DK, true>(tmem, k, parts);
@@ -1116,7 +1134,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   }
   tc_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_after();
     tmem_free(tmem);
     if (lane == 0 && failed) *error = kErrCopyTimeout;
