@@ -1,5 +1,6 @@
-// Linear attention with a decay for each head: entry points, the general kernel (every type,
-// size and stride, products on the FMA pipes), the sum over segments, and the single-token form.
+// Linear attention with a decay for each head: entry points, the general kernels (every type,
+// size and stride; products on the FMA pipes, or as pairs of TF32 values), the sum over segments,
+// and the single-token form.
 // The mathematics, the jobs and the segments are in linattn.cuh.
 #include <type_traits>
 
@@ -33,27 +34,63 @@ __device__ __forceinline__ int64_t token_of(int64_t l, int64_t n, int reverse) {
 }
 
 // rows x cols of a tensor (row l at base + token * stride) into shared memory, zeros past
-// `valid` rows and `cols` columns.
+// `valid` rows and `cols` columns.  256 threads; where no conversion is due and rows are aligned
+// the copies are asynchronous (tiles_wait() below), else all loads are issued before the stores:
+// one latency a tile instead of one a group (15.6 -> 4 us a chunk on one block).
 template <typename T, typename A, int ROWS, int COLS, int PITCH>
 __device__ __forceinline__ void load_tile(A* dst, const T* base, int64_t stride, int64_t l0,
                                           int64_t n, int reverse, int valid, int cols, int vec) {
   constexpr int V = 16 / sizeof(T);
   if (vec) {
-    for (int i = threadIdx.x; i < ROWS * (COLS / V); i += blockDim.x) {
-      const int r = i / (COLS / V), c = i % (COLS / V) * V;
-      Pack<T, V> p;
-      const bool in = r < valid && c < cols;
-      if (in) p = *reinterpret_cast<const Pack<T, V>*>(base + token_of(l0 + r, n, reverse) * stride + c);
+    constexpr int N = (ROWS * (COLS / V) + 255) / 256;
+    if constexpr (std::is_same<T, A>::value) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) dst[r * PITCH + c + j] = in ? A(to_acc(p.v[j])) : A(0);
+      for (int j = 0; j < N; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / (COLS / V), c = i % (COLS / V) * V;
+        if (r >= ROWS) break;
+        const bool in = r < valid && c < cols;
+        const T* src = in ? base + token_of(l0 + r, n, reverse) * stride + c : base;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * PITCH + c))),
+                     "l"(src), "r"(in ? 16 : 0)
+                     : "memory");
+      }
+    } else {
+      Pack<T, V> p[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / (COLS / V), c = i % (COLS / V) * V;
+        if (r < valid && c < cols)
+          p[j] = *reinterpret_cast<const Pack<T, V>*>(base + token_of(l0 + r, n, reverse) * stride + c);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / (COLS / V), c = i % (COLS / V) * V;
+        if (r >= ROWS) break;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          dst[r * PITCH + c + e] = r < valid && c < cols ? A(to_acc(p[j].v[e])) : A(0);
+      }
     }
   } else {
-    for (int i = threadIdx.x; i < ROWS * COLS; i += blockDim.x) {
-      const int r = i / COLS, c = i % COLS;
-      dst[r * PITCH + c] = r < valid && c < cols
-          ? A(to_acc(base[token_of(l0 + r, n, reverse) * stride + c])) : A(0);
+    constexpr int N = 8;  // loads in flight
+    for (int i0 = threadIdx.x; i0 < ROWS * COLS; i0 += 256 * N) {
+      T x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = i0 + 256 * j, r = i / COLS, c = i % COLS;
+        if (r < valid && c < cols) x[j] = base[token_of(l0 + r, n, reverse) * stride + c];
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = i0 + 256 * j, r = i / COLS, c = i % COLS;
+        if (r < ROWS) dst[r * PITCH + c] = r < valid && c < cols ? A(to_acc(x[j])) : A(0);
+      }
     }
   }
+}
+__device__ __forceinline__ void tiles_wait() {
+  asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename T, int DK, int C, int NV> struct Simt {
@@ -137,6 +174,7 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
       const int age = m - job.off - static_cast<int>(threadIdx.x);
       sw[threadIdx.x] = age < 0 ? A(0) : A(job.write) * decay_pow(a, A(age));
     }
+    tiles_wait();
     __syncthreads();
     if (!STATES) {
       // scores, blocks on and below the diagonal
@@ -290,6 +328,286 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
   }
 }
 
+// ------------------------------------------------------------------------------ 32 bits, warps' MMA
+// The same block for 32-bit precision on the tensor cores (warp-level TF32 products): each operand
+// is the sum of two TF32 values, a b = ah bh + ah bl + al bh, which leaves 2^-21 of a product out,
+// less than a 32-bit sum of this length rounds.  Three products at 275 TFLOP/s (measured) against
+// the FMA pipes' 70; and a fragment serves 8 or 16 rows, where the FMA form above is bound by its
+// shared-memory reads.  Also the 16-bit types where rows are not aligned for linattn_tc.cu.
+//
+// 8 warps: warp w owns rows 16 (w % 4) and columns 32 (w / 4) of the scores and of o, and of every
+// 64 rows of the state, which stays in its registers.  Pitches: rows 4 (8) words apart modulo 32
+// put the 32 lanes of a fragment's read on different banks.
+__device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;  // to nearest; the next binade is exact too
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4],
+                                         const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+struct FragA {
+  uint32_t hi[4], lo[4];
+  // element (row, k) of the 16 x 8 block at p[row * rs + k * ks]
+  __device__ __forceinline__ void load(const float* p, int rs, int ks, int lane) {
+    const float* q = p + lane / 4 * rs + lane % 4 * ks;
+    tf32_split(q[0], hi[0], lo[0]);
+    tf32_split(q[8 * rs], hi[1], lo[1]);
+    tf32_split(q[4 * ks], hi[2], lo[2]);
+    tf32_split(q[8 * rs + 4 * ks], hi[3], lo[3]);
+  }
+};
+struct FragB {
+  uint32_t hi[2], lo[2];
+  // element (k, column) of the 8 x 8 block at p[k * ks + column * cs], times wk[k]
+  __device__ __forceinline__ void load(const float* p, int ks, int cs, int lane) {
+    const float* q = p + lane % 4 * ks + lane / 4 * cs;
+    tf32_split(q[0], hi[0], lo[0]);
+    tf32_split(q[4 * ks], hi[1], lo[1]);
+  }
+  __device__ __forceinline__ void load(const float* p, int ks, int cs, int lane, float w0,
+                                       float w1) {
+    const float* q = p + lane % 4 * ks + lane / 4 * cs;
+    tf32_split(q[0] * w0, hi[0], lo[0]);
+    tf32_split(q[4 * ks] * w1, hi[1], lo[1]);
+  }
+};
+__device__ __forceinline__ void mma3(float (&c)[4], const FragA& a, const FragB& b) {
+  mma_tf32(c, a.lo, b.hi);
+  mma_tf32(c, a.hi, b.lo);
+  mma_tf32(c, a.hi, b.hi);
+}
+
+template <int DK> struct Tf32 {
+  static constexpr int C = 64, NV = 64, PK = DK + 4, PV = NV + 8, PP = C + 4;
+  static constexpr int words = 2 * C * PK + C * PV + DK * PV + C * PP + 2 * (C + 8);
+  static constexpr size_t smem = words * sizeof(float);
+};
+
+template <typename T, int DK, bool STATES>
+__global__ void __launch_bounds__(256, DK == 64 ? 2 : 1)
+linattn_tf32_kernel(const __grid_constant__ Call call) {
+  using Z = Tf32<DK>;
+  constexpr int C = Z::C, NV = Z::NV, PK = Z::PK, PV = Z::PV, PP = Z::PP, RT = DK / 64;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  float* sq = reinterpret_cast<float*>(smem_raw);
+  float* sk = sq + C * PK;
+  float* sv = sk + C * PK;
+  float* ss = sv + C * PV;
+  float* sp = ss + DK * PV;
+  float* dpow = sp + C * PP;      // d^n, n = 0 .. 64
+  float* weight = dpow + C + 8;   // of the chunk's values towards its end
+
+  int tile = blockIdx.x % call.tiles;
+  const int64_t rest = blockIdx.x / call.tiles;
+  const int64_t heads = call.batch * call.heads;
+  const int64_t bh = rest % heads;
+  const int seg = static_cast<int>(rest / heads);
+  int ji = 0;
+  while (tile >= call.job[ji].tiles) tile -= call.job[ji++].tiles;
+  const Job& job = call.job[ji];
+  const int64_t b = bh / call.heads;
+  const int h = static_cast<int>(bh % call.heads);
+  const int v0 = tile * NV;
+  const int vcols = job.dv - v0 < NV ? job.dv - v0 : NV;
+  const int64_t n = valid_tokens(call, b);
+  const int last = n == 0 ? 0 : static_cast<int>((n - 1) / call.seg_len);
+  if (STATES && seg >= last) return;
+  const float a = static_cast<const float*>(call.log_decay)[h];
+  const int64_t begin = int64_t(seg) * call.seg_len;
+  const int64_t row_end = imin(begin + call.seg_len, call.length);
+  const int64_t end = imin(row_end, n);
+
+  const T* q = static_cast<const T*>(job.q) + b * job.qs[0] + (h / job.q_group) * job.qs[2];
+  const T* k = static_cast<const T*>(job.k) + b * job.ks[0] + (h / job.k_group) * job.ks[2];
+  const T* v = static_cast<const T*>(job.v) + b * job.vs[0] + (h / job.v_group) * job.vs[2] + v0;
+  const int64_t o_head = b * job.os[0] + h * job.os[2] + v0;
+  T* o = static_cast<T*>(job.o) + o_head;
+  float* wide = static_cast<float*>(job.o) + o_head;
+  const int64_t state_size = int64_t(job.dk) * job.dv;
+  float* segs = static_cast<float*>(job.seg) + bh * (call.nseg - 1) * state_size;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int r0 = warp % 4 * 16, c0 = warp / 4 * 32;
+  const int g = lane / 4, t4 = lane % 4;
+
+  for (int i = threadIdx.x; i <= C; i += 256) dpow[i] = decay_pow(a, float(i));
+  float s[RT][4][4];  // the state: rows 64 rt + r0 + g (+ 8), columns c0 + 8 j + 2 t4 (+ 1)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 64 * rt + r0 + g + e / 2 * 8, col = c0 + 8 * j + 2 * t4 + e % 2;
+        const int c = v0 + col;
+        float x = 0.0f;
+        if (!STATES && r < job.dk && c < job.dv) {
+          if (seg > 0 && seg <= last) x = segs[(seg - 1) * state_size + int64_t(r) * job.dv + c];
+          else if (seg == 0 && job.init != nullptr)
+            x = static_cast<const float*>(job.init)[bh * state_size + r * job.init_row +
+                                                    c * job.init_col];
+        }
+        s[rt][j][e] = x;
+        if (!STATES) ss[r * PV + col] = x;
+      }
+
+  for (int64_t l0 = begin; l0 < end; l0 += C) {
+    const int m = static_cast<int>(imin(C, end - l0));
+    if (!STATES)
+      load_tile<T, float, C, DK, PK>(sq, q, job.qs[1], l0, n, job.reverse, m, job.dk, job.q_vec);
+    load_tile<T, float, C, DK, PK>(sk, k, job.ks[1], l0, n, job.reverse, m, job.dk, job.k_vec);
+    load_tile<T, float, C, NV, PV>(sv, v, job.vs[1], l0, n, job.reverse, m, vcols, job.v_vec);
+    if (threadIdx.x < C) {
+      const int age = m - job.off - static_cast<int>(threadIdx.x);
+      weight[threadIdx.x] = age < 0 ? 0.0f : decay_pow(a, float(age));
+    }
+    tiles_wait();
+    __syncthreads();
+    if (!STATES) {
+      // scores: columns above the diagonal of these rows drop out
+      float acc[4][4] = {};
+      const int cols = r0 + 16 - c0 < 0 ? 0 : (r0 + 16 - c0 > 32 ? 4 : (r0 + 16 - c0) / 8);
+      if (cols > 0) {
+#pragma unroll 2
+        for (int d = 0; d < DK; d += 8) {
+          FragA x;
+          x.load(sq + r0 * PK + d, PK, 1, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j < cols) {
+              FragB y;
+              y.load(sk + (c0 + 8 * j) * PK + d, 1, PK, lane);
+              mma3(acc[j], x, y);
+            }
+          }
+        }
+      }
+      const float intra = float(job.intra);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = r0 + g + e / 2 * 8, u = c0 + 8 * j + 2 * t4 + e % 2;
+          sp[t * PP + u] = u > t ? 0.0f : acc[j][e] * (intra * dpow[t - u]);
+        }
+      // what the state gives
+      float out[4][4] = {};
+#pragma unroll 2
+      for (int d = 0; d < DK; d += 8) {
+        FragA x;
+        x.load(sq + r0 * PK + d, PK, 1, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          FragB y;
+          y.load(ss + d * PV + c0 + 8 * j, PV, 1, lane);
+          mma3(out[j], x, y);
+        }
+      }
+      const float inter = float(job.inter);
+      const float f0 = inter * dpow[r0 + g + job.off], f1 = inter * dpow[r0 + g + 8 + job.off];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        out[j][0] *= f0;
+        out[j][1] *= f0;
+        out[j][2] *= f1;
+        out[j][3] *= f1;
+      }
+      __syncthreads();
+      // and the chunk's own tokens, up to the end of these rows
+#pragma unroll 2
+      for (int u = 0; u < r0 + 16; u += 8) {
+        FragA x;
+        x.load(sp + r0 * PP + u, PP, 1, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          FragB y;
+          y.load(sv + u * PV + c0 + 8 * j, PV, 1, lane);
+          mma3(out[j], x, y);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const int t = r0 + g + e / 2 * 8;
+        if (t < m) {
+          const int64_t at = token_of(l0 + t, n, job.reverse) * job.os[1];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int col = c0 + 8 * j + 2 * t4;
+            if (sizeof(T) == 4 && job.o_vec && col + 2 <= vcols) {
+              *reinterpret_cast<float2*>(wide + at + col) = make_float2(out[j][e], out[j][e + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (col + i < vcols) {
+                  if (job.o_wide) wide[at + col + i] = out[j][e + i];
+                  else o[at + col + i] = from_acc<T>(out[j][e + i]);
+                }
+            }
+          }
+        }
+      }
+    }
+    // state
+    const float keep = dpow[m], write = float(job.write);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[rt][j][e] *= keep;
+#pragma unroll 2
+    for (int u = 0; u < C; u += 8) {
+      FragA x[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) x[rt].load(sk + u * PK + 64 * rt + r0, 1, PK, lane);
+      const float w0 = write * weight[u + t4], w1 = write * weight[u + t4 + 4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        FragB y;
+        y.load(sv + u * PV + c0 + 8 * j, PV, 1, lane, w0, w1);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) mma3(s[rt][j], x[rt], y);
+      }
+    }
+    if (!STATES) {  // (every read of the old one came before the barrier above)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+            *reinterpret_cast<float2*>(ss + (64 * rt + r0 + g + e / 2 * 8) * PV + c0 + 8 * j +
+                                       2 * t4) = make_float2(s[rt][j][e], s[rt][j][e + 1]);
+    }
+    __syncthreads();
+  }
+  if (!STATES) {  // rows after the sequence's end
+    for (int64_t l = imax(begin, n) + warp; l < row_end; l += 8)
+      for (int c = lane; c < vcols; c += 32) {
+        if (job.o_wide) wide[l * job.os[1] + c] = 0.0f;
+        else o[l * job.os[1] + c] = from_acc<T>(0.0f);
+      }
+  }
+  float* dst = STATES ? segs + seg * state_size
+                      : (seg == last && job.fin != nullptr
+                             ? static_cast<float*>(job.fin) + bh * state_size : nullptr);
+  if (dst != nullptr) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 64 * rt + r0 + g + e / 2 * 8, c = v0 + c0 + 8 * j + 2 * t4 + e % 2;
+          if (r < job.dk && c < job.dv) dst[int64_t(r) * job.dv + c] = s[rt][j][e];
+        }
+  }
+}
+
 // The states between segments: slot i of a head holds segment i's own end state and receives the
 // state before segment i + 1.
 template <typename A>
@@ -410,32 +728,39 @@ linattn_step_kernel(const __grid_constant__ fdwt_linattn_desc d, const T* __rest
 }
 
 // ------------------------------------------------------------------------------ launches
-template <typename T> struct Tiles {  // chunk and value tile of the general kernel
-  static constexpr int C = 64, NV = 64;
-};
-template <> struct Tiles<double> {
-  static constexpr int C = 32, NV = 32;
-};
+int block_chunk(int dtype, int dk) { return dtype == FDWT_F64 || dk > 128 ? 32 : 64; }
 
-int simt_chunk(int dtype, int dk) { return dtype == FDWT_F64 || dk > 128 ? 32 : 64; }
-
-template <typename T, int DK, int C, int NV>
-int simt_launch_as(const Call& call, bool states, int64_t grid, cudaStream_t stream) {
-  auto kernel = states ? linattn_simt_kernel<T, DK, C, NV, true>
-                       : linattn_simt_kernel<T, DK, C, NV, false>;
+template <typename Kernel>
+int launch_block(Kernel kernel, size_t smem, const Call& call, int64_t grid, cudaStream_t stream) {
   int st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
   if (st == FDWT_OK) st = pre_launch(stream);
   if (st != FDWT_OK) return st;
-  kernel<<<static_cast<unsigned>(grid), 256, Simt<T, DK, C, NV>::smem, stream>>>(call);
+  kernel<<<static_cast<unsigned>(grid), 256, smem, stream>>>(call);
   return launch_status();
 }
+template <typename T, int DK>
+int simt_launch(const Call& call, bool states, int64_t grid, cudaStream_t stream) {
+  return launch_block(states ? linattn_simt_kernel<T, DK, 32, 32, true>
+                             : linattn_simt_kernel<T, DK, 32, 32, false>,
+                      Simt<T, DK, 32, 32>::smem, call, grid, stream);
+}
+template <typename T, int DK>
+int tf32_launch(const Call& call, bool states, int64_t grid, cudaStream_t stream) {
+  return launch_block(states ? linattn_tf32_kernel<T, DK, true> : linattn_tf32_kernel<T, DK, false>,
+                      Tf32<DK>::smem, call, grid, stream);
+}
 
+// fp64 and heads over 128 on the FMA pipes, the others by TF32 products.
 template <typename T>
-int simt_launch(const Call& call, int dk, bool states, int64_t grid, cudaStream_t stream) {
-  constexpr int C = Tiles<T>::C, NV = Tiles<T>::NV;
-  if (dk <= 64) return simt_launch_as<T, 64, C, NV>(call, states, grid, stream);
-  if (dk <= 128) return simt_launch_as<T, 128, C, NV>(call, states, grid, stream);
-  return simt_launch_as<T, 256, 32, 32>(call, states, grid, stream);
+int general_launch(const Call& call, int dk, bool states, int64_t grid, cudaStream_t stream) {
+  if constexpr (std::is_same<T, double>::value) {
+    if (dk <= 64) return simt_launch<T, 64>(call, states, grid, stream);
+    if (dk <= 128) return simt_launch<T, 128>(call, states, grid, stream);
+  } else {
+    if (dk <= 64) return tf32_launch<T, 64>(call, states, grid, stream);
+    if (dk <= 128) return tf32_launch<T, 128>(call, states, grid, stream);
+  }
+  return simt_launch<T, 256>(call, states, grid, stream);
 }
 
 // Accesses of `bytes` along the last axis are aligned (and the axis ends on one).
@@ -464,7 +789,7 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   Plan p{};
   p.tc = tc;
   const int dk = max_dk(call);
-  p.chunk = tc ? kTcChunk : simt_chunk(dtype, dk);
+  p.chunk = tc ? kTcChunk : block_chunk(dtype, dk);
   p.tile = tc ? kTcTile : (p.chunk == 64 ? 64 : 32);
   int64_t tiles = 0;
   for (int j = 0; j < call.jobs; ++j) tiles += cdiv(call.job[j].dv, p.tile);
@@ -542,10 +867,10 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
     if (p.tc) return tc_launch(dtype, call, states, stream);
     const int64_t blocks = states ? grid / p.nseg * (p.nseg - 1) : grid;
     switch (dtype) {
-      case FDWT_F32: return simt_launch<float>(call, dk, states, blocks, stream);
-      case FDWT_F64: return simt_launch<double>(call, dk, states, blocks, stream);
-      case FDWT_F16: return simt_launch<__half>(call, dk, states, blocks, stream);
-      default: return simt_launch<__nv_bfloat16>(call, dk, states, blocks, stream);
+      case FDWT_F32: return general_launch<float>(call, dk, states, blocks, stream);
+      case FDWT_F64: return general_launch<double>(call, dk, states, blocks, stream);
+      case FDWT_F16: return general_launch<__half>(call, dk, states, blocks, stream);
+      default: return general_launch<__nv_bfloat16>(call, dk, states, blocks, stream);
     }
   };
   call.scan_inside = p.tc && p.nseg <= kScanInside;
