@@ -376,11 +376,18 @@ struct FragB {
     tf32_split(q[4 * ks] * w1, hi[1], lo[1]);
   }
 };
-__device__ __forceinline__ void mma3(float (&c)[4], const FragA& a, const FragB& b) {
-  mma_tf32(c, a.lo, b.hi);
-  mma_tf32(c, a.hi, b.lo);
-  mma_tf32(c, a.hi, b.hi);
-}
+// A 16 x 8 block of a product.  The matrix unit's 32-bit sum is cut off, not rounded, at every
+// step: the large products and the small ones are summed apart, each over one chunk or head only,
+// and what is carried from chunk to chunk is added outside (6e-6 off on a long sequence else).
+struct Block {
+  float hi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  __device__ __forceinline__ void add(const FragA& a, const FragB& b) {
+    mma_tf32(lo, a.lo, b.hi);
+    mma_tf32(lo, a.hi, b.lo);
+    mma_tf32(hi, a.hi, b.hi);
+  }
+  __device__ __forceinline__ float value(int e) const { return hi[e] + lo[e]; }
+};
 
 template <int DK> struct Tf32 {
   static constexpr int C = 64, NV = 64, PK = DK + 4, PV = NV + 8, PP = C + 4;
@@ -469,7 +476,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
     __syncthreads();
     if (!STATES) {
       // scores: columns above the diagonal of these rows drop out
-      float acc[4][4] = {};
+      Block acc[4];
       const int cols = r0 + 16 - c0 < 0 ? 0 : (r0 + 16 - c0 > 32 ? 4 : (r0 + 16 - c0) / 8);
       if (cols > 0) {
 #pragma unroll 2
@@ -481,7 +488,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
             if (j < cols) {
               FragB y;
               y.load(sk + (c0 + 8 * j) * PK + d, 1, PK, lane);
-              mma3(acc[j], x, y);
+              acc[j].add(x, y);
             }
           }
         }
@@ -492,10 +499,10 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int t = r0 + g + e / 2 * 8, u = c0 + 8 * j + 2 * t4 + e % 2;
-          sp[t * PP + u] = u > t ? 0.0f : acc[j][e] * (intra * dpow[t - u]);
+          sp[t * PP + u] = u > t ? 0.0f : acc[j].value(e) * (intra * dpow[t - u]);
         }
       // what the state gives
-      float out[4][4] = {};
+      Block state[4];
 #pragma unroll 2
       for (int d = 0; d < DK; d += 8) {
         FragA x;
@@ -504,20 +511,22 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
         for (int j = 0; j < 4; ++j) {
           FragB y;
           y.load(ss + d * PV + c0 + 8 * j, PV, 1, lane);
-          mma3(out[j], x, y);
+          state[j].add(x, y);
         }
       }
       const float inter = float(job.inter);
       const float f0 = inter * dpow[r0 + g + job.off], f1 = inter * dpow[r0 + g + 8 + job.off];
+      float out[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        out[j][0] *= f0;
-        out[j][1] *= f0;
-        out[j][2] *= f1;
-        out[j][3] *= f1;
+        out[j][0] = f0 * state[j].value(0);
+        out[j][1] = f0 * state[j].value(1);
+        out[j][2] = f1 * state[j].value(2);
+        out[j][3] = f1 * state[j].value(3);
       }
       __syncthreads();
       // and the chunk's own tokens, up to the end of these rows
+      Block own[4];
 #pragma unroll 2
       for (int u = 0; u < r0 + 16; u += 8) {
         FragA x;
@@ -526,9 +535,13 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
         for (int j = 0; j < 4; ++j) {
           FragB y;
           y.load(sv + u * PV + c0 + 8 * j, PV, 1, lane);
-          mma3(out[j], x, y);
+          own[j].add(x, y);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[j][e] += own[j].value(e);
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
         const int t = r0 + g + e / 2 * 8;
@@ -553,12 +566,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
     }
     // state
     const float keep = dpow[m], write = float(job.write);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[rt][j][e] *= keep;
+    Block update[RT][4];
 #pragma unroll 2
     for (int u = 0; u < C; u += 8) {
       FragA x[RT];
@@ -570,9 +578,15 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
         FragB y;
         y.load(sv + u * PV + c0 + 8 * j, PV, 1, lane, w0, w1);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) mma3(s[rt][j], x[rt], y);
+        for (int rt = 0; rt < RT; ++rt) update[rt][j].add(x[rt], y);
       }
     }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[rt][j][e] = keep * s[rt][j][e] + update[rt][j].value(e);
     if (!STATES) {  // (every read of the old one came before the barrier above)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -771,6 +785,8 @@ inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t siz
          strides[1] % v == 0 && strides[2] % v == 0;
 }
 
+constexpr int kShort = 64;
+
 struct Plan {
   bool tc;
   int chunk, tile, nseg;
@@ -794,12 +810,12 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   int64_t tiles = 0;
   for (int j = 0; j < call.jobs; ++j) tiles += cdiv(call.job[j].dv, p.tile);
   const int64_t chunks = imax(1, cdiv(call.length, p.chunk));
-  // the general kernel: blocks an SM holds by its shared memory
-  const int64_t slots = int64_t(sm_count()) * (tc || dtype == FDWT_F64 || dk > 64 ? 1 : 2);
+  // One block a multiprocessor counts: a second one on it (the general kernels) doubles the time
+  // of both.  Times in microseconds a chunk (measured): 128 tokens on the tensor cores, 64 (or 32)
+  // by the general kernels.
+  const int64_t slots = sm_count();
   const int64_t units = tiles * call.batch * call.heads;
-  // microseconds for the tensor cores (measured; 128 tokens), chunks of 64 or 32 tokens for the
-  // general kernel
-  const Cost cost = tc ? Cost{dk <= 64 ? 1.9 : 2.3, 0.75, 6.0, 4.0} : Cost{1.0, 0.4, 1.5, 2.0};
+  const Cost cost = tc ? Cost{dk <= 64 ? 1.9 : 2.3, 0.75, 6.0, 4.0} : Cost{7.5, 3.0, 5.0, 4.0};
   const int64_t c = cdiv(chunks, plan_segments(units, chunks, slots, cost));
   p.nseg = static_cast<int>(cdiv(chunks, c));
   p.seg_len = c * p.chunk;
@@ -845,7 +861,10 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
     job.o_vec = vector_ok(job.o, job.os, job.dv, o_size, 16) +
                 vector_ok(job.o, job.os, job.dv, o_size, 32);
   }
-  const Plan p = make_plan(dtype, call, tc_supports(dtype, call));
+  // One short chunk goes to the general kernel: as fast there, and without the 16-bit rounding of
+  // the scores, which few rows do not average out.
+  const bool tc = call.length > kShort && tc_supports(dtype, call);
+  const Plan p = make_plan(dtype, call, tc);
   call.nseg = p.nseg;
   call.seg_len = p.seg_len;
   call.tiles = 0;
