@@ -335,8 +335,7 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
 // the FMA pipes' 70; and a fragment serves 8 or 16 rows, where the FMA form above is bound by its
 // shared-memory reads.  Also the 16-bit types where rows are not aligned for linattn_tc.cu.
 //
-// 8 warps: warp w owns rows 16 (w % 4) and columns 32 (w / 4) of the scores and of o, and of every
-// 64 rows of the state, which stays in its registers.  Pitches: rows 4 (8) words apart modulo 32
+// 8 warps, each of 16 rows and 32 columns of the scores and of o, and of every 64 rows of the state, which stays in its registers.  Pitches: rows 4 (8) words apart modulo 32
 // put the 32 lanes of a fragment's read on different banks.
 __device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;  // to nearest; the next binade is exact too
@@ -396,7 +395,7 @@ template <int DK> struct Tf32 {
 };
 
 template <typename T, int DK, bool STATES>
-__global__ void __launch_bounds__(256, DK == 64 ? 2 : 1)
+__global__ void __launch_bounds__(256, 1)
 linattn_tf32_kernel(const __grid_constant__ Call call) {
   using Z = Tf32<DK>;
   constexpr int C = Z::C, NV = Z::NV, PK = Z::PK, PV = Z::PV, PP = Z::PP, RT = DK / 64;
@@ -438,7 +437,8 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
   const int64_t state_size = int64_t(job.dk) * job.dv;
   float* segs = static_cast<float*>(job.seg) + bh * (call.nseg - 1) * state_size;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int r0 = warp % 4 * 16, c0 = warp / 4 * 32;
+  // the two warps of a scheduler share the work under the diagonal: rows 0 and 3, 1 and 2
+  const int r0 = (warp < 4 ? warp : 7 - warp) * 16, c0 = warp / 4 * 32;
   const int g = lane / 4, t4 = lane % 4;
 
   for (int i = threadIdx.x; i <= C; i += 256) dpow[i] = decay_pow(a, float(i));
@@ -479,7 +479,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
       Block acc[4];
       const int cols = r0 + 16 - c0 < 0 ? 0 : (r0 + 16 - c0 > 32 ? 4 : (r0 + 16 - c0) / 8);
       if (cols > 0) {
-#pragma unroll 2
+#pragma unroll 4
         for (int d = 0; d < DK; d += 8) {
           FragA x;
           x.load(sq + r0 * PK + d, PK, 1, lane);
@@ -503,7 +503,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
         }
       // what the state gives
       Block state[4];
-#pragma unroll 2
+#pragma unroll 4
       for (int d = 0; d < DK; d += 8) {
         FragA x;
         x.load(sq + r0 * PK + d, PK, 1, lane);
@@ -527,7 +527,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
       __syncthreads();
       // and the chunk's own tokens, up to the end of these rows
       Block own[4];
-#pragma unroll 2
+#pragma unroll 4
       for (int u = 0; u < r0 + 16; u += 8) {
         FragA x;
         x.load(sp + r0 * PP + u, PP, 1, lane);
@@ -567,7 +567,7 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
     // state
     const float keep = dpow[m], write = float(job.write);
     Block update[RT][4];
-#pragma unroll 2
+#pragma unroll 4
     for (int u = 0; u < C; u += 8) {
       FragA x[RT];
 #pragma unroll
