@@ -625,11 +625,12 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
 // The states between segments: slot i of a head holds segment i's own end state and receives the
 // state before segment i + 1.
 template <typename A>
-__global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant__ Call call) {
-  const Job& job = call.job[blockIdx.z];
-  const int64_t bh = blockIdx.y;
+__global__ void __launch_bounds__(256)
+linattn_scan_kernel(const __grid_constant__ Call call, int blocks) {  // blocks: a head's
+  const Job& job = call.job[blockIdx.y];
   const int64_t size = int64_t(job.dk) * job.dv;
-  const int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t bh = blockIdx.x / blocks;
+  const int64_t e = int64_t(blockIdx.x % blocks) * blockDim.x + threadIdx.x;
   if (e >= size) return;
   const int64_t n = valid_tokens(call, bh / call.heads);
   const int last = n == 0 ? 0 : static_cast<int>((n - 1) / call.seg_len);
@@ -880,7 +881,7 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
   }
   const int64_t heads = call.batch * call.heads;
   const int64_t grid = heads * call.tiles * p.nseg;
-  if (grid > INT32_MAX || heads > 65535) return FDWT_ERR_UNSUPPORTED;
+  if (grid > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   const int dk = max_dk(call);
   auto launch = [&](bool states) -> int {
     if (p.tc) return tc_launch(dtype, call, states, stream);
@@ -900,10 +901,11 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
   if (p.nseg > 1 && !call.scan_inside) {
     int st = pre_launch(stream);
     if (st != FDWT_OK) return st;
-    const dim3 blocks(static_cast<unsigned>(cdiv(elems, 256)), static_cast<unsigned>(heads),
-                      static_cast<unsigned>(call.jobs));
-    if (dtype == FDWT_F64) linattn_scan_kernel<double><<<blocks, 256, 0, stream>>>(call);
-    else linattn_scan_kernel<float><<<blocks, 256, 0, stream>>>(call);
+    const int per = static_cast<int>(cdiv(elems, 256));
+    if (per * heads > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+    const dim3 blocks(static_cast<unsigned>(per * heads), static_cast<unsigned>(call.jobs));
+    if (dtype == FDWT_F64) linattn_scan_kernel<double><<<blocks, 256, 0, stream>>>(call, per);
+    else linattn_scan_kernel<float><<<blocks, 256, 0, stream>>>(call, per);
     st = launch_status();
     if (st != FDWT_OK) return st;
   }
@@ -916,7 +918,7 @@ inline bool desc_ok(const fdwt_linattn_desc* d) {
          d->length >= 0;
 }
 inline bool desc_supported(const fdwt_linattn_desc* d) {
-  return d->dk <= 256 && d->dv <= 256 && d->batch * d->heads <= 65535;
+  return d->dk <= 256 && d->dv <= 256;
 }
 
 inline void copy3(int64_t* dst, const int64_t* src) {

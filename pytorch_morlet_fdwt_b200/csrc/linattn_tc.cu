@@ -59,22 +59,32 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Polls of a wait (each may sleep for a while in hardware): well under a second in all.
-constexpr int kWaitTries = 1 << 22;
+// What a block needs to give up: a flag in shared memory and the time limit of a wait, about a
+// second (less under the test hook).
+struct Limit {
+  volatile int* failed;
+  long long cycles;
+};
+constexpr long long kWaitCycles = 2000000000LL, kTestCycles = 2000000LL;
 // False: the wait ran out here or elsewhere in the block; the block then ends early.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const Limit& limit) {
+  if (bar_try(bar, parity)) return true;
+  const long long start = clock64();
 #pragma unroll 1
-  for (int i = 0; i < kWaitTries; ++i) {
-    if (bar_try(bar, parity)) return true;
-    if (*failed) return false;
+  while (!bar_try(bar, parity)) {
+    if (*limit.failed) return false;
+    if (clock64() - start > limit.cycles) {
+      *limit.failed = 1;
+      return false;
+    }
   }
-  *failed = 1;
-  return false;
+  return true;
 }
-// For what is in flight after a failure: no regard to `failed`.
-__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
+// For what is in flight after a failure: no regard to the flag.
+__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity, const Limit& limit) {
+  const long long start = clock64();
 #pragma unroll 1
-  for (int i = 0; i < kWaitTries && !bar_try(bar, parity); ++i) {
+  while (!bar_try(bar, parity) && clock64() - start < limit.cycles) {
   }
 }
 __device__ __forceinline__ void fence_async() {
@@ -276,17 +286,19 @@ struct Where {
   float a;
 };
 
-// Block (value tile of the jobs, sequence and head, segment).
+__device__ __forceinline__ bool first_block() { return blockIdx.x == 0 && blockIdx.y == 0; }
+
+// Block (value tile of the jobs of a sequence and head, segment).
 __device__ __forceinline__ Where locate(const Call& call) {
   Where w;
-  int tile = blockIdx.x;
-  w.bh = blockIdx.y;
-  w.seg = blockIdx.z;
+  w.bh = static_cast<int>(blockIdx.x / static_cast<unsigned>(call.tiles));
+  int tile = static_cast<int>(blockIdx.x) - w.bh * call.tiles;
+  w.seg = blockIdx.y;
   int ji = 0;
   while (tile >= call.job[ji].tiles) tile -= call.job[ji++].tiles;
   w.job = &call.job[ji];
   w.ji = ji;
-  w.b = static_cast<int>(blockIdx.y / static_cast<unsigned>(call.heads));
+  w.b = static_cast<int>(unsigned(w.bh) / static_cast<unsigned>(call.heads));
   w.h = w.bh - w.b * call.heads;
   w.v0 = tile * NV;
   w.vcols = w.job->dv - w.v0 < NV ? w.job->dv - w.v0 : NV;
@@ -490,7 +502,7 @@ __device__ __forceinline__ void store_wide(float* dst, const float (&x)[16], int
 template <typename T, int DK>
 __global__ void __launch_bounds__(kThreads, 1)
 linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Maps maps,
-                  int* error) {
+                  int* error, unsigned extra_tx) {
   using Z = Smem<T, DK>;
   constexpr bool kHalf = kIsHalf<T>;
   constexpr int S = Z::stages;
@@ -510,6 +522,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (warp == 0) tmem_alloc(&tmem_slot);
+  const Limit limit{&failed, extra_tx == 0 ? kWaitCycles : kTestCycles};
   const Where w = locate(call);
   const Job& job = *w.job;
   const uint32_t base = smem_addr(sm);
@@ -520,7 +533,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const CUtensorMap* map = maps.map[w.ji];
     const int l0 = w.begin + i * C, token = job.reverse ? w.n - C - l0 : l0;
     if (which == 2) {
-      bar_expect(&v_in[st], kPanel);
+      // (test hook: block 0 waits for bytes that never come)
+      bar_expect(&v_in[st], kPanel + (j == 2 && first_block() ? extra_tx : 0));
       Source(map + 2, job.vs, w.h / job.v_group, w.b)
           .template load<C>(base + Z::v + st * kPanel, w.v0, 1, token, &v_in[st]);
     } else {
@@ -596,7 +610,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const float* diagonal = power + 31 + lane;
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
-      ok = __all_sync(0xffffffffu, bar_wait(&sc_full[i & 1], (i >> 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&sc_full[i & 1], (i >> 1) & 1, limit));
       if (!ok) break;
       tc_after();
       const uint32_t sc = tmem + lanes + kSc + (i & 1) * 128;
@@ -678,13 +692,13 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           weight[j] = age < 0 ? 0.0f : dpow[age];
         }
       }
-      if (!bar_wait(&v_in[i % S], (i / S) & 1, &failed)) break;
+      if (!bar_wait(&v_in[i % S], (i / S) & 1, limit)) break;
       unsigned char* v = sm + Z::v + (i % S) * kPanel;
       if (m < C && !job.reverse && w.n < call.length) {
         // padding after the sequence's end: the products take zeros for its keys and values
         // (scores with them are masked, whichever of the two they read).  A thread clears the
         // values that it reads below.
-        if (!bar_wait(&k_full[i % S], (i / S) & 1, &failed)) break;
+        if (!bar_wait(&k_full[i % S], (i / S) & 1, limit)) break;
         unsigned char* k = sm + Z::k + (i % S) * Z::panels * kPanel;
         for (int r = half * 64 + tid / 8; r < half * 64 + 64; r += 16) {
           if (r < m) continue;
@@ -696,7 +710,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         }
       }
       const bool ok = split_values<T>(v + cell0, sm + Z::parts + cell0, kPanel, weight, tid, [&] {
-        return i == 0 || bar_wait(&v_free[half], (i - 1) & 1, &failed);
+        return i == 0 || bar_wait(&v_free[half], (i - 1) & 1, limit);
       });
       if (!ok) break;
       fence_async();
@@ -710,7 +724,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     const float read = float(job.inter) * dpow[l + job.off];
     const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
     for (int i = 0; i < chunks; ++i) {
-      if (!__all_sync(0xffffffffu, bar_wait(&oe_full, i & 1, &failed))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(&oe_full, i & 1, limit))) break;
       tc_after();
       const int l0 = w.begin + i * C;
       const bool in = l0 + l < w.end;
@@ -724,7 +738,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       for (int g = 0; g < NV / 16; ++g) tmem_ld_wait(y[g]);
       tc_before();
       bar_arrive(&oe_empty);
-      if (!__all_sync(0xffffffffu, bar_wait(&o_full, i & 1, &failed))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(&o_full, i & 1, limit))) break;
       tc_after();
       const float fi = kHalf ? p_inv[i & 1][t] : 1.0f;
 #pragma unroll
@@ -798,7 +812,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     bool ok = true;
     for (int i = 0; i <= chunks && ok; ++i) {
       if (i > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(&u_full, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&u_full, (i - 1) & 1, limit));
         if (!ok) break;
         tc_after();
         const int left = w.end - (w.begin + (i - 1) * C);
@@ -817,7 +831,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         tc_before();
         bar_arrive(&u_empty);
         if (i == chunks) break;
-        ok = __all_sync(0xffffffffu, bar_wait(&oe_full, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&oe_full, (i - 1) & 1, limit));
         if (!ok) break;
       }
       if (chunks == 0) break;
@@ -836,7 +850,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           s_most[warp - 20] = most;
           bar_arrive(&most_full);
         }
-        ok = __all_sync(0xffffffffu, bar_wait(&most_full, i & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&most_full, i & 1, limit));
         if (!ok) break;
         most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
         float inv;
@@ -874,7 +888,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     for (; issued < 3 * chunks; ++issued) {
       const int i = issued / 3, which = issued % 3, st = i % S;
       uint64_t* empty = which == 0 ? k_empty : (which == 1 ? q_empty : v_empty);
-      ok = __all_sync(0xffffffffu, bar_wait(&empty[st], (i / S - 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&empty[st], (i / S - 1) & 1, limit));
       if (!ok) break;
       if (one) load(issued);
       __syncwarp();
@@ -883,7 +897,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       for (int j = issued > 3 * S ? issued - 3 * S : 0; j < issued; ++j) {
         const int i = j / 3, which = j % 3;
         uint64_t* bar = which == 0 ? k_full : (which == 1 ? q_full : v_in);
-        bar_drain(&bar[i % S], (i / S) & 1);
+        bar_drain(&bar[i % S], (i / S) & 1, limit);
       }
     }
   } else if (warp > 1) {
@@ -905,8 +919,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       if (i >= 0) {
         const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
         const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
-        ok = bar_wait(&v_full[0], i & 1, &failed) &&
-             (i == 0 || bar_wait(&u_empty, (i - 1) & 1, &failed));
+        ok = bar_wait(&v_full[0], i & 1, limit) &&
+             (i == 0 || bar_wait(&u_empty, (i - 1) & 1, limit));
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (one) {
@@ -915,7 +929,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           tc_commit(&v_free[0]);
         }
         __syncwarp();
-        ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, &failed));
+        ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, limit));
         if (!ok) break;
         if (one) {
           tc_after();
@@ -925,8 +939,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           tc_commit(&k_empty[i % S]);
         }
         __syncwarp();
-        ok = bar_wait(&s_full, i & 1, &failed) &&
-             (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, &failed));
+        ok = bar_wait(&s_full, i & 1, limit) &&
+             (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, limit));
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (one) {
@@ -942,13 +956,13 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         // Oi of the chunk before is out: its buffer takes the next scores.  (The wait is also due
         // before P V, whose o frees the other buffer: no barrier may be two phases ahead of who
         // waits for it.)
-        ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, &failed));
+        ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, limit));
         if (!ok) break;
       }
       const int n = i + 1;
       if (n < chunks) {
-        ok = bar_wait(&k_full[n % S], (n / S) & 1, &failed) &&
-             bar_wait(&q_full[n % S], (n / S) & 1, &failed);
+        ok = bar_wait(&k_full[n % S], (n / S) & 1, limit) &&
+             bar_wait(&q_full[n % S], (n / S) & 1, limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (one) {
@@ -966,7 +980,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         __syncwarp();
       }
       if (i < 0) continue;
-      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, limit));
       if (!ok) break;
       if (one) {
         tc_after();
@@ -983,7 +997,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     if (!ok) {  // let the products in flight end before TMEM goes
       if (one) tc_commit(&drain);
       __syncwarp();
-      bar_drain(&drain, 0);
+      bar_drain(&drain, 0, limit);
     }
   }
   // rows after the sequence's end
@@ -1015,7 +1029,7 @@ constexpr int kStateThreads = 576;  // V' (and the result): 16 warps, products: 
 template <typename T, int DK>
 __global__ void __launch_bounds__(kStateThreads, 1)
 linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant__ Maps maps,
-                        int* error) {
+                        int* error, unsigned extra_tx) {
   using Z = Smem<T, DK>;
   constexpr int R = kStateRows;
   constexpr int S = Z::st_stages;
@@ -1025,6 +1039,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   __shared__ uint64_t full[S], v_full[NB], used[S], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
+  const Limit limit{&failed, extra_tx == 0 ? kWaitCycles : kTestCycles};
   const Where w = locate(call);
   const Job& job = *w.job;
   if (w.seg >= w.last) return;  // the whole block
@@ -1058,17 +1073,17 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
         const int age = w.end - job.off - (w.begin + i * R + (job.reverse ? R - 1 - r : r));
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
       }
-      if (!bar_wait(&full[i % S], (i / S) & 1, &failed)) break;
+      if (!bar_wait(&full[i % S], (i / S) & 1, limit)) break;
       const bool ok = split_values<T>(
           sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
           sm + Z::st_parts + i % NB * kParts<T> * kStatePanel, kStatePanel, weight, tid,
           // the products of block i - NB have ended
-          [&] { return i < NB || bar_wait(&used[(i - NB) % S], ((i - NB) / S) & 1, &failed); });
+          [&] { return i < NB || bar_wait(&used[(i - NB) % S], ((i - NB) / S) & 1, limit); });
       if (!ok) break;
       fence_async();
       bar_arrive(&v_full[i % NB]);
     }
-    if (warp < 4 && __all_sync(0xffffffffu, bar_wait(&done, 0, &failed)) && !failed) {
+    if (warp < 4 && __all_sync(0xffffffffu, bar_wait(&done, 0, limit)) && !failed) {
       tc_after();
       const int r = DK == 128 ? warp * 32 + lane : warp * 16 + (lane & 15);
       const bool in = (DK == 128 || lane < 16) && r < job.dk;
@@ -1095,27 +1110,27 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     bool ok = true;
     for (; issued < chunks && ok; ++issued) {
       const int i = issued, st = i % S;
-      ok = __all_sync(0xffffffffu, i < S || bar_wait(&used[st], (i / S - 1) & 1, &failed));
+      ok = __all_sync(0xffffffffu, i < S || bar_wait(&used[st], (i / S - 1) & 1, limit));
       if (!ok) break;
       if (one) {
         const int l0 = w.begin + i * R;
         const int token = job.reverse ? w.n - R - l0 : l0;
         const uint32_t at = base + st * Z::st_stage;
-        bar_expect(&full[st], Z::st_stage);
+        bar_expect(&full[st], Z::st_stage + (i == 0 && first_block() ? extra_tx : 0));
         k.template load<R>(at, 0, Z::panels, token, &full[st]);
         v.template load<R>(at + Z::panels * kStatePanel, w.v0, 1, token, &full[st]);
       }
       __syncwarp();
     }
     if (!ok) {  // copies in flight land before the block ends
-      for (int i = issued > S ? issued - S : 0; i < issued; ++i) bar_drain(&full[i % S], (i / S) & 1);
+      for (int i = issued > S ? issued - S : 0; i < issued; ++i) bar_drain(&full[i % S], (i / S) & 1, limit);
     }
   } else {
     const uint32_t ok0 = operand(base, kStatePanel), op0 = operand(base + Z::st_parts, kStatePanel);
     const bool one = elect_one();
     bool ok = true;
     for (int i = 0; i < chunks && ok; ++i) {
-      ok = __all_sync(0xffffffffu, bar_wait(&v_full[i % NB], (i / NB) & 1, &failed));
+      ok = __all_sync(0xffffffffu, bar_wait(&v_full[i % NB], (i / NB) & 1, limit));
       if (!ok) break;
       const uint32_t k = ok0 + (i % S) * (Z::st_stage / 16);
       const uint32_t parts = op0 + (i % NB) * (kParts<T> * kStatePanel / 16);
@@ -1130,7 +1145,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     // also after a failed wait: the products in flight end before TMEM goes
     if (one) tc_commit(&done);
     __syncwarp();
-    bar_drain(&done, 0);
+    bar_drain(&done, 0, limit);
   }
   tc_before();
   __syncthreads();
@@ -1187,7 +1202,7 @@ template <typename T, int DK>
 int launch_as(const Call& call, const Maps& maps, bool states, cudaStream_t stream) {
   auto kernel = states ? linattn_tc_state_kernel<T, DK> : linattn_tc_kernel<T, DK>;
   const int64_t heads = call.batch * call.heads;
-  const dim3 grid(static_cast<unsigned>(call.tiles), static_cast<unsigned>(heads),
+  const dim3 grid(static_cast<unsigned>(heads * call.tiles),
                   static_cast<unsigned>(states ? call.nseg - 1 : call.nseg));
   int* error = device_error_flag();
   if (error == nullptr) return FDWT_ERR_CUDA;
@@ -1195,7 +1210,8 @@ int launch_as(const Call& call, const Maps& maps, bool states, cudaStream_t stre
   if (st == FDWT_OK) st = pre_launch(stream);
   if (st != FDWT_OK) return st;
   kernel<<<grid, states ? kStateThreads : kThreads,
-           states ? Smem<T, DK>::st_bytes : Smem<T, DK>::bytes, stream>>>(call, maps, error);
+           states ? Smem<T, DK>::st_bytes : Smem<T, DK>::bytes, stream>>>(call, maps, error,
+                                                                          copy_wait_test().extra_tx);
   return launch_status();
 }
 
