@@ -40,46 +40,22 @@ class _Desc(ctypes.Structure):
                 ("o_stride", ctypes.c_int64 * 3), ("scale", ctypes.c_double)]
 
 
-@lru_cache(maxsize=1024)
-def _describe(dtype, batch, length, heads, kv_heads, dk, dv, qs, ks, vs, os, scale,
-              device_index) -> Tuple[_Desc, int, int, int]:
-    """The C descriptor of a call, its address and the workspace bytes of the forward and the
-    backward pass: pure functions of the sizes on one device (the library only reads it)."""
-    d = _Desc(dtype, heads, kv_heads, dk, dv, batch, length)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = qs, ks, vs, os
-    d.scale = scale
-    lib = _lib.load()
-    at = ctypes.addressof(d)
-    return (d, at, int(lib.fdwt_linattn_forward_workspace(at)),
-            int(lib.fdwt_linattn_backward_workspace(at)))
-
-
-def _acc(dtype: torch.dtype) -> torch.dtype:
-    return torch.float64 if dtype == torch.float64 else torch.float32
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with a contiguous last axis (any other strides are taken as they are)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
-    return t.stride()[:3]
-
-
-def _check_heads(q, k, v, log_decay, names):
-    """Types and sizes shared by both forms; the head axis is the last but one."""
-    _lib.require_cuda(q, k, v, log_decay)
-    code = _lib.dtype_code(q.dtype)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    qs, ks, vs = q.shape, k.shape, v.shape
-    if len(qs) != len(names) or len(ks) != len(qs) or len(vs) != len(qs):
-        raise ValueError(f"expected q, k, v of shape ({', '.join(names)}), got {tuple(qs)}, "
-                         f"{tuple(ks)}, {tuple(vs)}")
+@lru_cache(maxsize=2048)
+def _describe(names, dtypes, shapes, strides, out_stride, scale, device_index):
+    """What a call's types, sizes and strides come to, checked once for each combination on one
+    device: the C descriptor and its address, the workspace bytes of the forward and the backward
+    pass, and the type of states.  The shapes and strides are (..., heads, size) of q, k and v;
+    ``out_stride`` None stands for a contiguous result."""
+    code = _lib.dtype_code(dtypes[0])
+    if dtypes[1] != dtypes[0] or dtypes[2] != dtypes[0]:
+        raise TypeError("q, k and v must have one type, got "
+                        f"{dtypes[0]}, {dtypes[1]}, {dtypes[2]}")
+    qs, ks, vs = (tuple(s) for s in shapes)
+    if not len(qs) == len(ks) == len(vs) == len(names):
+        raise ValueError(f"expected q, k, v of shape ({', '.join(names)}), got {qs}, {ks}, {vs}")
     if ks[:-2] != qs[:-2] or vs[:-1] != ks[:-1]:
         raise ValueError(f"q, k and v must agree in {', '.join(names[:-2])} and k and v in their "
-                         f"heads, got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+                         f"heads, got {qs}, {ks}, {vs}")
     heads, dk = qs[-2:]
     kv_heads, dv = vs[-2:]
     if ks[-1] != dk:
@@ -89,12 +65,43 @@ def _check_heads(q, k, v, log_decay, names):
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"the query heads must be a multiple of the key and value heads, got "
                          f"{heads} and {kv_heads}")
+    batch, length = qs[0], qs[1] if len(qs) == 4 else 1
+
+    def three(stride):  # batch, token, head; the single-token form has no token axis
+        return stride[:3] if len(qs) == 4 else (stride[0], 0, stride[1])
+
+    d = _Desc(code, heads, kv_heads, dk, dv, batch, length)
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = (three(s) for s in strides)
+    d.o_stride[:] = ((length * heads * dv, heads * dv, dv) if out_stride is None
+                     else three(out_stride))
+    d.scale = float(dk) ** -0.5 if scale is None else float(scale)
+    lib = _lib.load()
+    at = ctypes.addressof(d)
+    state = torch.float64 if code == 1 else torch.float32
+    return (d, at, int(lib.fdwt_linattn_forward_workspace(at)),
+            int(lib.fdwt_linattn_backward_workspace(at)), state)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with a contiguous last axis (any other strides are taken as they are)."""
+    return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _plan(names, q, k, v, scale, out_stride=None):
+    return _describe(names, (q.dtype, k.dtype, v.dtype), (q.shape, k.shape, v.shape),
+                     (q.stride(), k.stride(), v.stride()), out_stride, scale, q.device.index)
+
+
+def _schedule(log_decay, heads: int, dtype: torch.dtype) -> torch.Tensor:
+    """``log_decay (heads,)`` contiguous in the states' type."""
     if log_decay.shape != (heads,) or not log_decay.is_floating_point():
         raise ValueError(f"log_decay must be floating point of shape ({heads},), got "
                          f"{log_decay.dtype} {tuple(log_decay.shape)}")
     if log_decay.requires_grad:
         raise ValueError("log_decay is a fixed schedule without a gradient; detach it")
-    return code, heads, kv_heads, dk, dv
+    if log_decay.dtype != dtype or not log_decay.is_contiguous():
+        log_decay = log_decay.to(dtype).contiguous()
+    return log_decay
 
 
 def _check_state(state, shape, dtype):
@@ -113,21 +120,24 @@ def _indexes(t: torch.Tensor, count: int, low: int, high: int, name: str) -> tor
     return t.contiguous()
 
 
-def _forward(q, k, v, log_decay, initial, lengths, scale, sizes):
-    code, heads, kv_heads, dk, dv = sizes
-    batch, length = q.shape[:2]
+_SEQUENCE, _TOKEN = ("B", "L", "H", "D"), ("B", "H", "D")
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(q, k, v, log_decay, initial, lengths, plan):
+    d, desc, nws, _, acc = plan
     dev = q.device
-    out = torch.empty((batch, length, heads, dv), device=dev, dtype=q.dtype)
-    final = torch.empty((batch, heads, dk, dv), device=dev, dtype=log_decay.dtype)
+    out = torch.empty((d.batch, d.length, d.heads, d.dv), device=dev, dtype=q.dtype)
+    final = torch.empty((d.batch, d.heads, d.dk, d.dv), device=dev, dtype=acc)
     with _lib.device_guard(dev):
-        _, desc, nws, _ = _describe(code, batch, length, heads, kv_heads, dk, dv, _strides(q),
-                                    _strides(k), _strides(v), _strides(out), scale, dev.index)
         ws = _lib.workspace(nws, dev)
         st = _lib.load().fdwt_linattn_forward(
-            desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-            None if initial is None else initial.data_ptr(),
-            None if lengths is None else lengths.data_ptr(), out.data_ptr(), final.data_ptr(),
-            None if ws is None else ws.data_ptr(), nws, _lib.raw_stream(dev.index))
+            desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(initial),
+            _ptr(lengths), out.data_ptr(), final.data_ptr(), _ptr(ws), nws,
+            _lib.raw_stream(dev.index))
     if st:
         _lib.check(st, "fdwt_linattn_forward")
     if config.check_device_errors:
@@ -140,11 +150,11 @@ class _LinearAttentionFunction(torch.autograd.Function):
     back in time (one C call)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, initial, lengths, scale, sizes):
+    def forward(ctx, q, k, v, log_decay, initial, lengths, scale, plan):
         ctx.set_materialize_grads(False)
-        ctx.scale, ctx.sizes = scale, sizes
+        ctx.scale, ctx.plan = scale, plan
         ctx.save_for_backward(q, k, v, log_decay, initial, lengths)
-        return _forward(q, k, v, log_decay, initial, lengths, scale, sizes)
+        return _forward(q, k, v, log_decay, initial, lengths, plan)
 
     @staticmethod
     @once_differentiable
@@ -152,28 +162,26 @@ class _LinearAttentionFunction(torch.autograd.Function):
         q, k, v, log_decay, initial, lengths = ctx.saved_tensors
         if d_out is None and d_final is None:
             return (None,) * 8
-        code, heads, kv_heads, dk, dv = ctx.sizes
-        batch, length = q.shape[:2]
+        plan = ctx.plan
+        d = plan[0]
         dev = q.device
         if d_out is None:
-            d_out = torch.zeros((batch, length, heads, dv), device=dev, dtype=q.dtype)
-        d_out = _rows(d_out)
-        d_final = None if d_final is None else d_final.contiguous()
+            d_out = torch.zeros((d.batch, d.length, d.heads, d.dv), device=dev, dtype=q.dtype)
+        elif not d_out.is_contiguous():
+            d_out = _rows(d_out)
+            plan = _plan(_SEQUENCE, q, k, v, ctx.scale, d_out.stride())
+        if d_final is not None:
+            d_final = d_final.contiguous()
         dq, dkk, dvv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
-        need_state = ctx.needs_input_grad[4]
-        d_initial = torch.empty_like(initial) if need_state else None
+        d_initial = torch.empty_like(initial) if ctx.needs_input_grad[4] else None
+        _, desc, _, nws, _ = plan
         with _lib.device_guard(dev):
-            _, desc, _, nws = _describe(code, batch, length, heads, kv_heads, dk, dv, _strides(q),
-                                        _strides(k), _strides(v), _strides(d_out), ctx.scale,
-                                        dev.index)
             ws = _lib.workspace(nws, dev)
             st = _lib.load().fdwt_linattn_backward(
                 desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-                None if initial is None else initial.data_ptr(),
-                None if lengths is None else lengths.data_ptr(), d_out.data_ptr(),
-                None if d_final is None else d_final.data_ptr(), dq.data_ptr(), dkk.data_ptr(),
-                dvv.data_ptr(), None if d_initial is None else d_initial.data_ptr(),
-                None if ws is None else ws.data_ptr(), nws, _lib.raw_stream(dev.index))
+                _ptr(initial), _ptr(lengths), d_out.data_ptr(), _ptr(d_final), dq.data_ptr(),
+                dkk.data_ptr(), dvv.data_ptr(), _ptr(d_initial), _ptr(ws), nws,
+                _lib.raw_stream(dev.index))
         if st:
             _lib.check(st, "fdwt_linattn_backward")
         if config.check_device_errors:
@@ -204,26 +212,22 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     and initial_state.  fp16 and bf16 round the scores and the state's copy that multiplies q to
     16 bits; the state itself is fp32.
     """
-    sizes = _check_heads(q, k, v, log_decay, ("B", "L", "H", "D"))
-    code, heads, kv_heads, dk, dv = sizes
-    batch, length = q.shape[:2]
-    acc = _acc(q.dtype)
-    if log_decay.dtype != acc or not log_decay.is_contiguous():
-        log_decay = log_decay.to(acc).contiguous()
-    if initial_state is not None:
-        _lib.require_cuda(q, initial_state)
-        _check_state(initial_state, (batch, heads, dk, dv), acc)
-        initial_state = initial_state.contiguous()
-    if lengths is not None:
-        _lib.require_cuda(q, lengths)
-        lengths = _indexes(lengths, batch, 0, length, "lengths")
-    scale = float(dk) ** -0.5 if scale is None else float(scale)
+    _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (
-            initial_state is not None and initial_state.requires_grad)):
+    plan = _plan(_SEQUENCE, q, k, v, scale)
+    d, acc = plan[0], plan[4]
+    log_decay = _schedule(log_decay, d.heads, acc)
+    needs = q.requires_grad or k.requires_grad or v.requires_grad
+    if initial_state is not None:
+        _check_state(initial_state, (d.batch, d.heads, d.dk, d.dv), acc)
+        initial_state = initial_state.contiguous()
+        needs = needs or initial_state.requires_grad
+    if lengths is not None:
+        lengths = _indexes(lengths, d.batch, 0, d.length, "lengths")
+    if needs and torch.is_grad_enabled():
         return _LinearAttentionFunction.apply(q, k, v, log_decay, initial_state, lengths, scale,
-                                              sizes)
-    return _forward(q, k, v, log_decay, initial_state, lengths, scale, sizes)
+                                              plan)
+    return _forward(q, k, v, log_decay, initial_state, lengths, plan)
 
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -239,37 +243,26 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     touches no state and gives a zero output row.  Two sequences must not name the same slot.
     No gradient: training runs on :func:`linear_attention`.
     """
-    sizes = _check_heads(q, k, v, log_decay, ("B", "H", "D"))
-    code, heads, kv_heads, dk, dv = sizes
-    batch = q.shape[0]
-    acc = _acc(q.dtype)
-    _lib.require_cuda(q, state, slots)
-    pool = state.shape[0] if state.dim() == 4 and slots is not None else batch
-    _check_state(state, (pool, heads, dk, dv), acc)
+    _lib.require_cuda(q, k, v, log_decay, state, slots)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    d, desc, _, _, acc = _plan(_TOKEN, q, k, v, scale)
+    log_decay = _schedule(log_decay, d.heads, acc)
+    pool = state.shape[0] if state.dim() == 4 and slots is not None else d.batch
+    _check_state(state, (pool, d.heads, d.dk, d.dv), acc)
     if not state.is_contiguous():
         raise ValueError("the state is updated in place and must be contiguous")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or state.requires_grad):
+    if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) \
+            and torch.is_grad_enabled():
         raise RuntimeError("linear_attention_step has no gradient: use linear_attention, or "
                            "torch.no_grad()")
     if slots is not None:
-        slots = _indexes(slots, batch, -1, pool, "slots")
-    if log_decay.dtype != acc or not log_decay.is_contiguous():
-        log_decay = log_decay.to(acc).contiguous()
-    scale = float(dk) ** -0.5 if scale is None else float(scale)
-    q, k, v = _rows(q), _rows(k), _rows(v)
+        slots = _indexes(slots, d.batch, -1, pool, "slots")
     dev = q.device
-    out = torch.empty((batch, heads, dv), device=dev, dtype=q.dtype)
-    # (batch, head) strides with an unused token stride between them
+    out = torch.empty((d.batch, d.heads, d.dv), device=dev, dtype=q.dtype)
     with _lib.device_guard(dev):
-        _, desc, _, _ = _describe(code, batch, 1, heads, kv_heads, dk, dv,
-                                  (q.stride(0), 0, q.stride(1)), (k.stride(0), 0, k.stride(1)),
-                                  (v.stride(0), 0, v.stride(1)), (heads * dv, 0, dv), scale,
-                                  dev.index)
         st = _lib.load().fdwt_linattn_step(
             desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-            state.data_ptr(), pool, None if slots is None else slots.data_ptr(), out.data_ptr(),
-            _lib.raw_stream(dev.index))
+            state.data_ptr(), pool, _ptr(slots), out.data_ptr(), _lib.raw_stream(dev.index))
     if st:
         _lib.check(st, "fdwt_linattn_step")
     return out
