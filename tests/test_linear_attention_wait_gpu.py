@@ -65,3 +65,39 @@ def test_many_sequences_and_heads():
     # scores, the state's copy and the result rounded once each (unit roundoff 2^-8)
     assert (out[part].float() - ref).square().mean().sqrt() <= 2 * 2.0 ** -8 * ref.square().mean().sqrt()
     assert (state[part] - last).abs().max() <= 1e-4 * last.abs().max()
+
+
+@pytest.mark.parametrize("word", [0xFFFFFFFF, 0x7F800000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("length,Dk,Dv", [(70, 24, 40), (1500, 128, 72), (3000, 64, 64)])
+def test_nothing_depends_on_what_shared_memory_held(length, Dk, Dv, dtype, word):
+    """With all of shared memory set to NaN (infinity) before every kernel the results keep their
+    bits: forward, gradients, a token, and the norm."""
+    torch.manual_seed(7)
+    q = torch.randn(2, length, 2, Dk, device=DEV).to(dtype)
+    k = torch.randn(2, length, 1, Dk, device=DEV).to(dtype)
+    v = torch.randn(2, length, 1, Dv, device=DEV).to(dtype)
+    do = torch.randn(2, length, 2, Dv, device=DEV).to(dtype)
+    a = torch.tensor([-0.3, -0.002], device=DEV)
+    n = torch.tensor([length, length // 3], device=DEV)
+    x, w = do.reshape(-1, 2 * Dv), torch.randn(2 * Dv, device=DEV).to(dtype)
+
+    def everything():
+        ts = [t.detach().requires_grad_() for t in (q, k, v)]
+        out, state = F.linear_attention(*ts, a, lengths=n)
+        results = [out, state, *torch.autograd.grad(out, ts, do)]
+        carried = state.detach().clone()
+        results += [F.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], a, carried), carried]
+        ps = [t.detach().requires_grad_() for t in (x, w)]
+        y = F.layer_norm(*ps)
+        return results + [y, *torch.autograd.grad(y, ps, y.detach())]
+
+    want = everything()
+    _lib.set_shared_memory_fill(True, word)
+    try:
+        got = everything()
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_shared_memory_fill(False)
+    for g, r in zip(got, want):
+        assert torch.equal(g, r)
