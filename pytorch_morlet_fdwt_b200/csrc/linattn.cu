@@ -786,7 +786,7 @@ inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t siz
          strides[1] % v == 0 && strides[2] % v == 0;
 }
 
-constexpr int kShort = 64;
+constexpr int kShort = 64, kFewRows = 2048;
 
 struct Plan {
   bool tc;
@@ -862,9 +862,12 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
     job.o_vec = vector_ok(job.o, job.os, job.dv, o_size, 16) +
                 vector_ok(job.o, job.os, job.dv, o_size, 32);
   }
-  // One short chunk goes to the general kernel: as fast there, and without the 16-bit rounding of
-  // the scores, which few rows do not average out.
-  const bool tc = call.length > kShort && tc_supports(dtype, call);
+  // One short chunk goes to the general kernel: as fast there (64 tokens of 4 heads of 64: 12.5 us
+  // against 10.5, less than a call's host time), and without the 16-bit rounding of the scores,
+  // which few rows do not average out.  So do two of them with few rows in all.
+  const int64_t rows = call.batch * call.heads * call.length;
+  const bool small = call.length <= kShort || (call.length <= 2 * kShort && rows <= kFewRows);
+  const bool tc = !small && tc_supports(dtype, call);
   const Plan p = make_plan(dtype, call, tc);
   call.nseg = p.nseg;
   call.seg_len = p.seg_len;

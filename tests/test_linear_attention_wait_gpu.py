@@ -17,7 +17,7 @@ DEV = "cuda"
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("D,length", [(64, 100), (128, 700), (64, 9000)])
+@pytest.mark.parametrize("D,length", [(64, 300), (128, 700), (64, 9000)])
 def test_wait_that_runs_out_sets_the_error_word(dtype, D, length):
     torch.manual_seed(5)
     q, k, v = (torch.randn(1, length, 2, D, device=DEV).to(dtype) for _ in range(3))
