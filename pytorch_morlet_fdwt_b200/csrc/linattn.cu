@@ -36,7 +36,8 @@ __device__ __forceinline__ int64_t token_of(int64_t l, int64_t n, int reverse) {
 // rows x cols of a tensor (row l at base + token * stride) into shared memory, zeros past
 // `valid` rows and `cols` columns.  256 threads; where no conversion is due and rows are aligned
 // the copies are asynchronous (tiles_wait() below), else all loads are issued before the stores:
-// one latency a tile instead of one a group (15.6 -> 4 us a chunk on one block).
+// one latency a tile instead of one a group (5 x 1537 tokens, 6 heads of 48 x 80, fp32: state
+// launch 50 -> 33 us, main launch 113 -> 96 us).
 template <typename T, typename A, int ROWS, int COLS, int PITCH>
 __device__ __forceinline__ void load_tile(A* dst, const T* base, int64_t stride, int64_t l0,
                                           int64_t n, int reverse, int valid, int cols, int vec) {
@@ -680,6 +681,8 @@ linattn_group_sum_kernel(const typename AccOf<T>::type* __restrict__ in, T* __re
 // S <- d S + k v^T, o = scale q^T S.  Bound by reading and writing S: a block holds all rows of
 // `lanes` groups of V columns, so that each S value is read and written once, in 16-byte
 // accesses, 8 rows of a thread in flight; the products of the rows are joined in shared memory.
+// Measured: 240 x 16 heads of 128 x 128 94 us (503 MB, 5.3 TB/s; streaming hints 92, but 20.1 in
+// place of 18.7 us where the states fit L2); one head's 64 x 64 4.3 us.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 linattn_step_kernel(const __grid_constant__ fdwt_linattn_desc d, const T* __restrict__ q,
