@@ -281,12 +281,13 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
         }
       }
     }
-    // state
+    // state: the chunk's sum first, so that long sequences add up by chunks
     const A keep = decay_pow(a, A(m));
+    A sum[TD][TN];
 #pragma unroll
     for (int i = 0; i < TD; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) s[i][j] *= keep;
+      for (int j = 0; j < TN; ++j) sum[i][j] = A(0);
 #pragma unroll 4
     for (int u = 0; u < C; ++u) {
       Pack<A, TN> y = *reinterpret_cast<const Pack<A, TN>*>(sv + u * NV + tx * TN);
@@ -297,9 +298,13 @@ linattn_simt_kernel(const __grid_constant__ Call call) {
       for (int i = 0; i < TD; ++i) {
         const A x = sk[u * PK + ty + 16 * i];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) s[i][j] += x * y.v[j];
+        for (int j = 0; j < TN; ++j) sum[i][j] += x * y.v[j];
       }
     }
+#pragma unroll
+    for (int i = 0; i < TD; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) s[i][j] = keep * s[i][j] + sum[i][j];
     if (!STATES) {
 #pragma unroll
       for (int i = 0; i < TD; ++i)
@@ -789,7 +794,7 @@ inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t siz
          strides[1] % v == 0 && strides[2] % v == 0;
 }
 
-constexpr int kShort = 64, kFewRows = 2048;
+constexpr int kShort = 64, kFewRows = 512;
 
 struct Plan {
   bool tc;

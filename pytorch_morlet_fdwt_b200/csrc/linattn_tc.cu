@@ -1045,11 +1045,26 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   const Limit limit{&failed, extra_tx == 0 ? kWaitCycles : kTestCycles};
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const Where w = locate(call);
   const Job& job = *w.job;
   if (w.seg >= w.last) return;  // the whole block
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) {
+  if (warp == 16) tmem_alloc(&tmem_slot);
+  const uint32_t base = smem_addr(sm);
+  const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
+  auto load = [&](int i) {
+    const int st = i % S, l0 = w.begin + i * R;
+    const int token = job.reverse ? w.n - R - l0 : l0;
+    const uint32_t at = base + st * Z::st_stage;
+    const CUtensorMap* map = maps.map[w.ji];
+    bar_expect(&full[st], Z::st_stage + (i == 0 && first_block() ? extra_tx : 0));
+    Source(map + 1, job.ks, w.h / job.k_group, w.b)
+        .template load<R>(at, 0, Z::panels, token, &full[st]);
+    Source(map + 2, job.vs, w.h / job.v_group, w.b)
+        .template load<R>(at + Z::panels * kStatePanel, w.v0, 1, token, &full[st]);
+  };
+  const int first_loads = chunks < S ? chunks : S;
+  if (threadIdx.x == 17 * 32) {
     for (int i = 0; i < NB; ++i) bar_init(&v_full[i], 128);
     for (int i = 0; i < S; ++i) {
       bar_init(&full[i], 1);
@@ -1058,16 +1073,17 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
     bar_init(&done, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+#pragma unroll 1
+    for (int i = 0; i < first_loads; ++i) load(i);
   }
-  if (warp == 16) tmem_alloc(&tmem_slot);
+  __syncwarp();
   tc_before();
   __syncthreads();
   tc_after();
   // every block is on its way: blocks of the main launch may take the multiprocessors left over
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  const uint32_t base = smem_addr(sm);
-  const int chunks = w.chunks * (C / R);  // whole ones: every segment before the last is full
 
   if (warp < 4 * kGroups) {
     // groups of four warps take the blocks of 64 tokens by turns
@@ -1103,33 +1119,25 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
         load_update<T>(tmem + (uint32_t(warp * 32) << 16) + g, x);
         if (in) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            if (g + c < w.vcols) dst[g + c] = write * x[c];
+          for (int c = 0; c < 8; ++c) x[c] *= write;
+          if (g < w.vcols)
+            store8(dst + g, __float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                   __float_as_uint(x[3]), __float_as_uint(x[4]), __float_as_uint(x[5]),
+                   __float_as_uint(x[6]), __float_as_uint(x[7]));
         }
       }
     }
   } else if (warp == 17) {
-    const CUtensorMap* map = maps.map[w.ji];
-    const Source k(map + 1, job.ks, w.h / job.k_group, w.b),
-        v(map + 2, job.vs, w.h / job.v_group, w.b);
     const bool one = elect_one();
-    int issued = 0;
+    int issued = first_loads;
     bool ok = true;
-    for (; issued < chunks && ok; ++issued) {
-      const int i = issued, st = i % S;
-      ok = __all_sync(0xffffffffu, i < S || bar_wait(&used[st], (i / S - 1) & 1, limit));
+    for (; issued < chunks; ++issued) {
+      ok = __all_sync(0xffffffffu, bar_wait(&used[issued % S], (issued / S - 1) & 1, limit));
       if (!ok) break;
-      if (one) {
-        const int l0 = w.begin + i * R;
-        const int token = job.reverse ? w.n - R - l0 : l0;
-        const uint32_t at = base + st * Z::st_stage;
-        bar_expect(&full[st], Z::st_stage + (i == 0 && first_block() ? extra_tx : 0));
-        k.template load<R>(at, 0, Z::panels, token, &full[st]);
-        v.template load<R>(at + Z::panels * kStatePanel, w.v0, 1, token, &full[st]);
-      }
+      if (one) load(issued);
       __syncwarp();
     }
-    if (!ok) {  // copies in flight land before the block ends
+    if (!ok || failed) {  // copies in flight land before the block ends
       for (int i = issued > S ? issued - S : 0; i < issued; ++i) bar_drain(&full[i % S], (i / S) & 1, limit);
     }
   } else {
