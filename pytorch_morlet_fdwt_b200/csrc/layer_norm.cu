@@ -9,8 +9,8 @@
 // Sums, statistics and the gradients' partial sums are 32 bits (64 for fp64 rows).
 //
 // Measured: 65536 x 2048 bf16 forward 96 us (5.6 TB/s), backward 166 us (4.9 TB/s); 65536 x 1024
-// fp32 89 and 133 us (6.0 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
-// 78 and 114 us (4.1 and 4.2 TB/s, bound by the latency of single-element loads).
+// fp32 88 and 132 us (6.1 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
+// 54 and 113 us (5.9 and 4.2 TB/s, the backward bound by its instructions for single elements).
 #include <type_traits>
 
 #include "common.cuh"
@@ -141,6 +141,18 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A* slot) {
   for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? slot[i * 32 + lane] : A(0));
 }
 
+// The sum of one value over the NT threads of a row, NT known when compiling (whole warps).
+template <int NT, typename A> __device__ __forceinline__ void row_sum_of(A& v, A* slot) {
+  v = warp_sum(v);
+  if constexpr (NT > 32) {
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = slot[0];
+#pragma unroll
+    for (int w = 1; w < NT / 32; ++w) v += slot[w];
+  }
+}
+
 template <typename A> __device__ __forceinline__ A inv_sqrt(A v);
 template <> __device__ __forceinline__ float inv_sqrt(float v) { return 1.0f / sqrtf(v); }
 template <> __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
@@ -152,11 +164,24 @@ constexpr int fwd_max_threads(int e) { return e <= 16 ? 1024 : (e <= 32 ? 512 : 
 // (65536 x 2048 bf16: 106 us without, 96 us with).
 constexpr int fwd_min_blocks(int e) { return e <= 8 ? 2 : (e <= 16 ? 1 : (e <= 32 ? 2 : 3)); }
 
+// Single elements and pairs cost many instructions a byte, and with addresses and conditions worked
+// out for every one of them the kernel is bound by those (85 % of issue slots, 40000 x 1001 fp32:
+// 78 us, bf16: 86 us).  Their rows of more than 128 groups therefore take a number of threads
+// known when compiling (NT, 32 to 512) and the 6 or 8 groups a thread that are enough: the offsets
+// become constants and only the last two groups need a condition (54 and 50 us).
+constexpr int fwd_row_threads(int nt) { return nt == 32 ? 128 : nt; }  // rows a block: 4 or 1
+constexpr int fwd_threads(int e, int nt) { return nt ? fwd_row_threads(nt) : fwd_max_threads(e); }
+constexpr int fwd_blocks(int e, int nt, int size) {
+  return nt ? (e * size <= 32 ? 2048 : (e * size <= 64 ? 1024 : 512)) / fwd_row_threads(nt)
+            : fwd_min_blocks(e);
+}
+
 // A row is held by blockDim.x threads, IT groups of V elements each (group i of thread t starts
 // at (i * blockDim.x + t) * V: neighbouring lanes read neighbouring groups), blockDim.y rows a
 // block (more than one only where a row has at most a warp).
-template <typename T, typename P, int V, int IT>
-__global__ void __launch_bounds__(fwd_max_threads(V * IT), fwd_min_blocks(V * IT))
+template <typename T, typename P, int V, int IT, int NT>
+__global__ void __launch_bounds__(fwd_threads(V * IT, NT),
+                                  fwd_blocks(V * IT, NT, sizeof(typename AccOf<T>::type)))
 layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
                       const P* __restrict__ bias, T* __restrict__ y,
                       typename AccOf<T>::type* __restrict__ stats, int64_t rows, int dim,
@@ -168,29 +193,31 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
   const bool in = row < rows;
   if (!in) row = rows - 1;  // the lanes of a warp stay together
   const T* xr = x + row * dim + threadIdx.x * V;
-  const int step = blockDim.x * V, left = dim - threadIdx.x * V;
+  const int step = (NT ? NT : int(blockDim.x)) * V, left = dim - threadIdx.x * V;
+  constexpr int SURE = NT ? IT - 2 : 0;  // groups that every thread has
   typename G::Raw raw[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i)
-    if (i * step < left) raw[i] = G::load(xr + i * step);
+    if (i < SURE || i * step < left) raw[i] = G::load(xr + i * step);
   A v[IT * V];
   A sum[1] = {A(0)}, part[4] = {A(0), A(0), A(0), A(0)};
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    if (i * step < left) {
+    if (i < SURE || i * step < left) {
       G::values(raw[i], v + i * V);
 #pragma unroll
       for (int j = 0; j < V; ++j) part[(i * V + j) % 4] += v[i * V + j];
     }
   }
   sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
-  row_sum(sum, slots[0]);
+  if constexpr (NT) row_sum_of<NT>(sum[0], slots[0]);
+  else row_sum(sum, slots[0]);
   const A mean = sum[0] / A(dim);
 #pragma unroll
   for (int k = 0; k < 4; ++k) part[k] = A(0);
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    if (i * step < left) {
+    if (i < SURE || i * step < left) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         A& d = v[i * V + j];
@@ -200,7 +227,8 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
     }
   }
   sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
-  row_sum(sum, slots[1]);
+  if constexpr (NT) row_sum_of<NT>(sum[0], slots[1]);
+  else row_sum(sum, slots[1]);
   const A rstd = inv_sqrt(sum[0] / A(dim) + eps);
   if (!in) return;
   if (stats != nullptr && threadIdx.x == 0) {
@@ -210,7 +238,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
   T* yr = y + row * dim + threadIdx.x * V;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    if (i * step < left) {
+    if (i < SURE || i * step < left) {
       A p[V];
       A* d = v + i * V;
 #pragma unroll
@@ -516,6 +544,27 @@ template <typename A> bool backward_shape(int64_t groups, int v, Shape* s) {
   return false;
 }
 
+// Rows of single elements or pairs, more than 128 and at most 4096 groups: threads a power of two,
+// groups a thread 6 or 8, all but the last two of them within the row for every thread.
+inline bool narrow_shape(int64_t groups, Shape* s) {
+  if (groups <= 128 || groups > 4096) return false;
+  int threads = 32;
+  while (threads * 8 < groups) threads *= 2;
+  *s = {threads, threads * 6 >= groups ? 6 : 8, fwd_row_threads(threads) / threads};
+  return true;
+}
+// fn(std::integral_constant<int, threads>) for the threads of narrow_shape.
+template <typename F> int with_threads(int threads, F fn) {
+  switch (threads) {
+    case 32: return fn(std::integral_constant<int, 32>{});
+    case 64: return fn(std::integral_constant<int, 64>{});
+    case 128: return fn(std::integral_constant<int, 128>{});
+    case 256: return fn(std::integral_constant<int, 256>{});
+    case 512: return fn(std::integral_constant<int, 512>{});
+    default: return FDWT_ERR_INVALID;
+  }
+}
+
 // fn(std::integral_constant<int, items>); items V at most `MOST` elements.
 template <int V, int MOST, typename F> int with_items(int items, F fn) {
   switch (items) {
@@ -543,21 +592,31 @@ int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const voi
               void* y, void* stats, bool* done, cudaStream_t stream) {
   using A = typename AccOf<T>::type;
   Shape s;
-  if (!forward_shape(dim / V, V, sizeof(A), &s)) return FDWT_OK;
+  const bool narrow = V <= 2 && narrow_shape(dim / V, &s);
+  if (!narrow && !forward_shape(dim / V, V, sizeof(A), &s)) return FDWT_OK;
   *done = true;
   const dim3 block(s.threads, s.rows);
   const int64_t grid = cdiv(rows, s.rows);
   if (grid > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   const int st = pre_launch(stream);
   if (st != FDWT_OK) return st;
-  return with_items<V, (sizeof(A) == 8 ? 32 : 64)>(s.items, [&](auto items) {
-    constexpr int IT = decltype(items)::value;
-    layer_norm_fwd_kernel<T, P, V, IT><<<static_cast<unsigned>(grid), block, 0, stream>>>(
-        static_cast<const T*>(x), static_cast<const P*>(w), static_cast<const P*>(b),
-        static_cast<T*>(y), static_cast<A*>(stats), rows, static_cast<int>(dim),
-        static_cast<A>(eps));
+  auto launch = [&](auto items, auto threads) {
+    layer_norm_fwd_kernel<T, P, V, decltype(items)::value, decltype(threads)::value>
+        <<<static_cast<unsigned>(grid), block, 0, stream>>>(
+            static_cast<const T*>(x), static_cast<const P*>(w), static_cast<const P*>(b),
+            static_cast<T*>(y), static_cast<A*>(stats), rows, static_cast<int>(dim),
+            static_cast<A>(eps));
     return launch_status();
-  });
+  };
+  if constexpr (V <= 2) {
+    if (narrow)
+      return with_threads(s.threads, [&](auto threads) {
+        return s.items == 6 ? launch(std::integral_constant<int, 6>{}, threads)
+                            : launch(std::integral_constant<int, 8>{}, threads);
+      });
+  }
+  return with_items<V, (V <= 2 ? 16 : sizeof(A) == 8 ? 32 : 64)>(
+      s.items, [&](auto items) { return launch(items, std::integral_constant<int, 0>{}); });
 }
 
 // Elements of a group: 16 bytes, two elements or one, whatever rows and pointers are aligned to.

@@ -83,6 +83,23 @@ def test_forward_and_gradients(rows, dim, dtype):
         assert torch.equal(F.layer_norm(x, w, b, eps), y)
 
 
+# rows that start anywhere, around the lengths at which the threads or the groups a thread change
+ODD = [(11, d) for d in (127, 129, 191, 193, 383, 385, 511, 513, 767, 769, 1023, 1025, 1535, 1537,
+                         2047, 2049, 2999, 4095)]
+PAIRS = [(9, d) for d in (258, 382, 386, 514, 770, 1022, 1026, 1538, 2050, 6146, 8190, 8194)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim", ODD + PAIRS)
+def test_rows_of_single_elements_and_pairs(rows, dim, dtype):
+    x, w, b, _ = _case(rows, dim, dtype, dtype, seed=dim)
+    ry, shift = _reference(x, w, b, 1e-5)
+    spread = (1 + shift + ry.abs()) * w.double().abs().amax() + 2 * b.double().abs().amax()
+    _check(F.layer_norm(x, w, b), ry, dtype, spread, "y")
+    plain, shift = _reference(x, None, None, 1e-5)
+    _check(F.layer_norm(x), plain, dtype, 1 + shift + plain.abs(), "y without parameters")
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_fp32_parameters_and_partial_needs(dtype):
     x, w, b, dy = _case(50, 384, dtype, torch.float32)
