@@ -10,7 +10,7 @@
 //
 // Measured: 65536 x 2048 bf16 forward 96 us (5.6 TB/s), backward 166 us (4.9 TB/s); 65536 x 1024
 // fp32 88 and 132 us (6.1 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
-// 54 and 113 us (5.9 and 4.2 TB/s, the backward bound by its instructions for single elements).
+// 54 and 88 us (5.9 and 5.4 TB/s).
 #include <type_traits>
 
 #include "common.cuh"
@@ -141,15 +141,23 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A* slot) {
   for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? slot[i * 32 + lane] : A(0));
 }
 
-// The sum of one value over the NT threads of a row, NT known when compiling (whole warps).
-template <int NT, typename A> __device__ __forceinline__ void row_sum_of(A& v, A* slot) {
-  v = warp_sum(v);
-  if constexpr (NT > 32) {
-    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = slot[0];
+// The same over NT threads, known when compiling (whole warps).
+template <int NT, typename A, int N>
+__device__ __forceinline__ void row_sum_of(A (&v)[N], A* slot) {
 #pragma unroll
-    for (int w = 1; w < NT / 32; ++w) v += slot[w];
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if constexpr (NT > 32) {
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[i * 32 + (threadIdx.x >> 5)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = slot[i * 32];
+#pragma unroll
+      for (int w = 1; w < NT / 32; ++w) v[i] += slot[i * 32 + w];
+    }
   }
 }
 
@@ -210,7 +218,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
     }
   }
   sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
-  if constexpr (NT) row_sum_of<NT>(sum[0], slots[0]);
+  if constexpr (NT) row_sum_of<NT>(sum, slots[0]);
   else row_sum(sum, slots[0]);
   const A mean = sum[0] / A(dim);
 #pragma unroll
@@ -227,7 +235,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ weight,
     }
   }
   sum[0] = (part[0] + part[1]) + (part[2] + part[3]);
-  if constexpr (NT) row_sum_of<NT>(sum[0], slots[1]);
+  if constexpr (NT) row_sum_of<NT>(sum, slots[1]);
   else row_sum(sum, slots[1]);
   const A rstd = inv_sqrt(sum[0] / A(dim) + eps);
   if (!in) return;
@@ -305,8 +313,15 @@ template <typename A> constexpr int bwd_max_threads(int e) {
   return words <= 4 ? 1024 : (words <= 16 ? 512 : 256);
 }
 
-template <typename T, typename P, int V, int IT>
-__global__ void __launch_bounds__(bwd_max_threads<typename AccOf<T>::type>(V * IT))
+// Rows of single elements and pairs take NT threads and constant offsets as in the forward pass
+// (40000 x 1001: fp32 113 -> 88 us, bf16 113 -> 70 us; 65536 x 491 fp16 118 -> 63 us).
+constexpr int bwd_row_threads(int nt) { return nt == 32 ? 256 : nt; }  // rows a block: 8 or 1
+template <typename A> constexpr int bwd_threads(int e, int nt) {
+  return nt ? bwd_row_threads(nt) : bwd_max_threads<A>(e);
+}
+
+template <typename T, typename P, int V, int IT, int NT>
+__global__ void __launch_bounds__(bwd_threads<typename AccOf<T>::type>(V * IT, NT))
 layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                       const P* __restrict__ weight,
                       const typename AccOf<T>::type* __restrict__ stats, T* __restrict__ dx,
@@ -317,7 +332,9 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
   extern __shared__ __align__(16) unsigned char smem_raw[];
   A* joined = reinterpret_cast<A*>(smem_raw);  // [blockDim.y][2][dim], only blockDim.y > 1
 
-  const int col = threadIdx.x * V, step = blockDim.x * V, left = dim - col;
+  const int col = threadIdx.x * V, left = dim - col;
+  const int step = (NT ? NT : int(blockDim.x)) * V;
+  constexpr int SURE = NT ? IT - 2 / V : 0;  // groups that every thread has
   A dw[IT * V], db[IT * V], w[IT * V];
 #pragma unroll
   for (int e = 0; e < IT * V; ++e) {
@@ -327,7 +344,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
   if (weight != nullptr) {
 #pragma unroll
     for (int i = 0; i < IT; ++i)
-      if (i * step < left) load_params<P, V>(weight + col + i * step, w + i * V);
+      if (i < SURE || i * step < left) load_params<P, V>(weight + col + i * step, w + i * V);
   }
   const int64_t rows_step = int64_t(gridDim.x) * blockDim.y;
   // rows of the block's last round past the end are read as the last row and left out of the sums
@@ -341,7 +358,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     const T* py = dy + r * dim + col;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (i * step < left) {
+      if (i < SURE || i * step < left) {
         nx[i] = G::load(px + i * step);
         ny[i] = G::load(py + i * step);
       }
@@ -358,7 +375,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     A s[2] = {A(0), A(0)}, s1[2] = {A(0), A(0)};
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (i * step < left) {
+      if (i < SURE || i * step < left) {
         A d[V];
         G::values(nx[i], h + i * V);
         G::values(ny[i], d);
@@ -378,13 +395,14 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     if (k + 1 < rounds) fetch(row + rows_step);
     s[0] += s[1];
     s[1] = s1[0] + s1[1];
-    row_sum(s, slots[k & 1]);
+    if constexpr (NT) row_sum_of<NT>(s, slots[k & 1]);
+    else row_sum(s, slots[k & 1]);
     const A mg = s[0] * inv, mgh = s[1] * inv;
     if (dx != nullptr && in) {
       T* out = dx + row * dim + col;
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        if (i * step < left) {
+        if (i < SURE || i * step < left) {
           A d[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) d[j] = r * (g[i * V + j] - mg - h[i * V + j] * mgh);
@@ -398,7 +416,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     A* mine = joined + int64_t(threadIdx.y) * 2 * dim;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (i * step < left) {
+      if (i < SURE || i * step < left) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           mine[col + i * step + j] = dw[i * V + j];
@@ -418,7 +436,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
   A* out = partial + int64_t(blockIdx.x) * 2 * dim + col;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    if (i * step < left) {
+    if (i < SURE || i * step < left) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         out[i * step + j] = dw[i * V + j];
@@ -504,6 +522,7 @@ layer_norm_params_kernel(const A* __restrict__ partial, int parts, int64_t dim,
 // Threads a row, groups a thread and rows a block for rows of `groups` groups.
 struct Shape {
   int threads, items, rows;
+  bool narrow = false;  // of narrow_shape: the kernels know the number of threads
 };
 
 // Lanes and groups of a row that one warp holds: with few elements a row several rows share a warp
@@ -518,41 +537,45 @@ inline bool warp_shape(int64_t groups, int v, int most_items, Shape* s, int bloc
     else items *= 2;
     if (items > most_items) return false;
   }
-  *s = {threads, items, block / threads};
+  *s = {threads, items, block / threads, false};
+  return true;
+}
+// Rows of single elements or pairs, up to 512 threads of `most` groups: threads a power of two, 3/4
+// of `most` or `most` groups a thread, of which the last quarter of `most` alone can be past the
+// row's end.  The lower bound is what 32 threads need for that.
+inline bool narrow_shape(int64_t groups, int most, int block, Shape* s) {
+  if (groups <= 16 * most || groups > 512 * most) return false;
+  int threads = 32;
+  while (threads * most < groups) threads *= 2;
+  *s = {threads, threads * (most * 3 / 4) >= groups ? most * 3 / 4 : most,
+        threads == 32 ? block / 32 : 1, true};
   return true;
 }
 inline bool forward_shape(int64_t groups, int v, int acc_size, Shape* s) {
+  if (v <= 2 && narrow_shape(groups, 8, 128, s)) return true;
   if (warp_shape(groups, v, v <= 2 ? 8 : (acc_size == 8 ? 32 : 64) / v, s, 128)) return true;
   for (int items = v >= 8 ? 4 : (v <= 2 ? 8 : 32 / v); items * v <= 32; items *= 2) {
     const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
     if (threads <= fwd_max_threads(items * v)) {
-      *s = {static_cast<int>(threads), items, 1};
+      *s = {static_cast<int>(threads), items, 1, false};
       return true;
     }
   }
   return false;
 }
 template <typename A> bool backward_shape(int64_t groups, int v, Shape* s) {
+  if (v <= 2 && narrow_shape(groups, 8 / v, 256, s)) return true;
   if (warp_shape(groups, v, (sizeof(A) == 8 ? 8 : (v > 2 ? 32 : 16)) / v, s, 256)) return true;
   for (int items = v >= 8 ? 2 : (v <= 2 ? 8 : 16) / v; items * v <= 32; items *= 2) {
     const int64_t threads = cdiv(cdiv(groups, items), 32) * 32;
     if (threads <= bwd_max_threads<A>(v * items)) {
-      *s = {static_cast<int>(threads), items, 1};
+      *s = {static_cast<int>(threads), items, 1, false};
       return true;
     }
   }
   return false;
 }
 
-// Rows of single elements or pairs, more than 128 and at most 4096 groups: threads a power of two,
-// groups a thread 6 or 8, all but the last two of them within the row for every thread.
-inline bool narrow_shape(int64_t groups, Shape* s) {
-  if (groups <= 128 || groups > 4096) return false;
-  int threads = 32;
-  while (threads * 8 < groups) threads *= 2;
-  *s = {threads, threads * 6 >= groups ? 6 : 8, fwd_row_threads(threads) / threads};
-  return true;
-}
 // fn(std::integral_constant<int, threads>) for the threads of narrow_shape.
 template <typename F> int with_threads(int threads, F fn) {
   switch (threads) {
@@ -592,8 +615,7 @@ int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const voi
               void* y, void* stats, bool* done, cudaStream_t stream) {
   using A = typename AccOf<T>::type;
   Shape s;
-  const bool narrow = V <= 2 && narrow_shape(dim / V, &s);
-  if (!narrow && !forward_shape(dim / V, V, sizeof(A), &s)) return FDWT_OK;
+  if (!forward_shape(dim / V, V, sizeof(A), &s)) return FDWT_OK;
   *done = true;
   const dim3 block(s.threads, s.rows);
   const int64_t grid = cdiv(rows, s.rows);
@@ -609,7 +631,7 @@ int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const voi
     return launch_status();
   };
   if constexpr (V <= 2) {
-    if (narrow)
+    if (s.narrow)
       return with_threads(s.threads, [&](auto threads) {
         return s.items == 6 ? launch(std::integral_constant<int, 6>{}, threads)
                             : launch(std::integral_constant<int, 8>{}, threads);
@@ -651,11 +673,13 @@ int forward(int64_t rows, int64_t dim, const void* x, const void* w, const void*
 }
 
 // Blocks of the backward pass: `resident` a multiprocessor, at most one a row group.  Their number
-// is that of the partial rows, so the workspace takes the most that can be resident.
+// is that of the partial rows, so the workspace takes the most that can be resident: at most 12
+// (blocks of 64 threads, 65536 x 491 fp16: 63 us, and 68 us with at most 8; 16 gain nothing more).
+constexpr int kLongParts = 64, kMostResident = 12;
 inline int64_t backward_blocks(int64_t rows, const Shape& s, int resident) {
-  return imin(cdiv(rows, s.rows), int64_t(sm_count()) * resident);
+  const int64_t most = imin(kMostResident, 2048 / (s.threads * s.rows));
+  return imin(cdiv(rows, s.rows), sm_count() * imin(resident, most));
 }
-constexpr int kLongParts = 64, kMostResident = 8;
 
 // The largest of the counts that the forms for every alignment use: the query has no pointers.
 inline int64_t backward_parts(int dtype, int64_t rows, int64_t dim) {
@@ -693,24 +717,32 @@ int backward_v(int64_t rows, int64_t dim, const void* dy, const void* x, const v
   const dim3 block(s.threads, s.rows);
   const size_t smem =
       partial == nullptr || s.rows == 1 ? 0 : size_t(s.rows) * 2 * dim * sizeof(A);
-  return with_items<V, 32>(s.items, [&](auto items) -> int {
-    constexpr int IT = decltype(items)::value;
-    auto kernel = layer_norm_bwd_kernel<T, P, V, IT>;
+  auto launch = [&](auto items, auto threads) -> int {
+    auto kernel =
+        layer_norm_bwd_kernel<T, P, V, decltype(items)::value, decltype(threads)::value>;
     int resident = 1;
     int st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
     if (st == FDWT_OK)
       st = occupancy(reinterpret_cast<const void*>(kernel), s.threads * s.rows, smem, &resident);
     if (st == FDWT_OK) st = pre_launch(stream);
     if (st != FDWT_OK) return st;
-    const int64_t grid =
-        backward_blocks(rows, s, resident < kMostResident ? (resident < 1 ? 1 : resident) : kMostResident);
+    const int64_t grid = backward_blocks(rows, s, resident < 1 ? 1 : resident);
     *parts = grid;
     kernel<<<static_cast<unsigned>(grid), block, smem, stream>>>(
         static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const P*>(w),
         static_cast<const A*>(stats), static_cast<T*>(dx), static_cast<A*>(partial), rows,
         static_cast<int>(dim));
     return launch_status();
-  });
+  };
+  if constexpr (V <= 2) {
+    if (s.narrow)
+      return with_threads(s.threads, [&](auto threads) {
+        return s.items == 6 / V ? launch(std::integral_constant<int, 6 / V>{}, threads)
+                                : launch(std::integral_constant<int, 8 / V>{}, threads);
+      });
+  }
+  return with_items<V, (V <= 2 && sizeof(A) == 4 ? 16 : 32)>(
+      s.items, [&](auto items) { return launch(items, std::integral_constant<int, 0>{}); });
 }
 
 template <typename T, typename P>

@@ -87,17 +87,28 @@ def test_forward_and_gradients(rows, dim, dtype):
 ODD = [(11, d) for d in (127, 129, 191, 193, 383, 385, 511, 513, 767, 769, 1023, 1025, 1535, 1537,
                          2047, 2049, 2999, 4095)]
 PAIRS = [(9, d) for d in (258, 382, 386, 514, 770, 1022, 1026, 1538, 2050, 6146, 8190, 8194)]
+MANY = [(20000, 193), (3000, 491), (3001, 490)]  # the backward pass's blocks take several rows each
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("rows,dim", ODD + PAIRS)
+@pytest.mark.parametrize("rows,dim", ODD + PAIRS + MANY)
 def test_rows_of_single_elements_and_pairs(rows, dim, dtype):
-    x, w, b, _ = _case(rows, dim, dtype, dtype, seed=dim)
+    x, w, b, dy = _case(rows, dim, dtype, dtype, seed=dim)
     ry, shift = _reference(x, w, b, 1e-5)
     spread = (1 + shift + ry.abs()) * w.double().abs().amax() + 2 * b.double().abs().amax()
     _check(F.layer_norm(x, w, b), ry, dtype, spread, "y")
     plain, shift = _reference(x, None, None, 1e-5)
     _check(F.layer_norm(x), plain, dtype, 1 + shift + plain.abs(), "y without parameters")
+    for t in (x, w, b):
+        t.requires_grad_()
+    dx, dw, db = torch.autograd.grad(F.layer_norm(x, w, b), (x, w, b), dy)
+    with torch.no_grad():
+        _, shift, rdx, rdw, rdb, rstd, h, g = _reference(x, w, b, 1e-5, dy)
+        gmax = g.abs().amax(-1, keepdim=True)
+        hmax = 1 + h.abs().amax(-1, keepdim=True)
+        _check(dx, rdx, dtype, rstd * gmax * hmax * (hmax + shift), "dx")
+        _check(dw, rdw, dtype, (dy.double().abs() * (h.abs() + shift + 1)).sum(0), "dweight")
+        _check(db, rdb, dtype, dy.double().abs().sum(0), "dbias")
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
