@@ -400,8 +400,10 @@ template <int DK> struct Tf32 {
   static constexpr size_t smem = words * sizeof(float);
 };
 
+// Two blocks leave 128 registers a thread, too few for 16-bit rows: 37 tokens of bf16 take 18 us
+// with them and 11.5 us with more.
 template <typename T, int DK, bool STATES>
-__global__ void __launch_bounds__(256, DK == 64 ? 2 : 1)
+__global__ void __launch_bounds__(256, DK == 64 && sizeof(T) == 4 ? 2 : 1)
 linattn_tf32_kernel(const __grid_constant__ Call call) {
   using Z = Tf32<DK>;
   constexpr int C = Z::C, NV = Z::NV, PK = Z::PK, PV = Z::PV, PP = Z::PP, RT = DK / 64;
@@ -819,10 +821,10 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   int64_t tiles = 0;
   for (int j = 0; j < call.jobs; ++j) tiles += cdiv(call.job[j].dv, p.tile);
   const int64_t chunks = imax(1, cdiv(call.length, p.chunk));
-  // Blocks a multiprocessor holds; two of the TF32 kernel up to heads of 64 (5 x 1537 tokens, 6
+  // Blocks a multiprocessor holds; two of the fp32 kernel up to heads of 64 (5 x 1537 tokens, 6
   // heads of 48 x 80: 120 us so, 132 us with one).  Times in microseconds a chunk (measured): 128
   // tokens on the tensor cores, 64 (or 32) by the general kernels.
-  const int64_t slots = int64_t(sm_count()) * (!tc && dtype != FDWT_F64 && dk <= 64 ? 2 : 1);
+  const int64_t slots = int64_t(sm_count()) * (dtype == FDWT_F32 && dk <= 64 ? 2 : 1);
   const int64_t units = tiles * call.batch * call.heads;
   const Cost cost = tc ? Cost{dk <= 64 ? 1.9 : 2.3, 0.75, 6.0, 4.0} : Cost{7.5, 3.0, 5.0, 4.0};
   const int64_t c = cdiv(chunks, plan_segments(units, chunks, slots, cost));
