@@ -826,7 +826,7 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   // tokens on the tensor cores, 64 (or 32) by the general kernels.
   const int64_t slots = int64_t(sm_count()) * (dtype == FDWT_F32 && dk <= 64 ? 2 : 1);
   const int64_t units = tiles * call.batch * call.heads;
-  const Cost cost = tc ? Cost{dk <= 64 ? 1.9 : 2.3, 0.75, 6.0, 4.0} : Cost{7.5, 3.0, 5.0, 4.0};
+  const Cost cost = tc ? Cost{dk <= 64 ? 2.3 : 2.8, 0.75, 6.0, 4.0} : Cost{7.5, 3.0, 5.0, 4.0};
   const int64_t c = cdiv(chunks, plan_segments(units, chunks, slots, cost));
   p.nseg = static_cast<int>(cdiv(chunks, c));
   p.seg_len = c * p.chunk;

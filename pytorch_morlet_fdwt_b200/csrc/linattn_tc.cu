@@ -4,18 +4,18 @@
 // One block per SM runs one head's segment, 64 value columns of it, in chunks of 128 tokens:
 //
 //   Sc = Q K^T            (128 x 128)    shared x shared   -> TMEM, two buffers
-//   P  = Sc * M           rounded to 16 bits, over the first half of Sc's columns
-//   Oi = P V              (128 x 64)     TMEM x shared     -> TMEM, the second half of them
-//   Oe = Q S              (128 x 64)     shared x shared   -> TMEM, S the 16-bit copy of the state
+//   P  = Sc * M           two 16-bit parts, over Sc's columns
+//   Oe = Q S              (128 x 64)     shared x shared   -> TMEM, S in two 16-bit parts
+//   Oi = P V              (128 x 64)     TMEM x shared     -> TMEM, Oe's columns once it is taken
 //   U  = K^T V'           (DK x 64 each part)  shared x shared -> TMEM
 //   o  = diag(d^{l+off}) inter Oe + Oi,  S <- d^m S + write U   in registers, 32 bits
 //
-// V' is diag(d^{m-off-l}) V in two 16-bit parts (fp16) or three (bf16): one part would leave the
-// state a 2^-9 (bf16) of each token off, two 2^-17, more than the 32-bit state's own rounding.
-// The scores and the copy of S that multiplies Q are rounded once to the operands' type, as the
-// products need it; their errors are of the size of the result's own rounding (together 1.41 times
-// it, measured).  fp16 would overflow or lose small values there: each row of P and each copy of S
-// is scaled by a power of two first, undone in the sum for o.
+// What a product needs in 16 bits goes in as the sum of parts, so that the result is that of the
+// operator in 32 bits, rounded once: two parts of the scores and of the state's copy that
+// multiplies Q (one would put the result 1.41 times as far off as its own rounding does), and of
+// V' = diag(d^{m-off-l}) V two (fp16) or three (bf16), which leave the 32-bit state as far off as
+// its own sums.  fp16 would overflow or lose small values: each row of P and each copy of S is
+// scaled by a power of two first, undone in the sum for o.
 //
 // Bound: 2 (2 Dk + 2 Dv) bytes of HBM a token and head against about 4 (Dk Dv + 128 (Dk + Dv))
 // operations, 96 a byte at 128 x 128, under half of the tensor rate at the HBM rate.  What costs
@@ -23,9 +23,9 @@
 // overlap: one warp issues the loads (TMA), one all products, four form P, eight V', four finish
 // o, four keep the state.  All parts of V' are one product (N = 64 parts), so that K is read once:
 // the shared-memory rate binds the products more than the tensor rate.  Measured with all SMs
-// busy: 1.9 us a chunk with heads of 64 (4 x 4096 x 37 heads, 67 us, 71 % of the HBM rate), 2.3 us
-// with heads of 128 (2 x 4096 x 37 heads, 87 us, 55 %; 368 KB a chunk through shared memory, 1.5 us
-// at its rate); the first chunk is out after 10 us.  Every wait on a barrier has a time limit.
+// busy, bf16: 2.3 us a chunk with heads of 64 (4 x 4096 tokens of 37 heads, 84 us), 2.8 us with
+// heads of 128 (2 x 4096 of 37 heads, 103 us); 67 and 87 us with P and S in one part.  Every wait
+// on a barrier has a time limit.
 #include <cuda.h>
 
 #include <type_traits>
@@ -259,6 +259,20 @@ template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b)
   typename Pair<T>::type p = Pair<T>::make(a, b);
   return *reinterpret_cast<uint32_t*>(&p);
 }
+// The first of the two 16-bit parts of (a, b), which keep what is left for the second one.  It is
+// cut off rather than rounded: one conversion less, and the second part, rounded, takes up the
+// rest (2^-16 of a value in bf16, 2^-21 in fp16).
+template <typename T>
+__device__ __forceinline__ uint32_t first_part(float& a, float& b) {
+  constexpr uint32_t mask = std::is_same<T, __half>::value ? 0xffffe000u : 0xffff0000u;
+  const float x = __uint_as_float(__float_as_uint(a) & mask);
+  const float y = __uint_as_float(__float_as_uint(b) & mask);
+  const uint32_t u = std::is_same<T, __half>::value
+                         ? pack<T>(x, y)
+                         : __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+  sub2(a, b, x, y);
+  return u;
+}
 template <typename T> __device__ __forceinline__ float2 unpack(uint32_t u) {
   return Pair<T>::split(*reinterpret_cast<typename Pair<T>::type*>(&u));
 }
@@ -373,36 +387,37 @@ __device__ __forceinline__ void split_group(const unsigned char* v, float weight
 #pragma unroll
   for (int p = 0; p < kParts<T>; ++p) out[p] = make_uint4(u[p][0], u[p][1], u[p][2], u[p][3]);
 }
-// 64 rows of it by 128 threads: thread tid takes the column group tid % 8 of the rows tid / 8 + 16 j.
+// ROWS (64 or 32) rows of it by 128 threads: thread tid takes the column group tid % 8 of the rows
+// tid / 8 + 16 j, whose weights are weight[from + j].  Part p goes to parts + p * ROWS * 128.
 // `ready()` (false: give up) is asked for between forming the first two groups and storing them.
-template <typename T, typename F>
-__device__ __forceinline__ bool split_values(const unsigned char* v, unsigned char* parts, int lead,
-                                             const float (&weight)[4], int tid, F ready) {
+template <typename T, int ROWS, typename F>
+__device__ __forceinline__ bool split_values(const unsigned char* v, unsigned char* parts,
+                                             const float (&weight)[4], int from, int tid, F ready) {
   const int r0 = tid / 8;
   const int cell = r0 * 128 + (((tid % 8) ^ (r0 & 7)) << 4);
 #pragma unroll 1
-  for (int j = 0; j < 4; j += 2) {
+  for (int j = 0; j < ROWS / 16; j += 2) {
     uint4 a[2][kParts<T>];
-    split_group<T>(v + cell + j * 2048, j == 0 ? weight[0] : weight[2], a[0]);
-    split_group<T>(v + cell + j * 2048 + 2048, j == 0 ? weight[1] : weight[3], a[1]);
+    split_group<T>(v + cell + j * 2048, from + j == 0 ? weight[0] : weight[2], a[0]);
+    split_group<T>(v + cell + j * 2048 + 2048, from + j == 0 ? weight[1] : weight[3], a[1]);
     if (j == 0 && !ready()) return false;
 #pragma unroll
     for (int p = 0; p < kParts<T>; ++p) {
-      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048) = a[0][p];
-      *reinterpret_cast<uint4*>(parts + p * lead + cell + j * 2048 + 2048) = a[1][p];
+      *reinterpret_cast<uint4*>(parts + p * ROWS * 128 + cell + j * 2048) = a[0][p];
+      *reinterpret_cast<uint4*>(parts + p * ROWS * 128 + cell + j * 2048 + 2048) = a[1][p];
     }
   }
   return true;
 }
 
-// D (+)= K^T V' over 64 tokens, all parts at once, 64 columns each (FIRST: the first product does
+// D (+)= K^T V' over ROWS tokens, all parts at once, 64 columns each (FIRST: the first product does
 // not add): M runs along the heads' size, the contraction over the tokens.  k, b: operand().
-template <typename T, int DK, bool FIRST>
+template <typename T, int DK, int ROWS, bool FIRST>
 __device__ __forceinline__ void issue_update(uint32_t d, uint32_t k, uint32_t b) {
   constexpr uint32_t id = instr<T>(DK, NV * kParts<T>, true, true);
   mma_ss<!FIRST>(d, k, b, id);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
+  for (int i = 1; i < ROWS / 16; ++i) mma_ss<true>(d, k + i * 128, b + i * 128, id);
 }
 // 8 columns of U from the parts' sums.
 template <typename T> __device__ __forceinline__ void load_update(uint32_t addr, float (&x)[8]) {
@@ -436,8 +451,8 @@ template <int N> __device__ __forceinline__ void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 constexpr uint32_t kColumns = 512;
-// TMEM columns: two buffers of Sc (P over its first 64 columns, Oi over the others), Oe, U
-constexpr uint32_t kSc = 0, kOi = 64, kOe = 256, kU = 320;
+// TMEM columns: two buffers of Sc (both parts of P over it), Oe and after it Oi, U
+constexpr uint32_t kSc = 0, kO = 256, kU = 320;
 // The state launch takes 64 tokens at a time.  A stage is held from its load to the end of its
 // product, some 2.5 us, so what counts is their number (4: 140 us for 1 x 65536 x 16 x 128).
 constexpr int kStateRows = 64, kStatePanel = kStateRows * 128, kStateGroups = 4, kStateParts = 2;
@@ -446,8 +461,12 @@ template <typename T, int DK> struct Smem {
   static constexpr int panels = DK / 64;
   static constexpr int stages = DK == 64 ? 3 : 2;
   static constexpr int q = 0, k = stages * panels * kPanel, v = 2 * k;  // rings of stages
-  static constexpr int parts = v + stages * kPanel, s = parts + kParts<T> * kPanel;
-  static constexpr int bytes = s + DK * 128 + 1024;  // 1024: room to align the base
+  // V' is formed and multiplied by blocks of v_rows tokens, two of them in turn; the smaller ones
+  // are what heads of 128 have room for
+  static constexpr int v_rows = DK == 64 ? 64 : 32, v_block = kParts<T> * v_rows * 128;
+  static constexpr int parts = v + stages * kPanel, s = parts + 2 * v_block;
+  static constexpr int s_part = DK * 128;              // two parts of the state's copy
+  static constexpr int bytes = s + 2 * s_part + 1024;  // 1024: room to align the base
   static constexpr int st_stages = DK == 64 ? 8 : 6;
   static constexpr int st_stage = (panels + 1) * kStatePanel;
   static constexpr int st_parts = st_stages * st_stage;
@@ -597,10 +616,10 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   if (warp >= 4 && warp < 8) {
     take_registers<96>();
     const int row_warp = warp - 4;
-    // ---- P = Sc * M.  Row t = 32 row_warp + lane, 32 columns at a time from the left: the 16-bit
-    // scores of a block go over columns whose scores have been read.  Off the diagonal block
-    // (forward; the mirror image back in time) d^{t-s} = d^{32(w-j-1)+lane+1} d^{31-c}: both
-    // powers are at least 0, nothing overflows.
+    // ---- P = Sc * M.  Row t = 32 row_warp + lane, 32 columns at a time: their two 16-bit parts (16
+    // columns each) go over the scores.  Off the diagonal block (forward; the mirror image back
+    // in time) d^{t-s} = d^{32(w-j-1)+lane+1} d^{31-c}: both powers are at least 0, nothing
+    // overflows.
     const bool rev = job.reverse != 0;
     float tab[32], lead[4];
 #pragma unroll
@@ -648,6 +667,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         if (rev ? j < row_warp : j > row_warp) {  // all masked
 #pragma unroll
           for (int c = 0; c < 16; ++c) u[c] = 0;
+          tmem_st16(sc + j * 32, u);
         } else {
           float x[32];
           tmem_ld32(sc + j * 32, x);
@@ -668,9 +688,12 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
             }
           }
 #pragma unroll
+          for (int c = 0; c < 16; ++c) u[c] = first_part<T>(x[2 * c], x[2 * c + 1]);
+          tmem_st16(sc + j * 32, u);
+#pragma unroll
           for (int c = 0; c < 16; ++c) u[c] = pack<T>(x[2 * c], x[2 * c + 1]);
         }
-        tmem_st16(sc + j * 16, u);
+        tmem_st16(sc + j * 32 + 16, u);
       }
       tmem_st_wait();
       tc_before();
@@ -678,20 +701,22 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     }
   } else if (warp >= 8 && warp < 16) {
     give_registers<56>();
-    // ---- V', four warps each for the first and the last 64 tokens, which are multiplied one
-    // after the other: a half is formed anew while the other one is still in use
-    const int tid = threadIdx.x % 128, half = (warp - 8) / 4;
-    const int cell0 = half * 64 * 128;
+    // ---- V', two groups of four warps take blocks of v_rows tokens by turns, each with its own
+    // buffer: a block is formed while the other group's is multiplied.  idx = 0 .. 3 are a
+    // thread's rows of a chunk, kIn of them in a block.
+    constexpr int R = Z::v_rows, kBlocks = C / R / 2, kIn = 4 / kBlocks;
+    const int tid = threadIdx.x % 128, group = (warp - 8) / 4;
+    auto row = [&](int idx) { return (group + idx / kIn * 2) * R + tid / 8 + idx % kIn * 16; };
     float weight[4];
     int weight_m = 0;
-    for (int i = 0; i < chunks; ++i) {
+    bool ok = true;
+    for (int i = 0; i < chunks && ok; ++i) {
       const int left = w.end - (w.begin + i * C), m = left < C ? left : C;
       if (m != weight_m) {
         weight_m = m;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int r = half * 64 + tid / 8 + 16 * j;
-          const int age = m - job.off - (job.reverse ? C - 1 - r : r);
+          const int r = row(j), age = m - job.off - (job.reverse ? C - 1 - r : r);
           weight[j] = age < 0 ? 0.0f : dpow[age];
         }
       }
@@ -703,7 +728,9 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         // values that it reads below.
         if (!bar_wait(&k_full[i % S], (i / S) & 1, limit)) break;
         unsigned char* k = sm + Z::k + (i % S) * Z::panels * kPanel;
-        for (int r = half * 64 + tid / 8; r < half * 64 + 64; r += 16) {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          const int r = row(j);
           if (r < m) continue;
           const int at = r * 128 + (((tid % 8) ^ (r & 7)) << 4);
 #pragma unroll
@@ -712,17 +739,22 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
           *reinterpret_cast<uint4*>(v + at) = make_uint4(0, 0, 0, 0);
         }
       }
-      const bool ok = split_values<T>(v + cell0, sm + Z::parts + cell0, kPanel, weight, tid, [&] {
-        return i == 0 || bar_wait(&v_free[half], (i - 1) & 1, limit);
-      });
-      if (!ok) break;
-      fence_async();
-      bar_arrive(&v_full[half]);
+#pragma unroll 1
+      for (int b = 0; b < kBlocks && ok; ++b) {
+        const int turn = i * kBlocks + b;
+        ok = split_values<T, R>(v + (group + 2 * b) * R * 128, sm + Z::parts + group * Z::v_block,
+                                weight, b * kIn, tid, [&] {
+          return turn == 0 || bar_wait(&v_free[group], (turn - 1) & 1, limit);
+        });
+        if (!ok) break;
+        fence_async();
+        bar_arrive(&v_full[group]);
+      }
     }
   } else if (warp >= 16 && warp < 20) {
     take_registers<96>();
     // ---- o = inter d^{l+off} Oe + Oi, a row of 64 columns a thread; Oe is taken as soon as it is
-    // there, so that the next chunk's can follow
+    // there, so that Oi can take its place
     const int t = warp % 4 * 32 + lane, l = job.reverse ? C - 1 - t : t;
     const float read = float(job.inter) * dpow[l + job.off];
     const int64_t head = int64_t(w.b) * job.os[0] + int64_t(w.h) * job.os[2] + w.v0;
@@ -736,7 +768,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       const float fe = kHalf ? read * s_inv[i & 1] : read;
       float y[NV / 16][16];
 #pragma unroll
-      for (int g = 0; g < NV / 16; ++g) tmem_ld16(tmem + lanes + kOe + g * 16, y[g]);
+      for (int g = 0; g < NV / 16; ++g) tmem_ld16(tmem + lanes + kO + g * 16, y[g]);
 #pragma unroll
       for (int g = 0; g < NV / 16; ++g) tmem_ld_wait(y[g]);
       tc_before();
@@ -747,7 +779,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
       for (int g = 0; g < NV / 16; ++g) {
         float x[16];
-        tmem_ld16(tmem + lanes + kSc + (i & 1) * 128 + kOi + g * 16, x);
+        tmem_ld16(tmem + lanes + kO + g * 16, x);
         tmem_ld_wait(x);
         if (g == NV / 16 - 1) {
           tc_before();
@@ -867,12 +899,18 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
           const float* y = &s[g / 4][g % 4 * 8];
-          uint32_t u[4];
+          uint32_t u[4], low[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            u[e] = kHalf ? pack<T>(y[2 * e] * scale, y[2 * e + 1] * scale)
-                         : pack<T>(y[2 * e], y[2 * e + 1]);
-          *reinterpret_cast<uint4*>(row + ((g ^ (r & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+          for (int e = 0; e < 4; ++e) {
+            float a = y[2 * e], b = y[2 * e + 1];
+            if (kHalf) mul2(a, b, scale, scale);
+            u[e] = first_part<T>(a, b);
+            low[e] = pack<T>(a, b);
+          }
+          const int at = (g ^ (r & 7)) << 4;
+          *reinterpret_cast<uint4*>(row + at) = make_uint4(u[0], u[1], u[2], u[3]);
+          *reinterpret_cast<uint4*>(row + Z::s_part + at) =
+              make_uint4(low[0], low[1], low[2], low[3]);
         }
       }
       fence_async();
@@ -915,7 +953,8 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     // operands of stage 0, and of what has one buffer
     const uint32_t oq = operand(base + Z::q, kPanel), ok0 = operand(base + Z::k, kPanel);
     const uint32_t ov = operand(base + Z::v, kPanel);
-    const uint32_t os = operand(base + Z::s, kPanel), op = operand(base + Z::parts, kPanel);
+    const uint32_t os = operand(base + Z::s, kPanel);
+    const uint32_t op = operand(base + Z::parts, Z::v_rows * 128);
     const bool one = elect_one();
     bool ok = true;
     // each turn: U, Oe of chunk i, the scores of chunk i + 1, Oi of chunk i (turn -1: the scores
@@ -924,45 +963,47 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       if (i >= 0) {
         const uint32_t q = oq + (i % S) * (Z::panels * kPanel / 16);
         const uint32_t k = ok0 + (i % S) * (Z::panels * kPanel / 16);
-        ok = bar_wait(&v_full[0], i & 1, limit) &&
-             (i == 0 || bar_wait(&u_empty, (i - 1) & 1, limit));
-        ok = __all_sync(0xffffffffu, ok);
+        constexpr int kBlocks = C / Z::v_rows;  // of V', in turn from the two groups that form them
+        ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&u_empty, (i - 1) & 1, limit));
         if (!ok) break;
-        if (one) {
-          tc_after();
-          issue_update<T, DK, true>(tmem + kU, k, op);
-          tc_commit(&v_free[0]);
-        }
-        __syncwarp();
-        ok = __all_sync(0xffffffffu, bar_wait(&v_full[1], i & 1, limit));
-        if (!ok) break;
-        if (one) {
-          tc_after();
-          issue_update<T, DK, false>(tmem + kU, k + 512, op + 512);
-          tc_commit(&v_free[1]);
-          tc_commit(&u_full);
-          tc_commit(&k_empty[i % S]);
-        }
-        __syncwarp();
-        ok = bar_wait(&s_full, i & 1, limit) &&
-             (i == 0 || bar_wait(&oe_empty, (i - 1) & 1, limit));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (one) {
-          tc_after();
-          mma_ss<false>(tmem + kOe, q, os, id_o);
 #pragma unroll
-          for (int j = 1; j < DK / 16; ++j)
-            mma_ss<true>(tmem + kOe, q + j / 4 * (kPanel / 16) + j % 4 * 2, os + j * 128, id_o);
+        for (int b = 0; b < kBlocks; ++b) {
+          const int turn = i * (kBlocks / 2) + b / 2;
+          ok = __all_sync(0xffffffffu, bar_wait(&v_full[b % 2], turn & 1, limit));
+          if (!ok) break;
+          if (one) {
+            tc_after();
+            const uint32_t kb = k + b * (Z::v_rows * 128 / 16), pb = op + b % 2 * (Z::v_block / 16);
+            if (b == 0) issue_update<T, DK, Z::v_rows, true>(tmem + kU, kb, pb);
+            else issue_update<T, DK, Z::v_rows, false>(tmem + kU, kb, pb);
+            tc_commit(&v_free[b % 2]);
+            if (b + 1 == kBlocks) {
+              tc_commit(&u_full);
+              tc_commit(&k_empty[i % S]);
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        // o of the chunk before is out: its columns take this chunk's, and its scores' buffer the
+        // next scores
+        ok = bar_wait(&s_full, i & 1, limit) &&
+             (i == 0 || bar_wait(&o_empty, (i - 1) & 1, limit));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (one) {
+          tc_after();
+          mma_ss<false>(tmem + kO, q, os, id_o);
+#pragma unroll
+          for (int j = 1; j < DK / 8; ++j) {  // both parts of the state's copy
+            const int d = j % (DK / 16);
+            mma_ss<true>(tmem + kO, q + d / 4 * (kPanel / 16) + d % 4 * 2,
+                         os + j / (DK / 16) * (Z::s_part / 16) + d * 128, id_o);
+          }
           tc_commit(&oe_full);
           tc_commit(&q_empty[i % S]);
         }
         __syncwarp();
-        // Oi of the chunk before is out: its buffer takes the next scores.  (The wait is also due
-        // before P V, whose o frees the other buffer: no barrier may be two phases ahead of who
-        // waits for it.)
-        ok = __all_sync(0xffffffffu, i == 0 || bar_wait(&o_empty, (i - 1) & 1, limit));
-        if (!ok) break;
       }
       const int n = i + 1;
       if (n < chunks) {
@@ -985,15 +1026,21 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         __syncwarp();
       }
       if (i < 0) continue;
-      ok = __all_sync(0xffffffffu, bar_wait(&p_full[i & 1], (i >> 1) & 1, limit));
+      // (no barrier may be two phases ahead of who waits for it: each Oe and Oi is taken before the
+      // next one is issued)
+      ok = bar_wait(&p_full[i & 1], (i >> 1) & 1, limit) && bar_wait(&oe_empty, i & 1, limit);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (one) {
         tc_after();
         const uint32_t v = ov + (i % S) * (kPanel / 16);
         const uint32_t p = tmem + kSc + (i & 1) * 128;
-        mma_ts<false>(p + kOi, p, v, id_o);
+        mma_ts<false>(tmem + kO, p, v, id_o);
 #pragma unroll
-        for (int j = 1; j < C / 16; ++j) mma_ts<true>(p + kOi, p + j * 8, v + j * 128, id_o);
+        for (int j = 1; j < C / 8; ++j) {  // the first part of P, then the second
+          const int t = j % (C / 16);
+          mma_ts<true>(tmem + kO, p + t / 2 * 32 + t % 2 * 8 + j / (C / 16) * 16, v + t * 128, id_o);
+        }
         tc_commit(&o_full);
         tc_commit(&v_empty[i % S]);
       }
@@ -1097,9 +1144,9 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
         weight[j] = age < 0 ? 0.0f : decay_pow(w.a, float(age));
       }
       if (!bar_wait(&full[i % S], (i / S) & 1, limit)) break;
-      const bool ok = split_values<T>(
+      const bool ok = split_values<T, R>(
           sm + (i % S) * Z::st_stage + Z::panels * kStatePanel,
-          sm + Z::st_parts + i % NB * kParts<T> * kStatePanel, kStatePanel, weight, tid,
+          sm + Z::st_parts + i % NB * kParts<T> * kStatePanel, weight, 0, tid,
           // the products of block i - NB have ended
           [&] { return i < NB || bar_wait(&used[(i - NB) % S], ((i - NB) / S) & 1, limit); });
       if (!ok) break;
@@ -1151,8 +1198,8 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
       const uint32_t parts = op0 + (i % NB) * (kParts<T> * kStatePanel / 16);
       if (one) {
         tc_after();
-        if (i == 0) issue_update<T, DK, true>(tmem, k, parts);
-        else issue_update<T, DK, false>(tmem, k, parts);
+        if (i == 0) issue_update<T, DK, R, true>(tmem, k, parts);
+        else issue_update<T, DK, R, false>(tmem, k, parts);
         tc_commit(&used[i % S]);
       }
       __syncwarp();

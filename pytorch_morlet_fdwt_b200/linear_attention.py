@@ -209,8 +209,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
             may hold anything.
 
     Returns ``(out (B, L, H, Dv), final_state (B, H, Dk, Dv))``, differentiable once in q, k, v
-    and initial_state.  fp16 and bf16 round the scores and the state's copy that multiplies q to
-    16 bits; the state itself is fp32.
+    and initial_state.  fp16 and bf16 inputs are computed to 32 bits, states too, and the result
+    rounded once.
     """
     _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _rows(q), _rows(k), _rows(v)

@@ -1,0 +1,48 @@
+"""What linear_attention rounds: 16-bit results are those of the operator in 32 bits, rounded once.
+
+Against the closed form in 64 bits the root mean square error may then be that of rounding the
+64-bit result to the type, e0 (0.3 to 0.4 unit roundoffs u of the result), and little more: the
+products take scores, states and weighted values in at least two 16-bit parts, u^2 of a term each
+(2^-16 for bf16, 1 % of e0; 2^-22 for fp16), and sum in 32 bits.  These are independent of e0, so
+1.05 e0 leaves room for them; one more value rounded to 16 bits would come to 1.2 e0 or more.
+"""
+
+import pytest
+import torch
+
+import pytorch_morlet_fdwt_b200 as F
+from .test_linear_attention_gpu import DEV, _inputs, _reference
+
+pytestmark = pytest.mark.gpu
+
+CASES = [  # B, L, H, Hkv, Dk, Dv, initial, lengths, fast decay
+    (2, 300, 4, 4, 64, 64, True, None, False),
+    (1, 1100, 2, 2, 128, 128, True, [1030], False),
+    (2, 700, 4, 2, 128, 72, True, [700, 259], False),
+    (3, 385, 4, 1, 40, 128, False, [385, 130, 0], False),
+    (2, 640, 3, 3, 64, 64, True, None, True),
+    (1, 2050, 1, 1, 128, 64, False, None, False),
+    (8, 129, 8, 8, 16, 32, True, None, False),
+]
+
+
+def _rms(x):
+    return x.double().square().mean().sqrt()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,Hk,Dk,Dv,initial,lengths,fast", CASES)
+def test_one_rounding(B, L, H, Hk, Dk, Dv, initial, lengths, fast, dtype):
+    q, k, v, a, s0, n = _inputs(B, L, H, Hk, Dk, Dv, dtype, L, initial, lengths, fast)
+    torch.manual_seed(L + 1)
+    do = torch.randn(B, L, H, Dv, device=DEV).to(dtype)
+    wrt = [t.requires_grad_() for t in (q, k, v)]
+    out, _ = F.linear_attention(q, k, v, a, initial_state=s0, lengths=n)
+    got = (out, *torch.autograd.grad(out, wrt, do))
+    leaves = [t.detach().double().requires_grad_() for t in wrt]
+    ref, _ = _reference(*leaves, a, s0, n, Dk ** -0.5)
+    want = (ref.detach(), *torch.autograd.grad(ref, leaves, do.double()))
+    for name, g, r in zip(("out", "dq", "dk", "dv"), got, want):
+        once = _rms(r.to(dtype).double() - r)
+        off = _rms(g.double() - r)
+        assert off <= 1.05 * once, f"{name}: {off / once:.3f} times the rounding of the result"
