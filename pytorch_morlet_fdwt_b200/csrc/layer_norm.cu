@@ -11,6 +11,7 @@
 // Measured: 65536 x 2048 bf16 forward 96 us (5.6 TB/s), backward 166 us (4.9 TB/s); 65536 x 1024
 // fp32 88 and 132 us (6.1 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
 // 54 and 88 us (5.9 and 5.4 TB/s).
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -94,7 +95,8 @@ template <> struct Group<__nv_bfloat16, 2> : Group4<__nv_bfloat16> {};
 template <> struct Group<__half, 8> : Group16<__half> {};
 template <> struct Group<__nv_bfloat16, 8> : Group16<__nv_bfloat16> {};
 
-// V parameters (weight or bias) as values; their group is 16 or 32 bytes.
+// V parameters (weight or bias) as values: V elements of their own type, loaded 16 bytes (all of
+// them, where they are fewer) at a time.  group_of() sees to their alignment.
 template <typename P, int V, typename A>
 __device__ __forceinline__ void load_params(const P* p, A* x) {
   if constexpr (sizeof(P) * V == 32) {
@@ -642,12 +644,16 @@ int forward_v(int64_t rows, int64_t dim, const void* x, const void* w, const voi
 }
 
 // Elements of a group: 16 bytes, two elements or one, whatever rows and pointers are aligned to.
-template <typename T, typename... Ptr> int group_of(int64_t dim, Ptr... p) {
-  uintptr_t all = 0;
-  for (const void* q : {static_cast<const void*>(p)...}) all |= reinterpret_cast<uintptr_t>(q);
+// Parameters of another type than the rows' have groups of another size (fp32 beside 16 bits: a
+// pair is 8 bytes, not 4), so each of the two is tested by its own.
+using Pointers = std::initializer_list<const void*>;
+template <typename T, typename P> int group_of(int64_t dim, Pointers rows, Pointers params) {
+  uintptr_t x = 0, p = 0;
+  for (const void* q : rows) x |= reinterpret_cast<uintptr_t>(q);
+  for (const void* q : params) p |= reinterpret_cast<uintptr_t>(q);
   constexpr int V = 16 / sizeof(T);
-  if (dim % V == 0 && all % 16 == 0) return V;
-  if (V > 2 && dim % 2 == 0 && all % (2 * sizeof(T)) == 0) return 2;
+  if (dim % V == 0 && x % 16 == 0 && p % 16 == 0) return V;
+  if (V > 2 && dim % 2 == 0 && x % (2 * sizeof(T)) == 0 && p % (2 * sizeof(P)) == 0) return 2;
   return 1;
 }
 
@@ -658,7 +664,7 @@ int forward(int64_t rows, int64_t dim, const void* x, const void* w, const void*
   constexpr int V = 16 / sizeof(T);
   bool done = false;
   int st;
-  const int v = group_of<T>(dim, x, y, w, b);
+  const int v = group_of<T, P>(dim, {x, y}, {w, b});
   if (v == V) st = forward_v<T, P, V>(rows, dim, x, w, b, eps, y, stats, &done, stream);
   else if (v == 2) st = forward_v<T, P, 2>(rows, dim, x, w, b, eps, y, stats, &done, stream);
   else st = forward_v<T, P, 1>(rows, dim, x, w, b, eps, y, stats, &done, stream);
@@ -753,7 +759,7 @@ int backward(int64_t rows, int64_t dim, const void* dy, const void* x, const voi
   void* partial = (dw != nullptr || db != nullptr) ? ws : nullptr;
   int64_t parts = 0;
   int st;
-  const int v = group_of<T>(dim, x, dy, dx, w);
+  const int v = group_of<T, P>(dim, {x, dy, dx}, {w});
   if (v == V) st = backward_v<T, P, V>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
   else if (v == 2) st = backward_v<T, P, 2>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
   else st = backward_v<T, P, 1>(rows, dim, dy, x, w, stats, dx, partial, &parts, stream);
