@@ -22,6 +22,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib, config
 
@@ -237,7 +238,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """One token of :func:`linear_attention` for each of B sequences: ``q (B, H, Dk)``,
     ``k (B, Hkv, Dk)``, ``v (B, Hkv, Dv)`` -> ``out (B, H, Dv)``.
 
-    ``state (N, H, Dk, Dv)``, contiguous fp32 (fp64 for fp64 inputs), is updated in place.
+    ``state (N, H, Dk, Dv)``, contiguous fp32 (fp64 for fp64 inputs), is updated in place (as by
+    any in-place operation, a graph that saved it then raises in its backward pass).
     Without ``slots`` sequence b has state b and N is B.  ``slots (B,)``, int32 or int64, names
     each sequence's state in a pool; a slot outside ``0..N-1`` (-1 for an empty row of a batch)
     touches no state and gives a zero output row.  Two sequences must not name the same slot.
@@ -265,4 +267,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             state.data_ptr(), pool, _ptr(slots), out.data_ptr(), _lib.raw_stream(dev.index))
     if st:
         _lib.check(st, "fdwt_linattn_step")
+    # written through its pointer: tell autograd, so that a graph that saved this state raises in
+    # its backward pass (inference tensors keep no count and are in no graph)
+    if not state.is_inference():
+        increment_version(state)
     return out
