@@ -279,14 +279,22 @@ class DecayTokenMixer(nn.Module):
         self._log_decay = [math.log1p(-2.0 ** -(5 + 7 * h / max(1, num_heads - 1)))
                            for h in range(num_heads)]
         self._on_device = {}
+        self.log_decay(self.norm.weight.device)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        # made with the move to a device, not in the first call: that one may be captured in a graph
+        self.log_decay(self.norm.weight.device)
+        return self
 
     def log_decay(self, device) -> torch.Tensor:
         """The schedule on ``device`` in fp64's nearest fp32 (kept out of the buffers: a module
         cast to 16 bits must not round it)."""
         device = torch.device(device)
         if device not in self._on_device:
-            self._on_device[device] = torch.tensor(self._log_decay, dtype=torch.float32,
-                                                   device=device)
+            with torch.inference_mode(False):  # kept for training calls, whoever asks first
+                self._on_device[device] = torch.tensor(self._log_decay, dtype=torch.float32,
+                                                       device=device)
         return self._on_device[device]
 
     def init_state(self, batch: int, device, dtype: torch.dtype = torch.float32) -> torch.Tensor:
