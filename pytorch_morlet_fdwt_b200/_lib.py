@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfdwt_b200.so")
@@ -161,6 +162,14 @@ def require_cuda(*tensors) -> torch.device:
         elif t.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     return dev
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation (it has no
+    ``requires_grad``; an autograd function without a ``jvp`` raises on it)."""
+    if forward_ad._current_level < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -98,7 +98,7 @@ def _schedule(log_decay, heads: int, dtype: torch.dtype) -> torch.Tensor:
     if log_decay.shape != (heads,) or not log_decay.is_floating_point():
         raise ValueError(f"log_decay must be floating point of shape ({heads},), got "
                          f"{log_decay.dtype} {tuple(log_decay.shape)}")
-    if log_decay.requires_grad:
+    if log_decay.requires_grad or _lib.has_tangent(log_decay):
         raise ValueError("log_decay is a fixed schedule without a gradient; detach it")
     if log_decay.dtype != dtype or not log_decay.is_contiguous():
         log_decay = log_decay.to(dtype).contiguous()
@@ -225,7 +225,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         needs = needs or initial_state.requires_grad
     if lengths is not None:
         lengths = _indexes(lengths, d.batch, 0, d.length, "lengths")
-    if needs and torch.is_grad_enabled():
+    if (needs and torch.is_grad_enabled()) or _lib.has_tangent(q, k, v, initial_state):
         return _LinearAttentionFunction.apply(q, k, v, log_decay, initial_state, lengths, scale,
                                               plan)
     return _forward(q, k, v, log_decay, initial_state, lengths, plan)
@@ -253,8 +253,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _check_state(state, (pool, d.heads, d.dk, d.dv), acc)
     if not state.is_contiguous():
         raise ValueError("the state is updated in place and must be contiguous")
-    if (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad) \
-            and torch.is_grad_enabled():
+    if ((q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)
+            and torch.is_grad_enabled()) or _lib.has_tangent(q, k, v, state):
         raise RuntimeError("linear_attention_step has no gradient: use linear_attention, or "
                            "torch.no_grad()")
     if slots is not None:

@@ -115,7 +115,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
             raise TypeError(f"weight and bias must have one type, got {weight.dtype} and "
                             f"{bias.dtype}")
         param, needs = _lib.DTYPES[bias.dtype], needs or bias.requires_grad
-    if needs and torch.is_grad_enabled():
+    if (needs and torch.is_grad_enabled()) or _lib.has_tangent(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, float(eps), (code, param))
     return _forward(x, weight, bias, float(eps), (code, param), False)[0]
 
