@@ -89,6 +89,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _plan(names, q, k, v, scale, out_stride=None):
+    if scale is not None and type(scale) is not float:
+        # a number by value: a tensor would be looked up by its identity
+        if isinstance(scale, torch.Tensor) and scale.requires_grad:
+            raise ValueError("scale is a number without a gradient; detach it")
+        scale = float(scale)
     return _describe(names, (q.dtype, k.dtype, v.dtype), (q.shape, k.shape, v.shape),
                      (q.stride(), k.stride(), v.stride()), out_stride, scale, q.device.index)
 
@@ -151,9 +156,9 @@ class _LinearAttentionFunction(torch.autograd.Function):
     back in time (one C call)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, initial, lengths, scale, plan):
+    def forward(ctx, q, k, v, log_decay, initial, lengths, plan):
         ctx.set_materialize_grads(False)
-        ctx.scale, ctx.plan = scale, plan
+        ctx.plan = plan
         ctx.save_for_backward(q, k, v, log_decay, initial, lengths)
         return _forward(q, k, v, log_decay, initial, lengths, plan)
 
@@ -162,7 +167,7 @@ class _LinearAttentionFunction(torch.autograd.Function):
     def backward(ctx, d_out, d_final):
         q, k, v, log_decay, initial, lengths = ctx.saved_tensors
         if d_out is None and d_final is None:
-            return (None,) * 8
+            return (None,) * 7
         plan = ctx.plan
         d = plan[0]
         dev = q.device
@@ -170,7 +175,7 @@ class _LinearAttentionFunction(torch.autograd.Function):
             d_out = torch.zeros((d.batch, d.length, d.heads, d.dv), device=dev, dtype=q.dtype)
         elif not d_out.is_contiguous():
             d_out = _rows(d_out)
-            plan = _plan(_SEQUENCE, q, k, v, ctx.scale, d_out.stride())
+            plan = _plan(_SEQUENCE, q, k, v, d.scale, d_out.stride())
         if d_final is not None:
             d_final = d_final.contiguous()
         dq, dkk, dvv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
@@ -187,7 +192,7 @@ class _LinearAttentionFunction(torch.autograd.Function):
             _lib.check(st, "fdwt_linattn_backward")
         if config.check_device_errors:
             _lib.check_device_error("fdwt_linattn_backward")
-        return dq, dkk, dvv, None, d_initial, None, None, None
+        return dq, dkk, dvv, None, d_initial, None, None
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -226,8 +231,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     if lengths is not None:
         lengths = _indexes(lengths, d.batch, 0, d.length, "lengths")
     if (needs and torch.is_grad_enabled()) or _lib.has_tangent(q, k, v, initial_state):
-        return _LinearAttentionFunction.apply(q, k, v, log_decay, initial_state, lengths, scale,
-                                              plan)
+        return _LinearAttentionFunction.apply(q, k, v, log_decay, initial_state, lengths, plan)
     return _forward(q, k, v, log_decay, initial_state, lengths, plan)
 
 
