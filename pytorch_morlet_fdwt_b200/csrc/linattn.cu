@@ -400,8 +400,8 @@ template <int DK> struct Tf32 {
   static constexpr size_t smem = words * sizeof(float);
 };
 
-// Two blocks leave 128 registers a thread, too few for 16-bit rows: 37 tokens of bf16 take 18 us
-// with them and 11.5 us with more.
+// Two blocks leave 128 registers a thread, too few for 16-bit rows: 37 tokens of bf16 (off 16-byte
+// boundaries) take 18 us with them and 11.5 us with more.
 template <typename T, int DK, bool STATES>
 __global__ void __launch_bounds__(256, DK == 64 && sizeof(T) == 4 ? 2 : 1)
 linattn_tf32_kernel(const __grid_constant__ Call call) {
@@ -796,8 +796,6 @@ inline bool vector_ok(const void* p, const int64_t* strides, int dim, size_t siz
          strides[1] % v == 0 && strides[2] % v == 0;
 }
 
-constexpr int kShort = 64, kFewRows = 512;
-
 struct Plan {
   bool tc;
   int chunk, tile, nseg;
@@ -872,12 +870,11 @@ int run(int dtype, Call& call, void* workspace, cudaStream_t stream) {
     job.o_vec = vector_ok(job.o, job.os, job.dv, o_size, 16) +
                 vector_ok(job.o, job.os, job.dv, o_size, 32);
   }
-  // One short chunk goes to the general kernel: as fast there (64 tokens of 4 heads of 64: 12.5 us
-  // against 10.5, less than a call's host time), and without the 16-bit rounding of the scores,
-  // which few rows do not average out.  So do two of them with few rows in all.
-  const int64_t rows = call.batch * call.heads * call.length;
-  const bool small = call.length <= kShort || (call.length <= 2 * kShort && rows <= kFewRows);
-  const bool tc = !small && tc_supports(dtype, call);
+  // The tensor cores wherever their kernel takes the call's types, sizes and strides: faster from
+  // one token on (bf16, one sequence of 4 heads of 64: 1 token 10.3 us against the general
+  // kernel's 12.4, 128 tokens 10.3 against 20.6; 32 sequences of 16 heads of 128: 79 against 117
+  // and 85 against 223), and as exact.
+  const bool tc = tc_supports(dtype, call);
   const Plan p = make_plan(dtype, call, tc);
   call.nseg = p.nseg;
   call.seg_len = p.seg_len;

@@ -23,6 +23,10 @@ CASES = [  # B, L, H, Hkv, Dk, Dv, initial, lengths, fast decay
     (2, 640, 3, 3, 64, 64, True, None, True),
     (1, 2050, 1, 1, 128, 64, False, None, False),
     (8, 129, 8, 8, 16, 32, True, None, False),
+    (4, 1, 8, 8, 64, 64, True, None, False),
+    (1, 37, 4, 4, 64, 64, False, None, False),
+    (2, 64, 4, 2, 128, 64, True, None, False),
+    (2, 100, 2, 2, 64, 128, False, [100, 63], False),
 ]
 
 
@@ -46,3 +50,42 @@ def test_one_rounding(B, L, H, Hk, Dk, Dv, initial, lengths, fast, dtype):
         once = _rms(r.to(dtype).double() - r)
         off = _rms(g.double() - r)
         assert off <= 1.05 * once, f"{name}: {off / once:.3f} times the rounding of the result"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("L", [1, 40, 64, 65, 100, 128])
+def test_a_sequence_alone_and_in_a_batch(L, dtype):
+    """The kernel goes by a sequence's own sizes: up to a chunk of tokens, which is never cut into
+    segments, the bits are the same whatever else is in the call."""
+    q, k, v, a, s0, _ = _inputs(7, L, 4, 2, 64, 64, dtype, L, True)
+    do = torch.randn(7, L, 4, 64, device=DEV).to(dtype)
+
+    def results(rows):
+        ts = [t[rows].detach().requires_grad_() for t in (q, k, v, s0)]
+        out, final = F.linear_attention(*ts[:3], a, initial_state=ts[3])
+        return (out, final, *torch.autograd.grad(out, ts, do[rows]))
+
+    batch = results(slice(0, 7))
+    for b in (0, 6):
+        for alone, whole in zip(results(slice(b, b + 1)), batch):
+            assert torch.equal(alone[0], whole[b])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("L", [129, 700])
+def test_a_long_sequence_alone_and_in_a_batch(L, dtype):
+    """Longer ones are cut into as many segments as the call's blocks leave room for, which adds
+    up the same 32-bit sums in another order: (64 + 64 + 128 + L / 32) 2^-24 of their magnitudes
+    at most, and 16-bit results a rounding (u of the result) where that decides one."""
+    q, k, v, a, s0, _ = _inputs(24, L, 8, 8, 64, 64, dtype, L, True)
+    unit = {torch.float32: 0.0, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -7}[dtype]
+    with torch.no_grad():
+        batch = F.linear_attention(q, k, v, a, initial_state=s0)
+        alone = F.linear_attention(q[5:6], k[5:6], v[5:6], a, initial_state=s0[5:6])
+        size = _reference(q[5:6].abs(), k[5:6].abs(), v[5:6].abs(), a, s0[5:6].abs(), None, 0.125)
+        growth = (256 + L / 32) * 2.0 ** -24
+        low = 0.0 if dtype == torch.float32 else 2.0 ** -16  # parts of scores and states
+        for one, all_, mag, u in zip(alone, batch, size, (unit, 0.0)):
+            one, whole = one[0].double(), all_[5].double()
+            assert ((one - whole).abs() <= (growth + (low if u else 0.0)) * mag[0]
+                    + u * one.abs()).all()
