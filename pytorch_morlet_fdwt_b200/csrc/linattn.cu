@@ -374,6 +374,12 @@ struct FragB {
     tf32_split(q[0], hi[0], lo[0]);
     tf32_split(q[4 * ks], hi[1], lo[1]);
   }
+  // with zeros for infinities and NaN
+  __device__ __forceinline__ void load_finite(const float* p, int ks, int cs, int lane) {
+    const float* q = p + lane % 4 * ks + lane / 4 * cs;
+    tf32_split(isfinite(q[0]) ? q[0] : 0.0f, hi[0], lo[0]);
+    tf32_split(isfinite(q[4 * ks]) ? q[4 * ks] : 0.0f, hi[1], lo[1]);
+  }
   __device__ __forceinline__ void load(const float* p, int ks, int cs, int lane, float w0,
                                        float w1) {
     const float* q = p + lane % 4 * ks + lane / 4 * cs;
@@ -545,6 +551,38 @@ linattn_tf32_kernel(const __grid_constant__ Call call) {
           y.load(sv + u * PV + c0 + 8 * j, PV, 1, lane);
           own[j].add(x, y);
         }
+      }
+      float worst = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) worst += own[j].value(e) * 0.0f;
+      if (__any_sync(0xffffffffu, worst != 0.0f)) {  // NaN
+        // Infinities or NaN among the values (or scores): the masked scores of the block on the
+        // diagonal, factors of zero, would bring them to earlier tokens.  Again with zeros in
+        // their place, and NaN from their token on.
+#pragma unroll
+        for (int j = 0; j < 4; ++j) own[j] = Block();
+#pragma unroll 1
+        for (int u = 0; u < r0 + 16; u += 8) {
+          FragA x;
+          x.load(sp + r0 * PP + u, PP, 1, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            FragB y;
+            y.load_finite(sv + u * PV + c0 + 8 * j, PV, 1, lane);
+            own[j].add(x, y);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = r0 + g + e / 2 * 8, col = c0 + 8 * j + 2 * t4 + e % 2;
+#pragma unroll 1
+            for (int u = 0; u <= t; ++u)
+              if (!isfinite(sv[u * PV + col])) own[j].hi[e] = nanf("");
+          }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)

@@ -306,11 +306,11 @@ struct Where {
 __device__ __forceinline__ bool first_block() { return blockIdx.x == 0 && blockIdx.y == 0; }
 
 // Block (value tile of the jobs of a sequence and head, segment).
-__device__ __forceinline__ Where locate(const Call& call) {
+__device__ __forceinline__ Where locate(const Call& call, unsigned x, unsigned y) {
   Where w;
-  w.bh = static_cast<int>(blockIdx.x / static_cast<unsigned>(call.tiles));
-  int tile = static_cast<int>(blockIdx.x) - w.bh * call.tiles;
-  w.seg = blockIdx.y;
+  w.bh = static_cast<int>(x / static_cast<unsigned>(call.tiles));
+  int tile = static_cast<int>(x) - w.bh * call.tiles;
+  w.seg = static_cast<int>(y);
   int ji = 0;
   while (tile >= call.job[ji].tiles) tile -= call.job[ji++].tiles;
   w.job = &call.job[ji];
@@ -520,6 +520,74 @@ __device__ __forceinline__ void store_wide(float* dst, const float (&x)[16], int
              __float_as_uint(x[g * 8 + 6]), __float_as_uint(x[g * 8 + 7]));
 }
 
+// ------------------------------------------------------------------------------ non-finite values
+// P V takes an infinity or NaN among a chunk's values to the chunk's earlier tokens too (a masked
+// score is a factor zero of the product).  Such a value also makes its column of the segment's end
+// state NaN, which costs nothing to see; what it spoilt, its column's outputs in its chunk before
+// its token, is then formed again by the recurrence.  The warp looks for column c's first such
+// token and walks to it from the segment's first one, lanes taking rows of the column:
+//   R_l = d R_{l-1} + k_l v_l,   o_l = q_l . (inter d^{l+off} S_0 + intra R_l).
+template <typename T, int DK>
+__device__ __forceinline__ void restore_column(const Call& call, const Where& w, int c, int lane) {
+  constexpr int N = DK / 32;
+  const Job& job = *w.job;
+  auto token = [&](int l) { return int64_t(job.reverse ? w.n - 1 - l : l); };
+  const T* v = static_cast<const T*>(job.v) + w.b * job.vs[0] + w.h / job.v_group * job.vs[2] +
+               w.v0 + c;
+  int first = w.begin;  // of the tokens not known to be finite
+  for (; first < w.end; first += 32) {
+    const int l = first + lane;
+    const unsigned odd = __ballot_sync(
+        0xffffffffu, l < w.end && !isfinite(to_acc(v[token(l < w.end ? l : first) * job.vs[1]])));
+    if (odd != 0) {
+      first += __ffs(odd) - 1;
+      break;
+    }
+  }
+  const int from = w.begin + (first - w.begin) / C * C;  // its chunk's first token
+  if (first >= w.end || first == from) return;
+  const T* q = static_cast<const T*>(job.q) + w.b * job.qs[0] + w.h / job.q_group * job.qs[2];
+  const T* k = static_cast<const T*>(job.k) + w.b * job.ks[0] + w.h / job.k_group * job.ks[2];
+  const int64_t size = int64_t(job.dk) * job.dv, head = w.bh * size;
+  const float* seg = static_cast<const float*>(job.seg) + head * (call.nseg - 1);
+  const bool inside = call.scan_inside != 0;
+  const float whole = inside ? decay_pow(w.a, float(call.seg_len)) : 0.0f;
+  const float keep = decay_pow(w.a, 1.0f);
+  float s0[N], r[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // the state before the segment
+    const int row = lane + 32 * i;
+    s0[i] = r[i] = 0.0f;
+    if (row >= job.dk) continue;
+    if (job.init != nullptr && (w.seg == 0 || inside))
+      s0[i] = static_cast<const float*>(job.init)[head + row * job.init_row +
+                                                  (w.v0 + c) * job.init_col];
+    for (int j = inside ? 0 : w.seg - 1; j < w.seg; ++j)
+      if (j >= 0) s0[i] = whole * s0[i] + seg[j * size + int64_t(row) * job.dv + w.v0 + c];
+  }
+  for (int l = w.begin; l < first; ++l) {
+    const float x = to_acc(v[token(l) * job.vs[1]]);
+    float sum = 0.0f;
+    const float read = float(job.inter) * decay_pow(w.a, float(l - w.begin + job.off));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = lane + 32 * i;
+      if (row >= job.dk) continue;
+      r[i] = keep * r[i] + to_acc(k[token(l) * job.ks[1] + row]) * x;
+      if (l >= from)
+        sum += to_acc(q[token(l) * job.qs[1] + row]) * (read * s0[i] + float(job.intra) * r[i]);
+    }
+    if (l < from) continue;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int64_t at = w.b * job.os[0] + w.h * job.os[2] + w.v0 + c + token(l) * job.os[1];
+    if (lane == 0) {
+      if (job.o_wide) static_cast<float*>(job.o)[at] = sum;
+      else static_cast<T*>(job.o)[at] = from_acc<T>(sum);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------ main launch
 template <typename T, int DK>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -541,11 +609,12 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
   __shared__ volatile float s_most[4];  // fp16: largest magnitude of each warp's rows
 
   __shared__ float dpow[C + 1];  // d^n
+  __shared__ unsigned odd[2];    // columns of the end state with infinities or NaN
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (warp == 0) tmem_alloc(&tmem_slot);
   const Limit limit{&failed, extra_tx == 0 ? kWaitCycles : kTestCycles};
-  const Where w = locate(call);
+  const Where w = locate(call, blockIdx.x, blockIdx.y);
   const Job& job = *w.job;
   const uint32_t base = smem_addr(sm);
   const int chunks = w.chunks;
@@ -594,6 +663,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
     bar_init(&most_full, 4);
     bar_init(&drain, 1);
     failed = 0;
+    odd[0] = odd[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async();
 #pragma unroll 1
@@ -798,6 +868,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
         }
       }
     }
+    asm volatile("bar.arrive 1, 256;" ::: "memory");
   } else if (warp >= 20) {
     take_registers<136>();
     // ---- the state, a row of 64 columns a thread (DK = 64: 16 rows a warp, the lanes that a
@@ -818,7 +889,9 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
                            w.v0 * job.init_col;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-          s[c / 32][c % 32] = c < cols ? *src : 0.0f;
+          const float x = c < cols ? *src : 0.0f;
+          // (fp16: as NaN an infinity leaves the scale of the other columns' copy alone)
+          s[c / 32][c % 32] = kHalf && isinf(x) ? nanf("") : x;
           src += job.init_col;
         }
       } else {
@@ -916,11 +989,30 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
       fence_async();
       bar_arrive(&s_full);
     }
+    float zeros[2] = {0.0f, 0.0f};  // 0 s: NaN for what is not finite
+#pragma unroll
+    for (int c = 0; c < NV; c += 2) {
+      float x = s[c / 32][c % 32], y = s[c / 32][c % 32 + 1];
+      fma2(x, y, 0.0f, zeros[0], zeros[1]);
+      zeros[0] = x;
+      zeros[1] = y;
+    }
+    if (ok && mine && r < job.dk && zeros[0] + zeros[1] != 0.0f) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+        if (!isfinite(s[c / 32][c % 32])) atomicOr(&odd[c / 32], 1u << (c % 32));
+    }
     if (ok && w.seg == w.last && job.fin != nullptr && mine && r < job.dk) {
       float* dst = static_cast<float*>(job.fin) + w.bh * size + int64_t(r) * job.dv + w.v0;
 #pragma unroll
       for (int c = 0; c < NV; ++c)
         if (c < w.vcols) dst[c] = s[c / 32][c % 32];
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // o is stored, odd is whole
+    if ((odd[0] | odd[1]) != 0) {
+#pragma unroll 1
+      for (int c = warp - 20; c < w.vcols; c += 4)
+        if (odd[c / 32] >> (c % 32) & 1) restore_column<T, DK>(call, w, c, lane);
     }
   } else if (warp == 1) {
     give_registers<40>();
@@ -1093,7 +1185,7 @@ linattn_tc_state_kernel(const __grid_constant__ Call call, const __grid_constant
   __shared__ volatile int failed;
   const Limit limit{&failed, extra_tx == 0 ? kWaitCycles : kTestCycles};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-  const Where w = locate(call);
+  const Where w = locate(call, blockIdx.x, blockIdx.y);
   const Job& job = *w.job;
   if (w.seg >= w.last) return;  // the whole block
   if (warp == 16) tmem_alloc(&tmem_slot);

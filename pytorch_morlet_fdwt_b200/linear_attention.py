@@ -216,7 +216,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     Returns ``(out (B, L, H, Dv), final_state (B, H, Dk, Dv))``, differentiable once in q, k, v
     and initial_state.  fp16 and bf16 inputs are computed to 32 bits, states too, and the result
-    rounded once.
+    rounded once.  An infinity or NaN reaches the outputs of its token and later ones only.
     """
     _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _rows(q), _rows(k), _rows(v)
