@@ -316,7 +316,7 @@ typedef struct {
 } fdwt_linattn_desc;
 
 /* out and the states after the sequences (final_state; may be NULL) from initial_state (NULL:
- * zeros). */
+ * zeros).  The workspaces of both calls begin on a multiple of 32 bytes. */
 size_t fdwt_linattn_forward_workspace(const fdwt_linattn_desc* desc);
 int fdwt_linattn_forward(const fdwt_linattn_desc* desc, const void* q, const void* k,
                          const void* v, const void* log_decay, const void* initial_state,

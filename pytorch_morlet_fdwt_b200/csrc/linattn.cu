@@ -869,6 +869,9 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   return p;
 }
 
+// States between segments and the heads' own gradients are stored 32 bytes at a time.
+constexpr uintptr_t kWorkspaceAlign = 32;
+
 inline size_t seg_bytes(const Call& call, const Job& job, int nseg, int dtype) {
   const size_t bytes = size_t(call.batch) * call.heads * (nseg - 1) * job.dk * job.dv *
                        (dtype == FDWT_F64 ? 8 : 4);
@@ -1075,6 +1078,7 @@ extern "C" int fdwt_linattn_forward(const fdwt_linattn_desc* desc, const void* q
   FDWT_CHECK(q != nullptr && k != nullptr && v != nullptr && log_decay != nullptr && out != nullptr);
   const size_t need = fdwt_linattn_forward_workspace(desc);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FDWT_ERR_WORKSPACE;
+  FDWT_CHECK(need == 0 || reinterpret_cast<uintptr_t>(workspace) % kWorkspaceAlign == 0);
   Call call{};
   shape_jobs(desc, false, &call);
   call.log_decay = log_decay;
@@ -1128,6 +1132,7 @@ extern "C" int fdwt_linattn_backward(const fdwt_linattn_desc* desc, const void* 
              d_out != nullptr && dq != nullptr && dk != nullptr && dv != nullptr);
   const size_t need = fdwt_linattn_backward_workspace(desc);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FDWT_ERR_WORKSPACE;
+  FDWT_CHECK(need == 0 || reinterpret_cast<uintptr_t>(workspace) % kWorkspaceAlign == 0);
   Call call{};
   shape_jobs(desc, true, &call);
   call.log_decay = log_decay;
