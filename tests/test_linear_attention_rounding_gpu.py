@@ -89,3 +89,26 @@ def test_a_long_sequence_alone_and_in_a_batch(L, dtype):
             one, whole = one[0].double(), all_[5].double()
             assert ((one - whole).abs() <= (growth + (low if u else 0.0)) * mag[0]
                     + u * one.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,Hk,Dk,Dv,lengths", [
+    (2, 37, 2, 2, 64, 64, None), (1, 128, 4, 2, 128, 128, None), (3, 200, 2, 1, 48, 80, [200, 77, 1]),
+    (2, 300, 2, 2, 128, 64, None), (1, 600, 1, 1, 64, 64, None)])
+def test_states_of_16_bit_inputs_keep_32_bits(B, L, H, Hk, Dk, Dv, lengths, dtype):
+    """Last states and the initial states' gradients: two fp16 parts of a value leave 2^-22 of it
+    out, three bf16 parts less; the matrix unit cuts its 32-bit sum off at each of the L / 16 steps,
+    2^-25 of it on average, and 2^-22 covers the sums outside.  Two bf16 parts would leave 2^-19."""
+    q, k, v, a, s0, n = _inputs(B, L, H, Hk, Dk, Dv, dtype, L, True, lengths)
+    do = torch.randn(B, L, H, Dv, device=DEV).to(dtype)
+    ds = torch.randn(B, H, Dk, Dv, device=DEV)
+    start = s0.clone().requires_grad_()
+    out, final = F.linear_attention(q, k, v, a, initial_state=start, lengths=n)
+    (ds0,) = torch.autograd.grad((out, final), start, (do, ds))
+    rstart = s0.double().requires_grad_()
+    rout, rfinal = _reference(q, k, v, a, rstart, n, Dk ** -0.5)
+    (rds0,) = torch.autograd.grad((rout, rfinal), rstart, (do.double(), ds.double()))
+    bound = 2.0 ** -21 + L / 16 * 2.0 ** -25
+    for name, got, ref in (("final state", final, rfinal), ("ds0", ds0, rds0)):
+        off = _rms(got.double() - ref) / _rms(ref)
+        assert off <= bound, f"{name}: {off:.3g}, bound {bound:.3g}"
