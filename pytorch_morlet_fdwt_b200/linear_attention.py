@@ -217,6 +217,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Returns ``(out (B, L, H, Dv), final_state (B, H, Dk, Dv))``, differentiable once in q, k, v
     and initial_state.  fp16 and bf16 inputs are computed to 32 bits, states too, and the result
     rounded once.  An infinity or NaN reaches the outputs of its token and later ones only.
+
+    The kernels for fp16 and bf16 wait on copies with a time limit (about a second; a machine in
+    order never gets near it).  Where one runs out the results are incomplete and the call does
+    not know: :func:`~pytorch_morlet_fdwt_b200._lib.device_error` does, and with
+    ``config.check_device_errors`` every call asks it, synchronising the device, and raises.
     """
     _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _rows(q), _rows(k), _rows(v)
