@@ -8,9 +8,10 @@
 // centred values, a second pass over registers, since E x^2 - m^2 cancels for a large mean.
 // Sums, statistics and the gradients' partial sums are 32 bits (64 for fp64 rows).
 //
-// Measured: 65536 x 2048 bf16 forward 96 us (5.6 TB/s), backward 166 us (4.9 TB/s); 65536 x 1024
-// fp32 88 and 132 us (6.1 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
-// 54 and 88 us (5.9 and 5.4 TB/s).
+// Measured: 65536 x 2048 bf16 forward 96 us (5.6 TB/s), backward 165 us (4.9 TB/s); 65536 x 1024
+// fp32 88 and 133 us (6.1 TB/s both); 40000 x 1001 fp32, whose rows start off 16-byte boundaries,
+// 55 and 88 us (5.8 and 5.5 TB/s); 32768 x 1024 fp64 84 and 132 us (6.4 and 6.1 TB/s).  Rows too
+// long for registers: 16384 x 12288 bf16 181 and 728 us (4.4 and 1.7 TB/s).
 #include <initializer_list>
 #include <type_traits>
 

@@ -36,8 +36,8 @@ __device__ __forceinline__ int64_t token_of(int64_t l, int64_t n, int reverse) {
 // rows x cols of a tensor (row l at base + token * stride) into shared memory, zeros past
 // `valid` rows and `cols` columns.  256 threads; where no conversion is due and rows are aligned
 // the copies are asynchronous (tiles_wait() below), else all loads are issued before the stores:
-// one latency a tile instead of one a group (5 x 1537 tokens, 6 heads of 48 x 80, fp32: state
-// launch 50 -> 33 us, main launch 113 -> 96 us).
+// one latency a tile instead of one a group (5 x 1537 tokens, 6 heads of 48 x 80, fp32: 163 -> 129 us
+// for both launches at that step, 123 us now).
 template <typename T, typename A, int ROWS, int COLS, int PITCH>
 __device__ __forceinline__ void load_tile(A* dst, const T* base, int64_t stride, int64_t l0,
                                           int64_t n, int reverse, int valid, int cols, int vec) {
@@ -858,8 +858,11 @@ inline Plan make_plan(int dtype, const Call& call, bool tc) {
   for (int j = 0; j < call.jobs; ++j) tiles += cdiv(call.job[j].dv, p.tile);
   const int64_t chunks = imax(1, cdiv(call.length, p.chunk));
   // Blocks a multiprocessor holds; two of the fp32 kernel up to heads of 64 (5 x 1537 tokens, 6
-  // heads of 48 x 80: 120 us so, 132 us with one).  Times in microseconds a chunk (measured): 128
-  // tokens on the tensor cores, 64 (or 32) by the general kernels.
+  // heads of 48 x 80: 120 us so, 132 us with one at that step).  Times in microseconds a chunk, all
+  // multiprocessors busy: measured for the tensor cores (128 tokens).  For the general kernels one
+  // set stands for all, near that of fp32 heads of 64 (64 tokens, 8.1 us with one block a
+  // multiprocessor, 11.9 with two); others measure 10 to 26 us, 16-bit rows of 128 off 16-byte
+  // boundaries 38 us.
   const int64_t slots = int64_t(sm_count()) * (dtype == FDWT_F32 && dk <= 64 ? 2 : 1);
   const int64_t units = tiles * call.batch * call.heads;
   const Cost cost = tc ? Cost{dk <= 64 ? 2.3 : 2.8, 0.75, 6.0, 4.0} : Cost{7.5, 3.0, 5.0, 4.0};

@@ -23,9 +23,10 @@
 // overlap: one warp issues the loads (TMA), one all products, four form P, eight V', four finish
 // o, four keep the state.  All parts of V' are one product (N = 64 parts), so that K is read once:
 // the shared-memory rate binds the products more than the tensor rate.  Measured with all SMs
-// busy, bf16: 2.3 us a chunk with heads of 64 (4 x 4096 tokens of 37 heads, 84 us), 2.8 us with
-// heads of 128 (2 x 4096 of 37 heads, 103 us); 67 and 87 us with P and S in one part.  Every wait
-// on a barrier has a time limit.
+// busy, bf16: 2.3 us a chunk with heads of 64 (4 x 4096 tokens of 37 heads, 85 us; 304 KB a chunk
+// through shared memory, 1.2 us at its rate), 2.8 us with heads of 128 (2 x 4096 of 37 heads, 102
+// us; 448 KB, 1.8 us); 67 and 87 us with P and S in one part.  The first chunk is out after 10 us.
+// Every wait on a barrier has a time limit.
 #include <cuda.h>
 
 #include <type_traits>
@@ -1369,7 +1370,7 @@ int launch_as(const Call& call, const Maps& maps, bool states, cudaStream_t stre
   config.dynamicSmemBytes = states ? Smem<T, DK>::st_bytes : Smem<T, DK>::bytes;
   config.stream = stream;
   // The main launch right after the state launch starts beside its end (1 x 1024 x 8 heads of 64:
-  // 23.1 us one after the other, 20.7 us so).  Its state warps wait for the state launch; nothing
+  // 19.0 us one after the other, 16.8 us so).  Its state warps wait for the state launch; nothing
   // else in it touches what that one reads or writes.
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
