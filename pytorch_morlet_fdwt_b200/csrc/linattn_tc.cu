@@ -890,9 +890,7 @@ linattn_tc_kernel(const __grid_constant__ Call call, const __grid_constant__ Map
                            w.v0 * job.init_col;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-          const float x = c < cols ? *src : 0.0f;
-          // (fp16: as NaN an infinity leaves the scale of the other columns' copy alone)
-          s[c / 32][c % 32] = kHalf && isinf(x) ? nanf("") : x;
+          s[c / 32][c % 32] = c < cols ? *src : 0.0f;
           src += job.init_col;
         }
       } else {

@@ -141,3 +141,29 @@ def test_many_values(dtype, L):
     assert torch.equal(final[0, 0].isfinite().all(0), first == L)
     keep = ~reached
     _close(out[0, :, 0][keep], clean[0, :, 0][keep], dtype)
+
+
+@pytest.mark.parametrize("dtype,Dk,Dv", CASES)
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_an_initial_state_that_is_not_finite(dtype, Dk, Dv, value):
+    """It passes through a sequence without tokens as it is, and stays in its column of another."""
+    torch.manual_seed(Dk)
+    L, H = 200, 2
+    acc = torch.float64 if dtype == torch.float64 else torch.float32
+    q, k = (torch.randn(2, L, H, Dk, device=DEV).to(dtype) for _ in range(2))
+    v = torch.randn(2, L, H, Dv, device=DEV).to(dtype)
+    s0 = torch.randn(2, H, Dk, Dv, device=DEV, dtype=acc)
+    a = torch.tensor([-0.02, -0.001], device=DEV, dtype=acc)
+    n = torch.tensor([0, L], device=DEV)
+    clean, last = F.linear_attention(q, k, v, a, initial_state=s0, lengths=n)
+    s0[:, 0, Dk // 2, Dv // 2] = value
+    out, final = F.linear_attention(q, k, v, a, initial_state=s0, lengths=n)
+    assert torch.equal(final[0].nan_to_num(7.0), s0[0].nan_to_num(7.0)) and not out[0].any()
+    keep = [i for i in range(Dv) if i != Dv // 2]
+    assert torch.equal(out[1, :, 1], clean[1, :, 1]) and torch.equal(final[1, 1], last[1, 1])
+    assert not out[1, :, 0, Dv // 2].isfinite().any()
+    # the entry itself: times the decay it is what it was
+    got = final[1, 0, Dk // 2, Dv // 2]
+    assert got.isnan() if value != value else got == value
+    _close(out[1, :, 0][:, keep], clean[1, :, 0][:, keep], dtype)
+    _close(final[1, 0][:, keep], last[1, 0][:, keep], dtype)
