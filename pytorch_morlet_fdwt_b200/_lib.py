@@ -167,7 +167,7 @@ def require_cuda(*tensors) -> torch.device:
 def has_tangent(*tensors) -> bool:
     """Whether one of them is a dual tensor of forward-mode differentiation (it has no
     ``requires_grad``; an autograd function without a ``jvp`` raises on it)."""
-    if forward_ad._current_level < 0:
+    if getattr(forward_ad, "_current_level", 0) < 0:  # (torch keeps it there; else ask each)
         return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
