@@ -340,6 +340,74 @@ int fdwt_linattn_step(const fdwt_linattn_desc* desc, const void* q, const void* 
                       const void* log_decay, void* state, int64_t state_slots,
                       const int32_t* slots, void* out, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Root-mean-square norm over the last axis with the residual's addition (no counterpart in the
+ * reference): rows of `dim` values,
+ *   total = x + residual, y = total / sqrt(mean total^2 + eps) * weight.
+ * residual (and total) are of the rows' type or FDWT_F32, total is rounded to that type before
+ * the norm; residual and total are both NULL for the norm of x itself.  weight may be NULL (1),
+ * of the rows' type or FDWT_F32 (fp64 rows: FDWT_F64 all).  rstd, (rows) fp32 (fp64 for fp64
+ * rows), receives 1 / sqrt(...) of each row for the backward pass; NULL skips it.
+ * ---------------------------------------------------------------------------------------- */
+int fdwt_rms_norm_forward(int dtype, int residual_dtype, int param_dtype, int64_t rows,
+                          int64_t dim, const void* x, const void* residual, const void* weight,
+                          double eps, void* y, void* total, void* rstd, void* stream);
+/* The same with y in 8 bits: groups of `group` neighbouring values (a divisor of dim) share the
+ * scale max |y| / 448 (FDWT_E4M3) or max |y| / 127 (FDWT_INT8), 1 where all are zero, and
+ * q = round(y / scale).  scales: (rows, dim / group) fp32.  Rows of fp64 are not supported. */
+enum { FDWT_E4M3 = 0, FDWT_INT8 = 1 };
+int fdwt_rms_norm_quantized(int dtype, int residual_dtype, int param_dtype, int out_type,
+                            int64_t rows, int64_t dim, int64_t group, const void* x,
+                            const void* residual, const void* weight, double eps, void* q,
+                            void* scales, void* total, void* stream);
+/* dL/dx = dL/dresidual (rows, dim) and dL/dweight (dim, param_dtype) from dL/dy and dL/dtotal
+ * (NULL: zeros) and the forward pass's total (x itself without a residual) and rstd.  dresidual
+ * is the same gradient in the residual's type where that is another; it and the others may be
+ * NULL.  The sums over rows are added in a fixed order (the same bits every run). */
+size_t fdwt_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t dim, int need_weight);
+int fdwt_rms_norm_backward(int dtype, int residual_dtype, int param_dtype, int64_t rows,
+                           int64_t dim, const void* dy, const void* dtotal, const void* total,
+                           const void* weight, const void* rstd, void* dx, void* dresidual,
+                           void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Short causal convolution over tokens (no counterpart in the reference), each channel with its
+ * own `width` taps:
+ *   p_t = bias + sum_j weight[j] x_{t - width + 1 + j},   y = p, or p sigmoid(p) with silu.
+ * x, addressed by (batch, token) strides in elements with contiguous channels; weight (dim,
+ * width) and bias (dim; may be NULL) of the rows' type or FDWT_F32; initial_state (batch,
+ * width - 1, dim), the inputs before the first token (NULL: zeros), and final_state, those
+ * before the token after the last (may be NULL), contiguous, of the rows' type.  lengths (batch,
+ * int32, may be NULL) gives the tokens that count, clamped to [0, length]: y and gradients after
+ * them are zero, and what stands there is not read.  y is contiguous.
+ * ---------------------------------------------------------------------------------------- */
+#define FDWT_MAX_CONV_WIDTH 8
+typedef struct {
+  int32_t dtype, param_dtype;
+  int32_t width; /* 2 to FDWT_MAX_CONV_WIDTH */
+  int32_t silu;
+  int64_t batch, length, dim;
+  int64_t x_stride[2], dy_stride[2]; /* batch, token */
+} fdwt_conv1d_desc;
+
+int fdwt_causal_conv1d_forward(const fdwt_conv1d_desc* desc, const void* x, const void* weight,
+                               const void* bias, const void* initial_state,
+                               const int32_t* lengths, void* y, void* final_state, void* stream);
+/* dL/dx (contiguous), dL/dweight, dL/dbias and dL/dinitial_state, each may be NULL, from dL/dy
+ * and dL/dfinal_state (NULL: zeros).  Sums over tokens are added in a fixed order. */
+size_t fdwt_causal_conv1d_backward_workspace(const fdwt_conv1d_desc* desc);
+int fdwt_causal_conv1d_backward(const fdwt_conv1d_desc* desc, const void* x, const void* weight,
+                                const void* bias, const void* initial_state,
+                                const int32_t* lengths, const void* dy,
+                                const void* d_final_state, void* dx, void* dweight, void* dbias,
+                                void* d_initial_state, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* One token for each of desc->batch sequences (desc->length is 1): the states in `state`
+ * (state_slots, width - 1, dim) move on by one in place; slots as in fdwt_linattn_step. */
+int fdwt_causal_conv1d_step(const fdwt_conv1d_desc* desc, const void* x, const void* weight,
+                            const void* bias, void* state, int64_t state_slots,
+                            const int32_t* slots, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,18 +9,22 @@
 * :func:`layer_norm`, :func:`linear_attention`, :func:`linear_attention_step` and the layers
   :class:`LayerNorm`, :class:`DecayTokenMixer` -- a causal token mixer for training, prompts and
   single tokens.
+* :func:`rms_norm`, :func:`rms_norm_quantized` (:class:`RMSNorm`), :func:`causal_conv1d` and
+  :func:`causal_conv1d_step` -- the norm with the residual's addition and the short convolution of
+  stacks of causal mixers.
 
 Every transform runs in hand-written CUDA kernels for sm_100a behind the C ABI of
 ``include/fdwt_b200.h`` (``libfdwt_b200.so``); inputs must be CUDA tensors.
 """
 
 from . import config
+from .causal_conv import causal_conv1d, causal_conv1d_step
 from .cwt import CWT1D, MorletPlan, cwt, freqs_to_scales, scales_to_freqs
 from .dwt import DWT1D, IDWT1D, dwt, dwt_max_level, idwt, wavedec, waverec
 from .layers import (DecayTokenMixer, MorletAttention, MorletChannelMixAttention,
                      MorletTokenMixer, WaveletTokenMixer)
 from .linear_attention import linear_attention, linear_attention_step
-from .norm import LayerNorm, layer_norm
+from .norm import LayerNorm, RMSNorm, layer_norm, rms_norm, rms_norm_quantized
 from .wavelets import FilterBank, get_filter_bank
 
 __version__ = "0.1.0"
@@ -30,5 +34,6 @@ __all__ = [
     "DWT1D", "IDWT1D", "dwt", "dwt_max_level", "idwt", "wavedec", "waverec",
     "MorletAttention", "MorletChannelMixAttention", "MorletTokenMixer", "WaveletTokenMixer",
     "DecayTokenMixer", "LayerNorm", "layer_norm", "linear_attention", "linear_attention_step",
+    "RMSNorm", "rms_norm", "rms_norm_quantized", "causal_conv1d", "causal_conv1d_step",
     "FilterBank", "get_filter_bank",
 ]

@@ -115,6 +115,20 @@ SIGNATURES = {
         ctypes.c_size_t, ctypes.c_void_p]),
     "fdwt_linattn_step": (ctypes.c_int, [ctypes.c_void_p] * 6 + [
         ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "fdwt_rms_norm_forward": (ctypes.c_int, [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [
+        ctypes.c_void_p] * 3 + [ctypes.c_double] + [ctypes.c_void_p] * 4),
+    "fdwt_rms_norm_quantized": (ctypes.c_int, [ctypes.c_int] * 4 + [ctypes.c_int64] * 3 + [
+        ctypes.c_void_p] * 3 + [ctypes.c_double] + [ctypes.c_void_p] * 4),
+    "fdwt_rms_norm_backward_workspace": (ctypes.c_size_t, [
+        ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "fdwt_rms_norm_backward": (ctypes.c_int, [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [
+        ctypes.c_void_p] * 9 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_causal_conv1d_forward": (ctypes.c_int, [ctypes.c_void_p] * 9),
+    "fdwt_causal_conv1d_backward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_causal_conv1d_backward": (ctypes.c_int, [ctypes.c_void_p] * 13 + [
+        ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_causal_conv1d_step": (ctypes.c_int, [ctypes.c_void_p] * 5 + [
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,547 @@
+// Short causal convolution of every channel with its own taps, over tokens: forward, gradients and
+// the single-token form.
+//
+//   p_t = bias + sum_j w[j] x_{t-W+1+j},   y = p   or   y = p sigmoid(p)
+//   dp = dy dy/dp,   dx_t = sum_j w[j] dp_{t+W-1-j},   dw[j] = sum_t dp_t x_{t-W+1+j},   db = sum_t dp_t
+//
+// Tokens before the first come from the state (the last W-1 inputs of what came before), zeros
+// without one.  Bound by HBM (2 W + 4 operations an element forward): a thread takes V
+// neighbouring channels (16 bytes, forward) and walks over a run of tokens with the last W inputs
+// in registers, so that every input is read once (and W-1 of a run's neighbours, from L2) and the
+// loads of several tokens are in flight.  Sums are 32 bits (64 for fp64); y and the gradients are
+// rounded once.
+#include "row_groups.cuh"
+
+namespace fdwt {
+namespace {
+
+struct ConvCall {
+  int64_t batch, length, dim, xs_b, xs_t, ds_b, ds_t;
+  bool silu, param_f32;
+  const void *x, *weight, *bias, *initial;
+  const int32_t* lengths;
+  cudaStream_t stream;
+};
+
+// 1 / (1 + e^-p): of a few roundings' error in 32 bits for rows of 32 bits, and by the fast
+// exponential and division for 16-bit rows, whose rounding is 2^12 times theirs.
+template <typename T, typename A> __device__ __forceinline__ A sigmoid(A p) {
+  if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-p));
+  else if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-p));
+  else return 1.0 / (1.0 + exp(-p));
+}
+
+// One parameter of the rows' type or of 32 bits.
+template <typename T>
+__device__ __forceinline__ typename AccOf<T>::type param(const void* p, bool f32, int64_t i) {
+  using A = typename AccOf<T>::type;
+  if (sizeof(T) == 2 && f32) return static_cast<A>(static_cast<const float*>(p)[i]);
+  return to_acc(static_cast<const T*>(p)[i]);
+}
+
+__device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, int64_t length) {
+  if (lengths == nullptr) return length;
+  const int64_t n = lengths[b];
+  return n < 0 ? 0 : (n < length ? n : length);
+}
+
+// V inputs of token t (before the first: of the state; none past the `count` valid ones).
+template <typename T, int V>
+__device__ __forceinline__ void input_at(const T* x, int64_t xs_t, const T* before, int64_t dim,
+                                         int width, int64_t t, int64_t count,
+                                         typename AccOf<T>::type* v) {
+  using G = Group<T, V>;
+  if (t >= 0 && t < count) {
+    G::values(G::load(x + t * xs_t), v);
+  } else if (t < 0 && before != nullptr) {
+    G::values(G::load(before + (t + width - 1) * dim), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0;
+  }
+}
+
+// Thread: V channels, `run` tokens.  Threads go over channels first, then runs, then sequences.
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(128)
+conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
+                const void* __restrict__ bias, const T* __restrict__ initial,
+                const int32_t* __restrict__ lengths, T* __restrict__ y,
+                T* __restrict__ final_state, int64_t batch, int64_t length, int64_t dim,
+                int64_t xs_b, int64_t xs_t, int run, bool silu, bool param_f32) {
+  using A = typename AccOf<T>::type;
+  using G = Group<T, V>;
+  constexpr int U = 4;  // tokens whose loads are issued together
+  const int64_t per = dim / V, runs = length > run ? (length + run - 1) / run : 1;
+  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t c = id % per * V, k = id / per % runs, b = id / per / runs;
+  if (b >= batch) return;
+  const int64_t count = tokens_of(lengths, b, length);
+  x += b * xs_b + c;
+  y += (b * length) * dim + c;
+  const T* before = initial == nullptr ? nullptr : initial + b * (W - 1) * dim + c;
+  if (final_state != nullptr && k == 0) {
+    for (int i = 0; i < W - 1; ++i) {
+      A v[V];
+      input_at<T, V>(x, xs_t, before, dim, W, count - (W - 1) + i, count, v);
+      G::store(final_state + (b * (W - 1) + i) * dim + c, v);
+    }
+  }
+  A w[W][V], at[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i][j] = param<T>(weight, param_f32, (c + j) * W + i);
+    at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
+  }
+  const int64_t t0 = k * run, t1 = t0 + run < length ? t0 + run : length;
+  A win[W - 1 + U][V];  // the inputs of tokens t - W + 1 ... t + U - 1
+#pragma unroll
+  for (int i = 0; i < W - 1; ++i)
+    input_at<T, V>(x, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i]);
+  for (int64_t t = t0; t < t1; t += U) {
+    typename G::Raw raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < count) raw[u] = G::load(x + (t + u) * xs_t);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) break;
+      A p[V];
+      if (t + u < count) {
+        G::values(raw[u], win[W - 1 + u]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          p[j] = at[j];
+#pragma unroll
+          for (int i = 0; i < W; ++i) p[j] += w[i][j] * win[u + i][j];
+        }
+        if (silu) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) p[j] *= sigmoid<T>(p[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[j] = win[W - 1 + u][j] = A(0);
+      }
+      G::store(y + (t + u) * dim, p);
+    }
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) win[i][j] = win[i + U][j];
+  }
+}
+
+// Backward.  A block is 32 threads of channels by 8 runs of tokens; a thread walks its run and the
+// W-1 tokens after it (whose dp its last inputs need), so dx is written once.  dw and db are summed
+// in registers over the run, joined over the block's runs in shared memory and written as one
+// partial row (dim x (W + 1)) a block row, added in a fixed order by conv_params_kernel.
+constexpr int kBwdLanes = 32, kBwdRuns = 8;
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(kBwdLanes* kBwdRuns)
+conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
+                const void* __restrict__ bias, const T* __restrict__ initial,
+                const int32_t* __restrict__ lengths, const T* __restrict__ dy,
+                const T* __restrict__ d_final, T* __restrict__ dx, T* __restrict__ d_initial,
+                typename AccOf<T>::type* __restrict__ partial, int64_t length, int64_t dim,
+                int64_t xs_b, int64_t xs_t, int64_t ds_b, int64_t ds_t, int run, int64_t rows,
+                int64_t columns, bool silu, bool param_f32) {
+  using A = typename AccOf<T>::type;
+  using G = Group<T, V>;
+  __shared__ A joined[kBwdRuns][kBwdLanes * V + 1];
+  const int64_t per = dim / V;
+  const int64_t column = blockIdx.x % columns, part = blockIdx.x / columns;
+  const int64_t cg = column * kBwdLanes + threadIdx.x;
+  const int64_t b = part / rows, row = part % rows;
+  const int64_t k = row * kBwdRuns + threadIdx.y;  // the thread's run
+  const bool in = cg < per;
+  const int64_t c = (in ? cg : per - 1) * V;
+  const int64_t count = tokens_of(lengths, b, length);
+  x += b * xs_b + c;
+  dy += b * ds_b + c;
+  const T* before = initial == nullptr ? nullptr : initial + b * (W - 1) * dim + c;
+  A w[W][V], at[V], dw[W][V], db[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      w[i][j] = param<T>(weight, param_f32, (c + j) * W + i);
+      dw[i][j] = A(0);
+    }
+    at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
+    db[j] = A(0);
+  }
+  const int64_t t0 = k * run;
+  const int64_t t1 = t0 + run < length ? t0 + run : length;  // (t1 <= t0: no tokens)
+  const bool first = k == 0;
+  if (in && (t0 < t1 || first)) {
+    A win[W][V], dp[W][V];  // inputs t-W+1 ... t and gradients of the sums p of the same tokens
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+      input_at<T, V>(x, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i + 1]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) dp[i + 1][j] = A(0);
+    }
+    constexpr int U = 4;
+    const int64_t end = t1 + W - 1;
+    for (int64_t s = t0; s < end; s += U) {
+      typename G::Raw rx[U], rd[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s + u < count && s + u < end) {
+          rx[u] = G::load(x + (s + u) * xs_t);
+          rd[u] = G::load(dy + (s + u) * ds_t);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t t = s + u;
+        if (t >= end) break;
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            win[i][j] = win[i + 1][j];
+            dp[i][j] = dp[i + 1][j];
+          }
+        if (t < count) {
+          G::values(rx[u], win[W - 1]);
+          G::values(rd[u], dp[W - 1]);
+          if (silu) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              A p = at[j];
+#pragma unroll
+              for (int i = 0; i < W; ++i) p += w[i][j] * win[i][j];
+              const A g = sigmoid<T>(p);
+              dp[W - 1][j] *= g * (A(1) + p * (A(1) - g));
+            }
+          }
+          if (t < t1) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              db[j] += dp[W - 1][j];
+#pragma unroll
+              for (int i = 0; i < W; ++i) dw[i][j] += dp[W - 1][j] * win[i][j];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) win[W - 1][j] = dp[W - 1][j] = A(0);
+        }
+        // all gradients that input t - W + 1 reaches are in dp[0 .. W-1] now
+        const int64_t to = t - (W - 1);
+        if (to < t0 && !(first && d_initial != nullptr)) continue;
+        A g[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          g[j] = A(0);
+#pragma unroll
+          for (int i = 0; i < W; ++i) g[j] += w[W - 1 - i][j] * dp[i][j];
+        }
+        if (d_final != nullptr && to >= count - (W - 1) && to < count) {
+          A f[V];
+          G::values(G::load(d_final + (b * (W - 1) + to - count + W - 1) * dim + c), f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] += f[j];
+        }
+        if (to >= 0) {
+          if (dx != nullptr) G::store(dx + (b * length + to) * dim + c, g);
+        } else {
+          G::store(d_initial + (b * (W - 1) + to + W - 1) * dim + c, g);
+        }
+      }
+    }
+  }
+  if (partial == nullptr) return;
+  // one tap (or the bias) after the other through shared memory
+#pragma unroll
+  for (int i = 0; i <= W; ++i) {
+    if (i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) joined[threadIdx.y][threadIdx.x * V + j] = i < W ? dw[i % W][j] : db[j];
+    __syncthreads();
+    for (int e = threadIdx.y * kBwdLanes + threadIdx.x; e < kBwdLanes * V;
+         e += kBwdLanes * kBwdRuns) {
+      const int64_t channel = column * kBwdLanes * V + e;
+      if (channel >= dim) continue;
+      A sum = joined[0][e];
+#pragma unroll
+      for (int r = 1; r < kBwdRuns; ++r) sum += joined[r][e];
+      partial[(part * (W + 1) + i) * dim + channel] = sum;
+    }
+  }
+}
+
+// dw (dim, W) and db from the partial rows [parts][W + 1][dim], added in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+conv_params_kernel(const typename AccOf<T>::type* __restrict__ partial, int64_t parts, int64_t dim,
+                   int width, void* __restrict__ dw, void* __restrict__ db, bool param_f32) {
+  using A = typename AccOf<T>::type;
+  __shared__ A cells[8][33];
+  const int64_t cols = (width + 1) * dim, c = int64_t(blockIdx.x) * 32 + threadIdx.x;
+  A sum = A(0);
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t p = threadIdx.y; p < parts; p += 8) sum += partial[p * cols + c];
+  }
+  cells[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.y != 0 || c >= cols) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sum += cells[k][threadIdx.x];
+  const int64_t tap = c / dim, channel = c % dim;
+  void* out = tap < width ? dw : db;
+  if (out == nullptr) return;
+  const int64_t i = tap < width ? channel * width + tap : channel;
+  if (sizeof(T) == 2 && param_f32) static_cast<float*>(out)[i] = static_cast<float>(sum);
+  else static_cast<T*>(out)[i] = from_acc<T>(sum);
+}
+
+// One token of every sequence: the window is the state's rows and x; the state moves on by one.
+template <typename T, int V>
+__global__ void __launch_bounds__(128)
+conv_step_kernel(const T* __restrict__ x, const void* __restrict__ weight,
+                 const void* __restrict__ bias, T* state, const int32_t* __restrict__ slots,
+                 T* __restrict__ y, int64_t batch, int64_t dim, int64_t xs_b, int64_t pool,
+                 int width, bool silu, bool param_f32) {
+  using A = typename AccOf<T>::type;
+  using G = Group<T, V>;
+  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t per = dim / V, c = id % per * V, b = id / per;
+  if (b >= batch) return;
+  const int64_t slot = slots == nullptr ? b : slots[b];
+  A p[V];
+  if (slot < 0 || slot >= pool) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p[j] = A(0);
+    G::store(y + b * dim + c, p);
+    return;
+  }
+  T* rows = state + slot * (width - 1) * dim + c;
+  typename G::Raw raw[8];
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < width - 1) raw[i] = G::load(rows + i * dim);
+  const typename G::Raw now = G::load(x + b * xs_b + c);
+#pragma unroll
+  for (int j = 0; j < V; ++j) p[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
+  A v[V];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i < width) {
+      if (i == width - 1) raw[i] = now;
+      G::values(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] += param<T>(weight, param_f32, (c + j) * width + i) * v[j];
+      if (i > 0) G::store(rows + (i - 1) * dim, v);
+    }
+  }
+  if (silu) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p[j] *= sigmoid<T>(p[j]);
+  }
+  G::store(y + b * dim + c, p);
+}
+
+// ------------------------------------------------------------------------------ launches
+// Whether rows of these strides and pointers take groups of v elements.
+template <typename T>
+bool grouped(int v, int64_t dim, std::initializer_list<int64_t> strides, Pointers pointers) {
+  uintptr_t bits = 0;
+  for (const void* q : pointers) bits |= reinterpret_cast<uintptr_t>(q);
+  if (dim % v != 0 || bits % (v * sizeof(T)) != 0) return false;
+  for (int64_t s : strides)
+    if (s % v != 0) return false;
+  return true;
+}
+
+template <typename F> int with_width(int width, F fn) {
+  switch (width) {
+    case 2: return fn(std::integral_constant<int, 2>{});
+    case 3: return fn(std::integral_constant<int, 3>{});
+    case 4: return fn(std::integral_constant<int, 4>{});
+    case 5: return fn(std::integral_constant<int, 5>{});
+    case 6: return fn(std::integral_constant<int, 6>{});
+    case 7: return fn(std::integral_constant<int, 7>{});
+    case 8: return fn(std::integral_constant<int, 8>{});
+    default: return FDWT_ERR_INVALID;
+  }
+}
+
+template <typename T, int V> int conv_forward_v(const ConvCall& c, int width, void* y, void* fin) {
+  // runs of 32 tokens where that leaves threads enough for every multiprocessor, else 8
+  const int64_t threads32 = c.batch * cdiv(c.length, 32) * (c.dim / V);
+  const int run = threads32 >= int64_t(sm_count()) * 512 ? 32 : 8;
+  const int64_t threads = c.batch * imax(1, cdiv(c.length, run)) * (c.dim / V);
+  const int64_t grid = cdiv(threads, 128);
+  if (grid > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+  const int st = pre_launch(c.stream);
+  if (st != FDWT_OK) return st;
+  return with_width(width, [&](auto w) {
+    conv_fwd_kernel<T, V, decltype(w)::value><<<static_cast<unsigned>(grid), 128, 0, c.stream>>>(
+        static_cast<const T*>(c.x), c.weight, c.bias, static_cast<const T*>(c.initial), c.lengths,
+        static_cast<T*>(y), static_cast<T*>(fin), c.batch, c.length, c.dim, c.xs_b, c.xs_t, run,
+        c.silu, c.param_f32);
+    return launch_status();
+  });
+}
+
+// Tokens a thread of the backward pass, and rows of blocks a sequence.
+struct BwdRuns {
+  int run;
+  int64_t rows;
+};
+inline BwdRuns bwd_runs(int64_t batch, int64_t length, int64_t dim, int v) {
+  int run = 32;
+  while (run > 8 && batch * cdiv(length, run) * cdiv(dim, v) < int64_t(sm_count()) * 512) run /= 2;
+  return {run, imax(1, cdiv(length, int64_t(run) * kBwdRuns))};
+}
+template <typename T> constexpr int bwd_group = sizeof(T) == 8 ? 2 : 4;
+
+template <typename T, int V>
+int conv_backward_v(const ConvCall& c, int width, const void* dy, const void* d_final, void* dx,
+                    void* dw, void* db, void* d_initial, void* ws) {
+  using A = typename AccOf<T>::type;
+  const BwdRuns r = bwd_runs(c.batch, c.length, c.dim, bwd_group<T>);
+  A* partial = dw != nullptr || db != nullptr ? static_cast<A*>(ws) : nullptr;
+  const int64_t parts = c.batch * r.rows;
+  const int64_t columns = cdiv(c.dim / V, kBwdLanes);
+  if (columns * parts > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+  int st = pre_launch(c.stream);
+  if (st != FDWT_OK) return st;
+  st = with_width(width, [&](auto w) {
+    conv_bwd_kernel<T, V, decltype(w)::value>
+        <<<static_cast<unsigned>(columns * parts), dim3(kBwdLanes, kBwdRuns), 0, c.stream>>>(
+            static_cast<const T*>(c.x), c.weight, c.bias, static_cast<const T*>(c.initial),
+            c.lengths, static_cast<const T*>(dy), static_cast<const T*>(d_final),
+            static_cast<T*>(dx), static_cast<T*>(d_initial), partial, c.length, c.dim, c.xs_b,
+            c.xs_t, c.ds_b, c.ds_t, r.run, r.rows, columns, c.silu, c.param_f32);
+    return launch_status();
+  });
+  if (st != FDWT_OK || partial == nullptr) return st;
+  st = pre_launch(c.stream);
+  if (st != FDWT_OK) return st;
+  conv_params_kernel<T><<<static_cast<unsigned>(cdiv((width + 1) * c.dim, 32)), dim3(32, 8), 0,
+                          c.stream>>>(partial, parts, c.dim, width, dw, db, c.param_f32);
+  return launch_status();
+}
+
+template <typename F> int with_type(int dtype, F fn) {
+  switch (dtype) {
+    case FDWT_F32: return fn(float{});
+    case FDWT_F64: return fn(double{});
+    case FDWT_F16: return fn(__half{});
+    default: return fn(__nv_bfloat16{});
+  }
+}
+
+// The largest sizes: token and element counts that the kernels' grids and 64-bit offsets hold.
+constexpr int64_t kMostTokens = int64_t(1) << 30;
+
+bool conv_ok(const fdwt_conv1d_desc* d) {
+  return d != nullptr && dtype_size(d->dtype) != 0 &&
+         (d->param_dtype == d->dtype || (d->param_dtype == FDWT_F32 && d->dtype != FDWT_F64)) &&
+         d->width >= 2 && d->width <= FDWT_MAX_CONV_WIDTH && d->batch >= 0 && d->length >= 0 &&
+         d->dim >= 1 && d->batch < kMostTokens && d->length < kMostTokens && d->dim < kMostTokens;
+}
+ConvCall conv_call(const fdwt_conv1d_desc* d, const void* x, const void* weight, const void* bias,
+                   const void* initial, const int32_t* lengths, void* stream) {
+  return {d->batch, d->length, d->dim, d->x_stride[0], d->x_stride[1], d->dy_stride[0],
+          d->dy_stride[1], d->silu != 0, d->param_dtype == FDWT_F32, x, weight, bias, initial,
+          lengths, static_cast<cudaStream_t>(stream)};
+}
+
+}  // namespace
+}  // namespace fdwt
+
+using namespace fdwt;
+
+extern "C" int fdwt_causal_conv1d_forward(const fdwt_conv1d_desc* desc, const void* x,
+                                          const void* weight, const void* bias,
+                                          const void* initial_state, const int32_t* lengths,
+                                          void* y, void* final_state, void* stream) {
+  FDWT_CHECK(conv_ok(desc));
+  if (desc->batch == 0 || (desc->length == 0 && final_state == nullptr)) return FDWT_OK;
+  FDWT_CHECK(weight != nullptr && (desc->length == 0 || (x != nullptr && y != nullptr)));
+  const ConvCall c = conv_call(desc, x, weight, bias, initial_state, lengths, stream);
+  return with_type(desc->dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    if (grouped<T>(V, c.dim, {c.xs_b, c.xs_t}, {x, y, initial_state, final_state}))
+      return conv_forward_v<T, V>(c, desc->width, y, final_state);
+    return conv_forward_v<T, 1>(c, desc->width, y, final_state);
+  });
+}
+
+extern "C" size_t fdwt_causal_conv1d_backward_workspace(const fdwt_conv1d_desc* desc) {
+  if (!conv_ok(desc) || desc->batch == 0) return 0;
+  const int v = desc->dtype == FDWT_F64 ? 2 : 4;
+  const BwdRuns r = bwd_runs(desc->batch, desc->length, desc->dim, v);
+  return size_t(desc->batch * r.rows) * (desc->width + 1) * desc->dim *
+         (desc->dtype == FDWT_F64 ? 8 : 4);
+}
+
+extern "C" int fdwt_causal_conv1d_backward(const fdwt_conv1d_desc* desc, const void* x,
+                                           const void* weight, const void* bias,
+                                           const void* initial_state, const int32_t* lengths,
+                                           const void* dy, const void* d_final_state, void* dx,
+                                           void* dweight, void* dbias, void* d_initial_state,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+  FDWT_CHECK(conv_ok(desc));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (desc->batch == 0) {
+    const size_t size = dtype_size(desc->param_dtype) * desc->dim;
+    if (dweight != nullptr) FDWT_CUDA(cudaMemsetAsync(dweight, 0, size * desc->width, s));
+    if (dbias != nullptr) FDWT_CUDA(cudaMemsetAsync(dbias, 0, size, s));
+    return FDWT_OK;
+  }
+  FDWT_CHECK(weight != nullptr && (desc->length == 0 || (x != nullptr && dy != nullptr)));
+  if ((dweight != nullptr || dbias != nullptr) &&
+      (workspace == nullptr || workspace_bytes < fdwt_causal_conv1d_backward_workspace(desc)))
+    return FDWT_ERR_WORKSPACE;
+  const ConvCall c = conv_call(desc, x, weight, bias, initial_state, lengths, stream);
+  return with_type(desc->dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = bwd_group<T>;
+    if (grouped<T>(V, c.dim, {c.xs_b, c.xs_t, c.ds_b, c.ds_t},
+                   {x, dy, dx, initial_state, d_final_state, d_initial_state}))
+      return conv_backward_v<T, V>(c, desc->width, dy, d_final_state, dx, dweight, dbias,
+                                   d_initial_state, workspace);
+    return conv_backward_v<T, 1>(c, desc->width, dy, d_final_state, dx, dweight, dbias,
+                                 d_initial_state, workspace);
+  });
+}
+
+extern "C" int fdwt_causal_conv1d_step(const fdwt_conv1d_desc* desc, const void* x,
+                                       const void* weight, const void* bias, void* state,
+                                       int64_t state_slots, const int32_t* slots, void* y,
+                                       void* stream) {
+  FDWT_CHECK(conv_ok(desc) && desc->length == 1 && state_slots >= 0);
+  FDWT_CHECK(slots != nullptr || state_slots >= desc->batch);
+  if (desc->batch == 0) return FDWT_OK;
+  FDWT_CHECK(x != nullptr && weight != nullptr && y != nullptr &&
+             (state != nullptr || state_slots == 0));
+  return with_type(desc->dtype, [&](auto t) {
+    using T = decltype(t);
+    auto launch = [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      const int64_t grid = cdiv(desc->batch * (desc->dim / V), 128);
+      if (grid > INT32_MAX) return static_cast<int>(FDWT_ERR_UNSUPPORTED);
+      const int st = pre_launch(static_cast<cudaStream_t>(stream));
+      if (st != FDWT_OK) return st;
+      conv_step_kernel<T, V><<<static_cast<unsigned>(grid), 128, 0,
+                               static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T*>(x), weight, bias, static_cast<T*>(state), slots,
+          static_cast<T*>(y), desc->batch, desc->dim, desc->x_stride[0], state_slots, desc->width,
+          desc->silu != 0, desc->param_dtype == FDWT_F32);
+      return launch_status();
+    };
+    constexpr int V = sizeof(T) == 8 ? 2 : 4;
+    if (grouped<T>(V, desc->dim, {desc->x_stride[0]}, {x, y, state}))
+      return launch(std::integral_constant<int, V>{});
+    return launch(std::integral_constant<int, 1>{});
+  });
+}
