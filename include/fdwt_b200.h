@@ -408,6 +408,57 @@ int fdwt_causal_conv1d_step(const fdwt_conv1d_desc* desc, const void* x, const v
                             const void* bias, void* state, int64_t state_slots,
                             const int32_t* slots, void* y, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Selective state space scan (no counterpart in the reference).  Channel d has `states` numbers
+ * h[n]; over the tokens t of a sequence, with v = dt_t + dt_bias and delta = v or, with
+ * dt_softplus, log(1 + e^v),
+ *   h[n] <- e^(delta a[n]) h[n] + delta x_t b_t[n],   p_t = sum_n c_t[n] h[n] + skip x_t,
+ *   y_t = p_t, or p_t gate_t / (1 + e^-gate_t) with a gate.
+ * Channel d reads b and c of group d / (dim / groups).  x, dt, gate (may be NULL) are addressed
+ * by (batch, token) strides in elements with contiguous channels, b and c by (batch, token,
+ * group) strides with contiguous states, all of desc->dtype.  a (dim, states), skip and dt_bias
+ * (dim; may be NULL) and the states (batch, dim, states) are contiguous fp32 (fp64 when dtype is
+ * FDWT_F64); a is finite or -inf.  lengths as in fdwt_causal_conv1d_forward.  y is contiguous.
+ * ---------------------------------------------------------------------------------------- */
+#define FDWT_MAX_SCAN_STATES 128
+typedef struct {
+  int32_t dtype;
+  int32_t groups, states;
+  int32_t dt_softplus;
+  int64_t batch, length, dim;
+  int64_t x_stride[2], dt_stride[2], gate_stride[2], dy_stride[2]; /* batch, token */
+  int64_t b_stride[3], c_stride[3];                                /* batch, token, group */
+} fdwt_scan_desc;
+
+/* y and the states after the sequences (final_state; may be NULL) from initial_state (NULL:
+ * zeros).  checkpoints (fdwt_selscan_checkpoint_bytes; NULL where no backward pass follows)
+ * receives states that the backward pass starts from.  Workspaces and checkpoints begin on a
+ * multiple of 16 bytes. */
+size_t fdwt_selscan_forward_workspace(const fdwt_scan_desc* desc);
+size_t fdwt_selscan_checkpoint_bytes(const fdwt_scan_desc* desc);
+int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, const void* dt, const void* a,
+                         const void* b, const void* c, const void* skip, const void* gate,
+                         const void* dt_bias, const void* initial_state, const int32_t* lengths,
+                         void* y, void* final_state, void* checkpoints, void* workspace,
+                         size_t workspace_bytes, void* stream);
+/* Gradients from dL/dy (strides dy_stride) and dL/dfinal_state (NULL: zeros), contiguous; those
+ * of a, b, c, skip, dt_bias and the initial state may be NULL, dgate without a gate.  Sums over
+ * tokens, channels and sequences are added in a fixed order. */
+size_t fdwt_selscan_backward_workspace(const fdwt_scan_desc* desc);
+int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, const void* dt,
+                          const void* a, const void* b, const void* c, const void* skip,
+                          const void* gate, const void* dt_bias, const int32_t* lengths,
+                          const void* checkpoints, const void* dy, const void* d_final_state,
+                          void* dx, void* ddt, void* da, void* db, void* dc, void* dskip,
+                          void* dgate, void* ddt_bias, void* d_initial_state, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* One token for each of desc->batch sequences (desc->length is 1): the states in `state`
+ * (state_slots, dim, states) are updated in place; slots as in fdwt_linattn_step. */
+int fdwt_selscan_step(const fdwt_scan_desc* desc, const void* x, const void* dt, const void* a,
+                      const void* b, const void* c, const void* skip, const void* gate,
+                      const void* dt_bias, void* state, int64_t state_slots, const int32_t* slots,
+                      void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,8 +10,9 @@
   :class:`LayerNorm`, :class:`DecayTokenMixer` -- a causal token mixer for training, prompts and
   single tokens.
 * :func:`rms_norm`, :func:`rms_norm_quantized` (:class:`RMSNorm`), :func:`causal_conv1d` and
-  :func:`causal_conv1d_step` -- the norm with the residual's addition and the short convolution of
-  stacks of causal mixers.
+  :func:`selective_scan` with their single-token forms :func:`causal_conv1d_step` and
+  :func:`selective_scan_step` -- the norm with the residual's addition, the short convolution and
+  the selective state space scan of stacks of causal mixers.
 
 Every transform runs in hand-written CUDA kernels for sm_100a behind the C ABI of
 ``include/fdwt_b200.h`` (``libfdwt_b200.so``); inputs must be CUDA tensors.
@@ -25,6 +26,7 @@ from .layers import (DecayTokenMixer, MorletAttention, MorletChannelMixAttention
                      MorletTokenMixer, WaveletTokenMixer)
 from .linear_attention import linear_attention, linear_attention_step
 from .norm import LayerNorm, RMSNorm, layer_norm, rms_norm, rms_norm_quantized
+from .selective_scan import selective_scan, selective_scan_step
 from .wavelets import FilterBank, get_filter_bank
 
 __version__ = "0.1.0"
@@ -35,5 +37,6 @@ __all__ = [
     "MorletAttention", "MorletChannelMixAttention", "MorletTokenMixer", "WaveletTokenMixer",
     "DecayTokenMixer", "LayerNorm", "layer_norm", "linear_attention", "linear_attention_step",
     "RMSNorm", "rms_norm", "rms_norm_quantized", "causal_conv1d", "causal_conv1d_step",
+    "selective_scan", "selective_scan_step",
     "FilterBank", "get_filter_bank",
 ]

@@ -129,6 +129,15 @@ SIGNATURES = {
         ctypes.c_size_t, ctypes.c_void_p]),
     "fdwt_causal_conv1d_step": (ctypes.c_int, [ctypes.c_void_p] * 5 + [
         ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "fdwt_selscan_forward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_selscan_checkpoint_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_selscan_forward": (ctypes.c_int, [ctypes.c_void_p] * 15 + [
+        ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_selscan_backward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_selscan_backward": (ctypes.c_int, [ctypes.c_void_p] * 23 + [
+        ctypes.c_size_t, ctypes.c_void_p]),
+    "fdwt_selscan_step": (ctypes.c_int, [ctypes.c_void_p] * 10 + [
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()

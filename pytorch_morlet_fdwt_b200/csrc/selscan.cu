@@ -1,0 +1,320 @@
+// Selective state space scan: the C entry points, how a call is cut, and the sums over blocks.
+#include "selscan.cuh"
+
+namespace fdwt {
+namespace {
+
+// db and dc (batch, length, groups, states) from the tiles' parts, added in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+scan_bc_kernel(const typename AccOf<T>::type* __restrict__ part, const int32_t* __restrict__ lengths,
+               int64_t batch, int64_t length, int groups, int64_t tiles, int states, int padded,
+               T* __restrict__ db, T* __restrict__ dc) {
+  using A = typename AccOf<T>::type;
+  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int e = static_cast<int>(id % (2 * padded));
+  const int64_t row = id / (2 * padded);  // (group, batch, token)
+  const int n = e % padded;
+  if (row >= groups * batch * length || n >= states) return;
+  T* out = e < padded ? db : dc;
+  if (out == nullptr) return;
+  const int64_t t = row % length, b = row / length % batch, g = row / length / batch;
+  A sum = A(0);
+  if (lengths == nullptr || t < lengths[b]) {
+    const int64_t step = batch * length * 2 * padded;
+    const A* q = part + g * tiles * step + (b * length + t) * 2 * padded + e;
+#pragma unroll 4
+    for (int64_t k = 0; k < tiles; ++k) sum += q[k * step];
+  }
+  out[((b * length + t) * groups + g) * states + n] = from_acc<T>(sum);
+}
+
+// Columns summed over rows in a fixed order: 32 columns by 8 row lanes a block.  Column c goes to
+// out[c / width * keep + c % width] where c % width < keep.
+template <typename A>
+__global__ void __launch_bounds__(256)
+scan_rows_kernel(const A* __restrict__ part, int64_t rows, int64_t stride, int64_t cols, int width,
+                 int keep, A* __restrict__ out) {
+  __shared__ A cells[8][33];
+  const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x;
+  A sum = A(0);
+  if (c < cols) {
+#pragma unroll 4
+    for (int64_t r = threadIdx.y; r < rows; r += 8) sum += part[r * stride + c];
+  }
+  cells[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.y != 0 || c >= cols || c % width >= keep) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sum += cells[k][threadIdx.x];
+  out[c / width * keep + c % width] = sum;
+}
+
+template <typename A>
+int sum_rows(const A* part, int64_t rows, int64_t stride, int64_t cols, int width, int keep,
+             void* out, cudaStream_t stream) {
+  if (out == nullptr) return FDWT_OK;
+  const int st = pre_launch(stream);
+  if (st != FDWT_OK) return st;
+  scan_rows_kernel<A><<<static_cast<unsigned>(cdiv(cols, 32)), dim3(32, 8), 0, stream>>>(
+      part, rows, stride, cols, width, keep, static_cast<A*>(out));
+  return launch_status();
+}
+
+constexpr int64_t kMostTokens = int64_t(1) << 30;
+
+bool scan_ok(const fdwt_scan_desc* d) {
+  return d != nullptr && dtype_size(d->dtype) != 0 && d->groups >= 1 && d->states >= 1 &&
+         d->batch >= 0 && d->length >= 0 && d->dim >= 1 && d->dim % d->groups == 0 &&
+         d->batch < kMostTokens && d->length < kMostTokens && d->dim < kMostTokens;
+}
+int lanes_of(int states) {
+  int lanes = 1;
+  while (4 * lanes < states) lanes *= 2;
+  return lanes;
+}
+size_t acc_size(int dtype) { return dtype == FDWT_F64 ? 8 : 4; }
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// How a launch is cut: channels into tiles, sequences into segments.
+struct Cut {
+  int64_t tiles;  // of one group
+  int segments;
+  int64_t seg_len;
+};
+constexpr int64_t kSegmentStep = 16;  // segments are multiples of the staged tokens
+Cut cut_of(const fdwt_scan_desc* d, int tile, int64_t blocks_wanted, int64_t shortest) {
+  Cut c;
+  c.tiles = cdiv(d->dim / d->groups, tile);
+  const int64_t blocks = c.tiles * d->groups * d->batch;
+  int64_t n = blocks >= blocks_wanted / 2 || blocks == 0 ? 1 : blocks_wanted / blocks;
+  n = imax(1, imin(n, d->length / shortest));
+  c.seg_len = imax(kSegmentStep, cdiv(cdiv(d->length, n), kSegmentStep) * kSegmentStep);
+  c.segments = static_cast<int>(imax(1, cdiv(d->length, c.seg_len)));
+  return c;
+}
+Cut forward_cut(const fdwt_scan_desc* d) {
+  return cut_of(d, scan_fwd_tile(lanes_of(d->states)), int64_t(sm_count()) * 4, 128);
+}
+bool wide_backward(const fdwt_scan_desc* d) {
+  const int64_t tiles = cdiv(d->dim / d->groups, scan_bwd_tile(lanes_of(d->states), true));
+  return d->dtype != FDWT_F64 && tiles * d->groups * d->batch >= sm_count();
+}
+Cut backward_cut(const fdwt_scan_desc* d, bool wide) {
+  return cut_of(d, scan_bwd_tile(lanes_of(d->states), wide), int64_t(sm_count()) * 3, 128);
+}
+struct Segments {
+  size_t state, sum, bytes;
+};
+Segments segment_bytes(const fdwt_scan_desc* d, const Cut& c) {
+  Segments s{0, 0, 0};
+  if (c.segments == 1) return s;
+  const size_t rows = size_t(d->batch) * c.segments * d->dim, a = acc_size(d->dtype);
+  s.sum = up256(rows * 4 * lanes_of(d->states) * a);
+  s.bytes = s.sum + up256(rows * a);
+  return s;
+}
+struct Parts {
+  size_t a, ch, bc, bytes;
+};
+Parts part_bytes(const fdwt_scan_desc* d, const Cut& c) {
+  const size_t size = acc_size(d->dtype), np = 4 * lanes_of(d->states);
+  const size_t rows = size_t(d->batch) * c.segments;
+  Parts p;
+  p.a = segment_bytes(d, c).bytes;
+  p.ch = p.a + up256(rows * d->dim * np * size);
+  p.bc = p.ch + up256(rows * 2 * d->dim * size);
+  p.bytes = p.bc + up256(size_t(c.tiles) * d->groups * d->batch * d->length * 2 * np * size);
+  return p;
+}
+
+bool aligned16(std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* q : pointers) bits |= reinterpret_cast<uintptr_t>(q);
+  return bits % 16 == 0;
+}
+
+ScanArgs args_of(const fdwt_scan_desc* d, const void* x, const void* dt, const void* a,
+                 const void* b, const void* c, const void* skip, const void* gate,
+                 const void* dt_bias, const void* initial, const int32_t* lengths) {
+  ScanArgs p{};
+  p.x = x, p.dt = dt, p.a = a, p.b = b, p.c = c, p.skip = skip, p.gate = gate;
+  p.dt_bias = dt_bias, p.initial = initial, p.lengths = lengths;
+  p.batch = d->batch, p.length = d->length, p.dim = d->dim;
+  p.groups = d->groups, p.states = d->states, p.softplus = d->dt_softplus != 0;
+  for (int i = 0; i < 2; ++i) {
+    p.xs[i] = d->x_stride[i], p.dts[i] = d->dt_stride[i];
+    p.gs[i] = d->gate_stride[i], p.dys[i] = d->dy_stride[i];
+  }
+  for (int i = 0; i < 3; ++i) p.bs[i] = d->b_stride[i], p.cs[i] = d->c_stride[i];
+  p.per = d->dim / d->groups;
+  p.segments = 1;
+  return p;
+}
+// Whether every row of channels begins on a 16-byte boundary.
+bool rows_aligned(const fdwt_scan_desc* d, const ScanArgs& p, bool backward) {
+  const int64_t v = 16 / static_cast<int64_t>(dtype_size(d->dtype));
+  int64_t bits = p.per | p.xs[0] | p.xs[1] | p.dts[0] | p.dts[1];
+  if (p.gate != nullptr) bits |= p.gs[0] | p.gs[1];
+  if (backward) bits |= p.dys[0] | p.dys[1];
+  return bits % v == 0 && aligned16({p.x, p.dt, p.gate, p.y, p.dy, p.dx, p.ddt, p.dgate});
+}
+void cut_into(ScanArgs* p, const fdwt_scan_desc* d, const Cut& c, void* ws) {
+  const Segments s = segment_bytes(d, c);
+  p->tiles = c.tiles, p->segments = c.segments, p->seg_len = c.seg_len;
+  p->seg_state = static_cast<char*>(ws) + s.state;
+  p->seg_sum = static_cast<char*>(ws) + s.sum;
+}
+
+template <typename F> int with_type(int dtype, F fn) {
+  switch (dtype) {
+    case FDWT_F32: return fn(float{});
+    case FDWT_F64: return fn(double{});
+    case FDWT_F16: return fn(__half{});
+    default: return fn(__nv_bfloat16{});
+  }
+}
+
+}  // namespace
+}  // namespace fdwt
+
+using namespace fdwt;
+
+extern "C" size_t fdwt_selscan_forward_workspace(const fdwt_scan_desc* desc) {
+  if (!scan_ok(desc) || desc->states > FDWT_MAX_SCAN_STATES) return 0;
+  return segment_bytes(desc, forward_cut(desc)).bytes;
+}
+
+extern "C" size_t fdwt_selscan_checkpoint_bytes(const fdwt_scan_desc* desc) {
+  if (!scan_ok(desc) || desc->states > FDWT_MAX_SCAN_STATES) return 0;
+  return size_t(desc->batch) * cdiv(desc->length, kScanCheck) * desc->dim * 4 *
+         lanes_of(desc->states) * acc_size(desc->dtype);
+}
+
+extern "C" int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, const void* dt,
+                                    const void* a, const void* b, const void* c, const void* skip,
+                                    const void* gate, const void* dt_bias,
+                                    const void* initial_state, const int32_t* lengths, void* y,
+                                    void* final_state, void* checkpoints, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  FDWT_CHECK(scan_ok(desc));
+  if (desc->states > FDWT_MAX_SCAN_STATES) return FDWT_ERR_UNSUPPORTED;
+  if (desc->batch == 0 || (desc->length == 0 && final_state == nullptr)) return FDWT_OK;
+  FDWT_CHECK(a != nullptr);
+  FDWT_CHECK(desc->length == 0 || (x != nullptr && dt != nullptr && b != nullptr && c != nullptr &&
+                                   y != nullptr));
+  const Cut cut = forward_cut(desc);
+  const size_t bytes = segment_bytes(desc, cut).bytes;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes)) return FDWT_ERR_WORKSPACE;
+  FDWT_CHECK(aligned16({workspace, checkpoints}));
+  ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths);
+  p.y = y, p.final_state = final_state, p.check = checkpoints;
+  p.vec = rows_aligned(desc, p, false);
+  cut_into(&p, desc, cut, workspace);
+  const int lanes = lanes_of(desc->states);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return with_type(desc->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (cut.segments > 1) {
+      const int st = scan_states<T>(p, lanes, false, s);
+      if (st != FDWT_OK) return st;
+    }
+    return scan_forward<T>(p, lanes, s);
+  });
+}
+
+extern "C" size_t fdwt_selscan_backward_workspace(const fdwt_scan_desc* desc) {
+  if (!scan_ok(desc) || desc->states > FDWT_MAX_SCAN_STATES) return 0;
+  return part_bytes(desc, backward_cut(desc, wide_backward(desc))).bytes;
+}
+
+extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, const void* dt,
+                                     const void* a, const void* b, const void* c, const void* skip,
+                                     const void* gate, const void* dt_bias, const int32_t* lengths,
+                                     const void* checkpoints, const void* dy,
+                                     const void* d_final_state, void* dx, void* ddt, void* da,
+                                     void* db, void* dc, void* dskip, void* dgate, void* ddt_bias,
+                                     void* d_initial_state, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  FDWT_CHECK(scan_ok(desc));
+  if (desc->states > FDWT_MAX_SCAN_STATES) return FDWT_ERR_UNSUPPORTED;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t size = acc_size(desc->dtype);
+  if (desc->batch == 0) {  // no sequences: the sums over them are zero
+    if (da != nullptr) FDWT_CUDA(cudaMemsetAsync(da, 0, size * desc->dim * desc->states, s));
+    if (dskip != nullptr) FDWT_CUDA(cudaMemsetAsync(dskip, 0, size * desc->dim, s));
+    if (ddt_bias != nullptr) FDWT_CUDA(cudaMemsetAsync(ddt_bias, 0, size * desc->dim, s));
+    return FDWT_OK;
+  }
+  FDWT_CHECK(a != nullptr && (gate == nullptr || dgate != nullptr || desc->length == 0));
+  FDWT_CHECK(desc->length == 0 || (x != nullptr && dt != nullptr && b != nullptr && c != nullptr &&
+                                   checkpoints != nullptr && dy != nullptr && dx != nullptr &&
+                                   ddt != nullptr));
+  const bool wide = wide_backward(desc);
+  const Cut cut = backward_cut(desc, wide);
+  const Parts parts = part_bytes(desc, cut);
+  if (workspace == nullptr || workspace_bytes < parts.bytes) return FDWT_ERR_WORKSPACE;
+  FDWT_CHECK(aligned16({workspace, checkpoints}));
+  ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, nullptr, lengths);
+  p.check = const_cast<void*>(checkpoints);
+  p.dy = dy, p.d_final = d_final_state, p.dx = dx, p.ddt = ddt, p.dgate = dgate;
+  p.d_initial = d_initial_state;
+  char* ws = static_cast<char*>(workspace);
+  p.part_a = ws + parts.a, p.part_ch = ws + parts.ch, p.part_bc = ws + parts.bc;
+  p.vec = rows_aligned(desc, p, true);
+  cut_into(&p, desc, cut, workspace);
+  const int lanes = lanes_of(desc->states), np = 4 * lanes;
+  return with_type(desc->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    using A = typename AccOf<T>::type;
+    int st = FDWT_OK;
+    if (cut.segments > 1) {
+      // the state launch has tiles of its own
+      ScanArgs r = p;
+      r.tiles = cdiv(p.per, scan_fwd_tile(lanes));
+      st = scan_states<T>(r, lanes, true, s);
+      if (st != FDWT_OK) return st;
+    }
+    st = scan_backward<T>(p, lanes, wide, s);
+    if (st != FDWT_OK) return st;
+    const int64_t rows = desc->batch * cut.segments;
+    if (desc->length > 0 && (db != nullptr || dc != nullptr)) {
+      const int64_t n = int64_t(desc->groups) * desc->batch * desc->length * 2 * np;
+      if (cdiv(n, 256) > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+      st = pre_launch(s);
+      if (st != FDWT_OK) return st;
+      scan_bc_kernel<T><<<static_cast<unsigned>(cdiv(n, 256)), 256, 0, s>>>(
+          static_cast<const A*>(p.part_bc), lengths, desc->batch, desc->length, desc->groups,
+          cut.tiles, desc->states, np, static_cast<T*>(db), static_cast<T*>(dc));
+      st = launch_status();
+      if (st != FDWT_OK) return st;
+    }
+    st = sum_rows(static_cast<const A*>(p.part_a), rows, desc->dim * np, desc->dim * np, np,
+                  desc->states, da, s);
+    if (st != FDWT_OK) return st;
+    const A* ch = static_cast<const A*>(p.part_ch);
+    st = sum_rows(ch, rows, 2 * desc->dim, desc->dim, 1, 1, dskip, s);
+    if (st != FDWT_OK) return st;
+    return sum_rows(ch + desc->dim, rows, 2 * desc->dim, desc->dim, 1, 1, ddt_bias, s);
+  });
+}
+
+extern "C" int fdwt_selscan_step(const fdwt_scan_desc* desc, const void* x, const void* dt,
+                                 const void* a, const void* b, const void* c, const void* skip,
+                                 const void* gate, const void* dt_bias, void* state,
+                                 int64_t state_slots, const int32_t* slots, void* y, void* stream) {
+  FDWT_CHECK(scan_ok(desc) && desc->length == 1 && state_slots >= 0);
+  FDWT_CHECK(slots != nullptr || state_slots >= desc->batch);
+  if (desc->states > FDWT_MAX_SCAN_STATES) return FDWT_ERR_UNSUPPORTED;
+  if (desc->batch == 0) return FDWT_OK;
+  FDWT_CHECK(x != nullptr && dt != nullptr && a != nullptr && b != nullptr && c != nullptr &&
+             y != nullptr && (state != nullptr || state_slots == 0));
+  ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, nullptr, nullptr);
+  p.y = y;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(state);
+  p.vec = desc->states % 4 == 0 && bits % (4 * acc_size(desc->dtype)) == 0;
+  return with_type(desc->dtype, [&](auto t) {
+    return scan_step<decltype(t)>(p, lanes_of(desc->states), slots, state_slots, state,
+                                  static_cast<cudaStream_t>(stream));
+  });
+}

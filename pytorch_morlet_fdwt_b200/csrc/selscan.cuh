@@ -1,0 +1,72 @@
+// Selective state space scan.  A channel d has `states` numbers h[n] that a token moves on by
+//
+//   v = dt + dt_bias,  delta = v or log(1 + e^v)
+//   h_t[n] = e^(delta_t a[n]) h_{t-1}[n] + delta_t x_t b_t[n]
+//   p_t = sum_n c_t[n] h_t[n] + skip x_t,   y_t = p_t, or p_t gate sigmoid(gate)
+//
+// with b and c shared by the channels of a group.  Its gradients, with dp = dy silu(gate):
+//
+//   g_t[n] = c_t[n] dp_t + r_{t+1}[n],   r_t[n] = e^(delta_t a[n]) g_t[n]     (back in time)
+//   k_t[n] = r_t[n] h_{t-1}[n]
+//   da[n] = sum_t delta_t k_t[n]            dx_t = delta_t sum_n g_t[n] b_t[n] + skip dp_t
+//   db_t[n] = sum_d g_t[n] delta_t x_t      ddelta_t = sum_n (a[n] k_t[n]) + x_t sum_n g_t[n] b_t[n]
+//   dc_t[n] = sum_d dp_t h_t[n]             dgate_t = dy_t p_t silu'(gate_t),  dskip = sum_t dp_t x_t
+//
+// The decays depend on channel, state and token, so there is no product of matrices in it: a state
+// and token cost one exponential (16 a clock and SM) and 4 (backward 12) operations of the FMA
+// pipes, which is the bound; bytes are 8 and 22 a token and channel in 16 bits.
+//
+// Split.  A thread keeps 4 neighbouring states; LN lanes hold a channel's states (up to 4 LN) and
+// the 32 / LN groups of lanes of a warp neighbouring channels.  Sums over states cross LN lanes,
+// those over channels (db, dc) the others; both are formed for 8 tokens at once, halving the
+// values a lane holds with each step.  A block of 4 warps stages some tokens of its channels in
+// shared memory in 32 bits: delta and delta x (as pairs, for the packed instructions), b and c.
+// Long sequences of few channels are cut into segments: a state launch forms each segment's end
+// state from zero and its sum of delta, and the main launch's blocks add up those before them.
+#pragma once
+
+#include "row_groups.cuh"
+
+namespace fdwt {
+
+constexpr int kScanCheck = 8;  // tokens from one kept state to the next (for the backward pass)
+
+struct ScanArgs {
+  const void *x, *dt, *a, *b, *c, *skip, *gate, *dt_bias, *initial;
+  const int32_t* lengths;
+  int64_t batch, length, dim;
+  int groups, states;
+  int softplus;
+  int64_t xs[2], dts[2], gs[2], dys[2], bs[3], cs[3];
+  int vec;            // rows begin on 16-byte boundaries throughout
+  int64_t per, tiles; // channels of a group, tiles of one
+  int segments;
+  int64_t seg_len;    // tokens, a multiple of kScanCheck and of the staged tokens
+  void *seg_state, *seg_sum;  // [batch][segments][dim][padded states], [batch][segments][dim]
+  void *y, *final_state;
+  void* check;        // states before tokens 0, 8, 16, ...: [batch][ceil(length / 8)][dim][padded]
+  // backward
+  const void *dy, *d_final;
+  void *dx, *ddt, *dgate, *d_initial;
+  void *part_bc;      // [groups * tiles][batch][length][2][padded states]
+  void *part_a;       // [batch][segments][dim][padded states]
+  void *part_ch;      // [batch][segments][2][dim]: dskip, ddt_bias
+};
+
+// Launchers by element type (selscan_*.cu).  `lanes` is LN, 1 to 32.
+template <typename T> int scan_forward(const ScanArgs& p, int lanes, cudaStream_t stream);
+template <typename T> int scan_states(const ScanArgs& p, int lanes, bool reverse, cudaStream_t stream);
+template <typename T> int scan_backward(const ScanArgs& p, int lanes, bool wide, cudaStream_t stream);
+template <typename T> int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool,
+                                    void* state, cudaStream_t stream);
+
+// Channels of a thread, and of a block, in the forward launches and (wide: 4 tiles of channels one
+// after the other where the block's shared memory holds them) in the backward launch.
+constexpr int scan_fwd_channels(int ln) { return ln == 1 ? 1 : (ln <= 4 ? 2 : 4); }
+constexpr int scan_fwd_tile(int ln) { return 4 * (32 / ln) * scan_fwd_channels(ln); }
+constexpr int scan_bwd_channels(int ln, bool wide) {
+  return !wide ? (ln <= 4 ? 1 : (ln == 8 ? 2 : 4)) : (ln == 1 ? 1 : (ln == 2 ? 2 : 4));
+}
+constexpr int scan_bwd_tile(int ln, bool wide) { return 4 * (32 / ln) * scan_bwd_channels(ln, wide); }
+
+}  // namespace fdwt

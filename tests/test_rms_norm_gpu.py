@@ -267,7 +267,7 @@ def test_another_stream_and_a_graph():
 
     def step():
         y, total = F.rms_norm(x, w, r)
-        return (y, total, *torch.autograd.grad((y, total), (x, r, w), (dy, dy)))
+        return (y.detach(), total.detach(), *torch.autograd.grad((y, total), (x, r, w), (dy, dy)))
 
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
