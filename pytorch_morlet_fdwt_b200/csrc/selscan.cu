@@ -76,6 +76,15 @@ int lanes_of(int states) {
 size_t acc_size(int dtype) { return dtype == FDWT_F64 ? 8 : 4; }
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+template <typename F> auto with_type(int dtype, F fn) {
+  switch (dtype) {
+    case FDWT_F32: return fn(float{});
+    case FDWT_F64: return fn(double{});
+    case FDWT_F16: return fn(__half{});
+    default: return fn(__nv_bfloat16{});
+  }
+}
+
 // How a launch is cut: channels into tiles, sequences into segments.
 struct Cut {
   int64_t tiles;  // of one group
@@ -83,25 +92,57 @@ struct Cut {
   int64_t seg_len;
 };
 constexpr int64_t kSegmentStep = 16;  // segments are multiples of the staged tokens
-Cut cut_of(const fdwt_scan_desc* d, int tile, int64_t blocks_wanted, int64_t shortest) {
-  Cut c;
-  c.tiles = cdiv(d->dim / d->groups, tile);
-  const int64_t blocks = c.tiles * d->groups * d->batch;
-  int64_t n = blocks >= blocks_wanted / 2 || blocks == 0 ? 1 : blocks_wanted / blocks;
-  n = imax(1, imin(n, d->length / shortest));
-  c.seg_len = imax(kSegmentStep, cdiv(cdiv(d->length, n), kSegmentStep) * kSegmentStep);
-  c.segments = static_cast<int>(imax(1, cdiv(d->length, c.seg_len)));
-  return c;
+constexpr int kMostSegments = 64;
+// Measured: microseconds a token of a block alone on its SM, and of each of several.
+struct Pace {
+  double alone, shared;
+};
+double launch_time(double blocks, double resident, int64_t tokens, const Pace& pace) {
+  const double sms = sm_count(), at_once = blocks < resident ? blocks : resident;
+  const double a_sm = static_cast<double>(cdiv(static_cast<int64_t>(at_once), sm_count()));
+  const double waves = static_cast<double>(cdiv(static_cast<int64_t>(blocks),
+                                                static_cast<int64_t>(resident)));
+  (void)sms;
+  const double each = pace.shared * a_sm;
+  return waves * tokens * (each > pace.alone ? each : pace.alone);
+}
+// The number of segments with the shortest modelled time: more of them fill the device, but cost a
+// state launch (for all segments but one) and waves.
+Cut cut_of(const fdwt_scan_desc* d, int tile, int state_tile, int64_t resident, const Pace& pace,
+           const Pace& state_pace) {
+  Cut best{cdiv(d->dim / d->groups, tile), 1, imax(kSegmentStep, cdiv(d->length, kSegmentStep) * kSegmentStep)};
+  const double blocks = double(best.tiles) * d->groups * d->batch;
+  const double state_blocks = double(cdiv(d->dim / d->groups, state_tile)) * d->groups * d->batch;
+  if (blocks == 0) return best;
+  double least = launch_time(blocks, resident, best.seg_len, pace);
+  for (int n = 2; n <= kMostSegments; ++n) {
+    const int64_t len = cdiv(cdiv(d->length, n), kSegmentStep) * kSegmentStep;
+    const int64_t count = len > 0 ? cdiv(d->length, len) : 1;
+    if (len < 4 * kSegmentStep || count != n) continue;
+    const double resident_states = 4.0 * sm_count();
+    const double t = launch_time(blocks * n, resident, len, pace) + 3.0 +
+                     launch_time(state_blocks * (n - 1), resident_states, len, state_pace);
+    if (t < least) {
+      least = t;
+      best.segments = n;
+      best.seg_len = len;
+    }
+  }
+  return best;
 }
 Cut forward_cut(const fdwt_scan_desc* d) {
-  return cut_of(d, scan_fwd_tile(lanes_of(d->states)), int64_t(sm_count()) * 4, 128);
+  const int lanes = lanes_of(d->states), tile = scan_fwd_tile(lanes);
+  return with_type(d->dtype, [&](auto t) {
+    return cut_of(d, tile, tile, scan_resident<decltype(t)>(lanes, false), {0.12, 0.07},
+                  {0.08, 0.048});
+  });
 }
-bool wide_backward(const fdwt_scan_desc* d) {
-  const int64_t tiles = cdiv(d->dim / d->groups, scan_bwd_tile(lanes_of(d->states), true));
-  return d->dtype != FDWT_F64 && tiles * d->groups * d->batch >= sm_count();
-}
-Cut backward_cut(const fdwt_scan_desc* d, bool wide) {
-  return cut_of(d, scan_bwd_tile(lanes_of(d->states), wide), int64_t(sm_count()) * 3, 128);
+Cut backward_cut(const fdwt_scan_desc* d) {
+  const int lanes = lanes_of(d->states);
+  return with_type(d->dtype, [&](auto t) {
+    return cut_of(d, scan_bwd_tile(lanes, d->dtype == FDWT_F64), scan_fwd_tile(lanes),
+                  scan_resident<decltype(t)>(lanes, true), {0.3, 0.2}, {0.1, 0.055});
+  });
 }
 struct Segments {
   size_t state, sum, bytes;
@@ -151,28 +192,27 @@ ScanArgs args_of(const fdwt_scan_desc* d, const void* x, const void* dt, const v
   p.segments = 1;
   return p;
 }
-// Whether every row of channels begins on a 16-byte boundary.
-bool rows_aligned(const fdwt_scan_desc* d, const ScanArgs& p, bool backward) {
-  const int64_t v = 16 / static_cast<int64_t>(dtype_size(d->dtype));
-  int64_t bits = p.per | p.xs[0] | p.xs[1] | p.dts[0] | p.dts[1];
-  if (p.gate != nullptr) bits |= p.gs[0] | p.gs[1];
-  if (backward) bits |= p.dys[0] | p.dys[1];
-  return bits % v == 0 && aligned16({p.x, p.dt, p.gate, p.y, p.dy, p.dx, p.ddt, p.dgate});
+// Whether rows of channels, and of b and c, begin on boundaries of 4 elements (and channels and
+// states come in whole fours).
+bool in_fours(const fdwt_scan_desc* d, int64_t counts, std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* q : pointers) bits |= reinterpret_cast<uintptr_t>(q);
+  return counts % 4 == 0 && bits % (4 * dtype_size(d->dtype)) == 0;
+}
+void see_alignment(ScanArgs* p, const fdwt_scan_desc* d, bool backward) {
+  int64_t rows = p->per | p->xs[0] | p->xs[1] | p->dts[0] | p->dts[1];
+  if (p->gate != nullptr) rows |= p->gs[0] | p->gs[1];
+  if (backward) rows |= p->dys[0] | p->dys[1];
+  p->vec = in_fours(d, rows, {p->x, p->dt, p->gate, p->y, p->dy, p->dx, p->ddt, p->dgate});
+  int64_t states = p->states;
+  for (int i = 0; i < 3; ++i) states |= p->bs[i] | p->cs[i];
+  p->vec_states = in_fours(d, states, {p->b, p->c});
 }
 void cut_into(ScanArgs* p, const fdwt_scan_desc* d, const Cut& c, void* ws) {
   const Segments s = segment_bytes(d, c);
   p->tiles = c.tiles, p->segments = c.segments, p->seg_len = c.seg_len;
   p->seg_state = static_cast<char*>(ws) + s.state;
   p->seg_sum = static_cast<char*>(ws) + s.sum;
-}
-
-template <typename F> int with_type(int dtype, F fn) {
-  switch (dtype) {
-    case FDWT_F32: return fn(float{});
-    case FDWT_F64: return fn(double{});
-    case FDWT_F16: return fn(__half{});
-    default: return fn(__nv_bfloat16{});
-  }
 }
 
 }  // namespace
@@ -209,7 +249,7 @@ extern "C" int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, c
   FDWT_CHECK(aligned16({workspace, checkpoints}));
   ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths);
   p.y = y, p.final_state = final_state, p.check = checkpoints;
-  p.vec = rows_aligned(desc, p, false);
+  see_alignment(&p, desc, false);
   cut_into(&p, desc, cut, workspace);
   const int lanes = lanes_of(desc->states);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -225,7 +265,7 @@ extern "C" int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, c
 
 extern "C" size_t fdwt_selscan_backward_workspace(const fdwt_scan_desc* desc) {
   if (!scan_ok(desc) || desc->states > FDWT_MAX_SCAN_STATES) return 0;
-  return part_bytes(desc, backward_cut(desc, wide_backward(desc))).bytes;
+  return part_bytes(desc, backward_cut(desc)).bytes;
 }
 
 extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, const void* dt,
@@ -250,8 +290,7 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
   FDWT_CHECK(desc->length == 0 || (x != nullptr && dt != nullptr && b != nullptr && c != nullptr &&
                                    checkpoints != nullptr && dy != nullptr && dx != nullptr &&
                                    ddt != nullptr));
-  const bool wide = wide_backward(desc);
-  const Cut cut = backward_cut(desc, wide);
+  const Cut cut = backward_cut(desc);
   const Parts parts = part_bytes(desc, cut);
   if (workspace == nullptr || workspace_bytes < parts.bytes) return FDWT_ERR_WORKSPACE;
   FDWT_CHECK(aligned16({workspace, checkpoints}));
@@ -261,7 +300,7 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
   p.d_initial = d_initial_state;
   char* ws = static_cast<char*>(workspace);
   p.part_a = ws + parts.a, p.part_ch = ws + parts.ch, p.part_bc = ws + parts.bc;
-  p.vec = rows_aligned(desc, p, true);
+  see_alignment(&p, desc, true);
   cut_into(&p, desc, cut, workspace);
   const int lanes = lanes_of(desc->states), np = 4 * lanes;
   return with_type(desc->dtype, [&](auto t) -> int {
@@ -275,7 +314,7 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
       st = scan_states<T>(r, lanes, true, s);
       if (st != FDWT_OK) return st;
     }
-    st = scan_backward<T>(p, lanes, wide, s);
+    st = scan_backward<T>(p, lanes, s);
     if (st != FDWT_OK) return st;
     const int64_t rows = desc->batch * cut.segments;
     if (desc->length > 0 && (db != nullptr || dc != nullptr)) {

@@ -38,7 +38,7 @@ struct ScanArgs {
   int groups, states;
   int softplus;
   int64_t xs[2], dts[2], gs[2], dys[2], bs[3], cs[3];
-  int vec;            // rows begin on 16-byte boundaries throughout
+  int vec, vec_states;  // rows of channels, of b and c begin on boundaries of 4 elements
   int64_t per, tiles; // channels of a group, tiles of one
   int segments;
   int64_t seg_len;    // tokens, a multiple of kScanCheck and of the staged tokens
@@ -56,17 +56,18 @@ struct ScanArgs {
 // Launchers by element type (selscan_*.cu).  `lanes` is LN, 1 to 32.
 template <typename T> int scan_forward(const ScanArgs& p, int lanes, cudaStream_t stream);
 template <typename T> int scan_states(const ScanArgs& p, int lanes, bool reverse, cudaStream_t stream);
-template <typename T> int scan_backward(const ScanArgs& p, int lanes, bool wide, cudaStream_t stream);
+template <typename T> int scan_backward(const ScanArgs& p, int lanes, cudaStream_t stream);
+// Blocks of the forward and the backward launch that are resident on the device.
+template <typename T> int64_t scan_resident(int lanes, bool backward);
 template <typename T> int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool,
                                     void* state, cudaStream_t stream);
 
-// Channels of a thread, and of a block, in the forward launches and (wide: 4 tiles of channels one
-// after the other where the block's shared memory holds them) in the backward launch.
+// Channels of a thread, and of a block.
 constexpr int scan_fwd_channels(int ln) { return ln == 1 ? 1 : (ln <= 4 ? 2 : 4); }
 constexpr int scan_fwd_tile(int ln) { return 4 * (32 / ln) * scan_fwd_channels(ln); }
-constexpr int scan_bwd_channels(int ln, bool wide) {
-  return !wide ? (ln <= 4 ? 1 : (ln == 8 ? 2 : 4)) : (ln == 1 ? 1 : (ln == 2 ? 2 : 4));
+constexpr int scan_bwd_channels(int ln, bool fp64) { return ln <= 2 || (fp64 && ln <= 8) ? 1 : 2; }
+constexpr int scan_bwd_tile(int ln, bool fp64) {
+  return 4 * (32 / ln) * scan_bwd_channels(ln, fp64);
 }
-constexpr int scan_bwd_tile(int ln, bool wide) { return 4 * (32 / ln) * scan_bwd_channels(ln, wide); }
 
 }  // namespace fdwt

@@ -28,14 +28,10 @@ __device__ __forceinline__ Two<float> two(float x, float y) {
 }
 __device__ __forceinline__ Two<double> two(double x, double y) { return {x, y}; }
 __device__ __forceinline__ float first(Two<float> a) {
-  float x, y;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
-  return x;
+  return __uint_as_float(static_cast<uint32_t>(a.v));
 }
 __device__ __forceinline__ float second(Two<float> a) {
-  float x, y;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
-  return y;
+  return __uint_as_float(static_cast<uint32_t>(a.v >> 32));
 }
 __device__ __forceinline__ double first(Two<double> a) { return a.x; }
 __device__ __forceinline__ double second(Two<double> a) { return a.y; }
@@ -82,19 +78,51 @@ template <typename A> __device__ __forceinline__ Two<A> exp_2(Two<A> x) {
 }
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
-// log(1 + e^v), to the last bits where it is small too: steps are often 1e-3.
-__device__ __forceinline__ float softplus(float v) {
-  return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
+// e^-a for a >= 0: the product with log2 e is rounded, so what it lost corrects the result.
+__device__ __forceinline__ float neg_exp(float a) {
+  constexpr float kHigh = 1.442695021629333f, kLow = 1.92596299e-8f;  // log2 e in two parts
+  const float t = a * kHigh;
+  const float lost = fmaf(a, kLow, fmaf(a, kHigh, -t));
+  const float e = exp_2(-t);
+  return fmaf(e, lost * -static_cast<float>(kLn2), e);
 }
-__device__ __forceinline__ double softplus(double v) {
-  return fmax(v, 0.0) + log1p(exp(-fabs(v)));
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
-// 1 / (1 + e^-v): of a few roundings' error for rows of 32 bits and where the result stays in 32
-// bits (EXACT), by the fast exponential and division where it is rounded to 16.
-template <typename T, bool EXACT, typename A> __device__ __forceinline__ A sigmoid_at(A v) {
-  if constexpr (sizeof(T) == 8) return 1.0 / (1.0 + exp(-v));
-  else if constexpr (sizeof(T) == 4 || EXACT) return 1.0f / (1.0f + expf(-v));
-  else return __fdividef(1.0f, 1.0f + __expf(-v));
+// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|), to the last bits where it is small too (steps are
+// often 1e-3), and its slope 1 / (1 + e^-v).  log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the
+// odd series of atanh, its coefficients fitted for s^2 up to 1/9 (8e-9 off).  Against log1pf and
+// expf of the library (35 instructions, this 17): 2 to 4 roundings off, as they are.
+__device__ __forceinline__ float softplus(float v, float* slope) {
+  const float e = neg_exp(fminf(fabsf(v), 128.0f));
+  const float s = e * reciprocal(2.0f + e), z = s * s;
+  float q = 0.2817465662956238f;
+  q = fmaf(q, z, 0.2796141803264618f);
+  q = fmaf(q, z, 0.40024852752685547f);
+  q = fmaf(q, z, 0.6666631698608398f);
+  q = fmaf(q, z, 2.0f);
+  if (slope != nullptr) {
+    const float w = reciprocal(1.0f + e);
+    *slope = v < 0.0f ? e * w : w;
+  }
+  return fmaf(s, q, v < 0.0f ? 0.0f : v);
+}
+__device__ __forceinline__ double softplus(double v, double* slope) {
+  const double e = exp(-fabs(v));
+  if (slope != nullptr) *slope = v < 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
+  return (v < 0.0 ? 0.0 : v) + log1p(e);
+}
+// 1 / (1 + e^-v) to a few roundings, or, where the result is rounded to 16 bits (FAST), by the
+// plain fast functions.
+template <bool FAST> __device__ __forceinline__ float sigmoid_at(float v) {
+  if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-v));
+  const float e = neg_exp(fminf(fabsf(v), 128.0f)), w = reciprocal(1.0f + e);
+  return v < 0.0f ? e * w : (v != v ? v : w);
+}
+template <bool FAST> __device__ __forceinline__ double sigmoid_at(double v) {
+  return 1.0 / (1.0 + exp(-v));
 }
 
 // A channel's rates times log2 e.  -inf (forgets everything) becomes the lowest finite value, so
@@ -130,29 +158,54 @@ template <int V, int L, int STRIDE, typename A> __device__ __forceinline__ void 
   }
 }
 
+// The same with values in another order in every lane, so that no lane has to choose: where place
+// p among L lanes holds its M values in the order 0 ^ p, 1 ^ p, ..., (bits of p from the top of the
+// order down, as many as both have), each step keeps the first half of the registers and hands over
+// the second.  v holds V runs of M values; afterwards register 0 of each run, or the first M / L, is
+// a sum over the first log2 M bits of the lanes; fold takes the others.
+template <int V, int M, int L, int STRIDE, typename A> __device__ __forceinline__ void fold_swapped(A* v) {
+  if constexpr (M > 1 && L > 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < M / 2; ++j)
+        v[i * (M / 2) + j] = v[i * M + j] + __shfl_xor_sync(0xffffffffu, v[i * M + M / 2 + j], STRIDE);
+    fold_swapped<V, M / 2, L / 2, 2 * STRIDE>(v);
+  }
+}
+// The order of the M values of a lane at place p among L: register j holds value j ^ order.  Bit i
+// of p decides about bit log2 M - 1 - i of the value.
+template <int M, int L> __device__ __forceinline__ int order_at(int p) {
+  if constexpr (M <= 1 || L <= 1) return 0;
+  else return (p & 1) * (M / 2) | order_at<M / 2, L / 2>(p >> 1);
+}
+template <typename A> __device__ __forceinline__ Four<A> reorder(Four<A> q, int order) {
+  if (order & 2) q = {q.v[2], q.v[3], q.v[0], q.v[1]};
+  if (order & 1) q = {q.v[1], q.v[0], q.v[3], q.v[2]};
+  return q;
+}
+
 __device__ __forceinline__ int64_t valid_tokens(const ScanArgs& p, int64_t b) {
   if (p.lengths == nullptr) return p.length;
   const int64_t n = p.lengths[b];
   return n < 0 ? 0 : (n < p.length ? n : p.length);
 }
 
-// Slots of a token's channels are staged by threads of 8 neighbouring ones and read by lanes of
-// neighbouring ones: the order within 8 goes by the place of the 8, so that both reach all banks.
-__device__ __forceinline__ int slot_of(int c) { return c ^ ((c >> 3) & 7); }
-
 // What a block works on.
 struct Place {
-  int64_t b, t0, t1, count;  // sequence, its segment's tokens, valid tokens of the sequence
+  int64_t b, t0, t1, count;  // sequence, its segment's tokens, the valid ones among them (an end)
   int64_t d0;                // first channel
   int group, segment, tile, width;  // width: channels of the tile
 };
-template <int CT> __device__ __forceinline__ Place place_of(const ScanArgs& p) {
+// `segments` of the sequence have a block, those from `first` on.
+template <int CT>
+__device__ __forceinline__ Place place_of(const ScanArgs& p, int segments, int first) {
   Place w;
   const int64_t tiles = p.tiles * p.groups;
   const int64_t id = blockIdx.x;
   w.tile = static_cast<int>(id % tiles);
-  w.segment = static_cast<int>(id / tiles % p.segments);
-  w.b = id / tiles / p.segments;
+  w.segment = static_cast<int>(id / tiles % segments) + first;
+  w.b = id / tiles / segments;
   w.group = static_cast<int>(w.tile / p.tiles);
   const int64_t within = (w.tile % p.tiles) * CT;
   w.d0 = w.group * p.per + within;
@@ -160,57 +213,186 @@ template <int CT> __device__ __forceinline__ Place place_of(const ScanArgs& p) {
   w.t0 = w.segment * p.seg_len;
   w.t1 = w.t0 + p.seg_len < p.length ? w.t0 + p.seg_len : p.length;
   w.count = valid_tokens(p, w.b);
+  if (w.count > w.t1) w.count = w.t1;
   return w;
 }
 
-// Rows of b or c: TT tokens from t on, in 32 bits, zeros past the states and the valid tokens.
-template <typename T, int TT, int NP, typename A>
-__device__ __forceinline__ void stage_states(const ScanArgs& p, const Place& w, const void* src,
-                                             const int64_t* stride, int64_t t, A* out) {
-  const T* q = static_cast<const T*>(src) + w.b * stride[0] + w.group * stride[2];
-  for (int e = threadIdx.x; e < TT * NP; e += 128) {
-    const int n = e % NP;
-    const int64_t at = t + e / NP;
-    out[e] = n < p.states && at < w.count ? to_acc(q[at * stride[1] + n]) : A(0);
+// 4 neighbouring elements of a row, the first `have` of which exist (4 or none where the rows begin
+// on their boundary); the others are zero.  16-bit elements stay packed until they are used: taken
+// apart at once, each load would be waited for where it is issued.
+template <typename T> struct Quad {
+  using Raw = Four<T>;
+  static __device__ __forceinline__ Raw some(const T* q, int have) {
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.v[j] = j < have ? q[j] : T(0);
+    return r;
+  }
+  static __device__ __forceinline__ void values(const Raw& r, T* x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = r.v[j];
+  }
+};
+template <typename T> struct Quad16 {
+  using Raw = uint2;
+  static __device__ __forceinline__ Raw some(const T* q, int have) {
+    const unsigned short* u = reinterpret_cast<const unsigned short*>(q);
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < have ? u[j] : 0;
+    return make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float* x) {
+    Half2<T>::split(r.x, x);
+    Half2<T>::split(r.y, x + 2);
+  }
+};
+template <> struct Quad<__half> : Quad16<__half> {};
+template <> struct Quad<__nv_bfloat16> : Quad16<__nv_bfloat16> {};
+template <typename T> using Raw4 = typename Quad<T>::Raw;
+template <typename T> __device__ __forceinline__ Raw4<T> load4(const T* q, int have, bool vec) {
+  if (vec) {
+    Raw4<T> r = {};
+    if (have >= 4) r = *reinterpret_cast<const Raw4<T>*>(q);
+    return r;
+  }
+  return Quad<T>::some(q, have);
+}
+template <typename T, typename A>
+__device__ __forceinline__ void store4(T* q, const A* x, int have, bool vec) {
+  if (vec && have >= 4) {
+    Group<T, 4>::store(q, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < have) q[j] = from_acc<T>(x[j]);
   }
 }
+template <typename A> __device__ __forceinline__ Four<A> params4(const void* q, int64_t at, int have) {
+  Four<A> r = {A(0), A(0), A(0), A(0)};
+  if (q != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < have) r.v[j] = static_cast<const A*>(q)[at + j];
+  }
+  return r;
+}
 
+// The threads of a block that stages TT tokens of CT channels: each takes 4 neighbouring channels
+// (always the same) of IT tokens, ROWS apart.
+template <int CT, int TT> struct Items {
+  static constexpr int COLS = CT / 4, ROWS = 128 / COLS, IT = (TT + ROWS - 1) / ROWS;
+};
+
+// A thread's share of b (and c) of TT tokens: 4 states a load, on the way to shared memory.
+template <typename T, int TT, int LN, int ARRAYS> struct States {
+  using A = typename AccOf<T>::type;
+  static constexpr int ALL = TT * LN * ARRAYS, IT = (ALL + 127) / 128;
+  // loads that lie whole rows of tokens apart in one array share a pointer
+  static constexpr int EACH = ARRAYS == 2 && TT * LN < 128 ? IT : (TT * LN + 127) / 128;
+  static constexpr int PTRS = (IT + EACH - 1) / EACH;
+  Raw4<T> raw[IT];
+  const T* at[PTRS];
+  int64_t stride[PTRS];
+  __device__ __forceinline__ void start(const ScanArgs& p, const Place& w, const void* b,
+                                        const int64_t* bs, const void* c, const int64_t* cs,
+                                        int64_t t) {
+#pragma unroll
+    for (int i = 0; i < PTRS; ++i) {
+      const int e = threadIdx.x + i * EACH * 128;
+      const bool second = ARRAYS == 2 && e >= TT * LN;
+      const int64_t* s = second ? cs : bs;
+      stride[i] = s[1];
+      at[i] = static_cast<const T*>(second ? c : b) + w.b * s[0] + w.group * s[2] +
+              (t + e / LN % TT) * s[1] + e % LN * 4;
+    }
+  }
+  // `left` tokens from the step's first on are valid; the next step is `step` tokens on.
+  __device__ __forceinline__ void fetch(const ScanArgs& p, int left, int step) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int e = threadIdx.x + i * 128;
+      if (ALL % 128 != 0 && e >= ALL) break;
+      const int k = i / EACH;
+      raw[i] = load4(at[k] + (i % EACH) * (128 / LN) * stride[k],
+                     e / LN % TT < left ? p.states - e % LN * 4 : 0, p.vec_states);
+    }
+#pragma unroll
+    for (int i = 0; i < PTRS; ++i) at[i] += step * stride[i];
+  }
+  __device__ __forceinline__ void store(Four<A>* out) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int e = threadIdx.x + i * 128;
+      if (ALL % 128 != 0 && e >= ALL) break;
+      Four<A> q;
+      Quad<T>::values(raw[i], q.v);
+      out[e] = q;
+    }
+  }
+  // [ARRAYS TT][COPIES][LN], copy k in the order of lanes at place k
+  template <int COPIES> __device__ __forceinline__ void store_orders(Four<A>* out) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int e = threadIdx.x + i * 128;
+      if (ALL % 128 != 0 && e >= ALL) break;
+      Four<A> q;
+      Quad<T>::values(raw[i], q.v);
+#pragma unroll
+      for (int k = 0; k < COPIES; ++k)
+        out[(e / LN * COPIES + k) * LN + e % LN] = reorder(q, order_at<4, COPIES>(k));
+    }
+  }
+};
+
+// Step and taken-in input of a token and channel.
+template <typename A> struct alignas(2 * sizeof(A)) Step {
+  A delta, u;
+};
 // ------------------------------------------------------------------------------ forward
 // MAIN: outputs and last states.  STATES: a segment's end state from zero, and its sum of delta.
 // REVERSE: the same back in time for the gradients, r = e^(delta a) (c dp + r).
+//
+// The next tokens' rows are loaded before the current ones' states are worked out, so that the
+// loads' latency passes behind the exponentials.
 enum ScanMode { MAIN, STATES, REVERSE };
 template <typename A> constexpr int scan_fwd_tokens() { return sizeof(A) == 8 ? 8 : 16; }
 
 template <typename T, int LN, int NC, int MODE>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, sizeof(T) == 8 ? 1 : (NC <= 2 ? 4 : 3))
 scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
   using A = typename AccOf<T>::type;
-  constexpr int LD = 32 / LN, CT = 4 * LD * NC, NP = 4 * LN, TT = scan_fwd_tokens<A>();
-  constexpr int V = 16 / sizeof(T) < CT ? 16 / sizeof(T) : CT;
+  constexpr int LD = 32 / LN, CT = 4 * LD * NC, TT = scan_fwd_tokens<A>();
   constexpr int PAD = CT + 8;
-  __shared__ Four<A> slots[TT * CT];           // delta, delta, delta x, delta x
-  __shared__ Four<A> into[TT * LN], out[MODE == MAIN ? TT * LN : 1];  // b and c
-  __shared__ A sums[MODE == MAIN ? TT * PAD : 1];
-  const Place w = place_of<CT>(p);
+  using I = Items<CT, TT>;
+  __shared__ Step<A> slots[TT * CT];
+  __shared__ Four<A> states[(MODE == MAIN ? 2 : 1) * TT * LN];  // b (REVERSE: c), then c
+  __shared__ __align__(4 * sizeof(A)) A sums[MODE == MAIN ? TT * PAD : 1];
+  // (no state is needed after the last segment, nor back in time before the first)
+  const Place w = place_of<CT>(p, MODE == MAIN ? p.segments : p.segments - 1, MODE == REVERSE);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nl = lane % LN, dl = lane / LN;
-  const int cl = (warp * LD + dl) * NC;  // the thread's first channel of the tile
+  // The thread's channels of the tile: cl + (k ^ swap), in an order by its lane (fold_swapped).
+  const int cl = (warp * LD + dl) * NC, swap = order_at<NC, LN>(nl);
+  constexpr int KEPT = NC < LN ? NC : LN, OTHERS = LN / KEPT;  // lanes that share out channels, tokens
+  static_assert(KEPT == NC || LN == 1);
   const A* rates = static_cast<const A*>(p.a);
 
   Two<A> ra[NC][2], h[NC][2];
   A total[NC];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
+    const int c = cl + (k ^ swap);
     A r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = nl * 4 + j;
-      r[j] = cl + k < w.width && n < p.states ? rate(rates[(w.d0 + cl + k) * p.states + n]) : A(0);
+      r[j] = c < w.width && n < p.states ? rate(rates[(w.d0 + c) * p.states + n]) : A(0);
     }
     ra[k][0] = two(r[0], r[1]);
     ra[k][1] = two(r[2], r[3]);
     A s[4] = {A(0), A(0), A(0), A(0)};
-    if (MODE == MAIN && cl + k < w.width) {
-      const int64_t d = w.d0 + cl + k;
+    if (MODE == MAIN && c < w.width) {
+      const int64_t d = w.d0 + c;
       if (p.initial != nullptr) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -218,6 +400,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
             s[j] = static_cast<const A*>(p.initial)[(w.b * p.dim + d) * p.states + nl * 4 + j];
       }
       // the segments before this one
+#pragma unroll 4
       for (int g = 0; g < w.segment; ++g) {
         const int64_t row = (w.b * p.segments + g) * p.dim + d;
         const A sum = static_cast<const A*>(p.seg_sum)[row];
@@ -231,156 +414,175 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     total[k] = A(0);
   }
 
+  // the thread's items
+  const int col = threadIdx.x % I::COLS * 4, row0 = threadIdx.x / I::COLS;
+  const int have = w.width - col;
   const T* px = static_cast<const T*>(MODE == REVERSE ? p.dy : p.x) +
-                w.b * (MODE == REVERSE ? p.dys[0] : p.xs[0]) + w.d0;
+                w.b * (MODE == REVERSE ? p.dys[0] : p.xs[0]) + w.d0 + col;
   const int64_t xs = MODE == REVERSE ? p.dys[1] : p.xs[1];
-  const T* pd = static_cast<const T*>(p.dt) + w.b * p.dts[0] + w.d0;
-  const T* pg = static_cast<const T*>(p.gate) + w.b * p.gs[0] + w.d0;
-  const A* bias = static_cast<const A*>(p.dt_bias) + w.d0;
-  const A* skip = static_cast<const A*>(p.skip) + w.d0;
-  T* py = static_cast<T*>(p.y) + w.b * p.length * p.dim + w.d0;
-
-  // G neighbouring channels of a token
-  auto stage = [&](auto g, int64_t t, int at, int c, bool in) {
-    constexpr int G = decltype(g)::value;
-    A dt[G], x[G];
-    if (in) {
-      Group<T, G>::values(Group<T, G>::load(pd + t * p.dts[1] + c), dt);
-      Group<T, G>::values(Group<T, G>::load(px + t * xs + c), x);
-      if (MODE == REVERSE && p.gate != nullptr) {
-        A z[G];
-        Group<T, G>::values(Group<T, G>::load(pg + t * p.gs[1] + c), z);
+  const T* pd = static_cast<const T*>(p.dt) + w.b * p.dts[0] + w.d0 + col;
+  const T* pg = static_cast<const T*>(p.gate) + w.b * p.gs[0] + w.d0 + col;
+  T* py = static_cast<T*>(p.y) + (w.b * p.length + w.t0 + row0) * p.dim + w.d0 + col;
+  const Four<A> bias = params4<A>(p.dt_bias, w.d0 + col, have);
+  const Four<A> skip = params4<A>(MODE == MAIN ? p.skip : nullptr, w.d0 + col, have);
+  const bool gated = MODE != STATES && p.gate != nullptr;
+  Raw4<T> xr[I::IT], dr[I::IT], zr[I::IT];
+  States<T, TT, LN, MODE == MAIN ? 2 : 1> bc;
+  const int64_t steps = w.count > w.t0 ? (w.count - w.t0 + TT - 1) / TT : 0;
+  auto begin = [&](int64_t i) { return w.t0 + (MODE == REVERSE ? steps - 1 - i : i) * TT; };
+  {  // from here on the pointers are those of the thread's first token of the step
+    const int64_t t = begin(0) + row0;
+    px += t * xs;
+    pd += t * p.dts[1];
+    pg += t * p.gs[1];
+    bc.start(p, w, MODE == REVERSE ? p.c : p.b, MODE == REVERSE ? p.cs : p.bs, p.c, p.cs, begin(0));
+  }
+  auto on = [&](const T*& q, int64_t stride) { q += MODE == REVERSE ? -TT * stride : TT * stride; };
+  auto rows = [&](const T* q, int64_t stride, Raw4<T>* raw, int left) {
 #pragma unroll
-        for (int j = 0; j < G; ++j) x[j] *= z[j] * sigmoid_at<T, true>(z[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      A delta = A(0), u = A(0);
-      if (in) {
-        delta = dt[j];
-        if (p.dt_bias != nullptr) delta += bias[c + j];
-        if (p.softplus) delta = softplus(delta);
-        u = MODE == REVERSE ? x[j] : delta * x[j];
-      }
-      slots[at * CT + slot_of(c + j)] = {delta, delta, u, u};
-    }
+    for (int i = 0; i < I::IT; ++i)
+      raw[i] = load4(q + i * (I::ROWS * stride), i * I::ROWS < left ? have : 0, p.vec);
   };
-  auto finish = [&](auto g, int64_t t, int at, int c) {
-    constexpr int G = decltype(g)::value;
-    A y[G];
-    if (t < w.count) {
-      A x[G], z[G];
-      Group<T, G>::values(Group<T, G>::load(px + t * xs + c), x);
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        y[j] = sums[at * PAD + c + j];
-        if (p.skip != nullptr) y[j] += skip[c + j] * x[j];
-      }
-      if (p.gate != nullptr) {
-        Group<T, G>::values(Group<T, G>::load(pg + t * p.gs[1] + c), z);
-#pragma unroll
-        for (int j = 0; j < G; ++j) y[j] *= z[j] * sigmoid_at<T, false>(z[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < G; ++j) y[j] = A(0);
-    }
-    Group<T, G>::store(py + t * p.dim + c, y);
+  // tokens from the thread's first one to the end of the valid ones and of the step
+  auto left_at = [&](int64_t t) {
+    return static_cast<int>((w.count - t < TT ? w.count - t : TT) - row0);
   };
-  // every (token, channels) of the staged tokens, by threads
-  auto each = [&](auto fn) {
-    if (p.vec) {
-      for (int e = threadIdx.x; e < TT * (CT / V); e += 128)
-        fn(std::integral_constant<int, V>{}, e / (CT / V), e % (CT / V) * V);
-    } else {
-      for (int e = threadIdx.x; e < TT * CT; e += 128)
-        fn(std::integral_constant<int, 1>{}, e / CT, e % CT);
-    }
+  auto fetch = [&](int64_t t) {
+    const int left = left_at(t);
+    rows(px, xs, xr, left);
+    rows(pd, p.dts[1], dr, left);
+    on(px, xs);
+    on(pd, p.dts[1]);
+    bc.fetch(p, static_cast<int>(w.count - t < TT ? w.count - t : TT), MODE == REVERSE ? -TT : TT);
   };
 
-  const int64_t steps = w.t1 > w.t0 ? (w.t1 - w.t0 + TT - 1) / TT : 0;
+  if (steps > 0) fetch(begin(0));
   for (int64_t i = 0; i < steps; ++i) {
-    const int64_t t = w.t0 + (MODE == REVERSE ? steps - 1 - i : i) * TT;
-    if (t < w.count) {
-      each([&](auto g, int at, int c) {
-        stage(g, t + at, at, c, t + at < w.count && c < w.width);
-      });
-      stage_states<T, TT, NP>(p, w, MODE == REVERSE ? p.c : p.b, MODE == REVERSE ? p.cs : p.bs, t,
-                              &into[0].v[0]);
-      if constexpr (MODE == MAIN) stage_states<T, TT, NP>(p, w, p.c, p.cs, t, &out[0].v[0]);
-      __syncthreads();
+    const int64_t t = begin(i);
+    const int left = left_at(t);
+    Raw4<T> xc[I::IT];
+    if (gated) {
+      rows(pg, p.gs[1], zr, left);
+      on(pg, p.gs[1]);
+    }
+#pragma unroll
+    for (int q = 0; q < I::IT; ++q) {
+      const int row = row0 + q * I::ROWS;
+      if (I::ROWS * I::IT > TT && row >= TT) break;
+      A x[4], dt[4], z[4];
+      Step<A> out[4];
+      Quad<T>::values(xr[q], x);
+      Quad<T>::values(dr[q], dt);
+      if (MODE == REVERSE && gated) Quad<T>::values(zr[q], z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        A delta = dt[j] + bias.v[j];
+        if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
+        if (MODE == REVERSE) {
+          if (gated) x[j] *= z[j] * sigmoid_at<false>(z[j]);
+          out[j] = {delta, x[j]};
+        } else {
+          out[j] = {delta, delta * x[j]};
+        }
+        if (q * I::ROWS >= left) out[j] = {A(0), A(0)};
+      }
+      Four<A>* to = reinterpret_cast<Four<A>*>(slots + row * CT + col);
+      to[0] = {out[0].delta, out[0].u, out[1].delta, out[1].u};
+      to[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
+      xc[q] = xr[q];
+    }
+    bc.store(states);
+    if (i + 1 < steps) fetch(begin(i + 1));
+    __syncthreads();
 #pragma unroll 1
-      for (int s = 0; s < TT; s += 8) {
-        if (MODE == MAIN && p.check != nullptr && t + s < p.length) {
-          const int64_t row = (w.b * ((p.length + 7) / 8) + (t + s) / 8) * p.dim + w.d0 + cl;
+    for (int s = 0; s < TT; s += 8) {
+      if (MODE == MAIN && p.check != nullptr && t + s < w.count) {
+        const int64_t row = (w.b * ((p.length + 7) / 8) + (t + s) / 8) * p.dim + w.d0 + cl;
 #pragma unroll
-          for (int k = 0; k < NC; ++k)
-            if (cl + k < w.width)
-              static_cast<Four<A>*>(p.check)[(row + k) * LN + nl] = {
-                  first(h[k][0]), second(h[k][0]), first(h[k][1]), second(h[k][1])};
-        }
-        A y[8 * NC];
+        for (int k = 0; k < NC; ++k)
+          if (cl + (k ^ swap) < w.width)
+            static_cast<Four<A>*>(p.check)[(row + (k ^ swap)) * LN + nl] = {
+                first(h[k][0]), second(h[k][0]), first(h[k][1]), second(h[k][1])};
+      }
+      A y[8 * NC];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int row = MODE == REVERSE ? TT - 1 - s - u : s + u;
-          const Four<A> bq = into[row * LN + nl];
-          Four<A> cq;
-          if constexpr (MODE == MAIN) cq = out[row * LN + nl];
+      for (int u = 0; u < 8; ++u) {
+        const int row = MODE == REVERSE ? TT - 1 - s - u : s + u;
+        const Four<A> bq = states[row * LN + nl];
+        Four<A> cq;
+        if constexpr (MODE == MAIN) cq = states[(TT + row) * LN + nl];
 #pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            const Four<A> q = slots[row * CT + slot_of(cl + k)];
-            const Two<A> d2 = low(q), u2 = high(q);
-            const Two<A> e0 = exp_2(mul(d2, ra[k][0])), e1 = exp_2(mul(d2, ra[k][1]));
-            if constexpr (MODE == REVERSE) {
-              h[k][0] = mul(e0, fma(u2, low(bq), h[k][0]));
-              h[k][1] = mul(e1, fma(u2, high(bq), h[k][1]));
-            } else {
-              h[k][0] = fma(e0, h[k][0], mul(u2, low(bq)));
-              h[k][1] = fma(e1, h[k][1], mul(u2, high(bq)));
-            }
-            if constexpr (MODE == MAIN) {
-              const Two<A> s2 = fma(h[k][1], high(cq), mul(h[k][0], low(cq)));
-              y[u * NC + k] = first(s2) + second(s2);
-            } else {
-              total[k] += first(d2);
-            }
+        for (int k = 0; k < NC; ++k) {
+          const Step<A> st = slots[row * CT + cl + (k ^ swap)];
+          const Two<A> d2 = two(st.delta, st.delta), u2 = two(st.u, st.u);
+          const Two<A> e0 = exp_2(mul(d2, ra[k][0])), e1 = exp_2(mul(d2, ra[k][1]));
+          if constexpr (MODE == REVERSE) {
+            h[k][0] = mul(e0, fma(u2, low(bq), h[k][0]));
+            h[k][1] = mul(e1, fma(u2, high(bq), h[k][1]));
+          } else {
+            h[k][0] = fma(e0, h[k][0], mul(u2, low(bq)));
+            h[k][1] = fma(e1, h[k][1], mul(u2, high(bq)));
           }
-        }
-        if constexpr (MODE == MAIN) {
-          fold<8 * NC, LN, 1>(y, lane);
-          constexpr int OWN = 8 * NC / LN;
-#pragma unroll
-          for (int o = 0; o < OWN; ++o) {
-            const int v = nl * OWN + o;
-            sums[(s + v / NC) * PAD + cl + v % NC] = y[o];
+          if constexpr (MODE == MAIN) {
+            const Two<A> s2 = fma(h[k][1], high(cq), mul(h[k][0], low(cq)));
+            y[u * NC + k] = first(s2) + second(s2);
+          } else {
+            total[k] += st.delta;
           }
         }
       }
-      __syncthreads();
+      if constexpr (MODE == MAIN) {
+        fold_swapped<8, NC, LN, 1>(y);
+        fold<8, OTHERS, KEPT>(y, lane);
+        constexpr int OWN = 8 / OTHERS;
+#pragma unroll
+        for (int o = 0; o < OWN; ++o)
+          sums[(s + nl / KEPT * OWN + o) * PAD + cl + (LN == 1 ? 0 : swap)] = y[o];
+      }
     }
+    __syncthreads();
     if constexpr (MODE == MAIN) {
-      each([&](auto g, int at, int c) {
-        if (t + at < w.t1 && c < w.width) finish(g, t + at, at, c);
-      });
+#pragma unroll
+      for (int q = 0; q < I::IT; ++q) {
+        const int row = row0 + q * I::ROWS;
+        if (q * I::ROWS >= left) break;
+        const Four<A> f = *reinterpret_cast<const Four<A>*>(sums + row * PAD + col);
+        A y[4], x[4], z[4];
+        if (p.skip != nullptr) Quad<T>::values(xc[q], x);
+        if (gated) Quad<T>::values(zr[q], z);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] = f.v[j];
+          if (p.skip != nullptr) y[j] += skip.v[j] * x[j];
+          if (gated) y[j] *= z[j] * sigmoid_at<sizeof(T) == 2>(z[j]);
+        }
+        store4(py + q * (I::ROWS * p.dim), y, have, p.vec);
+      }
+      py += TT * p.dim;
     }
   }
 
   if constexpr (MODE == MAIN) {
+    const A none[4] = {A(0), A(0), A(0), A(0)};
+    T* rest = static_cast<T*>(p.y) + w.b * p.length * p.dim + w.d0 + col;
+    for (int64_t t = (w.count > w.t0 ? w.count : w.t0) + row0; t < w.t1; t += I::ROWS)
+      store4(rest + t * p.dim, none, have, p.vec);
     if (w.segment != p.segments - 1 || p.final_state == nullptr) return;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const A s[4] = {first(h[k][0]), second(h[k][0]), first(h[k][1]), second(h[k][1])};
-      A* to = static_cast<A*>(p.final_state) + (w.b * p.dim + w.d0 + cl + k) * p.states;
+      const int c = cl + (k ^ swap);
+      A* to = static_cast<A*>(p.final_state) + (w.b * p.dim + w.d0 + c) * p.states;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (cl + k < w.width && nl * 4 + j < p.states) to[nl * 4 + j] = s[j];
+        if (c < w.width && nl * 4 + j < p.states) to[nl * 4 + j] = s[j];
     }
   } else {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      if (cl + k >= w.width) continue;
-      const int64_t row = (w.b * p.segments + w.segment) * p.dim + w.d0 + cl + k;
+      const int c = cl + (k ^ swap);
+      if (c >= w.width) continue;
+      const int64_t row = (w.b * p.segments + w.segment) * p.dim + w.d0 + c;
       static_cast<Four<A>*>(p.seg_state)[row * LN + nl] = {first(h[k][0]), second(h[k][0]),
                                                            first(h[k][1]), second(h[k][1])};
       if (nl == 0) static_cast<A*>(p.seg_sum)[row] = total[k];
@@ -389,284 +591,351 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
 }
 
 // ------------------------------------------------------------------------------ backward
-// A block walks its segment back in time, 8 tokens at a time.  From the state that the forward pass
-// kept before them a thread forms its states and decays of the 8 tokens again and keeps them in
-// registers, then goes back over them.  It does so for KC channels one after the other: their
-// shares of db and dc add up in registers, and cross the lanes once for all of them.
-template <typename T, int LN, int KC>
+// A block walks its segment back in time, 8 tokens at a time, in two halves.  From the state that
+// the forward pass kept before the 8 a thread forms the states and decays of a half's 4 tokens
+// again (for the later half after passing over the earlier one) and keeps them in registers, then
+// goes back over them.  Keeping 8 tokens' in registers would save the passing over, but takes 255
+// registers; a block's threads then wait on one another's latencies.
+template <typename T, int LN, int NC>
 __global__ void __launch_bounds__(128)
 scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
   using A = typename AccOf<T>::type;
-  constexpr int LD = 32 / LN, CT = 4 * LD * KC, NP = 4 * LN, TT = kScanCheck;
-  constexpr int V = 16 / sizeof(T) < CT ? 16 / sizeof(T) : CT;
+  constexpr int LD = 32 / LN, CT = 4 * LD * NC, NP = 4 * LN, TT = kScanCheck, SUB = TT / 2;
   constexpr int PAD = CT + 8;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  Four<A>* slots = reinterpret_cast<Four<A>*>(smem_raw);  // delta, delta, delta x, delta x
-  Four<A>* mine = slots + TT * CT;                        // [3][KC][128]: rates, r, da
-  Four<A>* into = mine + 3 * KC * 128;                    // b
-  Four<A>* from = into + TT * LN;                         // c
-  A* joined = reinterpret_cast<A*>(from + TT * LN);       // [4 warps][TT][2][NP]
-  A* dps = joined + 4 * TT * 2 * NP;                      // [TT][CT]
-  A* sums = dps + TT * CT;                                // [3][TT][PAD]: g b, p, a k
-  A* params = sums + 3 * TT * PAD;                        // [2][TT][CT]: dskip, ddt_bias
+  constexpr int COPIES = LD < 4 ? LD : 4;  // orders of 4 states
+  using I = Items<CT, TT>;
+  extern __shared__ __align__(32) unsigned char smem_raw[];
+  Four<A>* states = reinterpret_cast<Four<A>*>(smem_raw);  // b, then c: [TT][COPIES][LN]
+  Step<A>* slots = reinterpret_cast<Step<A>*>(states + 2 * TT * COPIES * LN);  // [TT][CT]
+  A* dps = reinterpret_cast<A*>(slots + TT * CT);                     // [TT][CT]
+  A* joined = dps + TT * CT;                                          // [4 warps][TT][2][NP]
+  A* sums = joined + 4 * TT * 2 * NP;                                 // [3][TT][PAD]: g b, p, a k
 
-  const Place w = place_of<CT>(p);
+  const Place w = place_of<CT>(p, p.segments, 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nl = lane % LN, dl = lane / LN;
-  const int c0 = warp * LD * KC + dl;  // the thread's channels: c0, c0 + LD, ...
-  for (int k = 0; k < KC; ++k) {
-    const int c = c0 + k * LD;
-    const bool in = c < w.width;
-    const int64_t d = w.d0 + c;
-    Four<A> r, s = {A(0), A(0), A(0), A(0)};
+  // The thread's channels of the tile and its 4 states: cl + (k ^ swap) and 4 nl + (j ^ order), by
+  // its lane (fold_swapped); b and c stand in shared memory in every order.
+  const int cl = (warp * LD + dl) * NC, swap = order_at<NC, LN>(nl), order = order_at<4, LD>(dl);
+  constexpr int KEPT = NC < LN ? NC : LN, OTHERS = LN / KEPT;  // lanes that share out channels, tokens
+  static_assert(KEPT == NC || LN == 1);
+  const Four<A>* my_b = states + dl % COPIES * LN + nl;
+  const Four<A>* my_c = my_b + TT * COPIES * LN;
+  const Two<A> none = two(A(0), A(0));
+  Two<A> ra[NC][2], r[NC][2], da[NC][2];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const bool in = cl + (k ^ swap) < w.width;
+    const int64_t d = w.d0 + cl + (k ^ swap);
+    A q[4], s[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int n = nl * 4 + j;
+      const int n = nl * 4 + (j ^ order);
       const bool live = in && n < p.states;
-      r.v[j] = live ? rate(static_cast<const A*>(p.a)[d * p.states + n]) : A(0);
-      if (live && p.d_final != nullptr)
-        s.v[j] = static_cast<const A*>(p.d_final)[(w.b * p.dim + d) * p.states + n];
+      q[j] = live ? rate(static_cast<const A*>(p.a)[d * p.states + n]) : A(0);
+      s[j] = live && p.d_final != nullptr
+                 ? static_cast<const A*>(p.d_final)[(w.b * p.dim + d) * p.states + n]
+                 : A(0);
     }
     if (in) {
+#pragma unroll 4
       for (int g = p.segments - 1; g > w.segment; --g) {  // the segments after this one
         const int64_t row = (w.b * p.segments + g) * p.dim + d;
         const A sum = static_cast<const A*>(p.seg_sum)[row];
-        const Four<A> e = static_cast<const Four<A>*>(p.seg_state)[row * LN + nl];
+        const Four<A> e = reorder(static_cast<const Four<A>*>(p.seg_state)[row * LN + nl], order);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s.v[j] = exp_2(sum * r.v[j]) * s.v[j] + e.v[j];
+        for (int j = 0; j < 4; ++j) s[j] = exp_2(sum * q[j]) * s[j] + e.v[j];
       }
     }
-    mine[(0 * KC + k) * 128 + threadIdx.x] = r;
-    mine[(1 * KC + k) * 128 + threadIdx.x] = s;
-    mine[(2 * KC + k) * 128 + threadIdx.x] = {A(0), A(0), A(0), A(0)};
+    ra[k][0] = two(q[0], q[1]), ra[k][1] = two(q[2], q[3]);
+    r[k][0] = two(s[0], s[1]), r[k][1] = two(s[2], s[3]);
+    da[k][0] = da[k][1] = none;
   }
-  for (int e = threadIdx.x; e < 2 * TT * CT; e += 128) params[e] = A(0);
 
-  const T* px = static_cast<const T*>(p.x) + w.b * p.xs[0] + w.d0;
-  const T* pd = static_cast<const T*>(p.dt) + w.b * p.dts[0] + w.d0;
-  const T* pg = static_cast<const T*>(p.gate) + w.b * p.gs[0] + w.d0;
-  const T* pq = static_cast<const T*>(p.dy) + w.b * p.dys[0] + w.d0;
-  const A* bias = static_cast<const A*>(p.dt_bias) + w.d0;
-  const A* skip = static_cast<const A*>(p.skip) + w.d0;
-  const int64_t to = w.b * p.length * p.dim + w.d0;
+  const int col = threadIdx.x % I::COLS * 4, row0 = threadIdx.x / I::COLS;
+  const int have = w.width - col;
+  const int64_t d0 = w.d0 + col;
+  const int64_t steps = w.count > w.t0 ? (w.count - w.t0 + TT - 1) / TT : 0;
+  const int64_t last = w.t0 + (steps - 1) * TT;  // the first token of the first step back in time
+  // pointers of the thread's first token of a step
+  const int64_t mine = last + row0;
+  const T* px = static_cast<const T*>(p.x) + w.b * p.xs[0] + d0 + mine * p.xs[1];
+  const T* pd = static_cast<const T*>(p.dt) + w.b * p.dts[0] + d0 + mine * p.dts[1];
+  const T* pg = static_cast<const T*>(p.gate) + w.b * p.gs[0] + d0 + mine * p.gs[1];
+  const T* pq = static_cast<const T*>(p.dy) + w.b * p.dys[0] + d0 + mine * p.dys[1];
+  const int64_t to = w.b * p.length * p.dim + d0;
   T *ox = static_cast<T*>(p.dx) + to, *od = static_cast<T*>(p.ddt) + to,
     *og = static_cast<T*>(p.dgate) + to;
-
-  auto stage = [&](auto g, int64_t t, int at, int c, bool in) {
-    constexpr int G = decltype(g)::value;
-    A dt[G], x[G], dp[G];
-    if (in) {
-      Group<T, G>::values(Group<T, G>::load(pd + t * p.dts[1] + c), dt);
-      Group<T, G>::values(Group<T, G>::load(px + t * p.xs[1] + c), x);
-      Group<T, G>::values(Group<T, G>::load(pq + t * p.dys[1] + c), dp);
-      if (p.gate != nullptr) {
-        A z[G];
-        Group<T, G>::values(Group<T, G>::load(pg + t * p.gs[1] + c), z);
+  const Four<A> bias = params4<A>(p.dt_bias, d0, have), skip = params4<A>(p.skip, d0, have);
+  const bool gated = p.gate != nullptr;
+  Raw4<T> xr[I::IT], dr[I::IT], zr[I::IT], qr[I::IT];
+  States<T, TT, LN, 2> bc;
+  A dskip[4] = {A(0), A(0), A(0), A(0)}, dbias[4] = {A(0), A(0), A(0), A(0)};
+  auto rows = [&](const T*& q, int64_t stride, Raw4<T>* raw, int left) {
 #pragma unroll
-        for (int j = 0; j < G; ++j) dp[j] *= z[j] * sigmoid_at<T, true>(z[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      A delta = A(0), u = A(0), q = A(0);
-      if (in) {
-        delta = dt[j];
-        if (p.dt_bias != nullptr) delta += bias[c + j];
-        if (p.softplus) delta = softplus(delta);
-        u = delta * x[j];
-        q = dp[j];
-      }
-      slots[at * CT + slot_of(c + j)] = {delta, delta, u, u};
-      dps[at * CT + c + j] = q;
-    }
+    for (int i = 0; i < I::IT; ++i)
+      raw[i] = load4(q + i * (I::ROWS * stride), i * I::ROWS < left ? have : 0, p.vec);
+    q -= TT * stride;
   };
-  auto finish = [&](auto g, int64_t t, int at, int c) {
-    constexpr int G = decltype(g)::value;
-    A gx[G], gd[G], gg[G];
-    if (t < w.count) {
-      A dt[G], x[G], z[G], dy[G];
-      Group<T, G>::values(Group<T, G>::load(px + t * p.xs[1] + c), x);
-      Group<T, G>::values(Group<T, G>::load(pd + t * p.dts[1] + c), dt);
-      if (p.gate != nullptr) {
-        Group<T, G>::values(Group<T, G>::load(pg + t * p.gs[1] + c), z);
-        Group<T, G>::values(Group<T, G>::load(pq + t * p.dys[1] + c), dy);
-      }
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const A delta = slots[at * CT + slot_of(c + j)].v[0], dp = dps[at * CT + c + j];
-        const A through = sums[at * PAD + c + j];
-        const A sk = p.skip != nullptr ? skip[c + j] : A(0);
-        const A pre = sums[(TT + at) * PAD + c + j] + sk * x[j];
-        gx[j] = delta * through + sk * dp;
-        gd[j] = A(kLn2) * sums[(2 * TT + at) * PAD + c + j] + x[j] * through;
-        if (p.softplus) {
-          const A v = p.dt_bias != nullptr ? dt[j] + bias[c + j] : dt[j];
-          gd[j] *= sigmoid_at<T, true>(v);
-        }
-        if (p.gate != nullptr) {
-          const A s = sigmoid_at<T, false>(z[j]);
-          gg[j] = dy[j] * pre * s * (A(1) + z[j] * (A(1) - s));
-        }
-        params[at * CT + c + j] += dp * x[j];
-        params[(TT + at) * CT + c + j] += gd[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < G; ++j) gx[j] = gd[j] = gg[j] = A(0);
-    }
-    Group<T, G>::store(ox + t * p.dim + c, gx);
-    Group<T, G>::store(od + t * p.dim + c, gd);
-    if (p.gate != nullptr) Group<T, G>::store(og + t * p.dim + c, gg);
+  // tokens from the thread's first one to the end of the valid ones and of the step
+  auto left_at = [&](int64_t t) {
+    return static_cast<int>((w.count - t < TT ? w.count - t : TT) - row0);
   };
-  auto each = [&](auto fn) {
-    if (p.vec) {
-      for (int e = threadIdx.x; e < TT * (CT / V); e += 128)
-        fn(std::integral_constant<int, V>{}, e / (CT / V), e % (CT / V) * V);
-    } else {
-      for (int e = threadIdx.x; e < TT * CT; e += 128)
-        fn(std::integral_constant<int, 1>{}, e / CT, e % CT);
-    }
+  bc.start(p, w, p.b, p.bs, p.c, p.cs, last);
+  auto fetch = [&](int64_t t) {
+    const int left = left_at(t);
+    rows(px, p.xs[1], xr, left);
+    rows(pd, p.dts[1], dr, left);
+    rows(pq, p.dys[1], qr, left);
+    if (gated) rows(pg, p.gs[1], zr, left);
+    bc.fetch(p, static_cast<int>(w.count - t < TT ? w.count - t : TT), -TT);
   };
 
-  const int64_t steps = w.t1 > w.t0 ? (w.t1 - w.t0 + TT - 1) / TT : 0;
   A* part_bc = static_cast<A*>(p.part_bc) + (w.tile * p.batch + w.b) * p.length * 2 * NP;
+  {  // what lies after the valid tokens
+    const A zero[4] = {A(0), A(0), A(0), A(0)};
+    for (int64_t t = (w.count > w.t0 ? w.count : w.t0) + row0; t < w.t1; t += I::ROWS) {
+      store4(ox + t * p.dim, zero, have, p.vec);
+      store4(od + t * p.dim, zero, have, p.vec);
+      if (gated) store4(og + t * p.dim, zero, have, p.vec);
+    }
+  }
+  if (steps > 0) fetch(last);
   for (int64_t i = steps - 1; i >= 0; --i) {
     const int64_t t = w.t0 + i * TT;
-    const bool any = t < w.count;
-    if (any) {
-      each([&](auto g, int at, int c) {
-        stage(g, t + at, at, c, t + at < w.count && c < w.width);
-      });
-      stage_states<T, TT, NP>(p, w, p.b, p.bs, t, &into[0].v[0]);
-      stage_states<T, TT, NP>(p, w, p.c, p.cs, t, &from[0].v[0]);
-      __syncthreads();
-      Two<A> db[TT][2], dc[TT][2];
-      const Two<A> none = two(A(0), A(0));
+    const int left = left_at(t);
+    Four<A> start[NC];
 #pragma unroll
-      for (int u = 0; u < TT; ++u) db[u][0] = db[u][1] = dc[u][0] = dc[u][1] = none;
+    for (int k = 0; k < NC; ++k) {
+      start[k] = {A(0), A(0), A(0), A(0)};
+      const int c = cl + (k ^ swap);
+      if (c < w.width)
+        start[k] = static_cast<const Four<A>*>(
+            p.check)[((w.b * ((p.length + 7) / 8) + t / 8) * p.dim + w.d0 + c) * LN + nl];
+    }
+    // kept for the results: x, the step's slope, dy silu'(gate)
+    A xk[I::IT][4], slope[I::IT][4], opening[I::IT][4];
+#pragma unroll
+    for (int q = 0; q < I::IT; ++q) {
+      const int row = row0 + q * I::ROWS;
+      if (I::ROWS * I::IT > TT && row >= TT) break;
+      Step<A> out[4];
+      Four<A> dp;
+      A dt[4], z[4];
+      Quad<T>::values(xr[q], xk[q]);
+      Quad<T>::values(dr[q], dt);
+      Quad<T>::values(qr[q], dp.v);
+      if (gated) Quad<T>::values(zr[q], z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        A delta = dt[j] + bias.v[j], sl = A(1), op = A(0);
+        if (p.softplus) delta = softplus(delta, &sl);
+        if (gated) {
+          const A sg = sigmoid_at<false>(z[j]);
+          op = dp.v[j] * (sg * (A(1) + z[j] * (A(1) - sg)));
+          dp.v[j] *= z[j] * sg;
+        }
+        out[j] = {delta, delta * xk[q][j]};
+        if (q * I::ROWS >= left) {
+          out[j] = {A(0), A(0)};
+          dp.v[j] = A(0);
+        }
+        slope[q][j] = sl, opening[q][j] = op;
+      }
+      Four<A>* st = reinterpret_cast<Four<A>*>(slots + row * CT + col);
+      st[0] = {out[0].delta, out[0].u, out[1].delta, out[1].u};
+      st[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
+      *reinterpret_cast<Four<A>*>(dps + row * CT + col) = dp;
+    }
+    bc.template store_orders<COPIES>(states);
+    if (i > 0) fetch(t - TT);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NC; ++k) start[k] = reorder(start[k], order);
+    Two<A> dat[NC][2];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) dat[k][0] = dat[k][1] = none;
 #pragma unroll 1
-      for (int k = 0; k < KC; ++k) {
-        const int c = c0 + k * LD;
-        const Four<A> rq = mine[(0 * KC + k) * 128 + threadIdx.x];
-        const Two<A> r0 = low(rq), r1 = high(rq);
-        Two<A> h[TT + 1][2], e[TT][2];
-        Four<A> start = {A(0), A(0), A(0), A(0)};
-        if (c < w.width)
-          start = static_cast<const Four<A>*>(
-              p.check)[((w.b * ((p.length + 7) / 8) + t / 8) * p.dim + w.d0 + c) * LN + nl];
-        h[0][0] = low(start);
-        h[0][1] = high(start);
+    for (int half = 1; half >= 0; --half) {
+      Two<A> h[SUB + 1][NC][2], e[SUB][NC][2];
 #pragma unroll
-        for (int u = 0; u < TT; ++u) {
-          const Four<A> q = slots[u * CT + slot_of(c)], bq = into[u * LN + nl];
-          e[u][0] = exp_2(mul(low(q), r0));
-          e[u][1] = exp_2(mul(low(q), r1));
-          h[u + 1][0] = fma(e[u][0], h[u][0], mul(high(q), low(bq)));
-          h[u + 1][1] = fma(e[u][1], h[u][1], mul(high(q), high(bq)));
-        }
-        const Four<A> sq = mine[(1 * KC + k) * 128 + threadIdx.x];
-        Two<A> s0 = low(sq), s1 = high(sq), a0 = none, a1 = none;
-        A through[TT], pre[TT], by_rate[TT];
+      for (int k = 0; k < NC; ++k) h[0][k][0] = low(start[k]), h[0][k][1] = high(start[k]);
+      if (half) {
 #pragma unroll
-        for (int u = TT - 1; u >= 0; --u) {
-          const Four<A> q = slots[u * CT + slot_of(c)], bq = into[u * LN + nl],
-                        cq = from[u * LN + nl];
-          const A dp = dps[u * CT + c];
-          const Two<A> dp2 = two(dp, dp);
-          const Two<A> g0 = fma(low(cq), dp2, s0), g1 = fma(high(cq), dp2, s1);
-          dc[u][0] = fma(dp2, h[u + 1][0], dc[u][0]);
-          dc[u][1] = fma(dp2, h[u + 1][1], dc[u][1]);
-          db[u][0] = fma(high(q), g0, db[u][0]);
-          db[u][1] = fma(high(q), g1, db[u][1]);
-          const Two<A> tb = fma(g1, high(bq), mul(g0, low(bq)));
-          const Two<A> tc = fma(h[u + 1][1], high(cq), mul(h[u + 1][0], low(cq)));
-          s0 = mul(e[u][0], g0);
-          s1 = mul(e[u][1], g1);
-          const Two<A> k0 = mul(s0, h[u][0]), k1 = mul(s1, h[u][1]);
-          const Two<A> ta = fma(r1, k1, mul(r0, k0));
-          a0 = fma(low(q), k0, a0);
-          a1 = fma(low(q), k1, a1);
-          through[u] = first(tb) + second(tb);
-          pre[u] = first(tc) + second(tc);
-          by_rate[u] = first(ta) + second(ta);
-        }
-        mine[(1 * KC + k) * 128 + threadIdx.x] = {first(s0), second(s0), first(s1), second(s1)};
-        Four<A> da = mine[(2 * KC + k) * 128 + threadIdx.x];
-        da.v[0] += first(a0), da.v[1] += second(a0), da.v[2] += first(a1), da.v[3] += second(a1);
-        mine[(2 * KC + k) * 128 + threadIdx.x] = da;
-        fold<TT, LN, 1>(through, lane);
-        fold<TT, LN, 1>(pre, lane);
-        fold<TT, LN, 1>(by_rate, lane);
-        constexpr int OWN = TT >= LN ? TT / LN : 1;
+        for (int u = 0; u < SUB; ++u) {
+          const Four<A> bq = my_b[u * COPIES * LN];
 #pragma unroll
-        for (int o = 0; o < OWN; ++o) {
-          const int u = TT >= LN ? nl * OWN + o : nl / (LN / TT);
-          sums[u * PAD + c] = through[o];
-          sums[(TT + u) * PAD + c] = pre[o];
-          sums[(2 * TT + u) * PAD + c] = by_rate[o];
+          for (int k = 0; k < NC; ++k) {
+            const Step<A> st = slots[u * CT + cl + (k ^ swap)];
+            const Two<A> d2 = two(st.delta, st.delta), u2 = two(st.u, st.u);
+            h[0][k][0] = fma(exp_2(mul(d2, ra[k][0])), h[0][k][0], mul(u2, low(bq)));
+            h[0][k][1] = fma(exp_2(mul(d2, ra[k][1])), h[0][k][1], mul(u2, high(bq)));
+          }
         }
       }
-      // over the warp's channels: value (token, b or c, state of the thread)
-      A v[TT * 8];
+      const int base = half * SUB;
+      Four<A> bq[SUB];
+      Step<A> st[SUB][NC];
 #pragma unroll
-      for (int u = 0; u < TT; ++u) {
-        v[u * 8 + 0] = first(db[u][0]), v[u * 8 + 1] = second(db[u][0]);
-        v[u * 8 + 2] = first(db[u][1]), v[u * 8 + 3] = second(db[u][1]);
-        v[u * 8 + 4] = first(dc[u][0]), v[u * 8 + 5] = second(dc[u][0]);
-        v[u * 8 + 6] = first(dc[u][1]), v[u * 8 + 7] = second(dc[u][1]);
+      for (int u = 0; u < SUB; ++u) {
+        bq[u] = my_b[(base + u) * COPIES * LN];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          st[u][k] = slots[(base + u) * CT + cl + (k ^ swap)];
+          const Two<A> d2 = two(st[u][k].delta, st[u][k].delta), u2 = two(st[u][k].u, st[u][k].u);
+          e[u][k][0] = exp_2(mul(d2, ra[k][0]));
+          e[u][k][1] = exp_2(mul(d2, ra[k][1]));
+          h[u + 1][k][0] = fma(e[u][k][0], h[u][k][0], mul(u2, low(bq[u])));
+          h[u + 1][k][1] = fma(e[u][k][1], h[u][k][1], mul(u2, high(bq[u])));
+        }
       }
-      fold<TT * 8, LD, LN>(v, lane);
-      constexpr int OWN = TT * 8 / LD;
+      A through[SUB * NC], pre[SUB * NC], by_rate[SUB * NC], v[SUB * 8];
+#pragma unroll
+      for (int u = SUB - 1; u >= 0; --u) {
+        const Four<A> cq = my_c[(base + u) * COPIES * LN];
+        A dp[NC];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) dp[k] = dps[(base + u) * CT + cl + (k ^ swap)];
+        Two<A> db[2], dc[2];
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          const Two<A> q2 = two(dp[k], dp[k]), d2 = two(st[u][k].delta, st[u][k].delta),
+                       u2 = two(st[u][k].u, st[u][k].u);
+          Two<A> g[2], kp[2];
+          const Two<A> bb[2] = {low(bq[u]), high(bq[u])}, cc[2] = {low(cq), high(cq)};
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            g[m] = fma(cc[m], q2, r[k][m]);
+            db[m] = k == 0 ? mul(u2, g[m]) : fma(u2, g[m], db[m]);
+            dc[m] = k == 0 ? mul(q2, h[u + 1][k][m]) : fma(q2, h[u + 1][k][m], dc[m]);
+            r[k][m] = mul(e[u][k][m], g[m]);
+            kp[m] = mul(r[k][m], h[u][k][m]);
+            dat[k][m] = fma(d2, kp[m], dat[k][m]);
+          }
+          const Two<A> tb = fma(g[1], bb[1], mul(g[0], bb[0]));
+          const Two<A> tc = fma(h[u + 1][k][1], cc[1], mul(h[u + 1][k][0], cc[0]));
+          const Two<A> ta = fma(ra[k][1], kp[1], mul(ra[k][0], kp[0]));
+          through[u * NC + k] = first(tb) + second(tb);
+          pre[u * NC + k] = first(tc) + second(tc);
+          by_rate[u * NC + k] = first(ta) + second(ta);
+        }
+        v[u * 8 + 0] = first(db[0]), v[u * 8 + 1] = second(db[0]);
+        v[u * 8 + 2] = first(db[1]), v[u * 8 + 3] = second(db[1]);
+        v[u * 8 + 4] = first(dc[0]), v[u * 8 + 5] = second(dc[0]);
+        v[u * 8 + 6] = first(dc[1]), v[u * 8 + 7] = second(dc[1]);
+      }
+      // over the states
+      fold_swapped<SUB, NC, LN, 1>(through);
+      fold_swapped<SUB, NC, LN, 1>(pre);
+      fold_swapped<SUB, NC, LN, 1>(by_rate);
+      fold<SUB, OTHERS, KEPT>(through, lane);
+      fold<SUB, OTHERS, KEPT>(pre, lane);
+      fold<SUB, OTHERS, KEPT>(by_rate, lane);
+      constexpr int OWN = SUB >= OTHERS ? SUB / OTHERS : 1, SAME = OTHERS > SUB ? OTHERS / SUB : 1;
 #pragma unroll
       for (int o = 0; o < OWN; ++o) {
-        const int at = dl * OWN + o;
-        joined[((warp * TT + at / 8) * 2 + at / 4 % 2) * NP + nl * 4 + at % 4] = v[o];
+        A* q = sums + (base + nl / KEPT / SAME * OWN + o) * PAD + cl + (LN == 1 ? 0 : swap);
+        q[0] = through[o];
+        q[TT * PAD] = pre[o];
+        q[2 * TT * PAD] = by_rate[o];
       }
-      __syncthreads();
-    }
-    each([&](auto g, int at, int c) {
-      if (t + at < w.t1 && c < w.width) finish(g, t + at, at, c);
-    });
-    for (int e = threadIdx.x; e < TT * 2 * NP; e += 128) {
-      if (t + e / (2 * NP) >= w.t1) continue;
-      A s = A(0);
-      if (any) {
+      // over the warp's channels: runs of the thread's 4 states by token, and b or c
+      fold_swapped<SUB * 2, 4, LD, LN>(v);
+      constexpr int LEFT = 4 / COPIES;                    // states of each run that a lane keeps
+      constexpr int FAR = LD / COPIES;                    // lanes that share out the runs
+      fold<SUB * 2, FAR, LN * COPIES>(v, lane);           // (FAR > 1 only where LEFT is 1)
+      constexpr int RUNS = SUB * 2 / FAR;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s += joined[q * TT * 2 * NP + e];
+      for (int o = 0; o < RUNS; ++o) {
+        const int run = dl / COPIES * RUNS + o;
+        A* q = joined + ((warp * TT + base) * 2 + run) * NP + nl * 4;
+#pragma unroll
+        for (int j = 0; j < LEFT; ++j) q[j ^ order] = v[o * LEFT + j];
       }
-      part_bc[t * 2 * NP + e] = s;
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      da[k][0] = add(da[k][0], dat[k][0]), da[k][1] = add(da[k][1], dat[k][1]);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < I::IT; ++q) {
+      const int row = row0 + q * I::ROWS;
+      if (q * I::ROWS >= left) break;
+      const Four<A> th = *reinterpret_cast<const Four<A>*>(sums + row * PAD + col);
+      const Four<A> pr = *reinterpret_cast<const Four<A>*>(sums + (TT + row) * PAD + col);
+      const Four<A> br = *reinterpret_cast<const Four<A>*>(sums + (2 * TT + row) * PAD + col);
+      const Four<A> dp = *reinterpret_cast<const Four<A>*>(dps + row * CT + col);
+      const Four<A>* st = reinterpret_cast<const Four<A>*>(slots + row * CT + col);
+      const Four<A> s0 = st[0], s1 = st[1];
+      const A delta[4] = {s0.v[0], s0.v[2], s1.v[0], s1.v[2]};
+      A gx[4], gd[4], gg[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        gx[j] = delta[j] * th.v[j] + skip.v[j] * dp.v[j];
+        gd[j] = (A(kLn2) * br.v[j] + xk[q][j] * th.v[j]) * slope[q][j];
+        gg[j] = opening[q][j] * (pr.v[j] + skip.v[j] * xk[q][j]);
+        dskip[j] += dp.v[j] * xk[q][j];
+        dbias[j] += gd[j];
+      }
+      store4(ox + (t + row) * p.dim, gx, have, p.vec);
+      store4(od + (t + row) * p.dim, gd, have, p.vec);
+      if (gated) store4(og + (t + row) * p.dim, gg, have, p.vec);
+    }
+    // (tokens past the valid ones have no part: scan_bc_kernel leaves them out)
+    for (int e = threadIdx.x; e < TT * 2 * LN; e += 128) {
+      if (t + e / (2 * LN) >= w.count) continue;
+      Four<A> s = reinterpret_cast<const Four<A>*>(joined)[e];
+#pragma unroll
+      for (int q = 1; q < 4; ++q) {
+        const Four<A> f = reinterpret_cast<const Four<A>*>(joined)[q * TT * 2 * LN + e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s.v[j] += f.v[j];
+      }
+      reinterpret_cast<Four<A>*>(part_bc + t * 2 * NP)[e] = s;
     }
     __syncthreads();
   }
 
-  if (steps == 0) __syncthreads();
   const int64_t row = w.b * p.segments + w.segment;
-  for (int k = 0; k < KC; ++k) {
-    const int c = c0 + k * LD;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int c = cl + (k ^ swap);
     if (c >= w.width) continue;
     const int64_t d = w.d0 + c;
-    static_cast<Four<A>*>(p.part_a)[(row * p.dim + d) * LN + nl] =
-        mine[(2 * KC + k) * 128 + threadIdx.x];
+    static_cast<Four<A>*>(p.part_a)[(row * p.dim + d) * LN + nl] = reorder(
+        Four<A>{first(da[k][0]), second(da[k][0]), first(da[k][1]), second(da[k][1])}, order);
     if (w.segment == 0 && p.d_initial != nullptr) {
-      const Four<A> s = mine[(1 * KC + k) * 128 + threadIdx.x];
+      const A s[4] = {first(r[k][0]), second(r[k][0]), first(r[k][1]), second(r[k][1])};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (nl * 4 + j < p.states)
-          static_cast<A*>(p.d_initial)[(w.b * p.dim + d) * p.states + nl * 4 + j] = s.v[j];
+      for (int j = 0; j < 4; ++j) {
+        const int n = nl * 4 + (j ^ order);
+        if (n < p.states) static_cast<A*>(p.d_initial)[(w.b * p.dim + d) * p.states + n] = s[j];
+      }
     }
   }
+  // dskip and ddt_bias over the block's tokens, in the order of the threads' rows
+  constexpr int ROWS = I::ROWS < TT ? I::ROWS : TT;
+  A* shares = sums;  // [2][ROWS][CT]
+  if (row0 < ROWS) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      shares[row0 * CT + col + j] = dskip[j];
+      shares[(ROWS + row0) * CT + col + j] = dbias[j];
+    }
+  }
+  __syncthreads();
   for (int e = threadIdx.x; e < 2 * CT; e += 128) {
     const int which = e / CT, c = e % CT;
     if (c >= w.width) continue;
     A s = A(0);
 #pragma unroll
-    for (int u = 0; u < TT; ++u) s += params[(which * TT + u) * CT + c];
+    for (int u = 0; u < ROWS; ++u) s += shares[(which * ROWS + u) * CT + c];
     static_cast<A*>(p.part_ch)[(row * 2 + which) * p.dim + w.d0 + c] = s;
   }
 }
-template <typename A> constexpr size_t scan_bwd_smem(int ln, int kc) {
-  const int ct = 4 * (32 / ln) * kc, np = 4 * ln, tt = kScanCheck;
-  return sizeof(A) * (4 * (size_t(tt) * ct + 3 * kc * 128 + 2 * tt * ln) + 4 * tt * 2 * np +
-                      tt * ct + 3 * tt * (ct + 8) + 2 * tt * ct);
+template <typename A> constexpr size_t scan_bwd_smem(int ln, int nc) {
+  const size_t ct = 4 * (32 / ln) * nc, np = 4 * ln, tt = kScanCheck;
+  const size_t copies = 32 / ln < 4 ? 32 / ln : 4;
+  return sizeof(A) * (2 * tt * np * copies + 3 * tt * ct + 4 * tt * 2 * np + 3 * tt * (ct + 8));
 }
 
 // ------------------------------------------------------------------------------ single tokens
@@ -690,7 +959,7 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     x = to_acc(static_cast<const T*>(p.x)[b * p.xs[0] + d]);
     A delta = to_acc(static_cast<const T*>(p.dt)[b * p.dts[0] + d]);
     if (p.dt_bias != nullptr) delta += static_cast<const A*>(p.dt_bias)[d];
-    if (p.softplus) delta = softplus(delta);
+    if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
     const int64_t group = d / p.per;
     const T* pb = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
     const T* pc = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
@@ -726,7 +995,7 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     if (p.skip != nullptr) y += static_cast<const A*>(p.skip)[d] * x;
     if (p.gate != nullptr) {
       const A z = to_acc(static_cast<const T*>(p.gate)[b * p.gs[0] + d]);
-      y *= z * sigmoid_at<T, false>(z);
+      y *= z * sigmoid_at<sizeof(T) == 2>(z);
     }
   }
   static_cast<T*>(p.y)[b * p.dim + d] = from_acc<T>(y);
@@ -744,8 +1013,8 @@ template <typename F> int with_lanes(int lanes, F fn) {
     default: return FDWT_ERR_INVALID;
   }
 }
-inline int scan_grid(const ScanArgs& p, unsigned* grid) {
-  const int64_t blocks = p.tiles * p.groups * p.segments * p.batch;
+inline int scan_grid(const ScanArgs& p, int segments, unsigned* grid) {
+  const int64_t blocks = p.tiles * p.groups * segments * p.batch;
   if (blocks > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   *grid = static_cast<unsigned>(blocks);
   return FDWT_OK;
@@ -755,7 +1024,7 @@ template <typename T, int MODE> int scan_launch(const ScanArgs& p, int lanes, cu
   return with_lanes(lanes, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
     unsigned grid;
-    int st = scan_grid(p, &grid);
+    int st = scan_grid(p, MODE == MAIN ? p.segments : p.segments - 1, &grid);
     if (st == FDWT_OK) st = pre_launch(stream);
     if (st != FDWT_OK) return st;
     scan_fwd_kernel<T, LN, scan_fwd_channels(LN), MODE><<<grid, 128, 0, stream>>>(p);
@@ -773,27 +1042,34 @@ int scan_states(const ScanArgs& p, int lanes, bool reverse, cudaStream_t stream)
   return reverse ? scan_launch<T, REVERSE>(p, lanes, stream) : scan_launch<T, STATES>(p, lanes, stream);
 }
 
-template <typename T> int scan_backward(const ScanArgs& p, int lanes, bool wide, cudaStream_t stream) {
+template <typename T> int scan_backward(const ScanArgs& p, int lanes, cudaStream_t stream) {
   using A = typename AccOf<T>::type;
   return with_lanes(lanes, [&](auto ln) {
-    constexpr int LN = decltype(ln)::value;
-    auto launch = [&](auto kc) {
-      constexpr int KC = decltype(kc)::value;
-      auto kernel = scan_bwd_kernel<T, LN, KC>;
-      unsigned grid;
-      int st = scan_grid(p, &grid);
-      if (st == FDWT_OK) st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
-      if (st == FDWT_OK) st = pre_launch(stream);
-      if (st != FDWT_OK) return st;
-      kernel<<<grid, 128, scan_bwd_smem<A>(LN, KC), stream>>>(p);
-      return launch_status();
-    };
-    constexpr int narrow = scan_bwd_channels(LN, false), broad = scan_bwd_channels(LN, true);
-    if constexpr (narrow != broad && sizeof(A) == 4) {
-      if (wide) return launch(std::integral_constant<int, broad>{});
-    }
-    return launch(std::integral_constant<int, narrow>{});
+    constexpr int LN = decltype(ln)::value, NC = scan_bwd_channels(LN, sizeof(A) == 8);
+    auto kernel = scan_bwd_kernel<T, LN, NC>;
+    unsigned grid;
+    int st = scan_grid(p, p.segments, &grid);
+    if (st == FDWT_OK) st = allow_max_dynamic_smem(reinterpret_cast<const void*>(kernel));
+    if (st == FDWT_OK) st = pre_launch(stream);
+    if (st != FDWT_OK) return st;
+    kernel<<<grid, 128, scan_bwd_smem<A>(LN, NC), stream>>>(p);
+    return launch_status();
   });
+}
+
+template <typename T> int64_t scan_resident(int lanes, bool backward) {
+  using A = typename AccOf<T>::type;
+  int blocks = 1;
+  with_lanes(lanes, [&](auto ln) {
+    constexpr int LN = decltype(ln)::value, NC = scan_bwd_channels(LN, sizeof(A) == 8);
+    if (!backward)
+      return occupancy(reinterpret_cast<const void*>(
+                           scan_fwd_kernel<T, LN, scan_fwd_channels(LN), MAIN>), 128, 0, &blocks);
+    const void* kernel = reinterpret_cast<const void*>(scan_bwd_kernel<T, LN, NC>);
+    const int st = allow_max_dynamic_smem(kernel);
+    return st != FDWT_OK ? st : occupancy(kernel, 128, scan_bwd_smem<A>(LN, NC), &blocks);
+  });
+  return int64_t(blocks < 1 ? 1 : blocks) * sm_count();
 }
 
 template <typename T>
@@ -814,7 +1090,8 @@ int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool, 
 #define FDWT_SCAN_TYPE(T)                                                            \
   template int scan_forward<T>(const ScanArgs&, int, cudaStream_t);                  \
   template int scan_states<T>(const ScanArgs&, int, bool, cudaStream_t);             \
-  template int scan_backward<T>(const ScanArgs&, int, bool, cudaStream_t);           \
+  template int scan_backward<T>(const ScanArgs&, int, cudaStream_t);                 \
+  template int64_t scan_resident<T>(int, bool);                                      \
   template int scan_step<T>(const ScanArgs&, int, const int32_t*, int64_t, void*, cudaStream_t);
 
 }  // namespace fdwt
