@@ -39,6 +39,26 @@ __device__ __forceinline__ typename AccOf<T>::type param(const void* p, bool f32
   return to_acc(static_cast<const T*>(p)[i]);
 }
 
+// The taps of V channels, contiguous in memory (`whole`: on a boundary of V elements).
+template <typename T, int V, int W, typename A>
+__device__ __forceinline__ void load_taps(const void* weight, bool f32, bool whole, int64_t c,
+                                          A (&w)[W][V]) {
+  if (whole && !(sizeof(T) == 2 && f32)) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      A x[V];
+      Group<T, V>::values(Group<T, V>::load(static_cast<const T*>(weight) + c * W + i * V), x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[(i * V + j) % W][(i * V + j) / W] = x[j];
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i][j] = param<T>(weight, f32, (c + j) * W + i);
+}
+
 __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, int64_t length) {
   if (lengths == nullptr) return length;
   const int64_t n = lengths[b];
@@ -62,13 +82,14 @@ __device__ __forceinline__ void input_at(const T* x, int64_t xs_t, const T* befo
 }
 
 // Thread: V channels, `run` tokens.  Threads go over channels first, then runs, then sequences.
+// The next U tokens are loaded before the current ones are worked out.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128)
 conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                 const void* __restrict__ bias, const T* __restrict__ initial,
                 const int32_t* __restrict__ lengths, T* __restrict__ y,
                 T* __restrict__ final_state, int64_t batch, int64_t length, int64_t dim,
-                int64_t xs_b, int64_t xs_t, int run, bool silu, bool param_f32) {
+                int64_t xs_b, int64_t xs_t, int run, bool silu, bool param_f32, bool whole) {
   using A = typename AccOf<T>::type;
   using G = Group<T, V>;
   constexpr int U = 4;  // tokens whose loads are issued together
@@ -78,7 +99,7 @@ conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
   if (b >= batch) return;
   const int64_t count = tokens_of(lengths, b, length);
   x += b * xs_b + c;
-  y += (b * length) * dim + c;
+  y += b * length * dim + c;
   const T* before = initial == nullptr ? nullptr : initial + b * (W - 1) * dim + c;
   if (final_state != nullptr && k == 0) {
     for (int i = 0; i < W - 1; ++i) {
@@ -87,57 +108,65 @@ conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
       G::store(final_state + (b * (W - 1) + i) * dim + c, v);
     }
   }
-  A w[W][V], at[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) w[i][j] = param<T>(weight, param_f32, (c + j) * W + i);
-    at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
-  }
   const int64_t t0 = k * run, t1 = t0 + run < length ? t0 + run : length;
+  const int valid = static_cast<int>((count < t1 ? count : t1) - t0);  // tokens of the run that count
+  const int all = static_cast<int>(t1 - t0);
+  x += t0 * xs_t;
+  y += t0 * dim;
+  typename G::Raw next[U];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < valid) next[u] = G::load(x + (t + u) * xs_t);
+  };
+  fetch(0);
+  A w[W][V], at[V];
+  load_taps<T, V, W>(weight, param_f32, whole, c, w);
+#pragma unroll
+  for (int j = 0; j < V; ++j) at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
   A win[W - 1 + U][V];  // the inputs of tokens t - W + 1 ... t + U - 1
 #pragma unroll
   for (int i = 0; i < W - 1; ++i)
-    input_at<T, V>(x, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i]);
-  for (int64_t t = t0; t < t1; t += U) {
-    typename G::Raw raw[U];
+    input_at<T, V>(x - t0 * xs_t, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i]);
+  for (int t = 0; t < valid; t += U) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t + u < count) raw[u] = G::load(x + (t + u) * xs_t);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t + u >= t1) break;
+    for (int u = 0; u < U; ++u) G::values(next[u], win[W - 1 + u]);  // (past the end: not used)
+    if (t + U < valid) fetch(t + U);
+    auto token = [&](int u) {
       A p[V];
-      if (t + u < count) {
-        G::values(raw[u], win[W - 1 + u]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          p[j] = at[j];
+      for (int j = 0; j < V; ++j) {
+        p[j] = at[j];
 #pragma unroll
-          for (int i = 0; i < W; ++i) p[j] += w[i][j] * win[u + i][j];
-        }
-        if (silu) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) p[j] *= sigmoid<T>(p[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = win[W - 1 + u][j] = A(0);
+        for (int i = 0; i < W; ++i) p[j] += w[i][j] * win[u + i][j];
+        if (silu) p[j] *= sigmoid<T>(p[j]);
       }
       G::store(y + (t + u) * dim, p);
+    };
+    if (t + U <= valid) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) token(u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t + u < valid) token(u);
     }
 #pragma unroll
     for (int i = 0; i < W - 1; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) win[i][j] = win[i + U][j];
   }
+  A none[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) none[j] = A(0);
+  for (int t = valid > 0 ? valid : 0; t < all; ++t) G::store(y + t * dim, none);
 }
 
-// Backward.  A block is 32 threads of channels by 8 runs of tokens; a thread walks its run and the
+// Backward.  A block is 32 threads of channels by 4 runs of tokens; a thread walks its run and the
 // W-1 tokens after it (whose dp its last inputs need), so dx is written once.  dw and db are summed
 // in registers over the run, joined over the block's runs in shared memory and written as one
 // partial row (dim x (W + 1)) a block row, added in a fixed order by conv_params_kernel.
-constexpr int kBwdLanes = 32, kBwdRuns = 8;
+constexpr int kBwdLanes = 32, kBwdRuns = 4;
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBwdLanes* kBwdRuns)
 conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
@@ -146,7 +175,7 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                 const T* __restrict__ d_final, T* __restrict__ dx, T* __restrict__ d_initial,
                 typename AccOf<T>::type* __restrict__ partial, int64_t length, int64_t dim,
                 int64_t xs_b, int64_t xs_t, int64_t ds_b, int64_t ds_t, int run, int64_t rows,
-                int64_t columns, bool silu, bool param_f32) {
+                int64_t columns, bool silu, bool param_f32, bool whole) {
   using A = typename AccOf<T>::type;
   using G = Group<T, V>;
   __shared__ A joined[kBwdRuns][kBwdLanes * V + 1];
@@ -162,20 +191,20 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
   dy += b * ds_b + c;
   const T* before = initial == nullptr ? nullptr : initial + b * (W - 1) * dim + c;
   A w[W][V], at[V], dw[W][V], db[V];
+  load_taps<T, V, W>(weight, param_f32, whole, c, w);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      w[i][j] = param<T>(weight, param_f32, (c + j) * W + i);
-      dw[i][j] = A(0);
-    }
+    for (int i = 0; i < W; ++i) dw[i][j] = A(0);
     at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
     db[j] = A(0);
   }
   const int64_t t0 = k * run;
-  const int64_t t1 = t0 + run < length ? t0 + run : length;  // (t1 <= t0: no tokens)
   const bool first = k == 0;
-  if (in && (t0 < t1 || first)) {
+  // relative to the run's first token: its tokens, and the valid ones of the sequence
+  const int all = static_cast<int>(length - t0 < run ? length - t0 : run);
+  const int valid = static_cast<int>(count - t0 < all + W - 1 ? count - t0 : all + W - 1);
+  if (in && (all > 0 || first)) {
     A win[W][V], dp[W][V];  // inputs t-W+1 ... t and gradients of the sums p of the same tokens
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
@@ -184,20 +213,31 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
       for (int j = 0; j < V; ++j) dp[i + 1][j] = A(0);
     }
     constexpr int U = 4;
-    const int64_t end = t1 + W - 1;
-    for (int64_t s = t0; s < end; s += U) {
-      typename G::Raw rx[U], rd[U];
+    const int end = all + W - 1, begin = first && d_initial != nullptr ? -(W - 1) : 0;
+    const T *px = x + t0 * xs_t, *pd = dy + t0 * ds_t;
+    T* out = dx + (b * length + t0) * dim + c;
+    typename G::Raw nx[U], nd[U];
+    auto fetch = [&](int t) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (s + u < count && s + u < end) {
-          rx[u] = G::load(x + (s + u) * xs_t);
-          rd[u] = G::load(dy + (s + u) * ds_t);
+        nx[u] = nd[u] = typename G::Raw{};
+        if (t + u < valid) {
+          nx[u] = G::load(px + u * xs_t);
+          nd[u] = G::load(pd + u * ds_t);
         }
       }
+      px += U * xs_t;
+      pd += U * ds_t;
+    };
+    fetch(0);
+    for (int s = 0; s < end; s += U) {
+      typename G::Raw rx[U], rd[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) rx[u] = nx[u], rd[u] = nd[u];
+      if (s + U < end) fetch(s + U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t t = s + u;
-        if (t >= end) break;
+        const int t = s + u;
 #pragma unroll
         for (int i = 0; i < W - 1; ++i)
 #pragma unroll
@@ -205,52 +245,42 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
             win[i][j] = win[i + 1][j];
             dp[i][j] = dp[i + 1][j];
           }
-        if (t < count) {
-          G::values(rx[u], win[W - 1]);
-          G::values(rd[u], dp[W - 1]);
-          if (silu) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              A p = at[j];
-#pragma unroll
-              for (int i = 0; i < W; ++i) p += w[i][j] * win[i][j];
-              const A g = sigmoid<T>(p);
-              dp[W - 1][j] *= g * (A(1) + p * (A(1) - g));
-            }
-          }
-          if (t < t1) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              db[j] += dp[W - 1][j];
-#pragma unroll
-              for (int i = 0; i < W; ++i) dw[i][j] += dp[W - 1][j] * win[i][j];
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) win[W - 1][j] = dp[W - 1][j] = A(0);
-        }
-        // all gradients that input t - W + 1 reaches are in dp[0 .. W-1] now
-        const int64_t to = t - (W - 1);
-        if (to < t0 && !(first && d_initial != nullptr)) continue;
+        G::values(rx[u], win[W - 1]);
+        G::values(rd[u], dp[W - 1]);
+        // (chosen, not multiplied by zero: what the window holds may be no number)
+        const bool counts = t < valid, own = t < all;
         A g[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+          if (silu) {
+            A p = at[j];
+#pragma unroll
+            for (int i = 0; i < W; ++i) p += w[i][j] * win[i][j];
+            const A q = sigmoid<T>(p);
+            dp[W - 1][j] *= q * (A(1) + p * (A(1) - q));
+          }
+          if (!counts) dp[W - 1][j] = A(0);
+          const A d = own ? dp[W - 1][j] : A(0);
+          db[j] += d;
           g[j] = A(0);
 #pragma unroll
-          for (int i = 0; i < W; ++i) g[j] += w[W - 1 - i][j] * dp[i][j];
+          for (int i = 0; i < W; ++i) {
+            dw[i][j] += d * win[i][j];
+            g[j] += w[W - 1 - i][j] * dp[i][j];
+          }
         }
-        if (d_final != nullptr && to >= count - (W - 1) && to < count) {
+        // g: the gradient of input t - W + 1, all of whose dp are there now
+        const int to = t - (W - 1);
+        if (to < begin || t >= end) continue;
+        const int64_t behind = count - t0 - to;  // 1: the last valid token
+        if (d_final != nullptr && behind >= 1 && behind <= W - 1) {
           A f[V];
-          G::values(G::load(d_final + (b * (W - 1) + to - count + W - 1) * dim + c), f);
+          G::values(G::load(d_final + (b * (W - 1) + W - 1 - behind) * dim + c), f);
 #pragma unroll
           for (int j = 0; j < V; ++j) g[j] += f[j];
         }
-        if (to >= 0) {
-          if (dx != nullptr) G::store(dx + (b * length + to) * dim + c, g);
-        } else {
-          G::store(d_initial + (b * (W - 1) + to + W - 1) * dim + c, g);
-        }
+        if (to < 0) G::store(d_initial + (b * (W - 1) + to + W - 1) * dim + c, g);
+        else if (dx != nullptr) G::store(out + to * dim, g);
       }
     }
   }
@@ -372,9 +402,9 @@ template <typename F> int with_width(int width, F fn) {
 }
 
 template <typename T, int V> int conv_forward_v(const ConvCall& c, int width, void* y, void* fin) {
-  // runs of 32 tokens where that leaves threads enough for every multiprocessor, else 8
-  const int64_t threads32 = c.batch * cdiv(c.length, 32) * (c.dim / V);
-  const int run = threads32 >= int64_t(sm_count()) * 512 ? 32 : 8;
+  // runs as long as leaves 512 threads for every multiprocessor, 8 to 64 tokens
+  int run = 64;
+  while (run > 8 && c.batch * cdiv(c.length, run) * (c.dim / V) < int64_t(sm_count()) * 512) run /= 2;
   const int64_t threads = c.batch * imax(1, cdiv(c.length, run)) * (c.dim / V);
   const int64_t grid = cdiv(threads, 128);
   if (grid > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
@@ -384,7 +414,7 @@ template <typename T, int V> int conv_forward_v(const ConvCall& c, int width, vo
     conv_fwd_kernel<T, V, decltype(w)::value><<<static_cast<unsigned>(grid), 128, 0, c.stream>>>(
         static_cast<const T*>(c.x), c.weight, c.bias, static_cast<const T*>(c.initial), c.lengths,
         static_cast<T*>(y), static_cast<T*>(fin), c.batch, c.length, c.dim, c.xs_b, c.xs_t, run,
-        c.silu, c.param_f32);
+        c.silu, c.param_f32, grouped<T>(V, c.dim, {}, {c.weight}));
     return launch_status();
   });
 }
@@ -395,11 +425,11 @@ struct BwdRuns {
   int64_t rows;
 };
 inline BwdRuns bwd_runs(int64_t batch, int64_t length, int64_t dim, int v) {
-  int run = 32;
+  int run = 64;
   while (run > 8 && batch * cdiv(length, run) * cdiv(dim, v) < int64_t(sm_count()) * 512) run /= 2;
   return {run, imax(1, cdiv(length, int64_t(run) * kBwdRuns))};
 }
-template <typename T> constexpr int bwd_group = sizeof(T) == 8 ? 2 : 4;
+template <typename T> constexpr int bwd_group = sizeof(T) == 8 ? 1 : 2;
 
 template <typename T, int V>
 int conv_backward_v(const ConvCall& c, int width, const void* dy, const void* d_final, void* dx,
@@ -418,7 +448,8 @@ int conv_backward_v(const ConvCall& c, int width, const void* dy, const void* d_
             static_cast<const T*>(c.x), c.weight, c.bias, static_cast<const T*>(c.initial),
             c.lengths, static_cast<const T*>(dy), static_cast<const T*>(d_final),
             static_cast<T*>(dx), static_cast<T*>(d_initial), partial, c.length, c.dim, c.xs_b,
-            c.xs_t, c.ds_b, c.ds_t, r.run, r.rows, columns, c.silu, c.param_f32);
+            c.xs_t, c.ds_b, c.ds_t, r.run, r.rows, columns, c.silu, c.param_f32,
+            grouped<T>(V, c.dim, {}, {c.weight}));
     return launch_status();
   });
   if (st != FDWT_OK || partial == nullptr) return st;
@@ -478,7 +509,7 @@ extern "C" int fdwt_causal_conv1d_forward(const fdwt_conv1d_desc* desc, const vo
 
 extern "C" size_t fdwt_causal_conv1d_backward_workspace(const fdwt_conv1d_desc* desc) {
   if (!conv_ok(desc) || desc->batch == 0) return 0;
-  const int v = desc->dtype == FDWT_F64 ? 2 : 4;
+  const int v = desc->dtype == FDWT_F64 ? 1 : 2;
   const BwdRuns r = bwd_runs(desc->batch, desc->length, desc->dim, v);
   return size_t(desc->batch * r.rows) * (desc->width + 1) * desc->dim *
          (desc->dtype == FDWT_F64 ? 8 : 4);
