@@ -10,6 +10,7 @@
 // in registers, so that every input is read once (and W-1 of a run's neighbours, from L2) and the
 // loads of several tokens are in flight.  Sums are 32 bits (64 for fp64); y and the gradients are
 // rounded once.
+#include "pairs.cuh"
 #include "row_groups.cuh"
 
 namespace fdwt {
@@ -31,6 +32,35 @@ template <typename T, typename A> __device__ __forceinline__ A sigmoid(A p) {
   else return 1.0 / (1.0 + exp(-p));
 }
 
+// V channels' values: pairs of them, or one.
+template <typename A, int V> struct Channels {
+  using E = std::conditional_t<V == 1, A, Two<A>>;
+  static constexpr int M = V == 1 ? 1 : V / 2;
+  E e[M];
+  __device__ __forceinline__ void set(const A* x) {
+    if constexpr (V == 1) {
+      e[0] = x[0];
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m) e[m] = two(x[2 * m], x[2 * m + 1]);
+    }
+  }
+  __device__ __forceinline__ void get(A* x) const {
+    if constexpr (V == 1) {
+      x[0] = e[0];
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m) x[2 * m] = first(e[m]), x[2 * m + 1] = second(e[m]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+    A zero[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) zero[j] = A(0);
+    set(zero);
+  }
+};
+
 // One parameter of the rows' type or of 32 bits.
 template <typename T>
 __device__ __forceinline__ typename AccOf<T>::type param(const void* p, bool f32, int64_t i) {
@@ -42,7 +72,8 @@ __device__ __forceinline__ typename AccOf<T>::type param(const void* p, bool f32
 // The taps of V channels, contiguous in memory (`whole`: on a boundary of V elements).
 template <typename T, int V, int W, typename A>
 __device__ __forceinline__ void load_taps(const void* weight, bool f32, bool whole, int64_t c,
-                                          A (&w)[W][V]) {
+                                          Channels<A, V> (&taps)[W]) {
+  A w[W][V];
   if (whole && !(sizeof(T) == 2 && f32)) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -51,12 +82,23 @@ __device__ __forceinline__ void load_taps(const void* weight, bool f32, bool who
 #pragma unroll
       for (int j = 0; j < V; ++j) w[(i * V + j) % W][(i * V + j) / W] = x[j];
     }
-    return;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i][j] = param<T>(weight, f32, (c + j) * W + i);
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j)
+  for (int i = 0; i < W; ++i) taps[i].set(w[i]);
+}
+template <typename T, int V, typename A>
+__device__ __forceinline__ Channels<A, V> load_bias(const void* bias, bool f32, int64_t c) {
+  A x[V];
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i][j] = param<T>(weight, f32, (c + j) * W + i);
+  for (int j = 0; j < V; ++j) x[j] = bias == nullptr ? A(0) : param<T>(bias, f32, c + j);
+  Channels<A, V> r;
+  r.set(x);
+  return r;
 }
 
 __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, int64_t length) {
@@ -66,10 +108,9 @@ __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, 
 }
 
 // V inputs of token t (before the first: of the state; none past the `count` valid ones).
-template <typename T, int V>
+template <typename T, int V, typename A>
 __device__ __forceinline__ void input_at(const T* x, int64_t xs_t, const T* before, int64_t dim,
-                                         int width, int64_t t, int64_t count,
-                                         typename AccOf<T>::type* v) {
+                                         int width, int64_t t, int64_t count, A* v) {
   using G = Group<T, V>;
   if (t >= 0 && t < count) {
     G::values(G::load(x + t * xs_t), v);
@@ -114,34 +155,50 @@ conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
   x += t0 * xs_t;
   y += t0 * dim;
   typename G::Raw next[U];
+  const T* px = x;
   auto fetch = [&](int t) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (t + u < valid) next[u] = G::load(x + (t + u) * xs_t);
+      if (t + u < valid) next[u] = G::load(px + u * xs_t);
+    px += U * xs_t;
   };
   fetch(0);
-  A w[W][V], at[V];
+  using C = Channels<A, V>;
+  C w[W];
   load_taps<T, V, W>(weight, param_f32, whole, c, w);
+  const C at = load_bias<T, V, A>(bias, param_f32, c);
+  C win[W - 1 + U];  // the inputs of tokens t - W + 1 ... t + U - 1
 #pragma unroll
-  for (int j = 0; j < V; ++j) at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
-  A win[W - 1 + U][V];  // the inputs of tokens t - W + 1 ... t + U - 1
-#pragma unroll
-  for (int i = 0; i < W - 1; ++i)
-    input_at<T, V>(x - t0 * xs_t, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i]);
+  for (int i = 0; i < W - 1; ++i) {
+    A v[V];
+    input_at<T, V>(x - t0 * xs_t, xs_t, before, dim, W, t0 - (W - 1) + i, count, v);
+    win[i].set(v);
+  }
+  T* out = y;
   for (int t = 0; t < valid; t += U) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) G::values(next[u], win[W - 1 + u]);  // (past the end: not used)
+    for (int u = 0; u < U; ++u) {  // (past the end: not used)
+      A v[V];
+      G::values(next[u], v);
+      win[W - 1 + u].set(v);
+    }
     if (t + U < valid) fetch(t + U);
     auto token = [&](int u) {
-      A p[V];
+      C p;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        p[j] = at[j];
+      for (int m = 0; m < C::M; ++m) {
+        p.e[m] = fma(w[0].e[m], win[u].e[m], at.e[m]);
 #pragma unroll
-        for (int i = 0; i < W; ++i) p[j] += w[i][j] * win[u + i][j];
-        if (silu) p[j] *= sigmoid<T>(p[j]);
+        for (int i = 1; i < W; ++i) p.e[m] = fma(w[i].e[m], win[u + i].e[m], p.e[m]);
       }
-      G::store(y + (t + u) * dim, p);
+      A v[V];
+      p.get(v);
+      if (silu) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] *= sigmoid<T>(v[j]);
+      }
+      G::store(out, v);
+      out += dim;
     };
     if (t + U <= valid) {
 #pragma unroll
@@ -152,9 +209,7 @@ conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
         if (t + u < valid) token(u);
     }
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) win[i][j] = win[i + U][j];
+    for (int i = 0; i < W - 1; ++i) win[i] = win[i + U];
   }
   A none[V];
 #pragma unroll
@@ -190,89 +245,121 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
   x += b * xs_b + c;
   dy += b * ds_b + c;
   const T* before = initial == nullptr ? nullptr : initial + b * (W - 1) * dim + c;
-  A w[W][V], at[V], dw[W][V], db[V];
+  using C = Channels<A, V>;
+  C w[W], dw[W], db;
   load_taps<T, V, W>(weight, param_f32, whole, c, w);
+  const C at = load_bias<T, V, A>(bias, param_f32, c);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) dw[i][j] = A(0);
-    at[j] = bias == nullptr ? A(0) : param<T>(bias, param_f32, c + j);
-    db[j] = A(0);
-  }
+  for (int i = 0; i < W; ++i) dw[i].clear();
+  db.clear();
   const int64_t t0 = k * run;
   const bool first = k == 0;
   // relative to the run's first token: its tokens, and the valid ones of the sequence
   const int all = static_cast<int>(length - t0 < run ? length - t0 : run);
   const int valid = static_cast<int>(count - t0 < all + W - 1 ? count - t0 : all + W - 1);
   if (in && (all > 0 || first)) {
-    A win[W][V], dp[W][V];  // inputs t-W+1 ... t and gradients of the sums p of the same tokens
+    C win[W], dp[W];  // inputs t-W+1 ... t and gradients of the sums p of the same tokens
+    win[0].clear();
+#pragma unroll
+    for (int i = 0; i < W; ++i) dp[i].clear();
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
-      input_at<T, V>(x, xs_t, before, dim, W, t0 - (W - 1) + i, count, win[i + 1]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) dp[i + 1][j] = A(0);
+      A v[V];
+      input_at<T, V>(x, xs_t, before, dim, W, t0 - (W - 1) + i, count, v);
+      win[i + 1].set(v);
     }
     constexpr int U = 4;
     const int end = all + W - 1, begin = first && d_initial != nullptr ? -(W - 1) : 0;
     const T *px = x + t0 * xs_t, *pd = dy + t0 * ds_t;
-    T* out = dx + (b * length + t0) * dim + c;
+    T* out = dx + (b * length + t0 - (W - 1)) * dim + c;  // of input t - W + 1
     typename G::Raw nx[U], nd[U];
     auto fetch = [&](int t) {
+      if (t + U <= valid) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        nx[u] = nd[u] = typename G::Raw{};
-        if (t + u < valid) {
-          nx[u] = G::load(px + u * xs_t);
-          nd[u] = G::load(pd + u * ds_t);
+        for (int u = 0; u < U; ++u) nx[u] = G::load(px + u * xs_t), nd[u] = G::load(pd + u * ds_t);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          nx[u] = nd[u] = typename G::Raw{};
+          if (t + u < valid) nx[u] = G::load(px + u * xs_t), nd[u] = G::load(pd + u * ds_t);
         }
       }
       px += U * xs_t;
       pd += U * ds_t;
     };
+    // Moves on by a token: its window, its dp (zero where it does not count) and its share of dw and
+    // db (where it is the run's own); g: the gradient of input t - W + 1, all of whose dp are there.
+    auto token = [&](const typename G::Raw& rx, const typename G::Raw& rd, bool counts, bool own,
+                     A* g) {
+#pragma unroll
+      for (int i = 0; i < W - 1; ++i) win[i] = win[i + 1], dp[i] = dp[i + 1];
+      A v[V], q[V];
+      G::values(rx, v);
+      win[W - 1].set(v);
+      G::values(rd, q);
+      if (silu) {
+        C p;
+#pragma unroll
+        for (int m = 0; m < C::M; ++m) {
+          p.e[m] = fma(w[0].e[m], win[0].e[m], at.e[m]);
+#pragma unroll
+          for (int i = 1; i < W; ++i) p.e[m] = fma(w[i].e[m], win[i].e[m], p.e[m]);
+        }
+        p.get(v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const A s = sigmoid<T>(v[j]);
+          q[j] *= s * (A(1) + v[j] * (A(1) - s));
+        }
+      }
+      // (chosen, not multiplied by zero: what the window holds may be no number)
+      C d;
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] = counts ? q[j] : A(0);
+      dp[W - 1].set(q);
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] = own ? q[j] : A(0);
+      d.set(q);
+      C r;
+#pragma unroll
+      for (int m = 0; m < C::M; ++m) {
+        db.e[m] = add(db.e[m], d.e[m]);
+        r.e[m] = mul(w[W - 1].e[m], dp[0].e[m]);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          dw[i].e[m] = fma(d.e[m], win[i].e[m], dw[i].e[m]);
+          if (i > 0) r.e[m] = fma(w[W - 1 - i].e[m], dp[i].e[m], r.e[m]);
+        }
+      }
+      r.get(g);
+    };
+    // up to here the tokens' shares are all the run's own, and their inputs not in the state
+    const int sure = valid < all ? valid : all;
+    const int64_t last = count - t0;
     fetch(0);
     for (int s = 0; s < end; s += U) {
       typename G::Raw rx[U], rd[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) rx[u] = nx[u], rd[u] = nd[u];
       if (s + U < end) fetch(s + U);
+      if (s >= W - 1 && s + U <= sure && dx != nullptr &&
+          (d_final == nullptr || s + U - (W - 1) <= last - (W - 1))) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = s + u;
-#pragma unroll
-        for (int i = 0; i < W - 1; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            win[i][j] = win[i + 1][j];
-            dp[i][j] = dp[i + 1][j];
-          }
-        G::values(rx[u], win[W - 1]);
-        G::values(rd[u], dp[W - 1]);
-        // (chosen, not multiplied by zero: what the window holds may be no number)
-        const bool counts = t < valid, own = t < all;
-        A g[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (silu) {
-            A p = at[j];
-#pragma unroll
-            for (int i = 0; i < W; ++i) p += w[i][j] * win[i][j];
-            const A q = sigmoid<T>(p);
-            dp[W - 1][j] *= q * (A(1) + p * (A(1) - q));
-          }
-          if (!counts) dp[W - 1][j] = A(0);
-          const A d = own ? dp[W - 1][j] : A(0);
-          db[j] += d;
-          g[j] = A(0);
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            dw[i][j] += d * win[i][j];
-            g[j] += w[W - 1 - i][j] * dp[i][j];
-          }
+        for (int u = 0; u < U; ++u) {
+          A g[V];
+          token(rx[u], rd[u], true, true, g);
+          G::store(out, g);
+          out += dim;
         }
-        // g: the gradient of input t - W + 1, all of whose dp are there now
-        const int to = t - (W - 1);
+        continue;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u, out += dim) {
+        const int t = s + u, to = t - (W - 1);
+        A g[V];
+        token(rx[u], rd[u], t < valid, t < all && t < valid, g);
         if (to < begin || t >= end) continue;
-        const int64_t behind = count - t0 - to;  // 1: the last valid token
+        const int64_t behind = last - to;  // 1: the last valid token
         if (d_final != nullptr && behind >= 1 && behind <= W - 1) {
           A f[V];
           G::values(G::load(d_final + (b * (W - 1) + W - 1 - behind) * dim + c), f);
@@ -280,7 +367,7 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
           for (int j = 0; j < V; ++j) g[j] += f[j];
         }
         if (to < 0) G::store(d_initial + (b * (W - 1) + to + W - 1) * dim + c, g);
-        else if (dx != nullptr) G::store(out + to * dim, g);
+        else if (dx != nullptr) G::store(out, g);
       }
     }
   }
@@ -289,8 +376,11 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
 #pragma unroll
   for (int i = 0; i <= W; ++i) {
     if (i > 0) __syncthreads();
+    A v[V];
+    if (i < W) dw[i % W].get(v);
+    else db.get(v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) joined[threadIdx.y][threadIdx.x * V + j] = i < W ? dw[i % W][j] : db[j];
+    for (int j = 0; j < V; ++j) joined[threadIdx.y][threadIdx.x * V + j] = v[j];
     __syncthreads();
     for (int e = threadIdx.y * kBwdLanes + threadIdx.x; e < kBwdLanes * V;
          e += kBwdLanes * kBwdRuns) {
@@ -339,9 +429,11 @@ conv_step_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                  int width, bool silu, bool param_f32) {
   using A = typename AccOf<T>::type;
   using G = Group<T, V>;
-  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t per = dim / V, c = id % per * V, b = id / per;
-  if (b >= batch) return;
+  // threads over channels, blocks over channels first, then sequences
+  const unsigned per = static_cast<unsigned>(dim / V), blocks = (per + 127) / 128;
+  const unsigned place = blockIdx.x % blocks * 128 + threadIdx.x;
+  const int64_t c = int64_t(place) * V, b = blockIdx.x / blocks;
+  if (place >= per) return;
   const int64_t slot = slots == nullptr ? b : slots[b];
   A p[V];
   if (slot < 0 || slot >= pool) {
@@ -559,7 +651,7 @@ extern "C" int fdwt_causal_conv1d_step(const fdwt_conv1d_desc* desc, const void*
     using T = decltype(t);
     auto launch = [&](auto v) {
       constexpr int V = decltype(v)::value;
-      const int64_t grid = cdiv(desc->batch * (desc->dim / V), 128);
+      const int64_t grid = desc->batch * cdiv(desc->dim / V, 128);
       if (grid > INT32_MAX) return static_cast<int>(FDWT_ERR_UNSUPPORTED);
       const int st = pre_launch(static_cast<cudaStream_t>(stream));
       if (st != FDWT_OK) return st;

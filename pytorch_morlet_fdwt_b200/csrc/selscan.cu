@@ -352,6 +352,9 @@ extern "C" int fdwt_selscan_step(const fdwt_scan_desc* desc, const void* x, cons
   p.y = y;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(state);
   p.vec = desc->states % 4 == 0 && bits % (4 * acc_size(desc->dtype)) == 0;
+  int64_t states = p.states;
+  for (int i : {0, 2}) states |= p.bs[i] | p.cs[i];
+  p.vec_states = in_fours(desc, states, {p.b, p.c});
   return with_type(desc->dtype, [&](auto t) {
     return scan_step<decltype(t)>(p, lanes_of(desc->states), slots, state_slots, state,
                                   static_cast<cudaStream_t>(stream));

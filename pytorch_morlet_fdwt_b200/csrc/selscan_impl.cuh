@@ -3,62 +3,17 @@
 
 #include <cfloat>
 
+#include "pairs.cuh"
 #include "selscan.cuh"
 
 namespace fdwt {
 namespace {
 
 // ------------------------------------------------------------------------------ arithmetic
-// Two neighbouring states: packed instructions for 32 bits.
-template <typename A> struct Two;
-template <> struct Two<float> {
-  unsigned long long v;
-};
-template <> struct Two<double> {
-  double x, y;
-};
 template <typename A> struct alignas(4 * sizeof(A)) Four {
   A v[4];
 };
 
-__device__ __forceinline__ Two<float> two(float x, float y) {
-  Two<float> r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ Two<double> two(double x, double y) { return {x, y}; }
-__device__ __forceinline__ float first(Two<float> a) {
-  return __uint_as_float(static_cast<uint32_t>(a.v));
-}
-__device__ __forceinline__ float second(Two<float> a) {
-  return __uint_as_float(static_cast<uint32_t>(a.v >> 32));
-}
-__device__ __forceinline__ double first(Two<double> a) { return a.x; }
-__device__ __forceinline__ double second(Two<double> a) { return a.y; }
-__device__ __forceinline__ Two<float> mul(Two<float> a, Two<float> b) {
-  Two<float> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two<double> mul(Two<double> a, Two<double> b) {
-  return {a.x * b.x, a.y * b.y};
-}
-__device__ __forceinline__ Two<float> add(Two<float> a, Two<float> b) {
-  Two<float> r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two<double> add(Two<double> a, Two<double> b) {
-  return {a.x + b.x, a.y + b.y};
-}
-__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
-  Two<float> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
-  return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
-}
 template <typename A> __device__ __forceinline__ Two<A> low(const Four<A>& q) {
   return two(q.v[0], q.v[1]);
 }
@@ -939,66 +894,84 @@ template <typename A> constexpr size_t scan_bwd_smem(int ln, int nc) {
 }
 
 // ------------------------------------------------------------------------------ single tokens
-// One token of every sequence: a pass over the states, read and written once.
-template <typename T, int LN>
+// One token of every sequence: a pass over the states, read and written once.  A thread takes 4 states
+// of a channel in up to SEQ sequences, whose loads are in flight together and share the rates.
+template <typename T, int LN, int SEQ>
 __global__ void __launch_bounds__(128)
 scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__ slots,
                  int64_t pool, typename AccOf<T>::type* state) {
   using A = typename AccOf<T>::type;
   constexpr int CW = 128 / LN;  // channels of a block
-  const int64_t blocks = (p.dim + CW - 1) / CW;
-  const int64_t b = blockIdx.x / blocks;
-  const int nl = threadIdx.x % LN;
-  int64_t d = blockIdx.x % blocks * CW + threadIdx.x / LN;
-  const bool in = d < p.dim;
-  if (!in) d = p.dim - 1;  // the lanes of a warp stay together
-  const int64_t slot = slots == nullptr ? b : slots[b];
-  const bool live = slot >= 0 && slot < pool;
-  A y = A(0), x = A(0);
-  if (live) {
-    x = to_acc(static_cast<const T*>(p.x)[b * p.xs[0] + d]);
-    A delta = to_acc(static_cast<const T*>(p.dt)[b * p.dts[0] + d]);
-    if (p.dt_bias != nullptr) delta += static_cast<const A*>(p.dt_bias)[d];
-    if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
-    const int64_t group = d / p.per;
-    const T* pb = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
-    const T* pc = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
-    const A* pa = static_cast<const A*>(p.a) + d * p.states;
-    A* ps = state + (slot * p.dim + d) * p.states;
-    if (p.vec) {  // states in whole fours
-      if (nl * 4 < p.states) {
-        Four<A> h = reinterpret_cast<Four<A>*>(ps)[nl];
-        const Four<A> r = reinterpret_cast<const Four<A>*>(pa)[nl];
+  const unsigned dim = static_cast<unsigned>(p.dim), blocks = (dim + CW - 1) / CW;
+  const unsigned b0 = blockIdx.x / blocks * SEQ;
+  const int nl = threadIdx.x % LN, n0 = nl * 4;
+  unsigned d = blockIdx.x % blocks * CW + threadIdx.x / LN;
+  const bool in = d < dim;
+  if (!in) d = dim - 1;  // the lanes of a warp stay together
+  const unsigned group = p.groups == 1 ? 0 : d / static_cast<unsigned>(p.per);
+  const bool whole = p.vec && n0 < p.states;
+  const int have = p.states - n0;
+  Four<A> r = {A(0), A(0), A(0), A(0)};
+  const A* pa = static_cast<const A*>(p.a) + int64_t(d) * p.states + n0;
+  if (whole) r = *reinterpret_cast<const Four<A>*>(pa);
+  else if (!p.vec) r = params4<A>(pa, 0, have);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          h.v[j] = exp_2(delta * rate(r.v[j])) * h.v[j] + delta * x * A(to_acc(pb[nl * 4 + j]));
-          y += h.v[j] * A(to_acc(pc[nl * 4 + j]));
-        }
-        if (in) reinterpret_cast<Four<A>*>(ps)[nl] = h;
-      }
-    } else {
+  for (int j = 0; j < 4; ++j) r.v[j] = rate(r.v[j]);
+  const A bias = p.dt_bias != nullptr ? static_cast<const A*>(p.dt_bias)[d] : A(0);
+  const A skip = p.skip != nullptr ? static_cast<const A*>(p.skip)[d] : A(0);
+
+  A* ps[SEQ];
+  Four<A> h[SEQ];
+  Raw4<T> rb[SEQ], rc[SEQ];
+  A x[SEQ], dt[SEQ], z[SEQ];
+#pragma unroll
+  for (int i = 0; i < SEQ; ++i) {
+    const int64_t b = b0 + i;
+    ps[i] = nullptr;
+    if (b >= p.batch) continue;
+    const int64_t slot = slots == nullptr ? b : slots[b];
+    if (slot < 0 || slot >= pool) continue;
+    ps[i] = state + (slot * p.dim + d) * p.states + n0;
+    h[i] = {A(0), A(0), A(0), A(0)};
+    if (whole) h[i] = *reinterpret_cast<const Four<A>*>(ps[i]);
+    else if (!p.vec) h[i] = params4<A>(ps[i], 0, have);
+    rb[i] = load4(static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2] + n0, have, p.vec_states);
+    rc[i] = load4(static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2] + n0, have, p.vec_states);
+    x[i] = to_acc(static_cast<const T*>(p.x)[b * p.xs[0] + d]);
+    dt[i] = to_acc(static_cast<const T*>(p.dt)[b * p.dts[0] + d]);
+    if (p.gate != nullptr) z[i] = to_acc(static_cast<const T*>(p.gate)[b * p.gs[0] + d]);
+  }
+#pragma unroll
+  for (int i = 0; i < SEQ; ++i) {
+    if (b0 + i >= p.batch) break;
+    A y = A(0);
+    if (ps[i] != nullptr) {  // (the same for all lanes)
+      A delta = dt[i] + bias, vb[4], vc[4];
+      if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
+      Quad<T>::values(rb[i], vb);
+      Quad<T>::values(rc[i], vc);
+      const A u = delta * x[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int n = nl * 4 + j;
-        if (n < p.states) {
-          const A h = exp_2(delta * rate(pa[n])) * ps[n] + delta * x * A(to_acc(pb[n]));
-          y += h * A(to_acc(pc[n]));
-          if (in) ps[n] = h;
+        h[i].v[j] = exp_2(delta * r.v[j]) * h[i].v[j] + u * vb[j];
+        y += h[i].v[j] * vc[j];
+      }
+      if (in) {
+        if (whole) {
+          *reinterpret_cast<Four<A>*>(ps[i]) = h[i];
+        } else if (!p.vec) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < have) ps[i][j] = h[i].v[j];
         }
       }
-    }
-  }
 #pragma unroll
-  for (int o = LN / 2; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (!in || nl != 0) return;
-  if (live) {
-    if (p.skip != nullptr) y += static_cast<const A*>(p.skip)[d] * x;
-    if (p.gate != nullptr) {
-      const A z = to_acc(static_cast<const T*>(p.gate)[b * p.gs[0] + d]);
-      y *= z * sigmoid_at<sizeof(T) == 2>(z);
+      for (int o = LN / 2; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (p.skip != nullptr) y += skip * x[i];
+      if (p.gate != nullptr) y *= z[i] * sigmoid_at<sizeof(T) == 2>(z[i]);
     }
+    if (in && nl == 0) static_cast<T*>(p.y)[(b0 + i) * p.dim + d] = from_acc<T>(y);
   }
-  static_cast<T*>(p.y)[b * p.dim + d] = from_acc<T>(y);
 }
 
 // ------------------------------------------------------------------------------ launches
@@ -1077,13 +1050,20 @@ int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool, 
               cudaStream_t stream) {
   return with_lanes(lanes, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    const int64_t grid = p.batch * cdiv(p.dim, 128 / LN);
-    if (grid > INT32_MAX) return static_cast<int>(FDWT_ERR_UNSUPPORTED);
-    const int st = pre_launch(stream);
-    if (st != FDWT_OK) return st;
-    scan_step_kernel<T, LN><<<static_cast<unsigned>(grid), 128, 0, stream>>>(
-        p, slots, pool, static_cast<typename AccOf<T>::type*>(state));
-    return launch_status();
+    auto launch = [&](auto seq) {
+      constexpr int SEQ = decltype(seq)::value;
+      const int64_t grid = cdiv(p.batch, SEQ) * cdiv(p.dim, 128 / LN);
+      if (grid > INT32_MAX) return static_cast<int>(FDWT_ERR_UNSUPPORTED);
+      const int st = pre_launch(stream);
+      if (st != FDWT_OK) return st;
+      scan_step_kernel<T, LN, SEQ><<<static_cast<unsigned>(grid), 128, 0, stream>>>(
+          p, slots, pool, static_cast<typename AccOf<T>::type*>(state));
+      return launch_status();
+    };
+    // several sequences a thread where there are blocks enough
+    if (p.batch * cdiv(p.dim, 128 / LN) >= int64_t(sm_count()) * 32)
+      return launch(std::integral_constant<int, 4>{});
+    return launch(std::integral_constant<int, 1>{});
   });
 }
 
