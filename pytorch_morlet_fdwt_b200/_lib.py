@@ -162,6 +162,15 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def needs_grad(*tensors) -> bool:
+    """Whether autograd follows a call of these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def check(status: int, what: str) -> None:
     if status != 0:
         lib = load()
@@ -172,7 +181,7 @@ def check(status: int, what: str) -> None:
 
 
 def require_cuda(*tensors) -> torch.device:
-    dev = None
+    dev = index = None
     for t in tensors:
         if t is None:
             continue
@@ -180,9 +189,10 @@ def require_cuda(*tensors) -> torch.device:
             raise RuntimeError(
                 "pytorch_morlet_fdwt_b200 computes on CUDA tensors only (sm_100a kernels, no CPU "
                 f"fallback); got a tensor on {t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        at = t.get_device()
+        if index is None:
+            index, dev = at, t.device
+        elif at != index:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     return dev
 

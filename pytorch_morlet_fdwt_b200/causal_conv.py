@@ -161,15 +161,13 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     bias = None if bias is None else bias.contiguous()
     plan = _plan(x, weight, bias, activation)
     d = plan[0]
-    needs = (x.requires_grad or weight.requires_grad
-             or (bias is not None and bias.requires_grad))
     if initial_state is not None:
         _check_state(initial_state, (d.batch, d.width - 1, d.dim), x.dtype)
         initial_state = initial_state.contiguous()
-        needs = needs or initial_state.requires_grad
     if lengths is not None:
         lengths = _indexes(lengths, d.batch, 0, d.length, "lengths")
-    if (needs and torch.is_grad_enabled()) or _lib.has_tangent(x, weight, bias, initial_state):
+    inputs = (x, weight, bias, initial_state)
+    if _lib.needs_grad(*inputs) or _lib.has_tangent(*inputs):
         return _CausalConvFunction.apply(x, weight, bias, initial_state, lengths, activation, plan)
     return _forward(x, weight, bias, initial_state, lengths, plan)
 
@@ -195,8 +193,7 @@ def causal_conv1d_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     _check_state(state, (pool, d.width - 1, d.dim), x.dtype)
     if not state.is_contiguous():
         raise ValueError("the state is updated in place and must be contiguous")
-    if (any(t is not None and t.requires_grad for t in (x, weight, bias, state))
-            and torch.is_grad_enabled()) or _lib.has_tangent(x, weight, bias, state):
+    if _lib.needs_grad(x, weight, bias, state) or _lib.has_tangent(x, weight, bias, state):
         raise RuntimeError("causal_conv1d_step has no gradient: use causal_conv1d, or "
                            "torch.no_grad()")
     if slots is not None:

@@ -895,83 +895,100 @@ template <typename A> constexpr size_t scan_bwd_smem(int ln, int nc) {
 
 // ------------------------------------------------------------------------------ single tokens
 // One token of every sequence: a pass over the states, read and written once.  A thread takes 4 states
-// of a channel in up to SEQ sequences, whose loads are in flight together and share the rates.
+// of a channel in SEQ sequences (at most LN), whose loads are in flight together and share the
+// rates.  The LN lanes of a channel share out the sequences' steps and gates, and hand them round.
 template <typename T, int LN, int SEQ>
 __global__ void __launch_bounds__(128)
 scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__ slots,
                  int64_t pool, typename AccOf<T>::type* state) {
   using A = typename AccOf<T>::type;
+  static_assert(SEQ <= LN);
   constexpr int CW = 128 / LN;  // channels of a block
   const unsigned dim = static_cast<unsigned>(p.dim), blocks = (dim + CW - 1) / CW;
-  const unsigned b0 = blockIdx.x / blocks * SEQ;
-  const int nl = threadIdx.x % LN, n0 = nl * 4;
+  const int64_t b0 = int64_t(blockIdx.x / blocks) * SEQ;
+  const int lane = threadIdx.x & 31, nl = lane % LN, n0 = nl * 4;
   unsigned d = blockIdx.x % blocks * CW + threadIdx.x / LN;
   const bool in = d < dim;
   if (!in) d = dim - 1;  // the lanes of a warp stay together
   const unsigned group = p.groups == 1 ? 0 : d / static_cast<unsigned>(p.per);
-  const bool whole = p.vec && n0 < p.states;
   const int have = p.states - n0;
+  const bool whole = p.vec && have > 0;
+
+  // the lane's own sequence of them
+  constexpr int SAME = LN / SEQ;
+  const int64_t own = b0 + nl / SAME;
+  int own_slot = -1;
+  if (own < p.batch) {
+    const int64_t slot = slots == nullptr ? own : slots[own];
+    if (slot >= 0 && slot < pool) own_slot = static_cast<int>(slot);
+  }
+  A x = A(0), dt = A(0), z = A(0);
+  if (own_slot >= 0) {
+    x = to_acc(static_cast<const T*>(p.x)[own * p.xs[0] + d]);
+    dt = to_acc(static_cast<const T*>(p.dt)[own * p.dts[0] + d]);
+    if (p.gate != nullptr) z = to_acc(static_cast<const T*>(p.gate)[own * p.gs[0] + d]);
+  }
+  A* ps[SEQ];
+  Four<A> h[SEQ];
+  Raw4<T> rb[SEQ], rc[SEQ];
+  const T* pb = static_cast<const T*>(p.b) + b0 * p.bs[0] + group * p.bs[2] + n0;
+  const T* pc = static_cast<const T*>(p.c) + b0 * p.cs[0] + group * p.cs[2] + n0;
+#pragma unroll
+  for (int i = 0; i < SEQ; ++i, pb += p.bs[0], pc += p.cs[0]) {
+    const int slot = SEQ == 1 ? own_slot : __shfl_sync(0xffffffffu, own_slot, i * SAME, LN);
+    ps[i] = nullptr;
+    if (slot < 0) continue;
+    ps[i] = state + (slot * p.dim + d) * p.states + n0;
+    h[i] = {A(0), A(0), A(0), A(0)};
+    if (whole) h[i] = *reinterpret_cast<const Four<A>*>(ps[i]);
+    else if (!p.vec) h[i] = params4<A>(ps[i], 0, have);
+    rb[i] = load4(pb, have, p.vec_states);
+    rc[i] = load4(pc, have, p.vec_states);
+  }
   Four<A> r = {A(0), A(0), A(0), A(0)};
   const A* pa = static_cast<const A*>(p.a) + int64_t(d) * p.states + n0;
   if (whole) r = *reinterpret_cast<const Four<A>*>(pa);
   else if (!p.vec) r = params4<A>(pa, 0, have);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r.v[j] = rate(r.v[j]);
-  const A bias = p.dt_bias != nullptr ? static_cast<const A*>(p.dt_bias)[d] : A(0);
-  const A skip = p.skip != nullptr ? static_cast<const A*>(p.skip)[d] : A(0);
 
-  A* ps[SEQ];
-  Four<A> h[SEQ];
-  Raw4<T> rb[SEQ], rc[SEQ];
-  A x[SEQ], dt[SEQ], z[SEQ];
+  A delta = dt;
+  if (p.dt_bias != nullptr) delta += static_cast<const A*>(p.dt_bias)[d];
+  if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
+  const A u = delta * x;
+  A y[SEQ];
 #pragma unroll
   for (int i = 0; i < SEQ; ++i) {
-    const int64_t b = b0 + i;
-    ps[i] = nullptr;
-    if (b >= p.batch) continue;
-    const int64_t slot = slots == nullptr ? b : slots[b];
-    if (slot < 0 || slot >= pool) continue;
-    ps[i] = state + (slot * p.dim + d) * p.states + n0;
-    h[i] = {A(0), A(0), A(0), A(0)};
-    if (whole) h[i] = *reinterpret_cast<const Four<A>*>(ps[i]);
-    else if (!p.vec) h[i] = params4<A>(ps[i], 0, have);
-    rb[i] = load4(static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2] + n0, have, p.vec_states);
-    rc[i] = load4(static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2] + n0, have, p.vec_states);
-    x[i] = to_acc(static_cast<const T*>(p.x)[b * p.xs[0] + d]);
-    dt[i] = to_acc(static_cast<const T*>(p.dt)[b * p.dts[0] + d]);
-    if (p.gate != nullptr) z[i] = to_acc(static_cast<const T*>(p.gate)[b * p.gs[0] + d]);
-  }
+    const A di = SEQ == 1 ? delta : __shfl_sync(0xffffffffu, delta, i * SAME, LN);
+    const A ui = SEQ == 1 ? u : __shfl_sync(0xffffffffu, u, i * SAME, LN);
+    y[i] = A(0);
+    if (ps[i] == nullptr) continue;
+    A vb[4], vc[4];
+    Quad<T>::values(rb[i], vb);
+    Quad<T>::values(rc[i], vc);
 #pragma unroll
-  for (int i = 0; i < SEQ; ++i) {
-    if (b0 + i >= p.batch) break;
-    A y = A(0);
-    if (ps[i] != nullptr) {  // (the same for all lanes)
-      A delta = dt[i] + bias, vb[4], vc[4];
-      if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
-      Quad<T>::values(rb[i], vb);
-      Quad<T>::values(rc[i], vc);
-      const A u = delta * x[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        h[i].v[j] = exp_2(delta * r.v[j]) * h[i].v[j] + u * vb[j];
-        y += h[i].v[j] * vc[j];
-      }
-      if (in) {
-        if (whole) {
-          *reinterpret_cast<Four<A>*>(ps[i]) = h[i];
-        } else if (!p.vec) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < have) ps[i][j] = h[i].v[j];
-        }
-      }
-#pragma unroll
-      for (int o = LN / 2; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (p.skip != nullptr) y += skip * x[i];
-      if (p.gate != nullptr) y *= z[i] * sigmoid_at<sizeof(T) == 2>(z[i]);
+    for (int j = 0; j < 4; ++j) {
+      h[i].v[j] = exp_2(di * r.v[j]) * h[i].v[j] + ui * vb[j];
+      y[i] += h[i].v[j] * vc[j];
     }
-    if (in && nl == 0) static_cast<T*>(p.y)[(b0 + i) * p.dim + d] = from_acc<T>(y);
+    if (!in) continue;
+    if (whole) {
+      *reinterpret_cast<Four<A>*>(ps[i]) = h[i];
+    } else if (!p.vec) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < have) ps[i][j] = h[i].v[j];
+    }
   }
+  fold<SEQ, LN, 1>(y, lane);
+  if (!in || nl % SAME != 0 || own >= p.batch) return;
+  A out = A(0);
+  if (own_slot >= 0) {
+    out = y[0];
+    if (p.skip != nullptr) out += static_cast<const A*>(p.skip)[d] * x;
+    if (p.gate != nullptr) out *= z * sigmoid_at<sizeof(T) == 2>(z);
+  }
+  static_cast<T*>(p.y)[own * p.dim + d] = from_acc<T>(out);
 }
 
 // ------------------------------------------------------------------------------ launches
@@ -1061,8 +1078,9 @@ int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool, 
       return launch_status();
     };
     // several sequences a thread where there are blocks enough
-    if (p.batch * cdiv(p.dim, 128 / LN) >= int64_t(sm_count()) * 32)
-      return launch(std::integral_constant<int, 4>{});
+    constexpr int MOST = LN < 4 ? LN : 4;
+    if (p.batch * cdiv(p.dim, 128 / LN) >= int64_t(sm_count()) * 4 * MOST)
+      return launch(std::integral_constant<int, MOST>{});
     return launch(std::integral_constant<int, 1>{});
   });
 }

@@ -249,8 +249,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     norm of its result.  Differentiable once in x, weight and residual; the gradients' sums over
     rows are added in a fixed order."""
     x, weight, residual, codes = _rms_inputs(x, weight, residual, eps)
-    needs = any(t is not None and t.requires_grad for t in (x, weight, residual))
-    if (needs and torch.is_grad_enabled()) or _lib.has_tangent(x, weight, residual):
+    if _lib.needs_grad(x, weight, residual) or _lib.has_tangent(x, weight, residual):
         return _RMSNormFunction.apply(x, residual, weight, float(eps), codes)
     y, total, _ = _rms_forward(x, residual, weight, float(eps), codes, False)
     return y if total is None else (y, total)
@@ -278,8 +277,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     group = dim if group_size is None else int(group_size)
     if group < 1 or dim % group:
         raise ValueError(f"group_size must divide {dim}, got {group_size}")
-    if (any(t is not None and t.requires_grad for t in (x, weight, residual))
-            and torch.is_grad_enabled()) or _lib.has_tangent(x, weight, residual):
+    if _lib.needs_grad(x, weight, residual) or _lib.has_tangent(x, weight, residual):
         raise RuntimeError("rms_norm_quantized has no gradient: use rms_norm, or torch.no_grad()")
     dev = x.device
     q = torch.empty(x.shape, device=dev, dtype=dtype)

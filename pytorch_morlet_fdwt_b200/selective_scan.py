@@ -94,12 +94,11 @@ def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, devic
 
 
 def _plan(lead, x, dt, a, b, c, gate, softplus, dy_stride=None):
-    return _describe(lead, (x.dtype, dt.dtype, b.dtype, c.dtype,
-                            None if gate is None else gate.dtype),
-                     (x.shape, dt.shape, b.shape, c.shape, None if gate is None else gate.shape),
-                     (x.stride(), dt.stride(), b.stride(), c.stride(),
-                      None if gate is None else gate.stride()),
-                     a.shape, dy_stride, bool(softplus), x.device.index)
+    dtypes, shapes = (x.dtype, dt.dtype, b.dtype, c.dtype), (x.shape, dt.shape, b.shape, c.shape)
+    strides = (x.stride(), dt.stride(), b.stride(), c.stride())
+    last = (None, None, None) if gate is None else (gate.dtype, gate.shape, gate.stride())
+    return _describe(lead, (*dtypes, last[0]), (*shapes, last[1]), (*strides, last[2]), a.shape,
+                     dy_stride, bool(softplus), x.get_device())
 
 
 _SEQUENCE, _TOKEN = ("B", "L"), ("B",)
@@ -107,8 +106,8 @@ _SEQUENCE, _TOKEN = ("B", "L"), ("B",)
 
 def _parameter(name: str, t: Optional[torch.Tensor], shape, dtype) -> Optional[torch.Tensor]:
     """``t`` contiguous and in the states' type (a cast that autograd follows)."""
-    if t is None:
-        return None
+    if t is None or (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+        return t
     if tuple(t.shape) != shape or not t.is_floating_point():
         raise ValueError(f"{name} must be floating point of shape {shape}, got {t.dtype} "
                          f"{tuple(t.shape)}")
@@ -222,8 +221,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     if lengths is not None:
         lengths = _indexes(lengths, d.batch, 0, d.length, "lengths")
     inputs = (x, dt, a, b, c, skip, gate, dt_bias, initial_state)
-    needs = any(t is not None and t.requires_grad for t in inputs)
-    if (needs and torch.is_grad_enabled()) or _lib.has_tangent(*inputs):
+    if _lib.needs_grad(*inputs) or _lib.has_tangent(*inputs):
         return _SelectiveScanFunction.apply(*inputs, lengths, bool(dt_softplus), plan)
     return _forward(*inputs, lengths, plan, False)[:2]
 
@@ -254,8 +252,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     if not state.is_contiguous():
         raise ValueError("the state is updated in place and must be contiguous")
     inputs = (x, dt, a, b, c, skip, gate, dt_bias, state)
-    if (any(t is not None and t.requires_grad for t in inputs)
-            and torch.is_grad_enabled()) or _lib.has_tangent(*inputs):
+    if _lib.needs_grad(*inputs) or _lib.has_tangent(*inputs):
         raise RuntimeError("selective_scan_step has no gradient: use selective_scan, or "
                            "torch.no_grad()")
     if slots is not None:
