@@ -33,51 +33,87 @@ template <typename A> __device__ __forceinline__ Two<A> exp_2(Two<A> x) {
 }
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
-// e^-a for a >= 0: the product with log2 e is rounded, so what it lost corrects the result.
-__device__ __forceinline__ float neg_exp(float a) {
-  constexpr float kHigh = 1.442695021629333f, kLow = 1.92596299e-8f;  // log2 e in two parts
-  const float t = a * kHigh;
-  const float lost = fmaf(a, kLow, fmaf(a, kHigh, -t));
-  const float e = exp_2(-t);
-  return fmaf(e, lost * -static_cast<float>(kLn2), e);
-}
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|), to the last bits where it is small too (steps are
-// often 1e-3), and its slope 1 / (1 + e^-v).  log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the
-// odd series of atanh, its coefficients fitted for s^2 up to 1/9 (8e-9 off).  Against log1pf and
-// expf of the library (35 instructions, this 17): 2 to 4 roundings off, as they are.
-__device__ __forceinline__ float softplus(float v, float* slope) {
-  const float e = neg_exp(fminf(fabsf(v), 128.0f));
-  const float s = e * reciprocal(2.0f + e), z = s * s;
-  float q = 0.2817465662956238f;
-  q = fmaf(q, z, 0.2796141803264618f);
-  q = fmaf(q, z, 0.40024852752685547f);
-  q = fmaf(q, z, 0.6666631698608398f);
-  q = fmaf(q, z, 2.0f);
-  if (slope != nullptr) {
-    const float w = reciprocal(1.0f + e);
-    *slope = v < 0.0f ? e * w : w;
+__device__ __forceinline__ Two<float> both(float x) { return two(x, x); }
+// e^-|v| of two values: the product with log2 e is rounded, so what it lost corrects the result.
+__device__ __forceinline__ Two<float> neg_exp(float v, float w) {
+  constexpr float kHigh = 1.442695021629333f, kLow = 1.92596299e-8f;  // log2 e in two parts
+  const Two<float> a = two(fminf(fabsf(v), 128.0f), fminf(fabsf(w), 128.0f));
+  const Two<float> t = mul(a, both(-kHigh));
+  const Two<float> lost = fma(a, both(kLow), fma(a, both(kHigh), t));
+  const Two<float> e = exp_2(t);
+  return fma(e, mul(lost, both(-static_cast<float>(kLn2))), e);
+}
+// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|) of 4 values, to the last bits where it is small too
+// (steps are often 1e-3), and with SLOPE its slope 1 / (1 + e^-v).  log(1 + e) = 2 atanh(s),
+// s = e / (2 + e) <= 1/3: the odd series of atanh, its coefficients fitted for s^2 up to 1/9 (8e-9
+// off).  Against expf and log1pf of the library: 11 instructions in place of 35, 2 to 4 roundings
+// off as they are.
+template <bool SLOPE>
+__device__ __forceinline__ void softplus(const float* v, float* d, float* slope) {
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const Two<float> e = neg_exp(v[j], v[j + 1]);
+    const Two<float> n = add(e, both(2.0f));
+    const Two<float> s = mul(e, two(reciprocal(first(n)), reciprocal(second(n))));
+    const Two<float> z = mul(s, s);
+    Two<float> q = fma(both(0.2817465662956238f), z, both(0.2796141803264618f));
+    q = fma(q, z, both(0.40024852752685547f));
+    q = fma(q, z, both(0.6666631698608398f));
+    q = fma(q, z, both(2.0f));
+    // (v + |v|) / 2: the larger of v and 0, and NaN for NaN
+    const Two<float> top = two(v[j] + fabsf(v[j]), v[j + 1] + fabsf(v[j + 1]));
+    const Two<float> r = fma(top, both(0.5f), mul(s, q));
+    if (SLOPE) {
+      const Two<float> o = add(e, both(1.0f));
+      const Two<float> w = two(reciprocal(first(o)), reciprocal(second(o))), ew = mul(e, w);
+      slope[j] = v[j] < 0.0f ? first(ew) : first(w);
+      slope[j + 1] = v[j + 1] < 0.0f ? second(ew) : second(w);
+    }
+    d[j] = first(r), d[j + 1] = second(r);
   }
-  return fmaf(s, q, v < 0.0f ? 0.0f : v);
 }
-__device__ __forceinline__ double softplus(double v, double* slope) {
-  const double e = exp(-fabs(v));
-  if (slope != nullptr) *slope = v < 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
-  return (v < 0.0 ? 0.0 : v) + log1p(e);
+template <bool SLOPE>
+__device__ __forceinline__ void softplus(const double* v, double* d, double* slope) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const double e = exp(-fabs(v[j])), x = v[j];
+    if (SLOPE) slope[j] = x < 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
+    d[j] = (x < 0.0 ? 0.0 : x) + log1p(e);
+  }
 }
-// 1 / (1 + e^-v) to a few roundings, or, where the result is rounded to 16 bits (FAST), by the
-// plain fast functions.
-template <bool FAST> __device__ __forceinline__ float sigmoid_at(float v) {
-  if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-v));
-  const float e = neg_exp(fminf(fabsf(v), 128.0f)), w = reciprocal(1.0f + e);
-  return v < 0.0f ? e * w : (v != v ? v : w);
+__device__ __forceinline__ float softplus(float v) {
+  const float x[4] = {v, v, v, v};
+  float d[4];
+  softplus<false>(x, d, nullptr);  // (one of the pairs is all that is kept)
+  return d[0];
 }
-template <bool FAST> __device__ __forceinline__ double sigmoid_at(double v) {
-  return 1.0 / (1.0 + exp(-v));
+__device__ __forceinline__ double softplus(double v) {
+  return (v < 0.0 ? 0.0 : v) + log1p(exp(-fabs(v)));
+}
+// 1 / (1 + e^-v) of 4 values to a few roundings (NaN gives a number: a product with v follows), or,
+// where the result is rounded to 16 bits (FAST), by the plain fast functions.
+template <bool FAST> __device__ __forceinline__ void sigmoid_at(const float* v, float* g) {
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    if constexpr (FAST) {
+      g[j] = __fdividef(1.0f, 1.0f + __expf(-v[j]));
+      g[j + 1] = __fdividef(1.0f, 1.0f + __expf(-v[j + 1]));
+    } else {
+      const Two<float> e = neg_exp(v[j], v[j + 1]), o = add(e, both(1.0f));
+      const Two<float> w = two(reciprocal(first(o)), reciprocal(second(o))), ew = mul(e, w);
+      g[j] = v[j] < 0.0f ? first(ew) : first(w);
+      g[j + 1] = v[j + 1] < 0.0f ? second(ew) : second(w);
+    }
+  }
+}
+template <bool FAST> __device__ __forceinline__ void sigmoid_at(const double* v, double* g) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = 1.0 / (1.0 + exp(-v[j]));
 }
 
 // A channel's rates times log2 e.  -inf (forgets everything) becomes the lowest finite value, so
@@ -411,6 +447,8 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     bc.fetch(p, static_cast<int>(w.count - t < TT ? w.count - t : TT), MODE == REVERSE ? -TT : TT);
   };
 
+  Four<A>* kept = static_cast<Four<A>*>(p.check) +
+                  ((w.b * ((p.length + 7) / 8) + w.t0 / 8) * p.dim + w.d0 + cl) * LN + nl;
   if (steps > 0) fetch(begin(0));
   for (int64_t i = 0; i < steps; ++i) {
     const int64_t t = begin(i);
@@ -424,23 +462,26 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     for (int q = 0; q < I::IT; ++q) {
       const int row = row0 + q * I::ROWS;
       if (I::ROWS * I::IT > TT && row >= TT) break;
-      A x[4], dt[4], z[4];
-      Step<A> out[4];
+      A x[4], delta[4];
       Quad<T>::values(xr[q], x);
-      Quad<T>::values(dr[q], dt);
-      if (MODE == REVERSE && gated) Quad<T>::values(zr[q], z);
+      Quad<T>::values(dr[q], delta);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        A delta = dt[j] + bias.v[j];
-        if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
-        if (MODE == REVERSE) {
-          if (gated) x[j] *= z[j] * sigmoid_at<false>(z[j]);
-          out[j] = {delta, x[j]};
-        } else {
-          out[j] = {delta, delta * x[j]};
-        }
-        if (q * I::ROWS >= left) out[j] = {A(0), A(0)};
+      for (int j = 0; j < 4; ++j) delta[j] += bias.v[j];
+      if (p.softplus) softplus<false>(delta, delta, nullptr);
+      if (q * I::ROWS >= left) {  // (x and the rest are zero there)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) delta[j] = A(0);
       }
+      if (MODE == REVERSE && gated) {
+        A z[4], g[4];
+        Quad<T>::values(zr[q], z);
+        sigmoid_at<false>(z, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] *= z[j] * g[j];
+      }
+      Step<A> out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = {delta[j], MODE == REVERSE ? x[j] : delta[j] * x[j]};
       Four<A>* to = reinterpret_cast<Four<A>*>(slots + row * CT + col);
       to[0] = {out[0].delta, out[0].u, out[1].delta, out[1].u};
       to[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
@@ -449,15 +490,15 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     bc.store(states);
     if (i + 1 < steps) fetch(begin(i + 1));
     __syncthreads();
-#pragma unroll 1
+#pragma unroll(MODE == MAIN && NC <= 2 ? TT / 8 : 1)
     for (int s = 0; s < TT; s += 8) {
-      if (MODE == MAIN && p.check != nullptr && t + s < w.count) {
-        const int64_t row = (w.b * ((p.length + 7) / 8) + (t + s) / 8) * p.dim + w.d0 + cl;
+      if (MODE == MAIN && p.check != nullptr && s < left + row0) {
 #pragma unroll
         for (int k = 0; k < NC; ++k)
           if (cl + (k ^ swap) < w.width)
-            static_cast<Four<A>*>(p.check)[(row + (k ^ swap)) * LN + nl] = {
-                first(h[k][0]), second(h[k][0]), first(h[k][1]), second(h[k][1])};
+            kept[(k ^ swap) * LN] = {first(h[k][0]), second(h[k][0]), first(h[k][1]),
+                                     second(h[k][1])};
+        kept += p.dim * LN;
       }
       A y[8 * NC];
 #pragma unroll
@@ -502,14 +543,19 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
         const int row = row0 + q * I::ROWS;
         if (q * I::ROWS >= left) break;
         const Four<A> f = *reinterpret_cast<const Four<A>*>(sums + row * PAD + col);
-        A y[4], x[4], z[4];
-        if (p.skip != nullptr) Quad<T>::values(xc[q], x);
-        if (gated) Quad<T>::values(zr[q], z);
+        A y[4] = {f.v[0], f.v[1], f.v[2], f.v[3]};
+        if (p.skip != nullptr) {
+          A x[4];
+          Quad<T>::values(xc[q], x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          y[j] = f.v[j];
-          if (p.skip != nullptr) y[j] += skip.v[j] * x[j];
-          if (gated) y[j] *= z[j] * sigmoid_at<sizeof(T) == 2>(z[j]);
+          for (int j = 0; j < 4; ++j) y[j] += skip.v[j] * x[j];
+        }
+        if (gated) {
+          A z[4], g[4];
+          Quad<T>::values(zr[q], z);
+          sigmoid_at<sizeof(T) == 2>(z, g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] *= z[j] * g[j];
         }
         store4(py + q * (I::ROWS * p.dim), y, have, p.vec);
       }
@@ -654,6 +700,11 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
       if (gated) store4(og + t * p.dim, zero, have, p.vec);
     }
   }
+  // of the step: the states kept before it, and the thread's results
+  const Four<A>* kept = static_cast<const Four<A>*>(p.check) +
+                        ((w.b * ((p.length + 7) / 8) + last / 8) * p.dim + w.d0 + cl) * LN + nl;
+  int64_t result = mine * p.dim;
+  part_bc += last * 2 * NP;
   if (steps > 0) fetch(last);
   for (int64_t i = steps - 1; i >= 0; --i) {
     const int64_t t = w.t0 + i * TT;
@@ -664,8 +715,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
       start[k] = {A(0), A(0), A(0), A(0)};
       const int c = cl + (k ^ swap);
       if (c < w.width)
-        start[k] = static_cast<const Four<A>*>(
-            p.check)[((w.b * ((p.length + 7) / 8) + t / 8) * p.dim + w.d0 + c) * LN + nl];
+        start[k] = kept[(k ^ swap) * LN];
     }
     // kept for the results: x, the step's slope, dy silu'(gate)
     A xk[I::IT][4], slope[I::IT][4], opening[I::IT][4];
@@ -673,34 +723,37 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     for (int q = 0; q < I::IT; ++q) {
       const int row = row0 + q * I::ROWS;
       if (I::ROWS * I::IT > TT && row >= TT) break;
-      Step<A> out[4];
       Four<A> dp;
-      A dt[4], z[4];
+      A delta[4];
       Quad<T>::values(xr[q], xk[q]);
-      Quad<T>::values(dr[q], dt);
+      Quad<T>::values(dr[q], delta);
       Quad<T>::values(qr[q], dp.v);
-      if (gated) Quad<T>::values(zr[q], z);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        A delta = dt[j] + bias.v[j], sl = A(1), op = A(0);
-        if (p.softplus) delta = softplus(delta, &sl);
-        if (gated) {
-          const A sg = sigmoid_at<false>(z[j]);
-          op = dp.v[j] * (sg * (A(1) + z[j] * (A(1) - sg)));
-          dp.v[j] *= z[j] * sg;
-        }
-        out[j] = {delta, delta * xk[q][j]};
-        if (q * I::ROWS >= left) {
-          out[j] = {A(0), A(0)};
-          dp.v[j] = A(0);
-        }
-        slope[q][j] = sl, opening[q][j] = op;
+      for (int j = 0; j < 4; ++j) delta[j] += bias.v[j], slope[q][j] = A(1);
+      if (p.softplus) softplus<true>(delta, delta, slope[q]);
+      if (q * I::ROWS >= left) {  // (x and dy are zero there)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) delta[j] = A(0);
       }
+      if (gated) {
+        A z[4], g[4];
+        Quad<T>::values(zr[q], z);
+        sigmoid_at<false>(z, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          opening[q][j] = dp.v[j] * (g[j] * (A(1) + z[j] * (A(1) - g[j])));
+          dp.v[j] *= z[j] * g[j];
+        }
+      }
+      Step<A> out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = {delta[j], delta[j] * xk[q][j]};
       Four<A>* st = reinterpret_cast<Four<A>*>(slots + row * CT + col);
       st[0] = {out[0].delta, out[0].u, out[1].delta, out[1].u};
       st[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
       *reinterpret_cast<Four<A>*>(dps + row * CT + col) = dp;
     }
+    kept -= p.dim * LN;
     bc.template store_orders<COPIES>(states);
     if (i > 0) fetch(t - TT);
     __syncthreads();
@@ -709,7 +762,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     Two<A> dat[NC][2];
 #pragma unroll
     for (int k = 0; k < NC; ++k) dat[k][0] = dat[k][1] = none;
-#pragma unroll 1
+#pragma unroll
     for (int half = 1; half >= 0; --half) {
       Two<A> h[SUB + 1][NC][2], e[SUB][NC][2];
 #pragma unroll
@@ -743,7 +796,9 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
           h[u + 1][k][1] = fma(e[u][k][1], h[u][k][1], mul(u2, high(bq[u])));
         }
       }
-      A through[SUB * NC], pre[SUB * NC], by_rate[SUB * NC], v[SUB * 8];
+      // sums over states and channels: each token's own first steps at once, so that few values live
+      constexpr int LEFT = 4 / COPIES;  // states of each run (token, b or c) that a lane keeps
+      A through[SUB], pre[SUB], by_rate[SUB], v[SUB * 2 * LEFT];
 #pragma unroll
       for (int u = SUB - 1; u >= 0; --u) {
         const Four<A> cq = my_c[(base + u) * COPIES * LN];
@@ -751,6 +806,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
 #pragma unroll
         for (int k = 0; k < NC; ++k) dp[k] = dps[(base + u) * CT + cl + (k ^ swap)];
         Two<A> db[2], dc[2];
+        A over[3][NC];
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
           const Two<A> q2 = two(dp[k], dp[k]), d2 = two(st[u][k].delta, st[u][k].delta),
@@ -769,19 +825,18 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
           const Two<A> tb = fma(g[1], bb[1], mul(g[0], bb[0]));
           const Two<A> tc = fma(h[u + 1][k][1], cc[1], mul(h[u + 1][k][0], cc[0]));
           const Two<A> ta = fma(ra[k][1], kp[1], mul(ra[k][0], kp[0]));
-          through[u * NC + k] = first(tb) + second(tb);
-          pre[u * NC + k] = first(tc) + second(tc);
-          by_rate[u * NC + k] = first(ta) + second(ta);
+          over[0][k] = first(tb) + second(tb);
+          over[1][k] = first(tc) + second(tc);
+          over[2][k] = first(ta) + second(ta);
         }
-        v[u * 8 + 0] = first(db[0]), v[u * 8 + 1] = second(db[0]);
-        v[u * 8 + 2] = first(db[1]), v[u * 8 + 3] = second(db[1]);
-        v[u * 8 + 4] = first(dc[0]), v[u * 8 + 5] = second(dc[0]);
-        v[u * 8 + 6] = first(dc[1]), v[u * 8 + 7] = second(dc[1]);
+        fold_swapped<3, NC, LN, 1>(&over[0][0]);
+        through[u] = over[0][0], pre[u] = (&over[0][0])[1], by_rate[u] = (&over[0][0])[2];
+        A runs[8] = {first(db[0]), second(db[0]), first(db[1]), second(db[1]),
+                     first(dc[0]), second(dc[0]), first(dc[1]), second(dc[1])};
+        fold_swapped<2, 4, LD, LN>(runs);
+#pragma unroll
+        for (int o = 0; o < 2 * LEFT; ++o) v[u * 2 * LEFT + o] = runs[o];
       }
-      // over the states
-      fold_swapped<SUB, NC, LN, 1>(through);
-      fold_swapped<SUB, NC, LN, 1>(pre);
-      fold_swapped<SUB, NC, LN, 1>(by_rate);
       fold<SUB, OTHERS, KEPT>(through, lane);
       fold<SUB, OTHERS, KEPT>(pre, lane);
       fold<SUB, OTHERS, KEPT>(by_rate, lane);
@@ -793,11 +848,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
         q[TT * PAD] = pre[o];
         q[2 * TT * PAD] = by_rate[o];
       }
-      // over the warp's channels: runs of the thread's 4 states by token, and b or c
-      fold_swapped<SUB * 2, 4, LD, LN>(v);
-      constexpr int LEFT = 4 / COPIES;                    // states of each run that a lane keeps
-      constexpr int FAR = LD / COPIES;                    // lanes that share out the runs
-      fold<SUB * 2, FAR, LN * COPIES>(v, lane);           // (FAR > 1 only where LEFT is 1)
+      constexpr int FAR = LD / COPIES;           // lanes that share out the runs
+      fold<SUB * 2, FAR, LN * COPIES>(v, lane);  // (FAR > 1 only where LEFT is 1)
       constexpr int RUNS = SUB * 2 / FAR;
 #pragma unroll
       for (int o = 0; o < RUNS; ++o) {
@@ -831,13 +883,15 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
         dskip[j] += dp.v[j] * xk[q][j];
         dbias[j] += gd[j];
       }
-      store4(ox + (t + row) * p.dim, gx, have, p.vec);
-      store4(od + (t + row) * p.dim, gd, have, p.vec);
-      if (gated) store4(og + (t + row) * p.dim, gg, have, p.vec);
+      const int64_t at = result + q * (I::ROWS * p.dim);
+      store4(ox + at, gx, have, p.vec);
+      store4(od + at, gd, have, p.vec);
+      if (gated) store4(og + at, gg, have, p.vec);
     }
+    result -= TT * p.dim;
     // (tokens past the valid ones have no part: scan_bc_kernel leaves them out)
     for (int e = threadIdx.x; e < TT * 2 * LN; e += 128) {
-      if (t + e / (2 * LN) >= w.count) continue;
+      if (e / (2 * LN) >= left + row0) continue;
       Four<A> s = reinterpret_cast<const Four<A>*>(joined)[e];
 #pragma unroll
       for (int q = 1; q < 4; ++q) {
@@ -845,8 +899,9 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s.v[j] += f.v[j];
       }
-      reinterpret_cast<Four<A>*>(part_bc + t * 2 * NP)[e] = s;
+      reinterpret_cast<Four<A>*>(part_bc)[e] = s;
     }
+    part_bc -= TT * 2 * NP;
     __syncthreads();
   }
 
@@ -954,7 +1009,7 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
 
   A delta = dt;
   if (p.dt_bias != nullptr) delta += static_cast<const A*>(p.dt_bias)[d];
-  if (p.softplus) delta = softplus(delta, static_cast<A*>(nullptr));
+  if (p.softplus) delta = softplus(delta);
   const A u = delta * x;
   A y[SEQ];
 #pragma unroll
@@ -986,7 +1041,12 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
   if (own_slot >= 0) {
     out = y[0];
     if (p.skip != nullptr) out += static_cast<const A*>(p.skip)[d] * x;
-    if (p.gate != nullptr) out *= z * sigmoid_at<sizeof(T) == 2>(z);
+    if (p.gate != nullptr) {
+      const A zs[4] = {z, z, z, z};
+      A g[4];
+      sigmoid_at<sizeof(T) == 2>(zs, g);
+      out *= z * g[0];
+    }
   }
   static_cast<T*>(p.y)[own * p.dim + d] = from_acc<T>(out);
 }
