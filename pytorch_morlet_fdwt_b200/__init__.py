@@ -12,7 +12,8 @@
 * :func:`rms_norm`, :func:`rms_norm_quantized` (:class:`RMSNorm`), :func:`causal_conv1d` and
   :func:`selective_scan` with their single-token forms :func:`causal_conv1d_step` and
   :func:`selective_scan_step` -- the norm with the residual's addition, the short convolution and
-  the selective state space scan of stacks of causal mixers.
+  the selective state space scan of a causal mixer, :class:`SelectiveTokenMixer`, and of stacks of
+  them, :class:`SelectiveTokenStack`.
 
 Every transform runs in hand-written CUDA kernels for sm_100a behind the C ABI of
 ``include/fdwt_b200.h`` (``libfdwt_b200.so``); inputs must be CUDA tensors.
@@ -23,7 +24,8 @@ from .causal_conv import causal_conv1d, causal_conv1d_step
 from .cwt import CWT1D, MorletPlan, cwt, freqs_to_scales, scales_to_freqs
 from .dwt import DWT1D, IDWT1D, dwt, dwt_max_level, idwt, wavedec, waverec
 from .layers import (DecayTokenMixer, MorletAttention, MorletChannelMixAttention,
-                     MorletTokenMixer, WaveletTokenMixer)
+                     MorletTokenMixer, SelectiveTokenMixer, SelectiveTokenStack,
+                     WaveletTokenMixer)
 from .linear_attention import linear_attention, linear_attention_step
 from .norm import LayerNorm, RMSNorm, layer_norm, rms_norm, rms_norm_quantized
 from .selective_scan import selective_scan, selective_scan_step
@@ -37,6 +39,6 @@ __all__ = [
     "MorletAttention", "MorletChannelMixAttention", "MorletTokenMixer", "WaveletTokenMixer",
     "DecayTokenMixer", "LayerNorm", "layer_norm", "linear_attention", "linear_attention_step",
     "RMSNorm", "rms_norm", "rms_norm_quantized", "causal_conv1d", "causal_conv1d_step",
-    "selective_scan", "selective_scan_step",
+    "selective_scan", "selective_scan_step", "SelectiveTokenMixer", "SelectiveTokenStack",
     "FilterBank", "get_filter_bank",
 ]

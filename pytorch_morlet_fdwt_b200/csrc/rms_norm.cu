@@ -70,10 +70,10 @@ template <typename O> constexpr bool is_quant = false;
 template <> constexpr bool is_quant<E4m3> = true;
 template <> constexpr bool is_quant<Int8> = true;
 
-// V values over their scale, rounded; 8, 4, 2 or 1 bytes in one store.  The division is a product
-// with the scale's reciprocal (`inv`, rounded once): a value is off by one rounding in 32 bits more,
-// which decides only between two neighbours as near as that, and 32768 x 2048 bf16 in groups of 128
-// take 132 us with divisions.
+// V values over their scale, rounded; 8, 4, 2 or 1 bytes in one store.  Both divisions, by the scale
+// and of the largest magnitude, are products with reciprocals: two or three roundings in 32 bits more
+// than one, which decide only between two neighbours in 8 bits as near as that (32768 x 2048 bf16 in
+// groups of 128: 132 us with divisions, 90 us without).
 template <typename O, int V>
 __device__ __forceinline__ void store_quant(O* p, const float* x, float inv) {
   if constexpr (V == 1) {
@@ -99,7 +99,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // The scale of a group whose largest magnitude is m: 1 where all are zero, else at least 2^-126, so
 // that its reciprocal is finite.  NaN stays NaN.
 template <typename O> __device__ __forceinline__ float scale_of(float m) {
-  return m == 0.0f ? 1.0f : max_nan(__fdiv_rn(m, Quant<O>::kMost), 0x1p-126f);
+  return m == 0.0f ? 1.0f : max_nan(m * (1.0f / Quant<O>::kMost), 0x1p-126f);
+}
+__device__ __forceinline__ float inverse(float scale) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
 }
 
 // The largest over the threads of a row, as row_sum adds.
@@ -203,7 +208,7 @@ rms_fwd_kernel(const T* __restrict__ x, const R* __restrict__ residual,
       for (int i = 1; i < IT; ++i) m[0] = max_nan(m[0], m[i]);
       const float scale = scale_of<O>(row_max(m[0], reinterpret_cast<float*>(slots[1])));
       if (in && threadIdx.x == 0) scales[row] = scale;
-      const float inv = __frcp_rn(scale);
+      const float inv = inverse(scale);
 #pragma unroll
       for (int i = 0; i < IT; ++i)
         if (in && i * step < left) store_quant<O, V>(y + at + i * step, v + i * V, inv);
@@ -216,7 +221,7 @@ rms_fwd_kernel(const T* __restrict__ x, const R* __restrict__ residual,
         const float scale = scale_of<O>(m[i]);
         if (in && i * step < left) {
           if (threadIdx.x % lanes == 0) scales[(at + i * step) / group] = scale;
-          store_quant<O, V>(y + at + i * step, v + i * V, __frcp_rn(scale));
+          store_quant<O, V>(y + at + i * step, v + i * V, inverse(scale));
         }
       }
     }
@@ -262,7 +267,7 @@ rms_fwd_long_kernel(const T* __restrict__ x, const R* __restrict__ residual,
       m = max_nan(m, fabsf(static_cast<float>(value(c))));
     const float scale = scale_of<O>(row_max(m, reinterpret_cast<float*>(slots[1])));
     if (threadIdx.x == 0) scales[row] = scale;
-    const float inv = __frcp_rn(scale);
+    const float inv = inverse(scale);
     for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
       const float v = static_cast<float>(value(c));
       store_quant<O, 1>(y + row * dim + c, &v, inv);
@@ -278,7 +283,7 @@ rms_fwd_long_kernel(const T* __restrict__ x, const R* __restrict__ residual,
       for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float scale = scale_of<O>(m);
       if (lane == 0) scales[row * (dim / group) + g] = scale;
-      const float inv = __frcp_rn(scale);
+      const float inv = inverse(scale);
       for (int64_t c = lane; c < group; c += 32) {
         const float v = static_cast<float>(value(g * group + c));
         store_quant<O, 1>(y + row * dim + g * group + c, &v, inv);
@@ -504,7 +509,9 @@ int rms_group(int64_t dim, Pointers rows, Pointers streams, Pointers params) {
   return v == 16 / sizeof(T) && s % 16 == 0 ? v : 0;
 }
 
-// Threads of a row whose 8-bit groups are `lanes` threads wide: at least so many.
+// Threads of a row whose 8-bit groups are `lanes` threads wide: at least so many.  32 elements a
+// thread: with the largest magnitudes beside the sums, 64 (as forward_shape takes) are slower
+// (32768 x 2048 bf16: 125 us; 32: 90, 16: 92, 8: 100).
 inline bool quant_shape(int64_t groups, int v, int lanes, Shape* s) {
   int threads = 32, items = 1;
   while (threads > 1 && threads / 2 >= groups && threads / 2 >= lanes) threads /= 2;
@@ -513,7 +520,7 @@ inline bool quant_shape(int64_t groups, int v, int lanes, Shape* s) {
     *s = {threads, items, 128 / threads, false};
     return lanes <= threads;
   }
-  for (items = v >= 8 ? 2 : 4; items * v <= 32; items *= 2) {
+  for (items = 4; items * v <= 32; items *= 2) {
     const int64_t wide = cdiv(cdiv(groups, items), 32) * 32;
     if (wide <= fwd_max_threads(items * v)) {
       *s = {static_cast<int>(wide), items, 1, false};
@@ -559,7 +566,7 @@ int rms_forward_v(const ForwardCall& c, bool* done) {
                             : launch(std::integral_constant<int, 8>{}, threads);
       });
   }
-  constexpr int most = is_quant<O> ? 32 : (V <= 2 ? 16 : sizeof(A) == 8 ? 32 : 64);
+  constexpr int most = V <= 2 ? 16 : sizeof(A) == 8 ? 32 : 64;
   return with_items<V, most>(
       s.items, [&](auto items) { return launch(items, std::integral_constant<int, 0>{}); });
 }

@@ -13,24 +13,31 @@ reference's parameters).  The forward passes run on this package's fused kernels
   frequencies weights learned per-channel values (or the channel-mixed input).
 - :class:`DecayTokenMixer`, ``(B, L, D) -> (B, L, D)`` (no counterpart in the reference): a causal
   mixer with a state, for training, prompts and single tokens.
+- :class:`SelectiveTokenMixer` and :class:`SelectiveTokenStack`, ``(B, L, D) -> (B, L, D)`` (no
+  counterpart in the reference): a causal mixer whose memory goes by the tokens, and a stack of
+  them.
 """
 
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import nn
 
+from .causal_conv import causal_conv1d, causal_conv1d_step
 from .cwt import CWT1D, morlet_mix_tokens, spectral_softmax
 from .dwt import wavedec, waverec
 from .linear_attention import linear_attention, linear_attention_step
-from .norm import LayerNorm
+from .norm import LayerNorm, RMSNorm
+from .selective_scan import selective_scan, selective_scan_step
 from .wavelets import WaveletLike
 
 __all__ = ["MorletTokenMixer", "WaveletTokenMixer", "MorletAttention", "MorletChannelMixAttention",
-           "DecayTokenMixer"]
+           "DecayTokenMixer", "SelectiveTokenMixer", "SelectiveTokenStack"]
+
+State = Tuple[torch.Tensor, torch.Tensor]
 
 
 def _randn_over(rows: int, cols: int, fan: int) -> torch.Tensor:
@@ -331,3 +338,156 @@ class DecayTokenMixer(nn.Module):
         q, k, v = self._qkv(x)
         mixed = linear_attention_step(q, k, v, self.log_decay(x.device), state, slots=slots)
         return x + self.out_proj(mixed.flatten(-2))
+
+
+class SelectiveTokenMixer(nn.Module):
+    """Causal token mixing by a selective state space scan after a short convolution, with the norm
+    before it and the residual around it::
+
+        u, gate = in_proj(norm(x));  u = silu(convolution(u))
+        dt, b, c = x_proj(u)
+        y = x + out_proj(scan(u, dt_proj(dt), -exp(log_rate), b, c, skip, gate, dt_bias))
+
+    Unlike :class:`DecayTokenMixer`, whose heads forget at fixed rates, every token sets the size of
+    its own step, and with it what its channels forget and take in.  It answers token by token: a
+    prompt's :meth:`forward` returns the state that :meth:`step` carries on, a pair of the
+    convolution's last inputs ``(B, conv_size - 1, E)`` and the scan's states ``(B, E, N)``.
+
+    Args: ``dim`` (D), ``state_size`` (N, numbers a channel remembers), ``conv_size`` (taps of the
+    convolution), ``expand`` (E = expand * dim channels inside), ``dt_rank`` (rank of the steps'
+    projection, ``ceil(dim / 16)`` by default), ``eps`` (of the norm).
+    """
+
+    def __init__(self, dim: int, state_size: int = 16, conv_size: int = 4, expand: int = 2,
+                 dt_rank: Optional[int] = None, eps: float = 1e-6):
+        super().__init__()
+        self.inner, self.state_size, self.conv_size = expand * dim, state_size, conv_size
+        self.dt_rank = -(-dim // 16) if dt_rank is None else dt_rank
+        self.norm = RMSNorm(dim, eps)
+        self.in_proj = nn.Linear(dim, 2 * self.inner, bias=False)
+        self.conv_weight = nn.Parameter(_randn_over(self.inner, conv_size, conv_size))
+        self.conv_bias = nn.Parameter(torch.zeros(self.inner))
+        self.x_proj = nn.Linear(self.inner, self.dt_rank + 2 * state_size, bias=False)
+        self.dt_proj = nn.Linear(self.dt_rank, self.inner, bias=False)
+        # steps of 1/1000 to 1/10 to begin with: the inverse of log(1 + e^v)
+        size = torch.exp(torch.rand(self.inner) * math.log(100.0) + math.log(1e-3))
+        self.dt_bias = nn.Parameter(torch.log(torch.expm1(size)))
+        self.log_rate = nn.Parameter(torch.log(torch.arange(1, state_size + 1,
+                                                            dtype=torch.float32)
+                                               ).repeat(self.inner, 1))
+        self.skip = nn.Parameter(torch.ones(self.inner))
+        self.out_proj = nn.Linear(self.inner, dim, bias=False)
+
+    def init_state(self, batch: int, device, dtype: torch.dtype = torch.float32) -> State:
+        """Zero states for ``batch`` sequences (or slots of a pool) of ``dtype`` tokens."""
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        return (torch.zeros(batch, self.conv_size - 1, self.inner, device=device, dtype=dtype),
+                torch.zeros(batch, self.inner, self.state_size, device=device, dtype=wide))
+
+    def _rates(self) -> torch.Tensor:
+        wide = torch.float64 if self.log_rate.dtype == torch.float64 else torch.float32
+        return -torch.exp(self.log_rate.to(wide))
+
+    def _steps(self, u: torch.Tensor):
+        low, b, c = self.x_proj(u).split((self.dt_rank, self.state_size, self.state_size), -1)
+        return self.dt_proj(low), b.unsqueeze(-2), c.unsqueeze(-2)
+
+    def mix(self, h: torch.Tensor, state: Optional[State] = None,
+            lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, State]:
+        """What is added to the residual, from the normed tokens ``h (B, L, D)``, and the state."""
+        u, gate = self.in_proj(h).split(self.inner, -1)
+        before, start = (None, None) if state is None else state
+        u, before = causal_conv1d(u, self.conv_weight, self.conv_bias, "silu", before, lengths)
+        dt, b, c = self._steps(u)
+        y, last = selective_scan(u, dt, self._rates(), b, c, self.skip, gate, self.dt_bias, True,
+                                 start, lengths)
+        return self.out_proj(y), (before, last)
+
+    def mix_step(self, h: torch.Tensor, state: State,
+                 slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """:meth:`mix` of one token for each sequence, ``h (B, D)``; ``state`` is updated in place."""
+        u, gate = self.in_proj(h).split(self.inner, -1)
+        u = causal_conv1d_step(u, self.conv_weight, state[0], self.conv_bias, "silu", slots)
+        dt, b, c = self._steps(u)
+        y = selective_scan_step(u, dt, self._rates(), b, c, state[1], self.skip, gate,
+                                self.dt_bias, True, slots)
+        return self.out_proj(y)
+
+    def forward(self, x: torch.Tensor, state: Optional[State] = None,
+                lengths: Optional[torch.Tensor] = None, return_state: bool = False):
+        """``x (B, L, D)`` -> ``y (B, L, D)``, or ``(y, state)`` with ``return_state``; ``state``
+        and ``lengths`` as ``initial_state`` and ``lengths`` of
+        :func:`~pytorch_morlet_fdwt_b200.selective_scan`."""
+        if x.dim() != 3:
+            raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
+        mixed, state = self.mix(self.norm(x), state, lengths)
+        y = x + mixed
+        return (y, state) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: State,
+             slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token for each sequence: ``x (B, D)`` -> ``y (B, D)``; ``state`` (of a prompt, or
+        pools indexed by ``slots``) is updated in place."""
+        if x.dim() != 2:
+            raise ValueError(f"expected (B, D) input, got shape {tuple(x.shape)}")
+        return x + self.mix_step(self.norm(x), state, slots)
+
+
+class SelectiveTokenStack(nn.Module):
+    """``depth`` :class:`SelectiveTokenMixer` layers and a norm after them.  Each layer's result is
+    added to the residual in the kernel of the next norm, which reads both and writes the sum and
+    its norm (:func:`~pytorch_morlet_fdwt_b200.rms_norm`).  Other arguments are the layers'."""
+
+    def __init__(self, dim: int, depth: int, state_size: int = 16, conv_size: int = 4,
+                 expand: int = 2, dt_rank: Optional[int] = None, eps: float = 1e-6):
+        super().__init__()
+        if depth < 1:
+            raise ValueError(f"depth must be at least 1, got {depth}")
+        self.layers = nn.ModuleList(
+            SelectiveTokenMixer(dim, state_size, conv_size, expand, dt_rank, eps)
+            for _ in range(depth))
+        self.norm = RMSNorm(dim, eps)
+
+    def init_state(self, batch: int, device, dtype: torch.dtype = torch.float32) -> List[State]:
+        """Zero states of every layer."""
+        return [layer.init_state(batch, device, dtype) for layer in self.layers]
+
+    def _run(self, x: torch.Tensor, mix):
+        total, mixed = x, None
+        for i, layer in enumerate(self.layers):
+            if mixed is None:
+                h = layer.norm(total)
+            else:
+                h, total = layer.norm(mixed, total)
+            mixed = mix(i, layer, h)
+        return self.norm(mixed, total)[0]
+
+    def forward(self, x: torch.Tensor, state: Optional[List[State]] = None,
+                lengths: Optional[torch.Tensor] = None, return_state: bool = False):
+        """``x (B, L, D)`` -> ``y (B, L, D)``, or ``(y, state)`` with ``return_state``; arguments
+        as :meth:`SelectiveTokenMixer.forward`, ``state`` a list of the layers'."""
+        if x.dim() != 3:
+            raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
+        if state is not None and len(state) != len(self.layers):
+            raise ValueError(f"expected {len(self.layers)} states, got {len(state)}")
+        states = []
+
+        def mix(i, layer, h):
+            mixed, last = layer.mix(h, None if state is None else state[i], lengths)
+            states.append(last)
+            return mixed
+
+        y = self._run(x, mix)
+        return (y, states) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: List[State],
+             slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token for each sequence, ``x (B, D)`` -> ``y (B, D)``; the states are updated in
+        place."""
+        if x.dim() != 2:
+            raise ValueError(f"expected (B, D) input, got shape {tuple(x.shape)}")
+        if len(state) != len(self.layers):
+            raise ValueError(f"expected {len(self.layers)} states, got {len(state)}")
+        return self._run(x, lambda i, layer, h: layer.mix_step(h, state[i], slots))
