@@ -14,6 +14,7 @@ import threading
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfdwt_b200.so")
@@ -162,6 +163,17 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def once(backward):
+    """A backward pass that is differentiable once, as ``once_differentiable`` makes it, without
+    that one's 7 us a call where no graph of the backward pass is asked for."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 def needs_grad(*tensors) -> bool:
     """Whether autograd follows a call of these tensors."""
     if torch.is_grad_enabled():
@@ -244,6 +256,12 @@ def f64_array(values):
 def ptr_array(tensors):
     return (ctypes.c_void_p * max(1, len(tensors)))(
         *[None if t is None else t.data_ptr() for t in tensors])
+
+
+def empty_like(t: torch.Tensor, dtype=None) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape and device (2 us less a call than
+    ``torch.empty`` with a shape and a device)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def workspace(nbytes: int, device: torch.device):

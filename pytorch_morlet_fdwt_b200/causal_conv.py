@@ -18,7 +18,6 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -82,8 +81,9 @@ def _check_state(state, shape, dtype):
 def _forward(x, weight, bias, initial, lengths, plan):
     d, desc, _ = plan
     dev = x.device
-    y = torch.empty((d.batch, d.length, d.dim), device=dev, dtype=x.dtype)
-    final = torch.empty((d.batch, d.width - 1, d.dim), device=dev, dtype=x.dtype)
+    y = _lib.empty_like(x)
+    final = (x.new_empty((d.batch, d.width - 1, d.dim)) if initial is None
+             else _lib.empty_like(initial))
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_causal_conv1d_forward(
             desc, x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial), _ptr(lengths),
@@ -102,7 +102,7 @@ class _CausalConvFunction(torch.autograd.Function):
         return _forward(x, weight, bias, initial, lengths, plan)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, dy, d_final):
         x, weight, bias, initial, lengths = ctx.saved_tensors
         if dy is None and d_final is None:
@@ -118,7 +118,7 @@ class _CausalConvFunction(torch.autograd.Function):
         if d_final is not None:
             d_final = d_final.contiguous()
         need_x, need_w, need_b, need_i = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_x else None
+        dx = _lib.empty_like(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
         di = torch.empty_like(initial) if need_i else None
@@ -199,7 +199,7 @@ def causal_conv1d_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     if slots is not None:
         slots = _indexes(slots, d.batch, -1, pool, "slots")
     dev = x.device
-    y = torch.empty((d.batch, d.dim), device=dev, dtype=x.dtype)
+    y = _lib.empty_like(x)
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_causal_conv1d_step(
             desc, x.data_ptr(), weight.data_ptr(), _ptr(bias), state.data_ptr(), pool,

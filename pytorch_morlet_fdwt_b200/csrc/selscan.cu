@@ -29,36 +29,38 @@ scan_bc_kernel(const typename AccOf<T>::type* __restrict__ part, const int32_t* 
   out[((b * length + t) * groups + g) * states + n] = from_acc<T>(sum);
 }
 
-// Columns summed over rows in a fixed order: 32 columns by 8 row lanes a block.  Column c goes to
-// out[c / width * keep + c % width] where c % width < keep.
+// da, dskip and ddt_bias: columns summed over the rows (sequences and segments) in a fixed order, 32
+// columns by 8 row lanes a block.  A row of `parts_a` has dim x padded columns, one of `parts_ch`
+// 2 dim.
 template <typename A>
 __global__ void __launch_bounds__(256)
-scan_rows_kernel(const A* __restrict__ part, int64_t rows, int64_t stride, int64_t cols, int width,
-                 int keep, A* __restrict__ out) {
+scan_rows_kernel(const A* __restrict__ parts_a, const A* __restrict__ parts_ch, int64_t rows,
+                 int64_t dim, int states, int padded, A* __restrict__ da, A* __restrict__ dskip,
+                 A* __restrict__ dbias) {
   __shared__ A cells[8][33];
-  const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x;
+  const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x, cols_a = dim * padded;
+  const bool of_a = c < cols_a;
+  A* out = nullptr;
+  if (of_a) {
+    if (da != nullptr && c % padded < states) out = da + c / padded * states + c % padded;
+  } else if (c < cols_a + dim) {
+    if (dskip != nullptr) out = dskip + (c - cols_a);
+  } else if (c < cols_a + 2 * dim && dbias != nullptr) {
+    out = dbias + (c - cols_a - dim);
+  }
   A sum = A(0);
-  if (c < cols) {
+  if (out != nullptr) {
+    const A* q = of_a ? parts_a + c : parts_ch + (c - cols_a);
+    const int64_t stride = of_a ? cols_a : 2 * dim;
 #pragma unroll 4
-    for (int64_t r = threadIdx.y; r < rows; r += 8) sum += part[r * stride + c];
+    for (int64_t r = threadIdx.y; r < rows; r += 8) sum += q[r * stride];
   }
   cells[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
-  if (threadIdx.y != 0 || c >= cols || c % width >= keep) return;
+  if (threadIdx.y != 0 || out == nullptr) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) sum += cells[k][threadIdx.x];
-  out[c / width * keep + c % width] = sum;
-}
-
-template <typename A>
-int sum_rows(const A* part, int64_t rows, int64_t stride, int64_t cols, int width, int keep,
-             void* out, cudaStream_t stream) {
-  if (out == nullptr) return FDWT_OK;
-  const int st = pre_launch(stream);
-  if (st != FDWT_OK) return st;
-  scan_rows_kernel<A><<<static_cast<unsigned>(cdiv(cols, 32)), dim3(32, 8), 0, stream>>>(
-      part, rows, stride, cols, width, keep, static_cast<A*>(out));
-  return launch_status();
+  *out = sum;
 }
 
 constexpr int64_t kMostTokens = int64_t(1) << 30;
@@ -328,13 +330,15 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
       st = launch_status();
       if (st != FDWT_OK) return st;
     }
-    st = sum_rows(static_cast<const A*>(p.part_a), rows, desc->dim * np, desc->dim * np, np,
-                  desc->states, da, s);
+    if (da == nullptr && dskip == nullptr && ddt_bias == nullptr) return FDWT_OK;
+    const int64_t columns = cdiv(desc->dim * (np + 2), 32);
+    if (columns > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
+    st = pre_launch(s);
     if (st != FDWT_OK) return st;
-    const A* ch = static_cast<const A*>(p.part_ch);
-    st = sum_rows(ch, rows, 2 * desc->dim, desc->dim, 1, 1, dskip, s);
-    if (st != FDWT_OK) return st;
-    return sum_rows(ch + desc->dim, rows, 2 * desc->dim, desc->dim, 1, 1, ddt_bias, s);
+    scan_rows_kernel<A><<<static_cast<unsigned>(columns), dim3(32, 8), 0, s>>>(
+        static_cast<const A*>(p.part_a), static_cast<const A*>(p.part_ch), rows, desc->dim,
+        desc->states, np, static_cast<A*>(da), static_cast<A*>(dskip), static_cast<A*>(ddt_bias));
+    return launch_status();
   });
 }
 

@@ -151,8 +151,7 @@ def _rms_forward(x, residual, weight, eps: float, codes, want_rstd: bool):
     total = None if residual is None else torch.empty_like(residual)
     rstd = None
     if want_rstd:
-        rstd = torch.empty(rows, device=dev,
-                           dtype=torch.float64 if codes[0] == 1 else torch.float32)
+        rstd = x.new_empty(rows, dtype=torch.float64 if codes[0] == 1 else torch.float32)
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_rms_norm_forward(
             *codes, rows, dim, x.data_ptr(), _ptr(residual), _ptr(weight), eps, y.data_ptr(),
@@ -178,7 +177,7 @@ class _RMSNormFunction(torch.autograd.Function):
         return y if total is None else (y, total)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, dy, dtotal=None):
         total, weight, rstd = ctx.saved_tensors
         need_x, need_r, need_w, _, _ = ctx.needs_input_grad
@@ -196,9 +195,9 @@ class _RMSNormFunction(torch.autograd.Function):
         rows = total.numel() // dim
         dev = total.device
         need = need_x or need_r
-        dx = torch.empty(total.shape, device=dev, dtype=dtype) if need else None
+        dx = torch.empty_like(dy) if need else None
         dr = torch.empty_like(total) if need_r and stream_code != code else None
-        dw = torch.empty(dim, device=dev, dtype=_lib.DTYPE_OF[param]) if need_w else None
+        dw = torch.empty_like(weight) if need_w else None
         with _lib.device_guard(dev):
             nws = _rms_backward_ws(code, rows, dim, int(need_w), dev.index)
             ws = _lib.workspace(nws, dev)
@@ -280,8 +279,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     if _lib.needs_grad(x, weight, residual) or _lib.has_tangent(x, weight, residual):
         raise RuntimeError("rms_norm_quantized has no gradient: use rms_norm, or torch.no_grad()")
     dev = x.device
-    q = torch.empty(x.shape, device=dev, dtype=dtype)
-    scales = torch.empty(*x.shape[:-1], dim // group, device=dev, dtype=torch.float32)
+    q = torch.empty_like(x, dtype=dtype)
+    scales = x.new_empty((*x.shape[:-1], dim // group), dtype=torch.float32)
     total = None if residual is None else torch.empty_like(residual)
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_rms_norm_quantized(

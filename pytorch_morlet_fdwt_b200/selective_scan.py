@@ -22,7 +22,6 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -117,9 +116,10 @@ def _parameter(name: str, t: Optional[torch.Tensor], shape, dtype) -> Optional[t
 def _forward(x, dt, a, b, c, skip, gate, dt_bias, initial, lengths, plan, keep: bool):
     d, desc, nws, ncheck, _, acc = plan
     dev = x.device
-    y = torch.empty((d.batch, d.length, d.dim), device=dev, dtype=x.dtype)
-    final = torch.empty((d.batch, d.dim, d.states), device=dev, dtype=acc)
-    check = torch.empty(ncheck, device=dev, dtype=torch.uint8) if keep else None
+    y = _lib.empty_like(x)
+    final = (x.new_empty((d.batch, d.dim, d.states), dtype=acc) if initial is None
+             else _lib.empty_like(initial))
+    check = x.new_empty(ncheck, dtype=torch.uint8) if keep else None
     with _lib.device_guard(dev):
         ws = _lib.workspace(nws, dev)
         st = _lib.load().fdwt_selscan_forward(
@@ -145,7 +145,7 @@ class _SelectiveScanFunction(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, dy, d_final):
         x, dt, a, b, c, skip, gate, dt_bias, initial, lengths, check = ctx.saved_tensors
         if dy is None and d_final is None:
@@ -161,12 +161,9 @@ class _SelectiveScanFunction(torch.autograd.Function):
             d_final = d_final.contiguous()
         need = ctx.needs_input_grad
 
-        def like(t, wanted=True):
-            return torch.empty(t.shape, device=dev, dtype=t.dtype) if wanted else None
-
-        dx, ddt = like(x), like(dt)
-        dgate = None if gate is None else like(gate)
-        da, db, dc, dskip, dbias, di = (like(t, need[i]) for i, t in
+        like = _lib.empty_like
+        dx, ddt, dgate = like(x), like(dt), None if gate is None else like(gate)
+        da, db, dc, dskip, dbias, di = (like(t) if need[i] else None for i, t in
                                         ((2, a), (3, b), (4, c), (5, skip), (7, dt_bias),
                                          (8, initial)))
         _, desc, _, _, nws, _ = plan
@@ -258,7 +255,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     if slots is not None:
         slots = _indexes(slots, d.batch, -1, pool, "slots")
     dev = x.device
-    y = torch.empty((d.batch, d.dim), device=dev, dtype=x.dtype)
+    y = _lib.empty_like(x)
     with _lib.device_guard(dev):
         st = _lib.load().fdwt_selscan_step(
             desc, x.data_ptr(), dt.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(),
