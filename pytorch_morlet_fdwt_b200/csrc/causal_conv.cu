@@ -24,14 +24,6 @@ struct ConvCall {
   cudaStream_t stream;
 };
 
-// 1 / (1 + e^-p): of a few roundings' error in 32 bits for rows of 32 bits, and by the fast
-// exponential and division for 16-bit rows, whose rounding is 2^12 times theirs.
-template <typename T, typename A> __device__ __forceinline__ A sigmoid(A p) {
-  if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-p));
-  else if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-p));
-  else return 1.0 / (1.0 + exp(-p));
-}
-
 // V channels' values: pairs of them, or one.
 template <typename A, int V> struct Channels {
   using E = std::conditional_t<V == 1, A, Two<A>>;
@@ -60,6 +52,30 @@ template <typename A, int V> struct Channels {
     set(zero);
   }
 };
+
+// 1 / (1 + e^-p): of a few roundings' error in 32 bits for rows of 32 bits, and by the fast
+// exponential and reciprocal, on pairs, for 16-bit rows, whose rounding is 2^12 times theirs.
+template <typename T, int V, typename A>
+__device__ __forceinline__ Channels<A, V> sigmoid(const Channels<A, V>& p) {
+  using E = typename Channels<A, V>::E;
+  Channels<A, V> r;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int m = 0; m < Channels<A, V>::M; ++m)
+      r.e[m] = reciprocal(add(exp_2(mul(p.e[m], splat<E>(-static_cast<float>(kLog2e)))),
+                              splat<E>(1.0f)));
+  } else {
+    A v[V];
+    p.get(v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if constexpr (sizeof(T) == 4) v[j] = 1.0f / (1.0f + expf(-v[j]));
+      else v[j] = 1.0 / (1.0 + exp(-v[j]));
+    }
+    r.set(v);
+  }
+  return r;
+}
 
 // One parameter of the rows' type or of 32 bits.
 template <typename T>
@@ -193,12 +209,13 @@ conv_fwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
 #pragma unroll
         for (int i = 1; i < W; ++i) p.e[m] = fma(w[i].e[m], win[u + i].e[m], p.e[m]);
       }
+      if (silu) {
+        const C g = sigmoid<T, V, A>(p);
+#pragma unroll
+        for (int m = 0; m < C::M; ++m) p.e[m] = mul(p.e[m], g.e[m]);
+      }
       A v[V];
       p.get(v);
-      if (silu) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= sigmoid<T>(v[j]);
-      }
       G::store(out, v);
       out += dim;
     };
@@ -307,12 +324,17 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
 #pragma unroll
           for (int i = 1; i < W; ++i) p.e[m] = fma(w[i].e[m], win[i].e[m], p.e[m]);
         }
-        p.get(v);
+        const C g = sigmoid<T, V, A>(p);
+        C slope;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const A s = sigmoid<T>(v[j]);
-          q[j] *= s * (A(1) + v[j] * (A(1) - s));
+        for (int m = 0; m < C::M; ++m) {  // g (1 + p (1 - g))
+          using E = typename C::E;
+          const E rest = fma(g.e[m], splat<E>(-1.0f), splat<E>(1.0f));
+          slope.e[m] = mul(g.e[m], fma(p.e[m], rest, splat<E>(1.0f)));
         }
+        slope.get(v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[j] *= v[j];
       }
       // (chosen, not multiplied by zero: what the window holds may be no number)
       C d;
@@ -465,7 +487,11 @@ conv_step_kernel(const T* __restrict__ x, const void* __restrict__ weight,
   }
   if (silu) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) p[j] *= sigmoid<T>(p[j]);
+    for (int j = 0; j < V; ++j) {
+      Channels<A, 1> one;
+      one.e[0] = p[j];
+      p[j] *= sigmoid<T, 1, A>(one).e[0];
+    }
   }
   G::store(y + b * dim + c, p);
 }

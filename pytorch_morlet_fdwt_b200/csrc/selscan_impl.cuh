@@ -21,24 +21,7 @@ template <typename A> __device__ __forceinline__ Two<A> high(const Four<A>& q) {
   return two(q.v[2], q.v[3]);
 }
 
-// 2^x: rates are kept times log2 e.
-__device__ __forceinline__ float exp_2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ double exp_2(double x) { return exp2(x); }
-template <typename A> __device__ __forceinline__ Two<A> exp_2(Two<A> x) {
-  return two(exp_2(first(x)), exp_2(second(x)));
-}
-constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
-__device__ __forceinline__ float reciprocal(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ Two<float> both(float x) { return two(x, x); }
 // e^-|v| of two values: the product with log2 e is rounded, so what it lost corrects the result.
 __device__ __forceinline__ Two<float> neg_exp(float v, float w) {
   constexpr float kHigh = 1.442695021629333f, kLow = 1.92596299e-8f;  // log2 e in two parts
