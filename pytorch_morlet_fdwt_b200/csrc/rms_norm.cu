@@ -228,9 +228,11 @@ rms_fwd_kernel(const T* __restrict__ x, const R* __restrict__ residual,
   }
 }
 
-// Rows too long for the registers of a block, and 8-bit groups that the lanes of a warp do not
-// share evenly: passes over the row, which find it in L2.
-template <typename T, typename R, typename P, typename O>
+// Rows too long for the registers of a block, rows off 16-byte boundaries with a result in 8 bits or an
+// fp32 residual, and 8-bit groups that the lanes of a warp do not share evenly: element by element,
+// the row kept in shared memory between the passes (CACHED) where that holds it, else found in L2.
+constexpr int64_t kCachedBytes = 32768;
+template <typename T, typename R, typename P, typename O, bool CACHED>
 __global__ void __launch_bounds__(1024)
 rms_fwd_long_kernel(const T* __restrict__ x, const R* __restrict__ residual,
                     const P* __restrict__ weight, O* __restrict__ y, R* total,
@@ -238,55 +240,66 @@ rms_fwd_long_kernel(const T* __restrict__ x, const R* __restrict__ residual,
                     int64_t group, int64_t dim, typename AccOf<T>::type eps) {
   using A = typename AccOf<T>::type;
   __shared__ A slots[2][32];
-  const int64_t row = blockIdx.x;
-  const T* xr = x + row * dim;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  A* cache = reinterpret_cast<A*>(smem_raw);
+  const int64_t row = blockIdx.x, at = row * dim;
   A sum[1] = {A(0)};
+#pragma unroll 4
   for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
-    A v = to_acc(xr[c]);
+    A v = to_acc(x[at + c]);
     if (residual != nullptr) {
-      const R t = from_acc<R>(v + A(to_acc(residual[row * dim + c])));
-      total[row * dim + c] = t;
+      const R t = from_acc<R>(v + A(to_acc(residual[at + c])));
+      total[at + c] = t;
       v = to_acc(t);
     }
+    if (CACHED) cache[c] = v;
     sum[0] += v * v;
   }
   row_sum(sum, slots[0]);
   const A rstd = inv_sqrt(sum[0] / A(dim) + eps);
   if (rstd_out != nullptr && threadIdx.x == 0) rstd_out[row] = rstd;
   auto value = [&](int64_t c) {
-    A v = (residual != nullptr ? A(to_acc(total[row * dim + c])) : A(to_acc(xr[c]))) * rstd;
+    A v;
+    if (CACHED) v = cache[c];
+    else v = residual != nullptr ? A(to_acc(total[at + c])) : A(to_acc(x[at + c]));
+    v *= rstd;
     if (weight != nullptr) v *= A(to_acc(weight[c]));
     return v;
   };
   if constexpr (!is_quant<O>) {
-    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
-      y[row * dim + c] = from_acc<T>(value(c));
+#pragma unroll 4
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) y[at + c] = from_acc<T>(value(c));
   } else if (group == dim) {
     float m = 0.0f;
-    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
-      m = max_nan(m, fabsf(static_cast<float>(value(c))));
+#pragma unroll 4
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
+      const A v = value(c);
+      if (CACHED) cache[c] = v;
+      m = max_nan(m, fabsf(static_cast<float>(v)));
+    }
     const float scale = scale_of<O>(row_max(m, reinterpret_cast<float*>(slots[1])));
     if (threadIdx.x == 0) scales[row] = scale;
     const float inv = inverse(scale);
+#pragma unroll 4
     for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
-      const float v = static_cast<float>(value(c));
-      store_quant<O, 1>(y + row * dim + c, &v, inv);
+      const float v = static_cast<float>(CACHED ? cache[c] : value(c));
+      store_quant<O, 1>(y + at + c, &v, inv);
     }
   } else {
-    __syncthreads();  // a group's lanes read sums that other threads have stored
+    __syncthreads();  // a group's lanes read what other threads have stored
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     for (int64_t g = threadIdx.x >> 5; g < dim / group; g += warps) {
       float m = 0.0f;
-      for (int64_t c = lane; c < group; c += 32)
-        m = max_nan(m, fabsf(static_cast<float>(value(g * group + c))));
+      for (int64_t c = g * group + lane; c < (g + 1) * group; c += 32)
+        m = max_nan(m, fabsf(static_cast<float>(value(c))));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float scale = scale_of<O>(m);
       if (lane == 0) scales[row * (dim / group) + g] = scale;
       const float inv = inverse(scale);
-      for (int64_t c = lane; c < group; c += 32) {
-        const float v = static_cast<float>(value(g * group + c));
-        store_quant<O, 1>(y + row * dim + g * group + c, &v, inv);
+      for (int64_t c = g * group + lane; c < (g + 1) * group; c += 32) {
+        const float v = static_cast<float>(value(c));
+        store_quant<O, 1>(y + at + c, &v, inv);
       }
     }
   }
@@ -587,13 +600,19 @@ template <typename T, typename R, typename P, typename O> int rms_forward(const 
   if (c.rows > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   st = pre_launch(c.stream);
   if (st != FDWT_OK) return st;
-  const int threads = c.dim <= 256 ? 128 : (c.dim <= 2048 ? 256 : 1024);
-  rms_fwd_long_kernel<T, R, P, O><<<static_cast<unsigned>(c.rows), threads, 0, c.stream>>>(
-      static_cast<const T*>(c.x), static_cast<const R*>(c.residual),
-      static_cast<const P*>(c.weight), static_cast<O*>(c.y), static_cast<R*>(c.total),
-      static_cast<A*>(c.rstd), static_cast<float*>(c.scales), c.group, c.dim,
-      static_cast<A>(c.eps));
-  return launch_status();
+  auto launch = [&](auto cached) {
+    constexpr bool CACHED = decltype(cached)::value;
+    const int threads = c.dim <= 1024 ? 128 : (c.dim <= 4096 ? 256 : 1024);
+    rms_fwd_long_kernel<T, R, P, O, CACHED>
+        <<<static_cast<unsigned>(c.rows), threads, CACHED ? c.dim * sizeof(A) : 0, c.stream>>>(
+            static_cast<const T*>(c.x), static_cast<const R*>(c.residual),
+            static_cast<const P*>(c.weight), static_cast<O*>(c.y), static_cast<R*>(c.total),
+            static_cast<A*>(c.rstd), static_cast<float*>(c.scales), c.group, c.dim,
+            static_cast<A>(c.eps));
+    return launch_status();
+  };
+  return c.dim * int64_t(sizeof(A)) <= kCachedBytes ? launch(std::true_type{})
+                                                    : launch(std::false_type{});
 }
 
 struct BackwardCall {

@@ -63,7 +63,7 @@ template <typename T> int scan_step(const ScanArgs& p, int lanes, const int32_t*
                                     void* state, cudaStream_t stream);
 
 // Channels of a thread, and of a block.
-constexpr int scan_fwd_channels(int ln) { return ln == 1 ? 1 : (ln <= 4 ? 2 : 4); }
+constexpr int scan_fwd_channels(int ln) { return ln == 1 ? 1 : 2; }
 constexpr int scan_fwd_tile(int ln) { return 4 * (32 / ln) * scan_fwd_channels(ln); }
 constexpr int scan_bwd_channels(int ln, bool fp64) { return ln <= 2 || (fp64 && ln <= 8) ? 1 : 2; }
 constexpr int scan_bwd_tile(int ln, bool fp64) {

@@ -333,7 +333,7 @@ enum ScanMode { MAIN, STATES, REVERSE };
 template <typename A> constexpr int scan_fwd_tokens() { return sizeof(A) == 8 ? 8 : 16; }
 
 template <typename T, int LN, int NC, int MODE>
-__global__ void __launch_bounds__(128, sizeof(T) == 8 ? 1 : (NC <= 2 ? 4 : 3))
+__global__ void __launch_bounds__(128, sizeof(T) == 8 ? 1 : 4)
 scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
   using A = typename AccOf<T>::type;
   constexpr int LD = 32 / LN, CT = 4 * LD * NC, TT = scan_fwd_tokens<A>();
@@ -473,7 +473,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     bc.store(states);
     if (i + 1 < steps) fetch(begin(i + 1));
     __syncthreads();
-#pragma unroll(MODE == MAIN && NC <= 2 ? TT / 8 : 1)
+#pragma unroll(MODE == MAIN ? TT / 8 : 1)
     for (int s = 0; s < TT; s += 8) {
       if (MODE == MAIN && p.check != nullptr && s < left + row0) {
 #pragma unroll
@@ -513,10 +513,10 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
       if constexpr (MODE == MAIN) {
         fold_swapped<8, NC, LN, 1>(y);
         fold<8, OTHERS, KEPT>(y, lane);
-        constexpr int OWN = 8 / OTHERS;
+        constexpr int OWN = 8 >= OTHERS ? 8 / OTHERS : 1, SAME = OTHERS > 8 ? OTHERS / 8 : 1;
 #pragma unroll
         for (int o = 0; o < OWN; ++o)
-          sums[(s + nl / KEPT * OWN + o) * PAD + cl + (LN == 1 ? 0 : swap)] = y[o];
+          sums[(s + nl / KEPT / SAME * OWN + o) * PAD + cl + (LN == 1 ? 0 : swap)] = y[o];
       }
     }
     __syncthreads();
