@@ -427,6 +427,10 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     rows(pd, p.dts[1], dr, left);
     on(px, xs);
     on(pd, p.dts[1]);
+    if (gated) {
+      rows(pg, p.gs[1], zr, left);
+      on(pg, p.gs[1]);
+    }
     bc.fetch(p, static_cast<int>(w.count - t < TT ? w.count - t : TT), MODE == REVERSE ? -TT : TT);
   };
 
@@ -436,11 +440,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
   for (int64_t i = 0; i < steps; ++i) {
     const int64_t t = begin(i);
     const int left = left_at(t);
-    Raw4<T> xc[I::IT];
-    if (gated) {
-      rows(pg, p.gs[1], zr, left);
-      on(pg, p.gs[1]);
-    }
+    Raw4<T> xc[I::IT], zc[I::IT];
 #pragma unroll
     for (int q = 0; q < I::IT; ++q) {
       const int row = row0 + q * I::ROWS;
@@ -468,7 +468,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
       Four<A>* to = reinterpret_cast<Four<A>*>(slots + row * CT + col);
       to[0] = {out[0].delta, out[0].u, out[1].delta, out[1].u};
       to[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
-      xc[q] = xr[q];
+      xc[q] = xr[q], zc[q] = zr[q];
     }
     bc.store(states);
     if (i + 1 < steps) fetch(begin(i + 1));
@@ -535,7 +535,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
         }
         if (gated) {
           A z[4], g[4];
-          Quad<T>::values(zr[q], z);
+          Quad<T>::values(zc[q], z);
           sigmoid_at<sizeof(T) == 2>(z, g);
 #pragma unroll
           for (int j = 0; j < 4; ++j) y[j] *= z[j] * g[j];
