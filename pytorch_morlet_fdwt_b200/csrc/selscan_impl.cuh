@@ -688,18 +688,22 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
                         ((w.b * ((p.length + 7) / 8) + last / 8) * p.dim + w.d0 + cl) * LN + nl;
   int64_t result = mine * p.dim;
   part_bc += last * 2 * NP;
-  if (steps > 0) fetch(last);
-  for (int64_t i = steps - 1; i >= 0; --i) {
-    const int64_t t = w.t0 + i * TT;
-    const int left = left_at(t);
-    Four<A> start[NC];
+  Four<A> start[NC];
+  auto fetch_start = [&] {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       start[k] = {A(0), A(0), A(0), A(0)};
-      const int c = cl + (k ^ swap);
-      if (c < w.width)
-        start[k] = kept[(k ^ swap) * LN];
+      if (cl + (k ^ swap) < w.width) start[k] = kept[(k ^ swap) * LN];
     }
+    kept -= p.dim * LN;
+  };
+  if (steps > 0) {
+    fetch(last);
+    fetch_start();
+  }
+  for (int64_t i = steps - 1; i >= 0; --i) {
+    const int64_t t = w.t0 + i * TT;
+    const int left = left_at(t);
     // kept for the results: x, the step's slope, dy silu'(gate)
     A xk[I::IT][4], slope[I::IT][4], opening[I::IT][4];
 #pragma unroll
@@ -736,7 +740,6 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
       st[1] = {out[2].delta, out[2].u, out[3].delta, out[3].u};
       *reinterpret_cast<Four<A>*>(dps + row * CT + col) = dp;
     }
-    kept -= p.dim * LN;
     bc.template store_orders<COPIES>(states);
     if (i > 0) fetch(t - TT);
     __syncthreads();
@@ -779,6 +782,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
           h[u + 1][k][1] = fma(e[u][k][1], h[u][k][1], mul(u2, high(bq[u])));
         }
       }
+      // (from here on nothing needs these; the next step's are there when it does)
+      if (half == 0 && i > 0) fetch_start();
       // sums over states and channels: each token's own first steps at once, so that few values live
       constexpr int LEFT = 4 / COPIES;  // states of each run (token, b or c) that a lane keeps
       A through[SUB], pre[SUB], by_rate[SUB], v[SUB * 2 * LEFT];
