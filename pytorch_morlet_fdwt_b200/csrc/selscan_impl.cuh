@@ -594,6 +594,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
   A* dps = reinterpret_cast<A*>(slots + TT * CT);                     // [TT][CT]
   A* joined = dps + TT * CT;                                          // [4 warps][TT][2][NP]
   A* sums = joined + 4 * TT * 2 * NP;                                 // [3][TT][PAD]: g b, p, a k
+  Four<A>* params = reinterpret_cast<Four<A>*>(sums + 3 * TT * PAD);  // the threads' dt_bias and skip
+  Four<A>* da = params + 256 + threadIdx.x;                           // theirs: [NC][128]
 
   const Place w = place_of<CT>(p, p.segments, 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nl = lane % LN, dl = lane / LN;
@@ -605,7 +607,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
   const Four<A>* my_b = states + dl % COPIES * LN + nl;
   const Four<A>* my_c = my_b + TT * COPIES * LN;
   const Two<A> none = two(A(0), A(0));
-  Two<A> ra[NC][2], r[NC][2], da[NC][2];
+  Two<A> ra[NC][2], r[NC][2];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
     const bool in = cl + (k ^ swap) < w.width;
@@ -632,7 +634,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     }
     ra[k][0] = two(q[0], q[1]), ra[k][1] = two(q[2], q[3]);
     r[k][0] = two(s[0], s[1]), r[k][1] = two(s[2], s[3]);
-    da[k][0] = da[k][1] = none;
+    da[k * 128] = {A(0), A(0), A(0), A(0)};
   }
 
   const int col = threadIdx.x % I::COLS * 4, row0 = threadIdx.x / I::COLS;
@@ -649,7 +651,9 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
   const int64_t to = w.b * p.length * p.dim + d0;
   T *ox = static_cast<T*>(p.dx) + to, *od = static_cast<T*>(p.ddt) + to,
     *og = static_cast<T*>(p.dgate) + to;
-  const Four<A> bias = params4<A>(p.dt_bias, d0, have), skip = params4<A>(p.skip, d0, have);
+  // (the thread's own: in registers they would be eight that most of the step has no use for)
+  params[threadIdx.x] = params4<A>(p.dt_bias, d0, have);
+  params[128 + threadIdx.x] = params4<A>(p.skip, d0, have);
   const bool gated = p.gate != nullptr;
   Raw4<T> xr[I::IT], dr[I::IT], zr[I::IT], qr[I::IT];
   States<T, TT, LN, 2> bc;
@@ -710,6 +714,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     for (int q = 0; q < I::IT; ++q) {
       const int row = row0 + q * I::ROWS;
       if (I::ROWS * I::IT > TT && row >= TT) break;
+      const Four<A> bias = params[threadIdx.x];
       Four<A> dp;
       A delta[4];
       Quad<T>::values(xr[q], xk[q]);
@@ -848,8 +853,12 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
       }
     }
 #pragma unroll
-    for (int k = 0; k < NC; ++k)
-      da[k][0] = add(da[k][0], dat[k][0]), da[k][1] = add(da[k][1], dat[k][1]);
+    for (int k = 0; k < NC; ++k) {
+      Four<A> sum = da[k * 128];
+      sum = {sum.v[0] + first(dat[k][0]), sum.v[1] + second(dat[k][0]),
+             sum.v[2] + first(dat[k][1]), sum.v[3] + second(dat[k][1])};
+      da[k * 128] = sum;
+    }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < I::IT; ++q) {
@@ -862,6 +871,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
       const Four<A>* st = reinterpret_cast<const Four<A>*>(slots + row * CT + col);
       const Four<A> s0 = st[0], s1 = st[1];
       const A delta[4] = {s0.v[0], s0.v[2], s1.v[0], s1.v[2]};
+      const Four<A> skip = params[128 + threadIdx.x];
       A gx[4], gd[4], gg[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -899,8 +909,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     const int c = cl + (k ^ swap);
     if (c >= w.width) continue;
     const int64_t d = w.d0 + c;
-    static_cast<Four<A>*>(p.part_a)[(row * p.dim + d) * LN + nl] = reorder(
-        Four<A>{first(da[k][0]), second(da[k][0]), first(da[k][1]), second(da[k][1])}, order);
+    static_cast<Four<A>*>(p.part_a)[(row * p.dim + d) * LN + nl] = reorder(da[k * 128], order);
     if (w.segment == 0 && p.d_initial != nullptr) {
       const A s[4] = {first(r[k][0]), second(r[k][0]), first(r[k][1]), second(r[k][1])};
 #pragma unroll
@@ -933,7 +942,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
 template <typename A> constexpr size_t scan_bwd_smem(int ln, int nc) {
   const size_t ct = 4 * (32 / ln) * nc, np = 4 * ln, tt = kScanCheck;
   const size_t copies = 32 / ln < 4 ? 32 / ln : 4;
-  return sizeof(A) * (2 * tt * np * copies + 3 * tt * ct + 4 * tt * 2 * np + 3 * tt * (ct + 8));
+  return sizeof(A) * (2 * tt * np * copies + 3 * tt * ct + 4 * tt * 2 * np + 3 * tt * (ct + 8) +
+                      (2 + nc) * 4 * 128);
 }
 
 // ------------------------------------------------------------------------------ single tokens
