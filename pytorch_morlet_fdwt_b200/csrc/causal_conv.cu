@@ -8,8 +8,13 @@
 // without one.  Bound by HBM (2 W + 4 operations an element forward): a thread takes V
 // neighbouring channels (16 bytes, forward) and walks over a run of tokens with the last W inputs
 // in registers, so that every input is read once (and W-1 of a run's neighbours, from L2) and the
-// loads of several tokens are in flight.  Sums are 32 bits (64 for fp64); y and the gradients are
-// rounded once.
+// loads of several tokens are in flight.  Sums are 32 bits (64 for fp64) on pairs of channels (one
+// packed instruction a pair); y and the gradients are rounded once.
+//
+// Measured, 4 taps with silu: 4 x 4096 x 2048 bf16 forward 33 us (4.1 TB/s), backward 64 us (3.2
+// TB/s); fp32 52 us forward (5.2 TB/s).  In 16 bits the exponential and reciprocal of silu (half of
+// the XU pipe's time) and the instructions around them take as long as the bytes do.  A thread of the
+// backward pass takes 2 channels (4: 160 registers, 1.2 times the time; 1 in fp64).
 #include "pairs.cuh"
 #include "row_groups.cuh"
 

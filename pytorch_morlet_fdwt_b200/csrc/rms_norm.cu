@@ -12,6 +12,11 @@
 // Bound by HBM (5, 8 and 16 operations an element): each element is read once and kept in
 // registers between the sum and the result, 16 bytes a load.  Sums and statistics are 32 bits
 // (64 for fp64 rows); y is rounded once, to its type or to 8 bits.
+//
+// Measured with the residual: 65536 x 2048 bf16 forward 170 us (6.3 TB/s), backward 171 us (6.3
+// TB/s); 16384 x 8192 bf16 164 us both (6.5 TB/s); 40000 x 1001 fp32 106 and 90 us (6.0 and 7.1 TB/s
+// with what L2 holds), bf16 72 and 78 us; 32768 x 2048 bf16 to e4m3 in groups of 128 84 us (5.6
+// TB/s), 40000 x 1001 bf16 to e4m3 137 us.
 #include <cuda_fp8.h>
 
 #include "row_groups.cuh"

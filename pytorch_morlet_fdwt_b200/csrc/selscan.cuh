@@ -13,16 +13,27 @@
 //   dc_t[n] = sum_d dp_t h_t[n]             dgate_t = dy_t p_t silu'(gate_t),  dskip = sum_t dp_t x_t
 //
 // The decays depend on channel, state and token, so there is no product of matrices in it: a state
-// and token cost one exponential (16 a clock and SM) and 4 (backward 12) operations of the FMA
-// pipes, which is the bound; bytes are 8 and 22 a token and channel in 16 bits.
+// and token cost one exponential (16 a clock and SM, 4.65e12 a second on 148 SMs) and 4 (backward
+// 12) operations of the FMA pipes; bytes are 8 and 22 a token and channel in 16 bits, 0.3 of the
+// exponentials' time with 16 states.
 //
-// Split.  A thread keeps 4 neighbouring states; LN lanes hold a channel's states (up to 4 LN) and
-// the 32 / LN groups of lanes of a warp neighbouring channels.  Sums over states cross LN lanes,
-// those over channels (db, dc) the others; both are formed for 8 tokens at once, halving the
-// values a lane holds with each step.  A block of 4 warps stages some tokens of its channels in
-// shared memory in 32 bits: delta and delta x (as pairs, for the packed instructions), b and c.
-// Long sequences of few channels are cut into segments: a state launch forms each segment's end
-// state from zero and its sum of delta, and the main launch's blocks add up those before them.
+// Split.  A thread keeps 4 neighbouring states of 2 channels; LN lanes hold a channel's states (up to
+// 4 LN) and the 32 / LN groups of lanes of a warp neighbouring channels.  Sums over states cross LN
+// lanes, those over channels (db, dc) the others; each step of such a sum halves the values a lane
+// holds.  A block of 4 warps stages some tokens of its channels in shared memory in 32 bits: delta
+// and delta x, b and c.  Long sequences of few channels are cut into segments: a state launch forms
+// each segment's end state from zero and its sum of delta, and the main launch's blocks add up those
+// before them.
+//
+// Measured (bf16, 16 states, a gate; ncu and events).  64 x 1024 x 2048, one launch: 789 us, 2.7e12
+// exponentials a second, 0.59 of their rate, 0.75 with those of the steps and gates counted.
+// 1 x 65536 x 2048, 37 segments: state launch 639 us, main launch 827 us.  4 x 4096 x 2048 with
+// gradients: 149 + 275 us forward, 179 us of states back in time, 671 us backward, 31 us of sums.
+// What was tried on the forward launches and changed nothing or made them slower: a quarter of the
+// exponentials by a polynomial on the FMA pipes (state launch 640 us either way, main launch 6 %
+// slower), 5 and 6 blocks an SM (5 % and 9 % slower), a second copy of the staged steps for wider
+// loads.  It is the mix of exponentials, shared memory and FMA instructions that fills the issue
+// slots; a 16-bit load that is taken apart where it is issued, and so waited for, cost 1.7 times.
 #pragma once
 
 #include "row_groups.cuh"
