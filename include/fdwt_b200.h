@@ -433,7 +433,7 @@ typedef struct {
 /* y and the states after the sequences (final_state; may be NULL) from initial_state (NULL:
  * zeros).  checkpoints (fdwt_selscan_checkpoint_bytes; NULL where no backward pass follows)
  * receives states that the backward pass starts from.  Workspaces and checkpoints begin on a
- * multiple of 16 bytes. */
+ * multiple of 32 bytes. */
 size_t fdwt_selscan_forward_workspace(const fdwt_scan_desc* desc);
 size_t fdwt_selscan_checkpoint_bytes(const fdwt_scan_desc* desc);
 int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, const void* dt, const void* a,

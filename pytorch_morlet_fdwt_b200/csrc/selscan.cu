@@ -171,10 +171,10 @@ Parts part_bytes(const fdwt_scan_desc* d, const Cut& c) {
   return p;
 }
 
-bool aligned16(std::initializer_list<const void*> pointers) {
+bool aligned32(std::initializer_list<const void*> pointers) {
   uintptr_t bits = 0;
   for (const void* q : pointers) bits |= reinterpret_cast<uintptr_t>(q);
-  return bits % 16 == 0;
+  return bits % 32 == 0;
 }
 
 ScanArgs args_of(const fdwt_scan_desc* d, const void* x, const void* dt, const void* a,
@@ -248,7 +248,7 @@ extern "C" int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, c
   const Cut cut = forward_cut(desc);
   const size_t bytes = segment_bytes(desc, cut).bytes;
   if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes)) return FDWT_ERR_WORKSPACE;
-  FDWT_CHECK(aligned16({workspace, checkpoints}));
+  FDWT_CHECK(aligned32({workspace, checkpoints}));
   ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths);
   p.y = y, p.final_state = final_state, p.check = checkpoints;
   see_alignment(&p, desc, false);
@@ -295,7 +295,7 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
   const Cut cut = backward_cut(desc);
   const Parts parts = part_bytes(desc, cut);
   if (workspace == nullptr || workspace_bytes < parts.bytes) return FDWT_ERR_WORKSPACE;
-  FDWT_CHECK(aligned16({workspace, checkpoints}));
+  FDWT_CHECK(aligned32({workspace, checkpoints}));
   ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, nullptr, lengths);
   p.check = const_cast<void*>(checkpoints);
   p.dy = dy, p.d_final = d_final_state, p.dx = dx, p.ddt = ddt, p.dgate = dgate;

@@ -126,7 +126,8 @@ def test_scan_entries_check_their_arguments():
     assert lib.fdwt_selscan_forward(at, None, *[PTR] * 13, 1 << 40, None) == INVALID
     need = lib.fdwt_selscan_forward_workspace(at)  # few channels: segments
     assert need > 0 and lib.fdwt_selscan_forward(at, *[PTR] * 14, need - 1, None) == WORKSPACE
-    assert lib.fdwt_selscan_forward(at, *[PTR] * 13, PTR + 4, need, None) == INVALID  # off 16 bytes
+    for off in (4, 16):  # off 32 bytes
+        assert lib.fdwt_selscan_forward(at, *[PTR] * 13, PTR + off, need, None) == INVALID
     need = lib.fdwt_selscan_backward_workspace(at)
     assert lib.fdwt_selscan_backward(at, *[PTR] * 22, need - 1, None) == WORKSPACE
     # the states before every eighth token, padded to a power of two
