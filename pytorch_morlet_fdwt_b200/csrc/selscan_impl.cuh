@@ -99,6 +99,15 @@ template <bool FAST> __device__ __forceinline__ void sigmoid_at(const double* v,
   for (int j = 0; j < 4; ++j) g[j] = 1.0 / (1.0 + exp(-v[j]));
 }
 
+// Added to the exponent of every decay.  The hardware's 2^x is 0.5e-8 to 2.7e-8 too small in the mean
+// for -1/2 < x < 0 (measured over 2^20 values for each power of two; 3e-8 to 4e-8 root mean square),
+// and a state is a product of hundreds of decays: this takes the mean back (2^lift = 1 + 1.4e-8) at no
+// cost, a product becoming a product and sum.  4 x 4096 x 2048 against 64 bits: last states 5e-7 off
+// without, 2.8e-7 with; dL/da 1.7e-6 and 0.75e-6.  2^lift itself comes out as 1, so that a step of zero
+// keeps the state as it is.
+template <typename A> __device__ __forceinline__ A lift() { return sizeof(A) == 4 ? A(2e-8) : A(0); }
+template <typename A> __device__ __forceinline__ Two<A> lift2() { return two(lift<A>(), lift<A>()); }
+
 // A channel's rates times log2 e.  -inf (forgets everything) becomes the lowest finite value, so
 // that a step of zero, as padding has, keeps the state.
 __device__ __forceinline__ float rate(float a) {
@@ -494,7 +503,7 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
         for (int k = 0; k < NC; ++k) {
           const Step<A> st = slots[row * CT + cl + (k ^ swap)];
           const Two<A> d2 = two(st.delta, st.delta), u2 = two(st.u, st.u);
-          const Two<A> e0 = exp_2(mul(d2, ra[k][0])), e1 = exp_2(mul(d2, ra[k][1]));
+          const Two<A> e0 = exp_2(fma(d2, ra[k][0], lift2<A>())), e1 = exp_2(fma(d2, ra[k][1], lift2<A>()));
           if constexpr (MODE == REVERSE) {
             h[k][0] = mul(e0, fma(u2, low(bq), h[k][0]));
             h[k][1] = mul(e1, fma(u2, high(bq), h[k][1]));
@@ -768,8 +777,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
           for (int k = 0; k < NC; ++k) {
             const Step<A> st = slots[u * CT + cl + (k ^ swap)];
             const Two<A> d2 = two(st.delta, st.delta), u2 = two(st.u, st.u);
-            h[0][k][0] = fma(exp_2(mul(d2, ra[k][0])), h[0][k][0], mul(u2, low(bq)));
-            h[0][k][1] = fma(exp_2(mul(d2, ra[k][1])), h[0][k][1], mul(u2, high(bq)));
+            h[0][k][0] = fma(exp_2(fma(d2, ra[k][0], lift2<A>())), h[0][k][0], mul(u2, low(bq)));
+            h[0][k][1] = fma(exp_2(fma(d2, ra[k][1], lift2<A>())), h[0][k][1], mul(u2, high(bq)));
           }
         }
       }
@@ -783,8 +792,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
         for (int k = 0; k < NC; ++k) {
           st[u][k] = slots[(base + u) * CT + cl + (k ^ swap)];
           const Two<A> d2 = two(st[u][k].delta, st[u][k].delta), u2 = two(st[u][k].u, st[u][k].u);
-          e[u][k][0] = exp_2(mul(d2, ra[k][0]));
-          e[u][k][1] = exp_2(mul(d2, ra[k][1]));
+          e[u][k][0] = exp_2(fma(d2, ra[k][0], lift2<A>()));
+          e[u][k][1] = exp_2(fma(d2, ra[k][1], lift2<A>()));
           h[u + 1][k][0] = fma(e[u][k][0], h[u][k][0], mul(u2, low(bq[u])));
           h[u + 1][k][1] = fma(e[u][k][1], h[u][k][1], mul(u2, high(bq[u])));
         }
@@ -1023,7 +1032,7 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     Quad<T>::values(rc[i], vc);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      h[i].v[j] = exp_2(di * r.v[j]) * h[i].v[j] + ui * vb[j];
+      h[i].v[j] = exp_2(fma(di, r.v[j], lift<A>())) * h[i].v[j] + ui * vb[j];
       y[i] += h[i].v[j] * vc[j];
     }
     if (!in) continue;

@@ -345,6 +345,18 @@ def test_rates_of_minus_infinity_forget():
     assert torch.equal(y, z) and torch.equal(final, last)
 
 
+def test_steps_of_zero_keep_the_state():
+    """A step of zero, and padding, leave a state as it is, bit by bit, over any number of tokens."""
+    for dtype in (F32, F64, BF16):
+        s = _case(2, 600, 40, 16, 1, dtype, softplus=False, bias=False, lengths=[600, 1])
+        s["dt"].zero_()
+        _, final = _call(s)
+        assert torch.equal(final, s["initial"])
+        for _ in range(3):
+            F.selective_scan_step(s["x"][:, 0], s["dt"][:, 0], s["a"], s["b"][:, 0], s["c"][:, 0], final)
+        assert torch.equal(final, s["initial"])
+
+
 def test_streams_graphs_and_workspaces():
     """Another stream; two captured forward and backward passes replayed in turn."""
     cases = [_case(1, 900, 64, 16, 1, BF16, seed=i) for i in range(2)]
