@@ -95,55 +95,52 @@ struct Cut {
 };
 constexpr int64_t kSegmentStep = 16;  // segments are multiples of the staged tokens
 constexpr int kMostSegments = 64;
-// Measured: microseconds a token of a block alone on its SM, and of each of several.
+// Microseconds of a token for each of the k blocks that share an SM, base + each k, and of a block's
+// beginning, start (with what it does for every other segment, other): fitted to calls of 64 channels
+// a block, 16 states, cut in 1 to 64 ways.
 struct Pace {
-  double alone, shared;
+  double base, each, start, other;
 };
-double launch_time(double blocks, double resident, int64_t tokens, const Pace& pace) {
-  const double sms = sm_count(), at_once = blocks < resident ? blocks : resident;
-  const double a_sm = static_cast<double>(cdiv(static_cast<int64_t>(at_once), sm_count()));
-  const double waves = static_cast<double>(cdiv(static_cast<int64_t>(blocks),
-                                                static_cast<int64_t>(resident)));
-  (void)sms;
-  const double each = pace.shared * a_sm;
-  return waves * tokens * (each > pace.alone ? each : pace.alone);
+double launch_time(double blocks, double resident, int64_t tokens, int segments, const Pace& pace) {
+  const double sms = sm_count(), whole = static_cast<double>(static_cast<int64_t>(blocks / resident));
+  const double rest = blocks - whole * resident, start = pace.start + pace.other * segments;
+  double t = whole * (tokens * (pace.base + pace.each * resident / sms) + start);
+  if (rest > 0) t += tokens * (pace.base + pace.each * (rest > sms ? rest / sms : 1.0)) + start;
+  // blocks that all begin together stage and compute together, and overlap less
+  return whole > 0 ? t : 1.1 * t;
 }
 // The number of segments with the shortest modelled time: more of them fill the device, but cost a
-// state launch (for all segments but one) and waves.
+// state launch (for all segments but one) and beginnings.
 Cut cut_of(const fdwt_scan_desc* d, int tile, int state_tile, int64_t resident, const Pace& pace,
            const Pace& state_pace) {
-  Cut best{cdiv(d->dim / d->groups, tile), 1, imax(kSegmentStep, cdiv(d->length, kSegmentStep) * kSegmentStep)};
+  Cut best{cdiv(d->dim / d->groups, tile), 1,
+           imax(kSegmentStep, cdiv(d->length, kSegmentStep) * kSegmentStep)};
   const double blocks = double(best.tiles) * d->groups * d->batch;
   const double state_blocks = double(cdiv(d->dim / d->groups, state_tile)) * d->groups * d->batch;
   if (blocks == 0) return best;
-  double least = launch_time(blocks, resident, best.seg_len, pace);
+  double least = launch_time(blocks, resident, best.seg_len, 1, pace);
   for (int n = 2; n <= kMostSegments; ++n) {
     const int64_t len = cdiv(cdiv(d->length, n), kSegmentStep) * kSegmentStep;
-    const int64_t count = len > 0 ? cdiv(d->length, len) : 1;
-    if (len < 4 * kSegmentStep || count != n) continue;
-    const double resident_states = 4.0 * sm_count();
-    const double t = launch_time(blocks * n, resident, len, pace) + 3.0 +
-                     launch_time(state_blocks * (n - 1), resident_states, len, state_pace);
-    if (t < least) {
-      least = t;
-      best.segments = n;
-      best.seg_len = len;
-    }
+    if (len < 4 * kSegmentStep || cdiv(d->length, len) != n) continue;
+    const double t = launch_time(blocks * n, resident, len, n, pace) + 3.0 +
+                     launch_time(state_blocks * (n - 1), 4.0 * sm_count(), len, n, state_pace);
+    if (t < least) least = t, best.segments = n, best.seg_len = len;
   }
   return best;
 }
 Cut forward_cut(const fdwt_scan_desc* d) {
   const int lanes = lanes_of(d->states), tile = scan_fwd_tile(lanes);
   return with_type(d->dtype, [&](auto t) {
-    return cut_of(d, tile, tile, scan_resident<decltype(t)>(lanes, false), {0.12, 0.07},
-                  {0.08, 0.048});
+    return cut_of(d, tile, tile, scan_resident<decltype(t)>(lanes, false),
+                  {0.08, 0.0355, 1.0, 0.1}, {0.04, 0.0363, 0.5, 0.0});
   });
 }
 Cut backward_cut(const fdwt_scan_desc* d) {
   const int lanes = lanes_of(d->states);
   return with_type(d->dtype, [&](auto t) {
     return cut_of(d, scan_bwd_tile(lanes, d->dtype == FDWT_F64), scan_fwd_tile(lanes),
-                  scan_resident<decltype(t)>(lanes, true), {0.3, 0.2}, {0.1, 0.055});
+                  scan_resident<decltype(t)>(lanes, true), {0.107, 0.133, 1.0, 0.04},
+                  {0.045, 0.037, 0.5, 0.0});
   });
 }
 struct Segments {
