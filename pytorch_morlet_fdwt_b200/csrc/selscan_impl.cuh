@@ -590,7 +590,9 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
 // goes back over them.  One channel a thread and 8 tokens at once (no passing over, one channel's
 // registers) was slower (4 x 4096 x 2048 with gradients: 4.7 ms against 3.1 ms then), as were 3
 // blocks an SM with spills (1.65 ms against 1.51 ms then): the kernel is bound by its instructions
-// (340 a token and channel of 16 states) at the 8 warps an SM that 255 registers leave.
+// (340 a token and channel of 16 states) at the 8 warps an SM that 255 registers leave.  What moved
+// out of registers (sums of da, dt_bias, skip) and loads a step ahead gained 7 %, the slopes and
+// openings in shared memory lost 2 %.
 template <typename T, int LN, int NC>
 __global__ void __launch_bounds__(128)
 scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
@@ -961,7 +963,7 @@ template <typename A> constexpr size_t scan_bwd_smem(int ln, int nc) {
 // One token of every sequence: a pass over the states, read and written once.  A thread takes 4 states
 // of a channel in SEQ sequences (at most LN), whose loads are in flight together and share the
 // rates.  The LN lanes of a channel share out the sequences' steps and gates, and hand them round.
-template <typename T, int LN, int SEQ>
+template <typename T, int LN, int SEQ, bool WHOLE>
 __global__ void __launch_bounds__(128)
 scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__ slots,
                  int64_t pool, typename AccOf<T>::type* state) {
@@ -975,8 +977,9 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
   const bool in = d < dim;
   if (!in) d = dim - 1;  // the lanes of a warp stay together
   const unsigned group = p.groups == 1 ? 0 : d / static_cast<unsigned>(p.per);
-  const int have = p.states - n0;
-  const bool whole = p.vec && have > 0;
+  const int have = WHOLE ? 4 : p.states - n0;
+  const bool whole = WHOLE || (p.vec && have > 0), vec = WHOLE || p.vec;
+  const bool vec_states = WHOLE || p.vec_states;
 
   // the lane's own sequence of them
   constexpr int SAME = LN / SEQ;
@@ -992,6 +995,8 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     dt = to_acc(static_cast<const T*>(p.dt)[own * p.dts[0] + d]);
     if (p.gate != nullptr) z = to_acc(static_cast<const T*>(p.gate)[own * p.gs[0] + d]);
   }
+  const int64_t row = p.dim * p.states;
+  A* first_state = state + (int64_t(d) * p.states + n0);
   A* ps[SEQ];
   Four<A> h[SEQ];
   Raw4<T> rb[SEQ], rc[SEQ];
@@ -1002,17 +1007,17 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     const int slot = SEQ == 1 ? own_slot : __shfl_sync(0xffffffffu, own_slot, i * SAME, LN);
     ps[i] = nullptr;
     if (slot < 0) continue;
-    ps[i] = state + (slot * p.dim + d) * p.states + n0;
+    ps[i] = first_state + slot * row;
     h[i] = {A(0), A(0), A(0), A(0)};
     if (whole) h[i] = *reinterpret_cast<const Four<A>*>(ps[i]);
-    else if (!p.vec) h[i] = params4<A>(ps[i], 0, have);
-    rb[i] = load4(pb, have, p.vec_states);
-    rc[i] = load4(pc, have, p.vec_states);
+    else if (!vec) h[i] = params4<A>(ps[i], 0, have);
+    rb[i] = load4(pb, have, vec_states);
+    rc[i] = load4(pc, have, vec_states);
   }
   Four<A> r = {A(0), A(0), A(0), A(0)};
   const A* pa = static_cast<const A*>(p.a) + int64_t(d) * p.states + n0;
   if (whole) r = *reinterpret_cast<const Four<A>*>(pa);
-  else if (!p.vec) r = params4<A>(pa, 0, have);
+  else if (!vec) r = params4<A>(pa, 0, have);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r.v[j] = rate(r.v[j]);
 
@@ -1030,15 +1035,16 @@ scan_step_kernel(const __grid_constant__ ScanArgs p, const int32_t* __restrict__
     A vb[4], vc[4];
     Quad<T>::values(rb[i], vb);
     Quad<T>::values(rc[i], vc);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h[i].v[j] = exp_2(fma(di, r.v[j], lift<A>())) * h[i].v[j] + ui * vb[j];
-      y[i] += h[i].v[j] * vc[j];
-    }
+    const Two<A> d2 = two(di, di), u2 = two(ui, ui);
+    const Two<A> h0 = fma(exp_2(fma(d2, low(r), lift2<A>())), low(h[i]), mul(u2, two(vb[0], vb[1])));
+    const Two<A> h1 = fma(exp_2(fma(d2, high(r), lift2<A>())), high(h[i]), mul(u2, two(vb[2], vb[3])));
+    const Two<A> sum = fma(h1, two(vc[2], vc[3]), mul(h0, two(vc[0], vc[1])));
+    y[i] = first(sum) + second(sum);
+    h[i] = {first(h0), second(h0), first(h1), second(h1)};
     if (!in) continue;
     if (whole) {
       *reinterpret_cast<Four<A>*>(ps[i]) = h[i];
-    } else if (!p.vec) {
+    } else if (!vec) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (j < have) ps[i][j] = h[i].v[j];
@@ -1142,7 +1148,10 @@ int scan_step(const ScanArgs& p, int lanes, const int32_t* slots, int64_t pool, 
       if (grid > INT32_MAX) return static_cast<int>(FDWT_ERR_UNSUPPORTED);
       const int st = pre_launch(stream);
       if (st != FDWT_OK) return st;
-      scan_step_kernel<T, LN, SEQ><<<static_cast<unsigned>(grid), 128, 0, stream>>>(
+      auto kernel = scan_step_kernel<T, LN, SEQ, false>;
+      // (without the conditions that other sizes need: 240 x 2048 of 16 states 15.4 us, with them 17)
+      if (p.vec && p.vec_states && p.states == 4 * LN) kernel = scan_step_kernel<T, LN, SEQ, true>;
+      kernel<<<static_cast<unsigned>(grid), 128, 0, stream>>>(
           p, slots, pool, static_cast<typename AccOf<T>::type*>(state));
       return launch_status();
     };

@@ -47,8 +47,8 @@ class _ScanDesc(ctypes.Structure):
 def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, device_index):
     """What a call's types, sizes and strides come to, checked once for each combination on one
     device: the C descriptor, its address, the bytes of the workspaces and of the kept states, and
-    the type of states.  In order x, dt, b, c and the gate (None without); ``lead`` names the axes
-    before the channels."""
+    the type of states; None where a last axis is not contiguous.  In order x, dt, b, c and the gate
+    (None without); ``lead`` names the axes before the channels."""
     code = _lib.dtype_code(dtypes[0])
     names = ("x", "dt", "b", "c", "gate")
     for name, dtype in zip(names, dtypes):
@@ -72,6 +72,8 @@ def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, devic
         raise ValueError(f"a channel must have 1 to {_MAX_STATES} states, got {states}")
     if tuple(a_shape) != (dim, states):
         raise ValueError(f"a must have shape ({dim}, {states}), got {tuple(a_shape)}")
+    if any(t is not None and t[-1] != 1 and s[-1] != 1 for t, s in zip(strides, shapes)):
+        return None
     length = x[1] if n == 2 else 1
     d = _ScanDesc(code, groups, states, bool(softplus), x[0], length, dim)
 
@@ -205,9 +207,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     inputs need gradients keeps ``L / 8`` states of every channel for the backward pass.
     """
     _lib.require_cuda(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths)
-    x, dt, b, c = _rows(x), _rows(dt), _rows(b), _rows(c)
-    gate = None if gate is None else _rows(gate)
     plan = _plan(_SEQUENCE, x, dt, a, b, c, gate, dt_softplus)
+    if plan is None:
+        x, dt, b, c = _rows(x), _rows(dt), _rows(b), _rows(c)
+        gate = None if gate is None else _rows(gate)
+        plan = _plan(_SEQUENCE, x, dt, a, b, c, gate, dt_softplus)
     d, acc = plan[0], plan[5]
     a = _parameter("a", a, (d.dim, d.states), acc)
     skip = _parameter("skip", skip, (d.dim,), acc)
@@ -238,9 +242,12 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     runs on :func:`selective_scan`.
     """
     _lib.require_cuda(x, dt, a, b, c, state, skip, gate, dt_bias, slots)
-    x, dt, b, c = _rows(x), _rows(dt), _rows(b), _rows(c)
-    gate = None if gate is None else _rows(gate)
-    d, desc, _, _, _, acc = _plan(_TOKEN, x, dt, a, b, c, gate, dt_softplus)
+    plan = _plan(_TOKEN, x, dt, a, b, c, gate, dt_softplus)
+    if plan is None:
+        x, dt, b, c = _rows(x), _rows(dt), _rows(b), _rows(c)
+        gate = None if gate is None else _rows(gate)
+        plan = _plan(_TOKEN, x, dt, a, b, c, gate, dt_softplus)
+    d, desc, _, _, _, acc = plan
     a = _parameter("a", a, (d.dim, d.states), acc)
     skip = _parameter("skip", skip, (d.dim,), acc)
     dt_bias = _parameter("dt_bias", dt_bias, (d.dim,), acc)

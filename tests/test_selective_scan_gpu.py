@@ -303,6 +303,25 @@ def test_strides_and_offsets(dtype):
         _check(h, ref["final"], F32, "state")
 
 
+def test_last_axes_that_are_not_contiguous():
+    """Inputs with another axis contiguous, or expanded over the channels or states: as their copies."""
+    s = _case(2, 21, 24, 8, 1, F32)
+    whole = _call(s)
+    turned = s | {k: s[k].transpose(1, -1).contiguous().transpose(1, -1)
+                  for k in ("x", "dt", "gate", "b", "c")}
+    assert all(torch.equal(p, q) for p, q in zip(_call(turned), whole))
+    wide = s | {"dt": s["dt"][..., :1].expand(2, 21, 24), "b": s["b"][..., :1].expand(2, 21, 1, 8)}
+    copy = s | {k: wide[k].contiguous() for k in ("dt", "b")}
+    assert all(torch.equal(p, q) for p, q in zip(_call(wide), _call(copy)))
+    one = {k: t[:, 4] if k in ("x", "dt", "b", "c", "gate") else t for k, t in s.items()}
+    states = [s["initial"].clone(), s["initial"].clone()]
+    outs = [F.selective_scan_step(f(one["x"]), one["dt"], s["a"], f(one["b"]), one["c"], h, s["skip"],
+                                  f(one["gate"]), s["dt_bias"], True)
+            for f, h in zip((lambda t: t.transpose(0, -1).contiguous().transpose(0, -1), lambda t: t),
+                            states)]
+    assert torch.equal(*outs) and torch.equal(*states)
+
+
 def test_parameters_in_16_bits_are_taken_in_32():
     s = _case(2, 20, 32, 8, 1, BF16)
     low = s | {k: s[k].to(BF16).requires_grad_() for k in ("a", "skip", "dt_bias")}
