@@ -21,7 +21,6 @@ template <typename A> __device__ __forceinline__ Two<A> high(const Four<A>& q) {
   return two(q.v[2], q.v[3]);
 }
 
-
 // e^-|v| of two values: the product with log2 e is rounded, so what it lost corrects the result.
 __device__ __forceinline__ Two<float> neg_exp(float v, float w) {
   constexpr float kHigh = 1.442695021629333f, kLow = 1.92596299e-8f;  // log2 e in two parts
