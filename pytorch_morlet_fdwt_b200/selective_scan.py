@@ -161,13 +161,15 @@ class _SelectiveScanFunction(torch.autograd.Function):
             plan = _plan(_SEQUENCE, x, dt, a, b, c, gate, ctx.softplus, dy.stride())
         if d_final is not None:
             d_final = d_final.contiguous()
-        need = ctx.needs_input_grad
-
+        _, _, need_a, need_b, need_c, need_skip, _, need_bias, need_i = ctx.needs_input_grad[:9]
         like = _lib.empty_like
         dx, ddt, dgate = like(x), like(dt), None if gate is None else like(gate)
-        da, db, dc, dskip, dbias, di = (like(t) if need[i] else None for i, t in
-                                        ((2, a), (3, b), (4, c), (5, skip), (7, dt_bias),
-                                         (8, initial)))
+        da = like(a) if need_a else None
+        db = like(b) if need_b else None
+        dc = like(c) if need_c else None
+        dskip = like(skip) if need_skip else None
+        dbias = like(dt_bias) if need_bias else None
+        di = like(initial) if need_i else None
         _, desc, _, _, nws, _ = plan
         with _lib.device_guard(dev):
             ws = _lib.workspace(nws, dev)

@@ -3,6 +3,10 @@ held before, tensors of more than 2^31 elements, two streams at once, dual tenso
 state that a graph has saved.  Tolerances where values are compared: those of the operators' tests,
 or the same bits."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -210,3 +214,39 @@ def test_shared_and_broadcast_inputs():
     assert torch.allclose(y, z, rtol=1e-13, atol=1e-13)
     assert torch.allclose(x.grad, sum(t.grad for t in xs), rtol=1e-11, atol=1e-11)
     assert torch.allclose(row.grad, sum(t.grad for t in bs).sum(1, keepdim=True), rtol=1e-11, atol=1e-11)
+
+
+FIRST_CALLS = """
+import torch
+import pytorch_morlet_fdwt_b200 as F
+t = lambda *s: torch.randn(*s, device="cuda").bfloat16().requires_grad_()
+x, w, g, bc, dy = t(2, 300, 64), t(64, 4), t(64), t(2, 300, 1, 16), t(2, 300, 64).detach()
+a = (-torch.rand(64, 16, device="cuda")).requires_grad_()
+states, inputs = torch.zeros(2, 64, 16, device="cuda"), torch.zeros(2, 3, 64, device="cuda").bfloat16()
+
+def run():
+    out = [*torch.autograd.grad(F.rms_norm(x, g, x)[0], (x, g), dy),
+           *torch.autograd.grad(F.causal_conv1d(x, w, None, "silu")[0], (x, w), dy),
+           *torch.autograd.grad(F.selective_scan(x, x, a, bc, bc, dt_softplus=True)[0], (x, a, bc), dy)]
+    with torch.no_grad():
+        out += F.rms_norm_quantized(x, g, group_size=32)
+        out.append(F.causal_conv1d_step(x[:, 0], w, inputs))
+        out.append(F.selective_scan_step(x[:, 0], x[:, 0], a, bc[:, 0], bc[:, 0], states,
+                                         dt_softplus=True))
+    return out
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = run()
+graph.replay()
+torch.cuda.synchronize()
+states.zero_(), inputs.zero_()
+want = run()
+assert all(torch.equal(p.float(), q.float()) for p, q in zip(held, want))
+"""
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first call of every operator is captured in a graph."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", FIRST_CALLS], check=True, cwd=root, timeout=300)
