@@ -93,6 +93,13 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_acc<__nv_bfloat16>(flo
   return __float2bfloat16_rn(v);
 }
 
+// max that keeps NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ------------------------------------------------------------------------------ index maps
 // Python-style floor division / modulo for signed 64-bit ints.
 __host__ __device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) {

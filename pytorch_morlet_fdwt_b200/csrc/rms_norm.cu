@@ -94,13 +94,6 @@ __device__ __forceinline__ void store_quant(O* p, const float* x, float inv) {
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
 }
-// max that keeps NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // The scale of a group whose largest magnitude is m: 1 where all are zero, else at least 2^-126, so
 // that its reciprocal is finite.  NaN stays NaN.
 template <typename O> __device__ __forceinline__ float scale_of(float m) {

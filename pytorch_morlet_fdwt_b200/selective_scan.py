@@ -197,7 +197,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
             strides (a last axis that is not contiguous is copied).  Up to 128 states N.
         a: ``(D, N)``, the rates (negative: the state decays; finite or ``-inf``); skip, dt_bias:
             ``(D,)``; taken in fp32 (fp64 for fp64 inputs).
-        dt_softplus: the step is ``log(1 + exp(dt + dt_bias))`` in place of ``dt + dt_bias``.
+        dt_softplus: the step is ``log(1 + exp(dt + dt_bias))`` in place of ``dt + dt_bias``; a dt
+            of ``-inf`` is then a step of zero, which keeps the state.
         initial_state: ``(B, D, N)`` fp32 (fp64 for fp64 inputs), zeros by default.
         lengths: ``(B,)`` int32 or int64, the tokens of each sequence that count (all by default;
             clamped to 0..L).  Outputs after them are zero and the state stops there; the padding
