@@ -342,22 +342,22 @@ conv_bwd_kernel(const T* __restrict__ x, const void* __restrict__ weight,
         for (int j = 0; j < V; ++j) q[j] *= v[j];
       }
       // (chosen, not multiplied by zero: what the window holds may be no number)
-      C d;
 #pragma unroll
       for (int j = 0; j < V; ++j) q[j] = counts ? q[j] : A(0);
       dp[W - 1].set(q);
-#pragma unroll
-      for (int j = 0; j < V; ++j) q[j] = own ? q[j] : A(0);
-      d.set(q);
       C r;
 #pragma unroll
       for (int m = 0; m < C::M; ++m) {
-        db.e[m] = add(db.e[m], d.e[m]);
         r.e[m] = mul(w[W - 1].e[m], dp[0].e[m]);
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          dw[i].e[m] = fma(d.e[m], win[i].e[m], dw[i].e[m]);
-          if (i > 0) r.e[m] = fma(w[W - 1 - i].e[m], dp[i].e[m], r.e[m]);
+        for (int i = 1; i < W; ++i) r.e[m] = fma(w[W - 1 - i].e[m], dp[i].e[m], r.e[m]);
+      }
+      if (own) {  // (the same for a warp's threads; and no product of zero with the window either)
+#pragma unroll
+        for (int m = 0; m < C::M; ++m) {
+          db.e[m] = add(db.e[m], dp[W - 1].e[m]);
+#pragma unroll
+          for (int i = 0; i < W; ++i) dw[i].e[m] = fma(dp[W - 1].e[m], win[i].e[m], dw[i].e[m]);
         }
       }
       r.get(g);
