@@ -244,6 +244,14 @@ def device_guard(device: torch.device):
     return torch.cuda.device(device)
 
 
+def index_guard(index):
+    """:func:`device_guard` by a tensor's device index; nothing to enter for one on the CPU (None or
+    -1)."""
+    if index is None or index < 0 or torch.cuda.current_device() == index:
+        return _NO_GUARD
+    return torch.cuda.device(index)
+
+
 def i64_array(values):
     arr = (ctypes.c_int64 * max(1, len(values)))(*[int(v) for v in values])
     return arr

@@ -63,7 +63,8 @@ def _describe(dtype, shape, stride, dy_stride, w_dtype, w_shape, bias, activatio
     d.x_stride[:] = stride[:2] if len(shape) == 3 else (stride[0], 0)
     d.dy_stride[:] = (d.length * d.dim, d.dim) if dy_stride is None else dy_stride[:2]
     at = ctypes.addressof(d)
-    return d, at, int(_lib.load().fdwt_causal_conv1d_backward_workspace(at))
+    with _lib.index_guard(device_index):  # runs of tokens go by the device
+        return d, at, int(_lib.load().fdwt_causal_conv1d_backward_workspace(at))
 
 
 def _plan(x, weight, bias, activation, dy_stride=None):

@@ -79,8 +79,9 @@ def _describe(names, dtypes, shapes, strides, out_stride, scale, device_index):
     lib = _lib.load()
     at = ctypes.addressof(d)
     state = torch.float64 if code == 1 else torch.float32
-    return (d, at, int(lib.fdwt_linattn_forward_workspace(at)),
-            int(lib.fdwt_linattn_backward_workspace(at)), state)
+    with _lib.index_guard(device_index):  # segments go by the device
+        return (d, at, int(lib.fdwt_linattn_forward_workspace(at)),
+                int(lib.fdwt_linattn_backward_workspace(at)), state)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:

@@ -88,10 +88,11 @@ def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, devic
     d.dy_stride[:] = (length * dim, dim) if dy_stride is None else dy_stride[:2]
     lib = _lib.load()
     at = ctypes.addressof(d)
-    return (d, at, int(lib.fdwt_selscan_forward_workspace(at)),
-            int(lib.fdwt_selscan_checkpoint_bytes(at)),
-            int(lib.fdwt_selscan_backward_workspace(at)),
-            torch.float64 if code == 1 else torch.float32)
+    with _lib.index_guard(device_index):  # the cut goes by the device
+        return (d, at, int(lib.fdwt_selscan_forward_workspace(at)),
+                int(lib.fdwt_selscan_checkpoint_bytes(at)),
+                int(lib.fdwt_selscan_backward_workspace(at)),
+                torch.float64 if code == 1 else torch.float32)
 
 
 def _plan(lead, x, dt, a, b, c, gate, softplus, dy_stride=None):
