@@ -29,7 +29,7 @@ from torch import nn
 from .causal_conv import causal_conv1d, causal_conv1d_step
 from .cwt import CWT1D, morlet_mix_tokens, spectral_softmax
 from .dwt import wavedec, waverec
-from .linear_attention import linear_attention, linear_attention_step
+from .linear_attention import _indexes, linear_attention, linear_attention_step
 from .norm import LayerNorm, RMSNorm
 from .selective_scan import selective_scan, selective_scan_step
 from .wavelets import WaveletLike
@@ -43,6 +43,15 @@ State = Tuple[torch.Tensor, torch.Tensor]
 def _randn_over(rows: int, cols: int, fan: int) -> torch.Tensor:
     """Standard normal ``(rows, cols)`` weights scaled by ``1 / sqrt(fan)``."""
     return torch.randn(rows, cols) / fan ** 0.5
+
+
+def _without_padding(t: torch.Tensor, lengths: Optional[torch.Tensor]) -> torch.Tensor:
+    """``t (B, L, D)`` with zeros after each sequence's tokens, and in its gradient: what stands there
+    must not reach a parameter's gradient, as zero times a NaN would."""
+    if lengths is None:
+        return t
+    at = torch.arange(t.shape[1], device=t.device)
+    return t.masked_fill((at >= lengths.unsqueeze(-1)).unsqueeze(-1), 0.0)
 
 
 def _compute_dtype(x: torch.Tensor) -> torch.dtype:
@@ -394,7 +403,8 @@ class SelectiveTokenMixer(nn.Module):
 
     def mix(self, h: torch.Tensor, state: Optional[State] = None,
             lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, State]:
-        """What is added to the residual, from the normed tokens ``h (B, L, D)``, and the state."""
+        """What is added to the residual, from the normed tokens ``h (B, L, D)`` (finite after the
+        ``lengths`` too, where the projections' gradients count them), and the state."""
         u, gate = self.in_proj(h).split(self.inner, -1)
         before, start = (None, None) if state is None else state
         u, before = causal_conv1d(u, self.conv_weight, self.conv_bias, "silu", before, lengths)
@@ -417,11 +427,15 @@ class SelectiveTokenMixer(nn.Module):
                 lengths: Optional[torch.Tensor] = None, return_state: bool = False):
         """``x (B, L, D)`` -> ``y (B, L, D)``, or ``(y, state)`` with ``return_state``; ``state``
         and ``lengths`` as ``initial_state`` and ``lengths`` of
-        :func:`~pytorch_morlet_fdwt_b200.selective_scan`."""
+        :func:`~pytorch_morlet_fdwt_b200.selective_scan`: outputs after them are zero, and the
+        padding may hold anything."""
         if x.dim() != 3:
             raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
+        if lengths is not None:
+            lengths = _indexes(lengths, x.shape[0], 0, x.shape[1], "lengths")
+        x = _without_padding(x, lengths)
         mixed, state = self.mix(self.norm(x), state, lengths)
-        y = x + mixed
+        y = _without_padding(x + mixed, lengths)
         return (y, state) if return_state else y
 
     @torch.no_grad()
@@ -471,6 +485,8 @@ class SelectiveTokenStack(nn.Module):
             raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
         if state is not None and len(state) != len(self.layers):
             raise ValueError(f"expected {len(self.layers)} states, got {len(state)}")
+        if lengths is not None:
+            lengths = _indexes(lengths, x.shape[0], 0, x.shape[1], "lengths")
         states = []
 
         def mix(i, layer, h):
@@ -478,7 +494,7 @@ class SelectiveTokenStack(nn.Module):
             states.append(last)
             return mixed
 
-        y = self._run(x, mix)
+        y = _without_padding(self._run(_without_padding(x, lengths), mix), lengths)
         return (y, states) if return_state else y
 
     @torch.no_grad()
