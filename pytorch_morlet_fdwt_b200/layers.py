@@ -328,13 +328,17 @@ class DecayTokenMixer(nn.Module):
                 lengths: Optional[torch.Tensor] = None, return_state: bool = False):
         """``x (B, L, D)`` -> ``y (B, L, D)``, or ``(y, state)`` with ``return_state``; ``state``
         and ``lengths`` as ``initial_state`` and ``lengths`` of
-        :func:`~pytorch_morlet_fdwt_b200.linear_attention`."""
+        :func:`~pytorch_morlet_fdwt_b200.linear_attention`: outputs after them are zero, and the
+        padding may hold anything."""
         if x.dim() != 3:
             raise ValueError(f"expected (B, L, D) input, got shape {tuple(x.shape)}")
+        if lengths is not None:
+            lengths = _indexes(lengths, x.shape[0], 0, x.shape[1], "lengths")
+        x = _without_padding(x, lengths)
         q, k, v = self._qkv(x)
         mixed, state = linear_attention(q, k, v, self.log_decay(x.device), initial_state=state,
                                         lengths=lengths)
-        y = x + self.out_proj(mixed.flatten(-2))
+        y = _without_padding(x + self.out_proj(mixed.flatten(-2)), lengths)
         return (y, state) if return_state else y
 
     @torch.no_grad()
