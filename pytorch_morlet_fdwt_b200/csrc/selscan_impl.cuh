@@ -118,6 +118,30 @@ __device__ __forceinline__ double rate(double a) {
   return r < -DBL_MAX ? -DBL_MAX : r;
 }
 
+// Four states carried over a segment: 2^(sum r) s + e, with the segment's sum of steps, the rates and the
+// states that it forms from zero; whether a 2^(sum r) leaves the type's range (rates above or steps below
+// zero, long segments).
+template <typename A>
+__device__ __forceinline__ bool carry(A* s, A sum, const A* r, const Four<A>& e) {
+  bool grows = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const A q = sum * r[j];
+    grows |= q > A(sizeof(A) == 4 ? 126 : 1022);
+    s[j] = fma(exp_2(q), s[j], e.v[j]);
+  }
+  return grows;
+}
+// The same in two halves where it does: a state of zero stays zero, as it does token by token.
+template <typename A>
+__device__ __forceinline__ void carry_growing(A* s, A sum, const A* r, const Four<A>& e) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const A q = sum * r[j], half = exp_2(A(0.5) * q);
+    s[j] = s[j] == A(0) && q > A(0) ? e.v[j] : fma(half * s[j], half, e.v[j]);
+  }
+}
+
 // Sums of V values each over L lanes `STRIDE` apart (powers of two): with each step a lane hands
 // over half of its values.  Afterwards v[0 .. max(V / L, 1)) are the sums of the values from
 // index * V / L on, index being the lane's place among the L (where L > V, lanes in runs of L / V
@@ -375,20 +399,26 @@ scan_fwd_kernel(const __grid_constant__ ScanArgs p) {
     A s[4] = {A(0), A(0), A(0), A(0)};
     if (MODE == MAIN && c < w.width) {
       const int64_t d = w.d0 + c;
-      if (p.initial != nullptr) {
+      auto initial = [&] {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (nl * 4 + j < p.states)
-            s[j] = static_cast<const A*>(p.initial)[(w.b * p.dim + d) * p.states + nl * 4 + j];
-      }
-      // the segments before this one
-#pragma unroll 4
-      for (int g = 0; g < w.segment; ++g) {
+          s[j] = p.initial != nullptr && nl * 4 + j < p.states
+                     ? static_cast<const A*>(p.initial)[(w.b * p.dim + d) * p.states + nl * 4 + j]
+                     : A(0);
+      };
+      auto segment = [&](int g, auto by) {
         const int64_t row = (w.b * p.segments + g) * p.dim + d;
-        const A sum = static_cast<const A*>(p.seg_sum)[row];
-        const Four<A> e = static_cast<const Four<A>*>(p.seg_state)[row * LN + nl];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = exp_2(sum * r[j]) * s[j] + e.v[j];
+        return by(s, static_cast<const A*>(p.seg_sum)[row], r,
+                  static_cast<const Four<A>*>(p.seg_state)[row * LN + nl]);
+      };
+      // the segments before this one
+      initial();
+      bool grows = false;
+#pragma unroll 4
+      for (int g = 0; g < w.segment; ++g) grows |= segment(g, carry<A>);
+      if (grows) {
+        initial();
+        for (int g = 0; g < w.segment; ++g) segment(g, carry_growing<A>);
       }
     }
     h[k][0] = two(s[0], s[1]);
@@ -628,20 +658,31 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = nl * 4 + (j ^ order);
-      const bool live = in && n < p.states;
-      q[j] = live ? rate(static_cast<const A*>(p.a)[d * p.states + n]) : A(0);
-      s[j] = live && p.d_final != nullptr
-                 ? static_cast<const A*>(p.d_final)[(w.b * p.dim + d) * p.states + n]
-                 : A(0);
+      q[j] = in && n < p.states ? rate(static_cast<const A*>(p.a)[d * p.states + n]) : A(0);
     }
-    if (in) {
-#pragma unroll 4
-      for (int g = p.segments - 1; g > w.segment; --g) {  // the segments after this one
-        const int64_t row = (w.b * p.segments + g) * p.dim + d;
-        const A sum = static_cast<const A*>(p.seg_sum)[row];
-        const Four<A> e = reorder(static_cast<const Four<A>*>(p.seg_state)[row * LN + nl], order);
+    auto behind = [&] {  // the gradients of the last states
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = exp_2(sum * q[j]) * s[j] + e.v[j];
+      for (int j = 0; j < 4; ++j) {
+        const int n = nl * 4 + (j ^ order);
+        s[j] = in && n < p.states && p.d_final != nullptr
+                   ? static_cast<const A*>(p.d_final)[(w.b * p.dim + d) * p.states + n]
+                   : A(0);
+      }
+    };
+    behind();
+    if (in) {
+      auto segment = [&](int g, auto by) {
+        const int64_t row = (w.b * p.segments + g) * p.dim + d;
+        return by(s, static_cast<const A*>(p.seg_sum)[row], q,
+                  reorder(static_cast<const Four<A>*>(p.seg_state)[row * LN + nl], order));
+      };
+      // the segments after this one
+      bool grows = false;
+#pragma unroll 4
+      for (int g = p.segments - 1; g > w.segment; --g) grows |= segment(g, carry<A>);
+      if (grows) {
+        behind();
+        for (int g = p.segments - 1; g > w.segment; --g) segment(g, carry_growing<A>);
       }
     }
     ra[k][0] = two(q[0], q[1]), ra[k][1] = two(q[2], q[3]);
