@@ -443,8 +443,11 @@ int fdwt_selscan_forward(const fdwt_scan_desc* desc, const void* x, const void* 
                          size_t workspace_bytes, void* stream);
 /* Gradients from dL/dy (strides dy_stride) and dL/dfinal_state (NULL: zeros), contiguous; those
  * of a, b, c, skip, dt_bias and the initial state may be NULL, dgate without a gate.  Sums over
- * tokens, channels and sequences are added in a fixed order. */
+ * tokens, channels and sequences are added in a fixed order.  The workspace holds parts of db and
+ * dc, up to 1 GiB of them at a time (or those of one tile of channels); _least is enough for a call
+ * where both are NULL. */
 size_t fdwt_selscan_backward_workspace(const fdwt_scan_desc* desc);
+size_t fdwt_selscan_backward_workspace_least(const fdwt_scan_desc* desc);
 int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, const void* dt,
                           const void* a, const void* b, const void* c, const void* skip,
                           const void* gate, const void* dt_bias, const int32_t* lengths,

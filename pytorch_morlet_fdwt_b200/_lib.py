@@ -135,6 +135,7 @@ SIGNATURES = {
     "fdwt_selscan_forward": (ctypes.c_int, [ctypes.c_void_p] * 15 + [
         ctypes.c_size_t, ctypes.c_void_p]),
     "fdwt_selscan_backward_workspace": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "fdwt_selscan_backward_workspace_least": (ctypes.c_size_t, [ctypes.c_void_p]),
     "fdwt_selscan_backward": (ctypes.c_int, [ctypes.c_void_p] * 23 + [
         ctypes.c_size_t, ctypes.c_void_p]),
     "fdwt_selscan_step": (ctypes.c_int, [ctypes.c_void_p] * 10 + [

@@ -4,29 +4,37 @@
 namespace fdwt {
 namespace {
 
-// db and dc (batch, length, groups, states) from the tiles' parts, added in a fixed order.
+// db and dc (batch, length, groups, states) of the groups from group0 on, from the parts of the tiles
+// tile0 ... tile1 - 1, added in a fixed order: a group's sum goes on from `sums` where earlier tiles of it
+// were in another launch, and into it where later ones are.
 template <typename T>
 __global__ void __launch_bounds__(256)
-scan_bc_kernel(const typename AccOf<T>::type* __restrict__ part, const int32_t* __restrict__ lengths,
-               int64_t batch, int64_t length, int groups, int64_t tiles, int states, int padded,
-               T* __restrict__ db, T* __restrict__ dc) {
+scan_bc_kernel(const typename AccOf<T>::type* __restrict__ part,
+               typename AccOf<T>::type* __restrict__ sums, const int32_t* __restrict__ lengths,
+               int64_t batch, int64_t length, int groups, int group0, int64_t tiles, int64_t tile0,
+               int64_t tile1, int states, int padded, T* __restrict__ db, T* __restrict__ dc) {
   using A = typename AccOf<T>::type;
   const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   const int e = static_cast<int>(id % (2 * padded));
-  const int64_t row = id / (2 * padded);  // (group, batch, token)
+  const int64_t row = id / (2 * padded) + group0 * batch * length;  // (group, batch, token)
   const int n = e % padded;
   if (row >= groups * batch * length || n >= states) return;
   T* out = e < padded ? db : dc;
   if (out == nullptr) return;
   const int64_t t = row % length, b = row / length % batch, g = row / length / batch;
+  const int64_t first = g * tiles > tile0 ? g * tiles : tile0;
+  const int64_t end = (g + 1) * tiles < tile1 ? (g + 1) * tiles : tile1;
+  if (first >= end) return;
   A sum = A(0);
   if (lengths == nullptr || t < lengths[b]) {
+    if (first != g * tiles) sum = sums[row * 2 * padded + e];
     const int64_t step = batch * length * 2 * padded;
-    const A* q = part + g * tiles * step + (b * length + t) * 2 * padded + e;
+    const A* q = part + (first - tile0) * step + (b * length + t) * 2 * padded + e;
 #pragma unroll 4
-    for (int64_t k = 0; k < tiles; ++k) sum += q[k * step];
+    for (int64_t k = first; k < end; ++k, q += step) sum += *q;
   }
-  out[((b * length + t) * groups + g) * states + n] = from_acc<T>(sum);
+  if (end == (g + 1) * tiles) out[((b * length + t) * groups + g) * states + n] = from_acc<T>(sum);
+  else sums[row * 2 * padded + e] = sum;
 }
 
 // da, dskip and ddt_bias: columns summed over the rows (sequences and segments) in a fixed order, 32
@@ -154,17 +162,27 @@ Segments segment_bytes(const fdwt_scan_desc* d, const Cut& c) {
   s.bytes = s.sum + up256(rows * a);
   return s;
 }
+// Parts of db and dc: one for each tile and token.  Tiles are the narrower the more states there are, so
+// with all of them at once this would take 4 KB a token of 2048 channels at 16 states and 256 KB at 128.
+// Above kMostPartBytes the backward pass is launched for some tiles at a time, and the sums go on from one
+// launch's tiles to the next's, in the same order.
+constexpr size_t kMostPartBytes = size_t(1) << 30;
 struct Parts {
-  size_t a, ch, bc, bytes;
+  size_t a, ch, bc, sums, least, bytes;  // least: without db and dc
+  int64_t tiles;  // of a launch
 };
 Parts part_bytes(const fdwt_scan_desc* d, const Cut& c) {
   const size_t size = acc_size(d->dtype), np = 4 * lanes_of(d->states);
   const size_t rows = size_t(d->batch) * c.segments;
+  const int64_t all = c.tiles * d->groups;
+  const size_t tile = size_t(d->batch) * d->length * 2 * np * size;
   Parts p;
+  p.tiles = tile == 0 ? all : imax(1, imin(all, static_cast<int64_t>(kMostPartBytes / tile)));
   p.a = segment_bytes(d, c).bytes;
   p.ch = p.a + up256(rows * d->dim * np * size);
-  p.bc = p.ch + up256(rows * 2 * d->dim * size);
-  p.bytes = p.bc + up256(size_t(c.tiles) * d->groups * d->batch * d->length * 2 * np * size);
+  p.bc = p.least = p.ch + up256(rows * 2 * d->dim * size);
+  p.sums = p.bc + up256(p.tiles * tile);
+  p.bytes = p.sums + (p.tiles < all ? up256(d->groups * tile) : 0);
   return p;
 }
 
@@ -210,6 +228,7 @@ void see_alignment(ScanArgs* p, const fdwt_scan_desc* d, bool backward) {
 void cut_into(ScanArgs* p, const fdwt_scan_desc* d, const Cut& c, void* ws) {
   const Segments s = segment_bytes(d, c);
   p->tiles = c.tiles, p->segments = c.segments, p->seg_len = c.seg_len;
+  p->tile_count = c.tiles * d->groups;
   p->seg_state = static_cast<char*>(ws) + s.state;
   p->seg_sum = static_cast<char*>(ws) + s.sum;
 }
@@ -267,6 +286,11 @@ extern "C" size_t fdwt_selscan_backward_workspace(const fdwt_scan_desc* desc) {
   return part_bytes(desc, backward_cut(desc)).bytes;
 }
 
+extern "C" size_t fdwt_selscan_backward_workspace_least(const fdwt_scan_desc* desc) {
+  if (!scan_ok(desc) || desc->states > FDWT_MAX_SCAN_STATES) return 0;
+  return part_bytes(desc, backward_cut(desc)).least;
+}
+
 extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, const void* dt,
                                      const void* a, const void* b, const void* c, const void* skip,
                                      const void* gate, const void* dt_bias, const int32_t* lengths,
@@ -291,14 +315,17 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
                                    ddt != nullptr));
   const Cut cut = backward_cut(desc);
   const Parts parts = part_bytes(desc, cut);
-  if (workspace == nullptr || workspace_bytes < parts.bytes) return FDWT_ERR_WORKSPACE;
+  const bool want_bc = db != nullptr || dc != nullptr;
+  if (workspace == nullptr || workspace_bytes < (want_bc ? parts.bytes : parts.least))
+    return FDWT_ERR_WORKSPACE;
   FDWT_CHECK(aligned32({workspace, checkpoints}));
   ScanArgs p = args_of(desc, x, dt, a, b, c, skip, gate, dt_bias, nullptr, lengths);
   p.check = const_cast<void*>(checkpoints);
   p.dy = dy, p.d_final = d_final_state, p.dx = dx, p.ddt = ddt, p.dgate = dgate;
   p.d_initial = d_initial_state;
   char* ws = static_cast<char*>(workspace);
-  p.part_a = ws + parts.a, p.part_ch = ws + parts.ch, p.part_bc = ws + parts.bc;
+  p.part_a = ws + parts.a, p.part_ch = ws + parts.ch;
+  p.part_bc = want_bc ? ws + parts.bc : nullptr;
   see_alignment(&p, desc, true);
   cut_into(&p, desc, cut, workspace);
   const int lanes = lanes_of(desc->states), np = 4 * lanes;
@@ -310,23 +337,30 @@ extern "C" int fdwt_selscan_backward(const fdwt_scan_desc* desc, const void* x, 
       // the state launch has tiles of its own
       ScanArgs r = p;
       r.tiles = cdiv(p.per, scan_fwd_tile(lanes));
+      r.tile_count = r.tiles * desc->groups;
       st = scan_states<T>(r, lanes, true, s);
       if (st != FDWT_OK) return st;
     }
-    st = scan_backward<T>(p, lanes, s);
-    if (st != FDWT_OK) return st;
-    const int64_t rows = desc->batch * cut.segments;
-    if (desc->length > 0 && (db != nullptr || dc != nullptr)) {
-      const int64_t n = int64_t(desc->groups) * desc->batch * desc->length * 2 * np;
+    const int64_t all = cut.tiles * desc->groups, each = want_bc ? parts.tiles : all;
+    for (int64_t tile = 0; tile < all; tile += each) {
+      const int64_t end = imin(all, tile + each);
+      p.tile0 = tile, p.tile_count = end - tile;
+      st = scan_backward<T>(p, lanes, s);
+      if (st != FDWT_OK) return st;
+      if (desc->length == 0 || !want_bc) continue;
+      const int64_t group0 = tile / cut.tiles, count = cdiv(end, cut.tiles) - group0;
+      const int64_t n = count * desc->batch * desc->length * 2 * np;
       if (cdiv(n, 256) > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
       st = pre_launch(s);
       if (st != FDWT_OK) return st;
       scan_bc_kernel<T><<<static_cast<unsigned>(cdiv(n, 256)), 256, 0, s>>>(
-          static_cast<const A*>(p.part_bc), lengths, desc->batch, desc->length, desc->groups,
-          cut.tiles, desc->states, np, static_cast<T*>(db), static_cast<T*>(dc));
+          static_cast<const A*>(p.part_bc), reinterpret_cast<A*>(ws + parts.sums), lengths,
+          desc->batch, desc->length, desc->groups, static_cast<int>(group0), cut.tiles, tile, end,
+          desc->states, np, static_cast<T*>(db), static_cast<T*>(dc));
       st = launch_status();
       if (st != FDWT_OK) return st;
     }
+    const int64_t rows = desc->batch * cut.segments;
     if (da == nullptr && dskip == nullptr && ddt_bias == nullptr) return FDWT_OK;
     const int64_t columns = cdiv(desc->dim * (np + 2), 32);
     if (columns > INT32_MAX) return FDWT_ERR_UNSUPPORTED;

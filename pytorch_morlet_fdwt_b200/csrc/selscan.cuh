@@ -52,6 +52,7 @@ struct ScanArgs {
   int64_t xs[2], dts[2], gs[2], dys[2], bs[3], cs[3];
   int vec, vec_states;  // rows of channels, of b and c begin on boundaries of 4 elements
   int64_t per, tiles; // channels of a group, tiles of one
+  int64_t tile0, tile_count;  // the launch's tiles among those of all groups
   int segments;
   int64_t seg_len;    // tokens, a multiple of kScanCheck and of the staged tokens
   void *seg_state, *seg_sum;  // [batch][segments][dim][padded states], [batch][segments][dim]
@@ -60,7 +61,7 @@ struct ScanArgs {
   // backward
   const void *dy, *d_final;
   void *dx, *ddt, *dgate, *d_initial;
-  void *part_bc;      // [groups * tiles][batch][length][2][padded states]
+  void *part_bc;      // [tile_count][batch][length][2][padded states]; null where none are wanted
   void *part_a;       // [batch][segments][dim][padded states]
   void *part_ch;      // [batch][segments][2][dim]: dskip, ddt_bias
 };

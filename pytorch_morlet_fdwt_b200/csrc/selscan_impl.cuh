@@ -207,9 +207,9 @@ struct Place {
 template <int CT>
 __device__ __forceinline__ Place place_of(const ScanArgs& p, int segments, int first) {
   Place w;
-  const int64_t tiles = p.tiles * p.groups;
+  const int64_t tiles = p.tile_count;
   const int64_t id = blockIdx.x;
-  w.tile = static_cast<int>(id % tiles);
+  w.tile = static_cast<int>(id % tiles + p.tile0);
   w.segment = static_cast<int>(id / tiles % segments) + first;
   w.b = id / tiles / segments;
   w.group = static_cast<int>(w.tile / p.tiles);
@@ -731,7 +731,8 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     bc.fetch(p, static_cast<int>(w.count - t < TT ? w.count - t : TT), -TT);
   };
 
-  A* part_bc = static_cast<A*>(p.part_bc) + (w.tile * p.batch + w.b) * p.length * 2 * NP;
+  A* part_bc =
+      static_cast<A*>(p.part_bc) + ((w.tile - p.tile0) * p.batch + w.b) * p.length * 2 * NP;
   {  // what lies after the valid tokens
     const A zero[4] = {A(0), A(0), A(0), A(0)};
     for (int64_t t = (w.count > w.t0 ? w.count : w.t0) + row0; t < w.t1; t += I::ROWS) {
@@ -941,7 +942,7 @@ scan_bwd_kernel(const __grid_constant__ ScanArgs p) {
     }
     result -= TT * p.dim;
     // (tokens past the valid ones have no part: scan_bc_kernel leaves them out)
-    for (int e = threadIdx.x; e < TT * 2 * LN; e += 128) {
+    for (int e = p.part_bc != nullptr ? threadIdx.x : TT * 2 * LN; e < TT * 2 * LN; e += 128) {
       if (e / (2 * LN) >= left + row0) continue;
       Four<A> s = reinterpret_cast<const Four<A>*>(joined)[e];
 #pragma unroll
@@ -1119,7 +1120,7 @@ template <typename F> int with_lanes(int lanes, F fn) {
   }
 }
 inline int scan_grid(const ScanArgs& p, int segments, unsigned* grid) {
-  const int64_t blocks = p.tiles * p.groups * segments * p.batch;
+  const int64_t blocks = p.tile_count * segments * p.batch;
   if (blocks > INT32_MAX) return FDWT_ERR_UNSUPPORTED;
   *grid = static_cast<unsigned>(blocks);
   return FDWT_OK;

@@ -46,8 +46,8 @@ class _ScanDesc(ctypes.Structure):
 @lru_cache(maxsize=2048)
 def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, device_index):
     """What a call's types, sizes and strides come to, checked once for each combination on one
-    device: the C descriptor, its address, the bytes of the workspaces and of the kept states, and
-    the type of states; None where a last axis is not contiguous.  In order x, dt, b, c and the gate
+    device: the C descriptor, its address, the bytes of the workspaces and of the kept states, the type
+    of states, and the bytes of a backward pass without dL/db and dL/dc; None where a last axis is not contiguous.  In order x, dt, b, c and the gate
     (None without); ``lead`` names the axes before the channels."""
     code = _lib.dtype_code(dtypes[0])
     names = ("x", "dt", "b", "c", "gate")
@@ -92,7 +92,8 @@ def _describe(lead, dtypes, shapes, strides, a_shape, dy_stride, softplus, devic
         return (d, at, int(lib.fdwt_selscan_forward_workspace(at)),
                 int(lib.fdwt_selscan_checkpoint_bytes(at)),
                 int(lib.fdwt_selscan_backward_workspace(at)),
-                torch.float64 if code == 1 else torch.float32)
+                torch.float64 if code == 1 else torch.float32,
+                int(lib.fdwt_selscan_backward_workspace_least(at)))
 
 
 def _plan(lead, x, dt, a, b, c, gate, softplus, dy_stride=None):
@@ -117,7 +118,7 @@ def _parameter(name: str, t: Optional[torch.Tensor], shape, dtype) -> Optional[t
 
 
 def _forward(x, dt, a, b, c, skip, gate, dt_bias, initial, lengths, plan, keep: bool):
-    d, desc, nws, ncheck, _, acc = plan
+    d, desc, nws, ncheck, _, acc, _ = plan
     dev = x.device
     y = _lib.empty_like(x)
     final = (x.new_empty((d.batch, d.dim, d.states), dtype=acc) if initial is None
@@ -171,7 +172,9 @@ class _SelectiveScanFunction(torch.autograd.Function):
         dskip = like(skip) if need_skip else None
         dbias = like(dt_bias) if need_bias else None
         di = like(initial) if need_i else None
-        _, desc, _, _, nws, _ = plan
+        _, desc, _, _, nws, _, least = plan
+        if not (need_b or need_c):
+            nws = least
         with _lib.device_guard(dev):
             ws = _lib.workspace(nws, dev)
             st = _lib.load().fdwt_selscan_backward(
@@ -251,7 +254,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
         x, dt, b, c = _rows(x), _rows(dt), _rows(b), _rows(c)
         gate = None if gate is None else _rows(gate)
         plan = _plan(_TOKEN, x, dt, a, b, c, gate, dt_softplus)
-    d, desc, _, _, _, acc = plan
+    d, desc, _, _, _, acc, _ = plan
     a = _parameter("a", a, (d.dim, d.states), acc)
     skip = _parameter("skip", skip, (d.dim,), acc)
     dt_bias = _parameter("dt_bias", dt_bias, (d.dim,), acc)
