@@ -47,9 +47,11 @@ __device__ __forceinline__ void softplus(const float* v, float* d, float* slope)
     q = fma(q, z, both(0.40024852752685547f));
     q = fma(q, z, both(0.6666631698608398f));
     q = fma(q, z, both(2.0f));
-    // (max, and not (v + |v|) / 2, which is NaN for -inf and infinite above half the largest float)
-    const Two<float> top = two(max_nan(v[j], 0.0f), max_nan(v[j + 1], 0.0f));
-    const Two<float> r = add(top, mul(s, q));
+    // (max, and not (v + |v|) / 2, which is NaN for -inf and infinite above half the largest float; sums
+    // that the compiler does not join with the product, so that other steps keep their last bits)
+    const Two<float> rest = mul(s, q);
+    const Two<float> r = two(__fadd_rn(max_nan(v[j], 0.0f), first(rest)),
+                             __fadd_rn(max_nan(v[j + 1], 0.0f), second(rest)));
     if (SLOPE) {
       const Two<float> o = add(e, both(1.0f));
       const Two<float> w = two(reciprocal(first(o)), reciprocal(second(o))), ew = mul(e, w);
