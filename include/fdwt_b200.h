@@ -353,8 +353,8 @@ int fdwt_rms_norm_forward(int dtype, int residual_dtype, int param_dtype, int64_
                           int64_t dim, const void* x, const void* residual, const void* weight,
                           double eps, void* y, void* total, void* rstd, void* stream);
 /* The same with y in 8 bits: groups of `group` neighbouring values (a divisor of dim) share the
- * scale max |y| / 448 (FDWT_E4M3) or max |y| / 127 (FDWT_INT8), 1 where all are zero, and
- * q = round(y / scale).  scales: (rows, dim / group) fp32.  Rows of fp64 are not supported. */
+ * scale max |y| / 448 (FDWT_E4M3) or max |y| / 127 (FDWT_INT8), at least 2^-126, 1 where all are
+ * zero, and q = round(y / scale).  scales: (rows, dim / group) fp32.  Rows of fp64 are not supported. */
 enum { FDWT_E4M3 = 0, FDWT_INT8 = 1 };
 int fdwt_rms_norm_quantized(int dtype, int residual_dtype, int param_dtype, int out_type,
                             int64_t rows, int64_t dim, int64_t group, const void* x,
@@ -411,7 +411,7 @@ int fdwt_causal_conv1d_step(const fdwt_conv1d_desc* desc, const void* x, const v
 /* ------------------------------------------------------------------------------------------
  * Selective state space scan (no counterpart in the reference).  Channel d has `states` numbers
  * h[n]; over the tokens t of a sequence, with v = dt_t + dt_bias and delta = v or, with
- * dt_softplus, log(1 + e^v),
+ * dt_softplus, log(1 + e^v) (0 for v = -inf),
  *   h[n] <- e^(delta a[n]) h[n] + delta x_t b_t[n],   p_t = sum_n c_t[n] h[n] + skip x_t,
  *   y_t = p_t, or p_t gate_t / (1 + e^-gate_t) with a gate.
  * Channel d reads b and c of group d / (dim / groups).  x, dt, gate (may be NULL) are addressed

@@ -11,10 +11,12 @@
 // loads of several tokens are in flight.  Sums are 32 bits (64 for fp64) on pairs of channels (one
 // packed instruction a pair); y and the gradients are rounded once.
 //
-// Measured, 4 taps with silu: 4 x 4096 x 2048 bf16 forward 33 us (4.1 TB/s), backward 64 us (3.2
-// TB/s); fp32 52 us forward (5.2 TB/s).  In 16 bits the exponential and reciprocal of silu (half of
-// the XU pipe's time) and the instructions around them take as long as the bytes do.  A thread of the
-// backward pass takes 2 channels (4: 160 registers, 1.2 times the time; 1 in fp64).
+// Measured, 4 taps with silu: 4 x 4096 x 2048 bf16 forward 33 us (4.1 TB/s), backward 62 us (3.2
+// TB/s); fp32 52 us forward (5.2 TB/s).  In 16 bits it is latency that bounds them, not bytes: forward
+// 143 registers, 12 warps an SM, 0.46 instructions issued a cycle and scheduler, DRAM 31 % busy, stalls on
+// results of fixed latency 1.5 and on loads 1.1 warps an issue; backward 96 registers, 20 warps, 0.61,
+// 32 %, and 82 instructions a token of two channels.  A thread of the backward pass takes 2 channels (4:
+// 160 registers, 1.2 times the time; 1 in fp64).
 #include "pairs.cuh"
 #include "row_groups.cuh"
 

@@ -94,8 +94,8 @@ __device__ __forceinline__ void store_quant(O* p, const float* x, float inv) {
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
 }
-// The scale of a group whose largest magnitude is m: 1 where all are zero, else at least 2^-126, so
-// that its reciprocal is finite.  NaN stays NaN.
+// The scale of a group whose largest magnitude is m: 1 where all are zero, else at least 2^-126 (the
+// smallest normal number), so that its reciprocal is finite.  NaN stays NaN.
 template <typename O> __device__ __forceinline__ float scale_of(float m) {
   return m == 0.0f ? 1.0f : max_nan(m * (1.0f / Quant<O>::kMost), 0x1p-126f);
 }

@@ -25,11 +25,13 @@
 // each segment's end state from zero and its sum of delta, and the main launch's blocks add up those
 // before them.
 //
-// Measured (bf16, 16 states, a gate; ncu and events).  64 x 1024 x 2048, one launch: 786 us, 2.7e12
-// exponentials a second, 0.59 of their rate, 0.74 with those of the steps and gates counted.
-// 1 x 65536 x 2048, 37 segments: state launch 639 us, main launch 827 us.  4 x 4096 x 2048 with
-// gradients, 9 and 16 segments: 148 + 224 us forward, 165 us of states back in time, 611 us backward,
-// 29 us of sums.  240 single tokens of 2048 channels: 15.4 us (4.4 TB/s).
+// Measured (bf16, 16 states, a gate; ncu and events).  64 x 1024 x 2048, one launch: 794 us, 2.7e12
+// exponentials a second, 0.58 of their rate, 0.73 with those of the steps and gates counted.
+// 1 x 65536 x 2048, 37 segments: state launch 642 us, main launch 838 us.  4 x 4096 x 2048 with
+// gradients, 9 and 16 segments: 154 + 235 us forward, 173 us of states back in time, 637 us backward,
+// 29 us of sums.  240 single tokens of 2048 channels: 15.4 us (4.4 TB/s).  With few states the steps and
+// gates, some 35 instructions and 4 exponentials or reciprocals a token and channel, are as much work as
+// the states: 64 x 1024 x 1024 with 4 states 238 us, 1.1e12 exponentials of decays a second.
 // What was tried on the forward launches and changed nothing or made them slower: a quarter of the
 // exponentials by a polynomial on the FMA pipes (state launch 640 us either way, main launch 6 %
 // slower), 5 and 6 blocks an SM (5 % and 9 % slower), a second copy of the staged steps for wider

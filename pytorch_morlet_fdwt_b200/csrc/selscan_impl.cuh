@@ -100,12 +100,13 @@ template <bool FAST> __device__ __forceinline__ void sigmoid_at(const double* v,
   for (int j = 0; j < 4; ++j) g[j] = 1.0 / (1.0 + exp(-v[j]));
 }
 
-// Added to the exponent of every decay.  The hardware's 2^x is 0.5e-8 to 2.7e-8 too small in the mean
-// for -1/2 < x < 0 (measured over 2^20 values for each power of two; 3e-8 to 4e-8 root mean square),
-// and a state is a product of hundreds of decays: this takes the mean back (2^lift = 1 + 1.4e-8) at no
-// cost, a product becoming a product and sum.  4 x 4096 x 2048 against 64 bits: last states 5e-7 off
-// without, 2.8e-7 with; dL/da 1.7e-6 and 0.75e-6.  2^lift itself comes out as 1, so that a step of zero
-// keeps the state as it is.
+// Added to the exponent of every decay.  The hardware's 2^x is 1.8e-8 to 2.7e-8 too small in the mean
+// for -1/2 < x < -2^-8 (measured over 2^20 values for each power of two; 3e-8 to 4e-8 root mean square),
+// and a state is a product of hundreds of decays: this takes half of the mean back or more (2^lift = 1 +
+// 1.4e-8) at no cost, a product becoming a product and sum.  Nearer to zero, where the mean is -0.5e-8 to
+// -0.8e-8, it becomes one of the same size and the other sign.  4 x 4096 x 2048 against 64 bits: last
+// states 5e-7 off without, 2.8e-7 with; dL/da 1.7e-6 and 0.75e-6.  2^lift itself comes out as 1, so that a
+// step of zero keeps the state as it is.
 template <typename A> __device__ __forceinline__ A lift() { return sizeof(A) == 4 ? A(2e-8) : A(0); }
 template <typename A> __device__ __forceinline__ Two<A> lift2() { return two(lift<A>(), lift<A>()); }
 

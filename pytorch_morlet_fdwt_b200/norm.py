@@ -263,9 +263,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``scales (..., D // group_size)``, so that ``q * scale`` is the result.
 
     Groups of ``group_size`` neighbouring values (a divisor of D; the whole row by default) share
-    a scale, their largest magnitude over 448 (e4m3) or 127 (int8), 1 where all are zero; the
-    result is formed in 32 bits and rounded once, to 8.  A NaN makes its group's scale NaN.  For
-    fp32, fp16 and bf16 inputs.  No gradient."""
+    a scale, their largest magnitude over 448 (e4m3) or 127 (int8), at least ``2 ** -126``, and 1
+    where all are zero; the result is formed in 32 bits and rounded once, to 8.  A NaN makes its
+    group's scale NaN.  For fp32, fp16 and bf16 inputs.  No gradient."""
     x, weight, residual, codes = _rms_inputs(x, weight, residual, eps)
     if dtype not in _QUANTIZED:
         raise TypeError(f"dtype must be one of {', '.join(map(str, _QUANTIZED))}, got {dtype}")

@@ -210,8 +210,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
 
     Returns ``(y (B, L, D), final_state (B, D, N))``, differentiable once in every input but the
     lengths.  fp16 and bf16 inputs are computed in 32 bits, states too, and the result rounded
-    once.  An infinity or NaN reaches the outputs of its token and later ones only.  A call whose
-    inputs need gradients keeps ``L / 8`` states of every channel for the backward pass.
+    once.  An infinity or NaN reaches the outputs of its token and later ones only (an infinity may
+    reach them as a NaN).  A call whose inputs need gradients keeps ``L / 8`` states of every channel
+    for the backward pass, which has up to 1 GiB of scratch besides (or one tile's, if that is more).
     """
     _lib.require_cuda(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths)
     plan = _plan(_SEQUENCE, x, dt, a, b, c, gate, dt_softplus)
